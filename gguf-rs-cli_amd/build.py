@@ -6,6 +6,7 @@ Produces gguf-rs-cli_amd/libgs_sampler.so (HIP, --offload-arch=gfx950) and
 oracle/liboracle.so.  This replaces the reference's build.rs shader step
 (GLSL -> SPIR-V via shaderc, build.rs:24-43) with hipcc code objects.
 """
+import concurrent.futures
 import os
 import subprocess
 import sys
@@ -25,7 +26,7 @@ HIP_FLAGS = [
     "-mllvm", "-amdgpu-function-calls=false",
     "-Wall", "-Wno-unused-function",
 ]
-SOURCES = ["gs_kernels.hip", "gs_api.cpp", "gs_gemv.hip", "gs_decode.hip", "gs_tokens.cpp"]
+SOURCES = ["gs_kernels.hip", "gs_api.cpp", "gs_gemv.hip", "gs_decode.hip", "gs_tokens.cpp", "gs_rope.hip", "gs_cache.hip", "gs_attn.hip"]
 
 
 def _run(cmd, cwd=None):
@@ -37,14 +38,16 @@ def _run(cmd, cwd=None):
 
 
 def build_library(verbose=False):
-    objs = []
-    for src in SOURCES:
+    def compile_one(src):
         obj = os.path.join(CSRC, os.path.splitext(src)[0] + ".o")
-        cmd = [HIPCC] + HIP_FLAGS + ["-x", "hip", "-c", os.path.join(CSRC, src), "-o", obj]
-        out = _run(cmd)
-        if verbose and out:
-            print(out)
-        objs.append(obj)
+        return obj, _run([HIPCC] + HIP_FLAGS + ["-x", "hip", "-c", os.path.join(CSRC, src), "-o", obj])
+
+    objs = []
+    with concurrent.futures.ThreadPoolExecutor(4) as pool:
+        for obj, out in pool.map(compile_one, SOURCES):
+            if verbose and out:
+                print(out)
+            objs.append(obj)
     tmp = LIB + ".tmp"
     _run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", tmp] + objs)
     os.replace(tmp, LIB)

@@ -1,0 +1,623 @@
+// gs_attn.hip -- attention of new tokens over the paged cache
+// (include/gs_attn.h).
+//
+// The work of a call is cut the same way for every shape.  A unit is one head
+// of keys and values of one sequence and up to R of its query rows (row r of a
+// sequence is token r / G and head r % G of the G that share the keys); a unit
+// has one tile per kTile keys that its rows see.  The tiles of all units, one
+// after the other, are dealt to the workgroups in equal runs.  So a long row
+// and a short one, many and few, cost what their keys cost; a unit that a
+// run's end cuts leaves its parts (maximum, sum, weighted values) in the
+// workspace, and a second kernel joins them in order.
+//
+// Each run goes through its keys once, with the running maximum and sum of the
+// softmax; the weights do not leave the registers.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "../../include/gs_attn.h"
+#include "gs_cache.hpp"
+
+namespace gs {
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ f4 mfma(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f4 mfma(b8 a, b8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+struct AttnArgs {
+    const char *k, *v;              // the layer's pages
+    const void *q;
+    void *out;
+    size_t ld_q, ld_out;
+    const uint32_t *table, *len, *rows, *start;
+    uint32_t n, n_tokens, n_rows, n_pages, ld_table, n_kv, group, d;
+    int shift;                      // log2 of the page size
+    float scale;                    // of the scores, times log2(e)
+    uint32_t window;                // (0xffffffff: none)
+    uint32_t n_wg;                  // runs
+    float *parts;                   // [2 n_wg][R][D + 2]: a run's cut units: the one it begins with, the one it ends with
+    struct Cut *cuts;               // [n_wg]
+};
+
+// A unit that a run begins and does not end.
+struct Cut {
+    uint32_t last;                  // the run that ends it; 0: none
+    uint32_t first_token, row0, rows, kvh;
+    uint32_t keyless;               // rows before this one see no key
+};
+
+// One sequence of the call.
+struct Seq {
+    uint32_t row, len, first, nq;
+};
+
+__device__ __forceinline__ Seq seq_of(const AttnArgs &a, uint32_t i)
+{
+    Seq s;
+    s.first = a.start ? min(a.start[i], a.n_tokens) : i;
+    const uint32_t end = a.start ? min(a.start[i + 1], a.n_tokens) : i + 1;
+    s.nq = end > s.first ? end - s.first : 0;
+    s.row = a.rows ? a.rows[i] : i;
+    s.len = s.row < a.n_rows ? min(a.len[s.row], a.ld_table << a.shift) : 0;
+    return s;
+}
+
+// The keys that rows r0 .. r1 - 1 of a sequence see, [lo, hi), and the first
+// tile; `tiles` is at least 1, so that rows without keys are written too.
+template <int kTile> struct Span {
+    uint32_t lo, hi, tile0, tiles;
+    __device__ __forceinline__ Span(const AttnArgs &a, const Seq &s, uint32_t r0, uint32_t r1)
+    {
+        const int64_t p0 = (int64_t)s.len - s.nq + r0 / a.group, p1 = (int64_t)s.len - s.nq + (r1 - 1) / a.group;
+        hi = (uint32_t)max((int64_t)0, p1 + 1);
+        lo = (uint32_t)max((int64_t)0, p0 + 1 - (int64_t)a.window);
+        tile0 = lo / kTile;
+        tiles = hi > lo ? (hi + kTile - 1) / kTile - tile0 : 1;
+    }
+};
+
+template <int R, int kTile> __device__ __forceinline__ uint32_t tiles_of(const AttnArgs &a, const Seq &s)
+{
+    uint32_t t = 0;
+    const uint32_t rows = s.nq * a.group;
+    for (uint32_t r = 0; r < rows; r += R) t += Span<kTile>(a, s, r, min(r + R, rows)).tiles;
+    return t;
+}
+
+// The run of this workgroup: its tiles [t0, t1) of `total`, the sequence the
+// first of them is in, and how many tiles of that sequence come before it.
+// Each thread counts a stretch of the sequences.
+struct Run {
+    uint64_t t0, t1, total;
+    uint32_t n_wg, seq;
+    uint64_t skip;
+};
+
+template <int R, int kTile, int kThreads> __device__ __forceinline__ Run run_of(const AttnArgs &a)
+{
+    __shared__ uint64_t s_wave[kThreads / 64];
+    __shared__ uint32_t s_seq;
+    __shared__ uint64_t s_skip;
+    const uint32_t each = (a.n + kThreads - 1) / kThreads;
+    const uint32_t i0 = min(threadIdx.x * each, a.n), i1 = min(i0 + each, a.n);
+    uint64_t mine = 0;
+    for (uint32_t i = i0; i < i1; i++) mine += (uint64_t)tiles_of<R, kTile>(a, seq_of(a, i)) * a.n_kv;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    uint64_t x = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint64_t y = __shfl_up(x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 63) s_wave[w] = x;
+    __syncthreads();
+    uint64_t before = x - mine;
+    Run r;
+    r.total = 0;
+#pragma unroll
+    for (int i = 0; i < kThreads / 64; i++) {
+        if (i < w) before += s_wave[i];
+        r.total += s_wave[i];
+    }
+    r.n_wg = (uint32_t)min((uint64_t)a.n_wg, r.total);
+    const uint32_t g = blockIdx.x;
+    if (g >= r.n_wg) { r.t0 = r.t1 = 0; r.seq = 0; r.skip = 0; return r; }
+    r.t0 = r.total * g / r.n_wg;
+    r.t1 = r.total * (g + 1) / r.n_wg;
+    if (r.t0 >= before && r.t0 < before + mine) {
+        uint32_t i = i0;
+        for (;; i++) {
+            const uint64_t t = (uint64_t)tiles_of<R, kTile>(a, seq_of(a, i)) * a.n_kv;
+            if (r.t0 < before + t) break;
+            before += t;
+        }
+        s_seq = i;
+        s_skip = r.t0 - before;
+    }
+    __syncthreads();
+    r.seq = s_seq;
+    r.skip = s_skip;
+    return r;
+}
+
+// An infinity or NaN among 8 values.
+template <class T> __device__ __forceinline__ bool not_finite(u4v x)
+{
+    constexpr uint32_t e = sizeof(T) == 2 && __is_same(T, _Float16) ? 0x7c00u : 0x7f80u;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; i++) bad |= (x[i] & e) == e || (x[i] >> 16 & e) == e;
+    return bad;
+}
+
+template <class T> struct Vec;
+template <> struct Vec<_Float16> { typedef h8 v8; };
+template <> struct Vec<__bf16> { typedef b8 v8; };
+
+// Weights are held times 2^15 where the type's smallest numbers are near: f16
+// weights of 2^-15 of the largest would lose bits below 2^-14.
+template <class T> constexpr float kLift = __is_same(T, _Float16) ? 15.0f : 0.0f;
+
+constexpr int kRowTile = 128;           // keys of a tile: 32 for each wave
+
+// Up to 16 NT query rows against the keys, for single tokens and few of them:
+// what bounds it is the read of K and V, so each wave reads its 32 keys of a
+// tile straight to registers, once, K for the next tile while it works on
+// this tile's V and the other way round.  The products are S^T = K Q^T and
+// O^T = V^T P^T, 16 x 16 x 32: a lane then holds the weights of one query row
+// (lane & 15) for exactly the 8 keys that it has to give to the second
+// product, if row m of the two K tiles is key 8 (m / 4) + 4 t + m % 4.  V^T's
+// columns come from the 8 rows of V in a lane by a transposition of 8 x 8
+// values in registers (the value a lane's row m stands for is 8 m + i in
+// product i).  Four waves' sums meet in LDS at a unit's end.
+// F32: q in three parts of T whose sum is q (scaled by a power of two into
+// f16's range), and the weights too, so the products keep 24 bits.
+template <class T, int D, int NT, bool F32>
+__global__ void __launch_bounds__(256) attn_rows_kernel(const AttnArgs a)
+{
+    constexpr int R = 16 * NT, NP = F32 ? 3 : 1, KS = D / 32;
+    constexpr int CW = D >= 128 ? 8 : D / 16, NC = D / (16 * CW);       // values of a lane's V chunk, chunks
+    typedef typename Vec<T>::v8 v8;
+    typedef T vw __attribute__((ext_vector_type(CW)));
+    __shared__ float s_o[4][16][D + 4];
+    __shared__ float s_m[4][16], s_l[4][16];
+
+    Run run = run_of<R, kRowTile, 256>(a);
+    if (threadIdx.x == 0 && blockIdx.x < a.n_wg) a.cuts[blockIdx.x].last = 0;
+    if (run.t0 >= run.t1) return;
+
+    const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t page = 1u << a.shift;
+    const size_t head = (size_t)a.d << a.shift;         // values of a head's page
+
+    uint32_t si = run.seq;
+    Seq s = seq_of(a, si);
+    uint32_t per = tiles_of<R, kRowTile>(a, s);
+    uint64_t t = run.t0;
+    uint32_t kvh = (uint32_t)(run.skip / max(per, 1u)), skip = (uint32_t)(run.skip % max(per, 1u)), r0 = 0;
+    while (t < run.t1) {
+        const uint32_t rows = s.nq * a.group;
+        if (kvh == a.n_kv || rows == 0) {               // the next sequence
+            si++;
+            s = seq_of(a, si);
+            per = tiles_of<R, kRowTile>(a, s);
+            kvh = 0; r0 = 0; skip = 0;
+            continue;
+        }
+        const uint32_t r1 = min(r0 + R, rows);
+        const Span<kRowTile> span(a, s, r0, r1);
+        if (skip >= span.tiles) { skip -= span.tiles; r0 += R; continue; }
+        const uint32_t left = (uint32_t)min((uint64_t)(span.tiles - skip), run.t1 - t);
+
+        // ---- queries: row r0 + 16 nt + m, values 32 s + 8 g .. + 7
+        v8 qf[NT][NP][KS];
+        float unscale[NT];
+        int64_t pos[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const uint32_t r = min(r0 + 16 * nt + m, r1 - 1);
+            const uint32_t tok = r / a.group, h = kvh * a.group + (r - tok * a.group);
+            pos[nt] = (int64_t)s.len - s.nq + tok;
+            const size_t at = (size_t)(s.first + tok) * a.ld_q + (size_t)h * a.d;
+            unscale[nt] = a.scale;
+            if constexpr (F32) {
+                float x[KS][8], top = 0.0f;
+#pragma unroll
+                for (int c = 0; c < KS; c++) {
+                    if (32 * c + 8 * g < a.d) load8((const float *)a.q + at + 32 * c + 8 * g, x[c]);
+                    else
+#pragma unroll
+                        for (int e = 0; e < 8; e++) x[c][e] = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[c][e]));
+                }
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                int ex = 0;
+                if (__is_same(T, _Float16) && top > 0.0f && top < INFINITY) ex = 14 - ilogbf(top);
+                unscale[nt] *= ldexpf(1.0f, -ex);       // (0 for rows below 2^-135: their scores are 0)
+#pragma unroll
+                for (int c = 0; c < KS; c++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float y = ldexpf(x[c][e], ex);
+                        const T p0 = (T)y;
+                        const float y1 = y - (float)p0;
+                        const T p1 = (T)y1;
+                        qf[nt][0][c][e] = p0;
+                        qf[nt][1][c][e] = p1;
+                        qf[nt][2][c][e] = (T)(y1 - (float)p1);
+                    }
+            } else {
+#pragma unroll
+                for (int c = 0; c < KS; c++) {
+                    v8 x = {};
+                    if (32 * c + 8 * g < a.d) x = *(const v8 *)((const T *)a.q + at + 32 * c + 8 * g);
+                    qf[nt][0][c] = x;
+                }
+            }
+        }
+
+        // ---- the keys
+        const uint32_t *table = a.table + (size_t)min(s.row, a.n_rows - 1) * a.ld_table;
+        const uint32_t last = span.hi > 0 ? span.hi - 1 : 0;
+        auto place = [&](uint32_t key) {                // of a key's page for this head, in values; the key is held to the unit's
+            const uint32_t p = min(table[min(key, last) >> a.shift], a.n_pages - 1);
+            return ((size_t)p * a.n_kv + kvh) * head;
+        };
+        v8 kf[2][KS];
+        vw vf[8][NC];
+        auto load_k = [&](uint32_t key0) {
+            const T *p = (const T *)a.k + place(key0 + 8 * (m >> 2));
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const T *row = p + (size_t)((key0 + 8 * (m >> 2) + 4 * x + (m & 3)) & (page - 1)) * a.d;
+#pragma unroll
+                for (int c = 0; c < KS; c++) {
+                    v8 y = {};
+                    if (32 * c + 8 * g < a.d) y = *(const v8 *)(row + 32 * c + 8 * g);
+                    kf[x][c] = y;
+                }
+            }
+        };
+        auto load_v = [&](uint32_t key0) {
+            const T *p = (const T *)a.v + place(key0 + 8 * g);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const T *row = p + (size_t)((key0 + 8 * g + j) & (page - 1)) * a.d;
+#pragma unroll
+                for (int c = 0; c < NC; c++) {
+                    vw y = {};
+                    if (16 * CW * c + CW * m < a.d) y = *(const vw *)(row + 16 * CW * c + CW * m);
+                    vf[j][c] = y;
+                }
+            }
+        };
+
+        f4 o[NT][NC][CW];
+        float mx[NT], sum[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            mx[nt] = -INFINITY;
+            sum[nt] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int i = 0; i < CW; i++) o[nt][c][i] = f4{0, 0, 0, 0};
+        }
+        uint32_t key0 = (span.tile0 + skip) * kRowTile + 32 * w;
+        load_k(key0);
+        load_v(key0);
+        for (uint32_t x = 0; x < left; x++, key0 += kRowTile) {
+            // rows that see a part of the 32 keys only
+            const bool edge = key0 + 32 > (uint32_t)max((int64_t)0, (int64_t)s.len - s.nq + r0 / a.group + 1) ||
+                              (int64_t)key0 < (int64_t)s.len - s.nq + (r1 - 1) / a.group + 1 - (int64_t)a.window;
+            f4 sc[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int y = 0; y < 2; y++) {
+                    f4 z = {0, 0, 0, 0};
+#pragma unroll
+                    for (int q = NP - 1; q >= 0; q--)           // (the small parts first)
+#pragma unroll
+                        for (int c = 0; c < KS; c++) z = mfma(kf[y][c], qf[nt][q][c], z);
+                    sc[nt][y] = z;
+                }
+            load_k(key0 + kRowTile);
+
+            float p[NT][8];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    p[nt][j] = sc[nt][j >> 2][j & 3] * unscale[nt];
+                    if (edge) {
+                        const int64_t key = (int64_t)key0 + 8 * g + j;
+                        if (key > pos[nt] || key <= pos[nt] - (int64_t)a.window) p[nt][j] = -INFINITY;
+                    }
+                    top = fmaxf(top, p[nt][j]);
+                }
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                top = fmaxf(top, mx[nt]);
+                const float ref = top == -INFINITY ? 0.0f : top;
+                const float by = __builtin_amdgcn_exp2f(mx[nt] - ref);
+                mx[nt] = top;
+                float add = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    p[nt][j] = __builtin_amdgcn_exp2f(p[nt][j] - ref + kLift<T>);
+                    add += p[nt][j];
+                }
+                sum[nt] = sum[nt] * by + add;
+#pragma unroll
+                for (int c = 0; c < NC; c++)
+#pragma unroll
+                    for (int i = 0; i < CW; i++) o[nt][c][i] *= by;
+            }
+
+            uint32_t bad = 0;               // keys 8 g + j of the edge with an infinity or a NaN, bit 8 g + j
+            if (edge) {
+                const uint32_t see = span.hi;           // keys past these are no row's
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const uint32_t key = key0 + 8 * g + j;
+                    bool out = key >= see || key < span.lo, inf = false;
+#pragma unroll
+                    for (int c = 0; c < NC; c++) {
+                        if (out) vf[j][c] = vw{};
+                        u4v raw = {};
+                        __builtin_memcpy(&raw, &vf[j][c], sizeof(vw));
+                        inf |= not_finite<T>(raw);
+                    }
+                    const uint64_t b = __ballot(inf);
+#pragma unroll
+                    for (int y = 0; y < 4; y++)
+                        if (b >> (16 * y) & 0xffff) bad |= 1u << (8 * y + j);
+                    if (bad >> (8 * g + j) & 1)
+#pragma unroll
+                        for (int c = 0; c < NC; c++) vf[j][c] = vw{};
+                }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                v8 pf[NP];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    pf[0][j] = (T)p[nt][j];
+                    if constexpr (F32) {
+                        const float y = p[nt][j] - (float)pf[0][j];
+                        pf[1][j] = (T)y;
+                        pf[2][j] = (T)(y - (float)pf[1][j]);
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < NC; c++)
+#pragma unroll
+                    for (int i = 0; i < CW; i++) {
+                        v8 x8;
+#pragma unroll
+                        for (int j = 0; j < 8; j++) x8[j] = vf[j][c][i];
+#pragma unroll
+                        for (int q = NP - 1; q >= 0; q--) o[nt][c][i] = mfma(x8, pf[q], o[nt][c][i]);
+                    }
+            }
+            // Those keys count for the rows that see them, and only for those.
+            for (; bad; bad &= bad - 1) {
+                const uint32_t y = __ffs(bad) - 1, key = key0 + y;
+                const T *row = (const T *)a.v + place(key) + (size_t)(key & (page - 1)) * a.d;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    float wt = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const float z = __shfl(p[nt][j], (y >> 3) * 16 + m);
+                        if (j == (int)(y & 7)) wt = z;
+                    }
+                    if ((int64_t)key > pos[nt] || (int64_t)key <= pos[nt] - (int64_t)a.window) continue;
+#pragma unroll
+                    for (int c = 0; c < NC; c++)
+#pragma unroll
+                        for (int i = 0; i < CW; i++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const uint32_t dv = 16 * CW * c + CW * (4 * g + e) + i;
+                                if (dv < a.d) o[nt][c][i][e] += wt * (float)row[dv];
+                            }
+                }
+            }
+            load_v(key0 + kRowTile);
+        }
+
+        // ---- the waves' sums together; the unit's rows or its part
+        const bool whole = skip == 0 && left == span.tiles;
+        float *part = a.parts + (size_t)(2 * blockIdx.x + (skip == 0)) * R * (D + 2);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            float l = sum[nt];
+            l += __shfl_xor(l, 16);
+            l += __shfl_xor(l, 32);
+            __syncthreads();
+            if (g == 0) { s_m[w][m] = mx[nt]; s_l[w][m] = l; }
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+#pragma unroll
+                    for (int i = 0; i < CW; i += 4)
+                        *(f4 *)&s_o[w][m][16 * CW * c + CW * (4 * g + e) + i] =
+                            f4{o[nt][c][i][e], o[nt][c][i + 1][e], o[nt][c][i + 2][e], o[nt][c][i + 3][e]};
+            __syncthreads();
+            const uint32_t rr = threadIdx.x >> 4, r = r0 + 16 * nt + rr, c0 = threadIdx.x & 15;
+            if (r >= r1) continue;
+            float top = fmaxf(fmaxf(s_m[0][rr], s_m[1][rr]), fmaxf(s_m[2][rr], s_m[3][rr])), total = 0.0f, by[4];
+            const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+            for (int y = 0; y < 4; y++) {
+                by[y] = __builtin_amdgcn_exp2f(s_m[y][rr] - ref);
+                total += by[y] * s_l[y][rr];
+            }
+            const uint32_t tok = r / a.group;
+            const int64_t at = (int64_t)s.len - s.nq + tok;
+            const float inv = at < 0 ? 0.0f : 1.0f / total;             // (no key: zeros)
+            if (!whole && c0 == 0) { part[R * D + 16 * nt + rr] = top; part[R * D + R + 16 * nt + rr] = total; }
+            const size_t to = (size_t)(s.first + tok) * a.ld_out + (size_t)(kvh * a.group + r - tok * a.group) * a.d;
+#pragma unroll
+            for (int c = 0; c < D / 64; c++) {
+                const int dv = 64 * c + 4 * c0;
+                f4 x = {0, 0, 0, 0};
+#pragma unroll
+                for (int y = 0; y < 4; y++) x += *(const f4 *)&s_o[y][rr][dv] * by[y];
+                if (!whole) *(f4 *)(part + (size_t)(16 * nt + rr) * D + dv) = x;
+                else if (dv < (int)a.d) {
+                    x *= inv;
+                    if constexpr (F32) *(f4 *)((float *)a.out + to + dv) = x;
+                    else {
+                        typedef T v4 __attribute__((ext_vector_type(4)));
+                        *(v4 *)((T *)a.out + to + dv) = v4{(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
+                    }
+                }
+            }
+        }
+        if (!whole && skip == 0 && threadIdx.x == 0) {
+            Cut c;
+            c.last = (uint32_t)(((t + span.tiles) * run.n_wg - 1) / run.total);
+            c.first_token = s.first; c.row0 = r0; c.rows = r1 - r0; c.kvh = kvh;
+            c.keyless = s.nq > s.len ? (s.nq - s.len) * a.group : 0;
+            a.cuts[blockIdx.x] = c;
+        }
+        t += left;
+        skip = 0;
+        r0 += R;
+        if (r0 >= rows) { r0 = 0; kvh++; }
+    }
+}
+
+// The parts of the unit that run blockIdx.x begins and another ends, in order:
+// a thread has 4 values of one row.
+template <class TO, int D, int R>
+__global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a)
+{
+    const Cut c = a.cuts[blockIdx.x];
+    if (c.last == 0) return;
+    constexpr int kCols = D / 4, kRows = 256 / kCols;
+    const uint32_t rr = blockIdx.y * kRows + threadIdx.x / kCols, dv = 4 * (threadIdx.x % kCols);
+    if (rr >= c.rows || dv >= a.d) return;
+    constexpr size_t kPart = (size_t)R * (D + 2);
+    const float *p0 = a.parts + (size_t)(2 * blockIdx.x + 1) * kPart, *p1 = a.parts + (size_t)(2 * blockIdx.x + 2) * kPart;
+    const uint32_t more = c.last - blockIdx.x;          // parts after the first, two slots apart
+    float top = p0[R * D + rr];
+    for (uint32_t i = 0; i < more; i++) top = fmaxf(top, p1[2 * i * kPart + R * D + rr]);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float by = __builtin_amdgcn_exp2f(p0[R * D + rr] - ref), total = by * p0[R * D + R + rr];
+    f4 x = *(const f4 *)(p0 + (size_t)rr * D + dv) * by;
+    for (uint32_t i = 0; i < more; i++) {
+        const float *p = p1 + 2 * i * kPart;
+        by = __builtin_amdgcn_exp2f(p[R * D + rr] - ref);
+        total += by * p[R * D + R + rr];
+        x += *(const f4 *)(p + (size_t)rr * D + dv) * by;
+    }
+    const uint32_t r = c.row0 + rr, tok = r / a.group;
+    x *= r < c.keyless ? 0.0f : 1.0f / total;
+    const size_t to = (size_t)(c.first_token + tok) * a.ld_out + (size_t)(c.kvh * a.group + r - tok * a.group) * a.d + dv;
+    if constexpr (sizeof(TO) == 4) *(f4 *)((float *)a.out + to) = x;
+    else {
+        typedef TO v4 __attribute__((ext_vector_type(4)));
+        *(v4 *)((TO *)a.out + to) = v4{(TO)x[0], (TO)x[1], (TO)x[2], (TO)x[3]};
+    }
+}
+
+} // namespace gs
+
+namespace {
+
+constexpr uint32_t kRuns = 512;         // two workgroups per CU
+constexpr int kMostRows = 64;
+
+int padded(uint32_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+
+size_t cuts_bytes() { return kRuns * ((sizeof(gs::Cut) + 15) / 16 * 16); }
+
+template <class T, int D, int NT, bool F32> int rows_call(gs::AttnArgs &a, hipStream_t st)
+{
+    a.n_wg = kRuns;
+    hipLaunchKernelGGL((gs::attn_rows_kernel<T, D, NT, F32>), dim3(kRuns), dim3(256), 0, st, a);
+    using TO = std::conditional_t<F32, float, T>;
+    constexpr int kRows = 256 / (D / 4);
+    hipLaunchKernelGGL((gs::attn_join_kernel<TO, D, 16 * NT>), dim3(kRuns, (16 * NT + kRows - 1) / kRows), dim3(256), 0, st, a);
+    return hipGetLastError() == hipSuccess ? GS_OK : GS_ERR_HIP;
+}
+
+template <class T, int D, bool F32> int by_rows(gs::AttnArgs &a, uint64_t rows, hipStream_t st)
+{
+    if (rows <= 16) return rows_call<T, D, 1, F32>(a, st);
+    if constexpr (D == 256) return rows_call<T, D, 1, F32>(a, st);      // (two tiles of rows spill)
+    else if constexpr (F32) return rows_call<T, D, 2, F32>(a, st);
+    else {
+        if (rows <= 32) return rows_call<T, D, 2, F32>(a, st);
+        return rows_call<T, D, 4, F32>(a, st);
+    }
+}
+
+template <class T, bool F32> int by_head(gs::AttnArgs &a, uint64_t rows, hipStream_t st)
+{
+    switch (padded(a.d)) {
+    case 64: return by_rows<T, 64, F32>(a, rows, st);
+    case 128: return by_rows<T, 128, F32>(a, rows, st);
+    default: return by_rows<T, 256, F32>(a, rows, st);
+    }
+}
+
+} // namespace
+
+extern "C" {
+
+size_t gs_attn_workspace(const gs_kv_cache *c, uint32_t n_heads)
+{
+    if (check_cache(c) || n_heads == 0 || n_heads % c->n_kv) return 0;
+    return cuts_bytes() + (size_t)2 * kRuns * kMostRows * (padded(c->d) + 2) * sizeof(float);
+}
+
+int gs_attn(const gs_kv_cache *c, uint32_t layer, const gs_kv_batch *b, const gs_attn_args *x, void *stream)
+{
+    if (int rc = check_cache(c)) return rc;
+    if (int rc = check_batch(c, b)) return rc;
+    if (!x || layer >= c->n_layers || x->n_heads == 0 || x->n_heads % c->n_kv || x->n_heads > 65535) return GS_ERR_INVALID;
+    if (x->type != GS_TYPE_F32 && x->type != c->type) return GS_ERR_UNSUPPORTED;
+    if (!std::isfinite(x->scale)) return GS_ERR_INVALID;
+    if (b->n_tokens == 0) return GS_OK;
+    const size_t width = (size_t)x->n_heads * c->d;
+    if (!x->q || !x->out || x->q == x->out || x->ld_q < width || x->ld_out < width) return GS_ERR_INVALID;
+    if ((((uintptr_t)x->q | (uintptr_t)x->out) & 15u) || x->ld_q % 8 || x->ld_out % 8) return GS_ERR_INVALID;
+    if (!x->ws || ((uintptr_t)x->ws & 15u) || x->ws_bytes < gs_attn_workspace(c, x->n_heads)) return GS_ERR_INVALID;
+    // (rows of a sequence are counted in 32 bits)
+    if ((uint64_t)b->n_tokens * (x->n_heads / c->n_kv) > 0x7fffffffull) return GS_ERR_UNSUPPORTED;
+    gs::AttnArgs a = {};
+    const size_t plane = (size_t)c->n_pages * c->n_kv * c->page_size * c->d * 2;
+    a.k = (const char *)c->k + layer * plane;
+    a.v = (const char *)c->v + layer * plane;
+    a.q = x->q; a.out = x->out; a.ld_q = x->ld_q; a.ld_out = x->ld_out;
+    a.table = c->table; a.len = c->len; a.rows = b->rows; a.start = b->start;
+    a.n = b->n; a.n_tokens = b->n_tokens; a.n_rows = c->rows; a.n_pages = c->n_pages; a.ld_table = c->ld_table;
+    a.n_kv = c->n_kv; a.group = x->n_heads / c->n_kv; a.d = c->d;
+    a.shift = log2_of(c->page_size);
+    a.scale = (float)((x->scale == 0.0f ? 1.0 / sqrt((double)c->d) : (double)x->scale) * M_LOG2E);
+    a.window = x->window ? x->window : 0xffffffffu;
+    a.cuts = (gs::Cut *)x->ws;
+    a.parts = (float *)((char *)x->ws + cuts_bytes());
+    const uint32_t most = !b->start ? 1 : x->max_q && x->max_q < b->n_tokens ? x->max_q : b->n_tokens;
+    const uint64_t rows = (uint64_t)most * a.group;
+    hipStream_t st = (hipStream_t)stream;
+    const bool f16 = c->type == GS_TYPE_F16;
+    if (x->type == GS_TYPE_F32) return f16 ? by_head<_Float16, true>(a, rows, st) : by_head<__bf16, true>(a, rows, st);
+    return f16 ? by_head<_Float16, false>(a, rows, st) : by_head<__bf16, false>(a, rows, st);
+}
+
+} // extern "C"

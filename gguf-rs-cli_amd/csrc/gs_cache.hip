@@ -1,0 +1,582 @@
+// gs_cache.hip -- the pages of the cache of keys and values: rows grow, are
+// forked, freed and lose tokens (include/gs_cache.h).
+//
+// The bookkeeping is whole numbers in a fixed order, so a call's result does
+// not depend on timing: pages are counted over the rows by a scan, taken from
+// the free ones in ascending order, and reference counts change by atomic
+// additions, whose order does not matter.  A call that takes pages does that
+// in one workgroup (the order makes it one chain), and the data moves in a
+// second launch over all CUs, which reads the list the first one left in ws.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/gs_cache.h"
+#include "gs_cache.hpp"
+
+namespace gs {
+
+constexpr int kBook = 1024;             // threads of the bookkeeping workgroup
+constexpr int kScan = 16;               // reference counts per thread and step of the search
+
+// One row of a fork or a drop, in ws.
+struct Move {
+    uint32_t row, from;         // fork: dst, src (GS_KV_NONE: none); drop: the row, its first token that leaves
+    uint32_t len, left;         // tokens before and after
+    uint32_t old_len;           // fork: tokens of dst before
+    uint32_t base;              // its first new page in the list
+    uint32_t ok;                // 0: leave the row as it is
+    uint32_t in_place;          // drop: a written page keeps its place
+};
+
+struct Cache {
+    char *k, *v;
+    uint32_t n_layers, n_pages, n_kv, d, rows, ld;
+    int shift;                  // log2 of the page size
+    uint32_t *table, *len, *ref;
+    uint32_t *list;             // [n_pages] the pages taken by the call
+    uint32_t *owner;            // [rows] the first i that names a row
+    Move *moves;                // [rows]
+    uint32_t *stage;            // [rows][ld]
+};
+
+__device__ __forceinline__ uint32_t pages_of(const Cache &c, uint32_t len) { return (uint32_t)(((uint64_t)len + (1u << c.shift) - 1) >> c.shift); }
+
+// Tokens of a row, held to what its table has room for.
+__device__ __forceinline__ uint32_t row_len(const Cache &c, uint32_t row) { return min(c.len[row], c.ld << c.shift); }
+
+// Exclusive sum over the workgroup's kBook threads; `total` to all.
+__device__ __forceinline__ uint32_t scan(uint32_t x, uint32_t &total)
+{
+    __shared__ uint32_t wave[kBook / 64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    uint32_t s = x;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t y = __shfl_up(s, o);
+        if (lane >= o) s += y;
+    }
+    __syncthreads();            // (the last call's readers are done)
+    if (lane == 63) wave[w] = s;
+    __syncthreads();
+    uint32_t before = 0, sum = 0;
+#pragma unroll
+    for (int i = 0; i < kBook / 64; i++) {
+        const uint32_t y = wave[i];
+        before += i < w ? y : 0;
+        sum += y;
+    }
+    total = sum;
+    return before + s - x;
+}
+
+// The free pages from `page` on, ascending, to list[found ..] until it has
+// `want`; both run on from call to call of one kernel.
+__device__ __forceinline__ void take(const Cache &c, uint32_t want, uint32_t &page, uint32_t &found)
+{
+    while (found < want && page < c.n_pages) {
+        const uint32_t p0 = page + threadIdx.x * kScan;
+        uint32_t mask = 0;
+#pragma unroll
+        for (int i = 0; i < kScan; i++)
+            if (p0 + i < c.n_pages) mask |= (uint32_t)(c.ref[p0 + i] == 0) << i;
+        uint32_t total, at = found + scan(__popc(mask), total);
+        for (; mask; mask &= mask - 1) c.list[at++] = p0 + __ffs(mask) - 1;     // (at most n_pages in all)
+        found += total;
+        page += kBook * kScan;
+    }
+    __syncthreads();
+}
+
+__global__ void reset_kernel(const Cache c)
+{
+    const size_t n = (size_t)c.rows * c.ld, step = (size_t)gridDim.x * blockDim.x;
+    for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += step) {
+        c.table[i] = GS_KV_NONE;
+        if (i < c.rows) c.len[i] = 0;
+    }
+    for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < c.n_pages; i += step) c.ref[i] = 0;
+}
+
+// The rows' needs are summed 1024 at a time; then each thread writes pages of
+// the 1024, whose row it finds in the sums, so one row's many pages (a prompt)
+// take no longer than many rows' few.
+__global__ void __launch_bounds__(kBook) extend_kernel(const Cache c, const uint32_t *rows, uint32_t n, const uint32_t *add,
+                                                       uint32_t add_all, int32_t *status)
+{
+    __shared__ uint32_t s_first[kBook], s_row[kBook], s_was[kBook];
+    uint32_t page = 0, found = 0, given = 0;    // given: needed by the rows before
+    for (uint32_t i0 = 0; i0 < n; i0 += kBook) {
+        const uint32_t i = i0 + threadIdx.x;
+        uint32_t row = 0, len = 0, more = 0, need = 0, was = 0;
+        int32_t rc = GS_OK;
+        if (i < n) {
+            row = rows ? rows[i] : i;
+            more = add ? add[i] : add_all;
+            if (row >= c.rows) rc = GS_ERR_INVALID;
+            else {
+                len = row_len(c, row);
+                if ((uint64_t)len + more > (uint64_t)c.ld << c.shift) rc = GS_ERR_UNSUPPORTED;
+                else { was = pages_of(c, len); need = pages_of(c, len + more) - was; }
+            }
+        }
+        uint32_t total;
+        const uint32_t first = scan(need, total);       // (below 2^31: rows * ld fits the table's words)
+        take(c, (uint32_t)min((uint64_t)given + total, (uint64_t)c.n_pages), page, found);
+        const uint32_t have = found > given ? found - given : 0;
+        if (rc == GS_OK && need && (uint64_t)first + need > have) { rc = GS_ERR_NOMEM; }
+        s_first[threadIdx.x] = first;
+        s_row[threadIdx.x] = rc == GS_OK ? row : GS_KV_NONE;
+        s_was[threadIdx.x] = was;
+        __syncthreads();
+        for (uint32_t p = threadIdx.x; p < min(total, have); p += kBook) {
+            uint32_t lo = 0, hi = kBook - 1;            // the last thread whose pages begin at or before p
+            while (lo < hi) {
+                const uint32_t mid = (lo + hi + 1) >> 1;
+                if (s_first[mid] <= p) lo = mid;
+                else hi = mid - 1;
+            }
+            if (s_row[lo] == GS_KV_NONE) continue;
+            const uint32_t id = c.list[given + p];
+            c.table[(size_t)s_row[lo] * c.ld + s_was[lo] + (p - s_first[lo])] = id;
+            c.ref[id] = 1;
+        }
+        if (i < n) {
+            if (rc == GS_OK) c.len[row] = len + more;
+            if (status) status[i] = rc;
+        }
+        given = (uint32_t)min((uint64_t)given + total, 0xffffffffull);
+        __syncthreads();
+    }
+}
+
+// Marks, for each row named, the first i that names it.  (Device-scope loads:
+// the marks are in L2.)
+__device__ __forceinline__ void claim(const Cache &c, const uint32_t *rows, uint32_t n)
+{
+    for (uint32_t i = threadIdx.x; i < n; i += kBook)
+        if (rows[i] < c.rows) __hip_atomic_store(&c.owner[rows[i]], GS_KV_NONE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __threadfence();
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n; i += kBook)
+        if (rows[i] < c.rows) atomicMin(&c.owner[rows[i]], i);
+    __threadfence();
+    __syncthreads();
+}
+
+__device__ __forceinline__ bool claimed(const Cache &c, uint32_t row, uint32_t i)
+{
+    return __hip_atomic_load(&c.owner[row], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == i;
+}
+
+// Fork, 1 of 3: which pairs go ahead, and the page for each partial last page.
+__global__ void __launch_bounds__(kBook) fork_plan_kernel(const Cache c, const uint32_t *src, const uint32_t *dst, uint32_t n,
+                                                          int32_t *status)
+{
+    claim(c, dst, n);
+    uint32_t page = 0, found = 0, given = 0;
+    for (uint32_t i0 = 0; i0 < n; i0 += kBook) {
+        const uint32_t i = i0 + threadIdx.x;
+        Move m = {};
+        uint32_t need = 0;
+        int32_t rc = GS_OK;
+        if (i < n) {
+            m.row = dst[i];
+            m.from = src[i];
+            if (m.row >= c.rows || (m.from >= c.rows && m.from != GS_KV_NONE) || !claimed(c, m.row, i)) rc = GS_ERR_INVALID;
+            else if (m.from != m.row) {
+                m.ok = 1;
+                m.old_len = row_len(c, m.row);
+                m.len = m.from == GS_KV_NONE ? 0 : row_len(c, m.from);
+                need = (m.len & ((1u << c.shift) - 1)) != 0;
+            }
+        }
+        uint32_t total;
+        const uint32_t first = scan(need, total);
+        take(c, min(given + total, c.n_pages), page, found);
+        if (need) {
+            if (given + first >= found) { rc = GS_ERR_NOMEM; m.ok = 0; }
+            else {
+                m.base = c.list[given + first];
+                c.ref[m.base] = 1;
+            }
+        }
+        if (i < n) {
+            c.moves[i] = m;
+            if (status) status[i] = rc;
+        }
+        given += total;
+        __syncthreads();
+    }
+}
+
+// Fork, 2 of 3: pair blockIdx.x.  The new table to `stage` (rows of the call
+// may be each other's sources), the shared pages counted, and the partial
+// page's tokens copied: a wave moves one (k or v, layer, head) piece, which is
+// contiguous; blockIdx.y shares the pieces out.
+__global__ void __launch_bounds__(256) fork_copy_kernel(const Cache c)
+{
+    const Move m = c.moves[blockIdx.x];
+    if (!m.ok || m.from == GS_KV_NONE) return;
+    const uint32_t full = m.len >> c.shift, rest = m.len & ((1u << c.shift) - 1);
+    const uint32_t *from = c.table + (size_t)m.from * c.ld;
+    for (uint32_t j = blockIdx.y * 256 + threadIdx.x; j < full; j += gridDim.y * 256) {
+        const uint32_t p = from[j];
+        c.stage[(size_t)blockIdx.x * c.ld + j] = p;
+        if (p < c.n_pages) atomicAdd(&c.ref[p], 1u);
+    }
+    if (!rest) return;
+    const uint32_t old = from[full];
+    if (old >= c.n_pages) return;
+    const size_t slot = (size_t)c.d * 2, head = slot << c.shift, plane = (size_t)c.n_pages * c.n_kv * head;
+    const uint32_t lane = threadIdx.x & 63, pieces = 2 * c.n_layers * c.n_kv;
+    const size_t bytes = rest * slot;
+    for (uint32_t q = blockIdx.y * 4 + (threadIdx.x >> 6); q < pieces; q += gridDim.y * 4) {
+        const uint32_t h = q % c.n_kv, l = q / c.n_kv >> 1;
+        char *base = (q / c.n_kv & 1 ? c.v : c.k) + l * plane;
+        const char *a = base + ((size_t)old * c.n_kv + h) * head;
+        char *b = base + ((size_t)m.base * c.n_kv + h) * head;
+        for (size_t o = lane * 16; o < bytes; o += 64 * 16) *(u4v *)(b + o) = *(const u4v *)(a + o);
+    }
+}
+
+// Fork, 3 of 3: pair blockIdx.x's old pages released, the new table written.
+__global__ void __launch_bounds__(256) fork_write_kernel(const Cache c)
+{
+    const Move m = c.moves[blockIdx.x];
+    if (!m.ok) return;
+    uint32_t *table = c.table + (size_t)m.row * c.ld;
+    const uint32_t full = m.len >> c.shift, now = pages_of(c, m.len), was = pages_of(c, m.old_len);
+    for (uint32_t j = threadIdx.x; j < max(now, was); j += 256) {
+        if (j < was && table[j] < c.n_pages) atomicSub(&c.ref[table[j]], 1u);
+        table[j] = j < full ? c.stage[(size_t)blockIdx.x * c.ld + j] : j < now ? m.base : GS_KV_NONE;
+    }
+    if (threadIdx.x == 0) c.len[m.row] = m.len;
+}
+
+// Row rows[blockIdx.x] emptied.  Its length is taken by an exchange: a row
+// named twice is released once.
+__global__ void __launch_bounds__(256) free_kernel(const Cache c, const uint32_t *rows)
+{
+    __shared__ uint32_t held;
+    const uint32_t row = rows[blockIdx.x];
+    if (row >= c.rows) return;
+    if (threadIdx.x == 0) held = min(atomicExch(&c.len[row], 0u), c.ld << c.shift);
+    __syncthreads();
+    uint32_t *table = c.table + (size_t)row * c.ld;
+    for (uint32_t j = threadIdx.x; j < pages_of(c, held); j += 256) {
+        if (table[j] < c.n_pages) atomicSub(&c.ref[table[j]], 1u);
+        table[j] = GS_KV_NONE;
+    }
+}
+
+// Drop, 1 of 3: what leaves each row, and the new pages for its written pages
+// that others hold too.  A wave counts a row's pages; stage[i][j] is the
+// number of new pages before place j, with the top bit where j gets one.
+__global__ void __launch_bounds__(kBook) drop_plan_kernel(const Cache c, const uint32_t *rows, uint32_t n, const uint32_t *from,
+                                                          const uint32_t *to, int32_t *status)
+{
+    claim(c, rows, n);
+    const uint32_t lane = threadIdx.x & 63;
+    for (uint32_t i = threadIdx.x >> 6; i < n; i += kBook / 64) {
+        Move m = {};
+        m.row = rows[i];
+        m.ok = m.row < c.rows && claimed(c, m.row, i);
+        uint32_t need = 0, written = 0;
+        if (m.ok) {
+            m.len = row_len(c, m.row);
+            m.from = min(from[i], m.len);
+            m.left = m.len - (min(max(to[i], m.from), m.len) - m.from);
+            const uint32_t first = m.from >> c.shift, now = pages_of(c, m.left);
+            if (m.left < m.len) {
+                for (uint32_t j = first; j < now; j += 64) {
+                    bool fresh = false;
+                    if (j + lane < now) {
+                        const uint32_t p = c.table[(size_t)m.row * c.ld + j + lane];
+                        fresh = p < c.n_pages && c.ref[p] > 1;
+                    }
+                    const uint64_t b = __ballot(fresh);
+                    if (j + lane < now)
+                        c.stage[(size_t)i * c.ld + j + lane] = (need + __popcll(b & ((1ull << lane) - 1))) | (fresh ? 0x80000000u : 0u);
+                    need += __popcll(b);
+                }
+                written = now > first ? now - first : 0;
+            }
+        }
+        m.in_place = need < written;
+        m.base = need;                  // (for the moment)
+        if (lane == 0) c.moves[i] = m;
+    }
+    __threadfence_block();
+    __syncthreads();
+    uint32_t page = 0, found = 0, given = 0;
+    for (uint32_t i0 = 0; i0 < n; i0 += kBook) {
+        const uint32_t i = i0 + threadIdx.x;
+        Move m = {};
+        uint32_t total;
+        if (i < n) m = c.moves[i];
+        const uint32_t need = m.base, first = scan(need, total);
+        take(c, (uint32_t)min((uint64_t)given + total, (uint64_t)c.n_pages), page, found);
+        if (i < n) {
+            int32_t rc = m.ok ? GS_OK : GS_ERR_INVALID;
+            if (need && (uint64_t)given + first + need > found) { m.ok = 0; rc = GS_ERR_NOMEM; }
+            m.base = given + first;
+            m.ok = m.ok && m.left < m.len;
+            c.moves[i] = m;
+            if (status) status[i] = rc;
+        }
+        given = (uint32_t)min((uint64_t)given + total, 0xffffffffull);
+        __syncthreads();
+    }
+}
+
+// The page that place j of row i of a drop has after it.
+__device__ __forceinline__ uint32_t new_page(const Cache &c, const Move &m, uint32_t i, uint32_t j)
+{
+    if (j >= m.from >> c.shift) {
+        const uint32_t s = c.stage[(size_t)i * c.ld + j];
+        if (s >> 31) return c.list[m.base + (s & 0x7fffffffu)];
+    }
+    return c.table[(size_t)m.row * c.ld + j];
+}
+
+// Drop, 2 of 3: the tokens move.  blockIdx.x: a stream (k or v, layer, head)
+// of row blockIdx.z; tokens go down in ascending order, kStep values of 16
+// bytes per thread and step, all read before any is written, so a workgroup
+// that has the stream alone may write over what it has read.  Rows all of
+// whose written pages are new are read from other pages than they are written
+// to, and their steps are shared by gridDim.y workgroups.
+// An item is 16 bytes of a token, or for turned keys two that belong together
+// (the pairs of the half layout; neighbours): a read, a write and little else,
+// bound by the traffic.
+template <class T, bool VEC>
+__global__ void __launch_bounds__(256) drop_move_kernel(const Cache c, const uint64_t *turns, int rot, int half)
+{
+    constexpr int kStep = 4;
+    const uint32_t i = blockIdx.z, stream = blockIdx.x;
+    const Move m = c.moves[i];
+    if (!m.ok) return;
+    const uint32_t slice = m.in_place ? 0 : blockIdx.y, slices = m.in_place ? 1 : gridDim.y;
+    if (slice != blockIdx.y) return;
+    const uint32_t h = stream % c.n_kv, l = stream / c.n_kv >> 1;
+    const bool keys = !(stream / c.n_kv & 1);
+    const uint32_t first = m.from >> c.shift, size = 1u << c.shift, gone = m.len - m.left;
+    // tokens before `from` move only where their page is a new one
+    const bool fresh = first < pages_of(c, m.left) && (c.stage[(size_t)i * c.ld + first] >> 31);
+    const uint32_t t0 = fresh ? first << c.shift : m.from;
+    const size_t head = (size_t)c.d << c.shift;
+    T *base = (T *)(keys ? c.k : c.v) + (size_t)l * c.n_pages * c.n_kv * head;
+    const uint32_t *table = c.table + (size_t)m.row * c.ld;
+
+    const bool turn = keys && rot > 0;
+    const uint32_t pairs = rot >> 1;
+    // items of a token
+    const uint32_t nturn = !turn ? 0 : VEC ? rot / 16 : pairs, per = nturn + (VEC ? (c.d - (turn ? rot : 0)) / 8 : (c.d - (turn ? rot : 0)) / 2);
+    __shared__ float2 cs[128];
+    if (turn) {
+        for (uint32_t e = threadIdx.x; e < pairs; e += 256) cs[e] = turn_of(turns[e], -(int64_t)gone, 1.0f);
+        __syncthreads();
+    }
+    const uint32_t fit = 256 / per, each = fit ? fit : 1;                   // tokens of a step's round
+    const uint32_t tl = threadIdx.x / per, item = threadIdx.x - tl * per;   // (per <= 128)
+    const bool works = tl < each;
+    // the two vectors of an item
+    uint32_t p, q;
+    const bool turned = item < nturn;
+    if (VEC) {
+        p = turned ? (half ? 8 * item : 16 * item) : (turn ? rot : 0) + 8 * (item - nturn);
+        q = turned ? (half ? p + pairs : p + 8) : p;
+    } else {
+        p = turned && half ? item : 2 * item;
+        q = turned && half ? item + pairs : p + 1;
+    }
+    constexpr int kW = VEC ? 8 : 1;
+    typedef T vec __attribute__((ext_vector_type(kW)));
+    for (uint32_t t = t0 + slice * each * kStep; t < m.left; t += slices * each * kStep) {
+        vec a[kStep], b[kStep];
+        T *to[kStep];
+        bool late[kStep];
+#pragma unroll
+        for (int s = 0; s < kStep; s++) {
+            const uint32_t x = t + s * each + tl;
+            to[s] = nullptr;
+            if (!works || x >= m.left) continue;
+            late[s] = x >= m.from;
+            const uint32_t y = late[s] ? x + gone : x;
+            const uint32_t np = new_page(c, m, i, x >> c.shift), op = table[y >> c.shift];
+            if (np >= c.n_pages || op >= c.n_pages) continue;
+            const T *f = base + ((size_t)op * c.n_kv + h) * head + (y & (size - 1)) * c.d;
+            to[s] = base + ((size_t)np * c.n_kv + h) * head + (x & (size - 1)) * c.d;
+            a[s] = *(const vec *)(f + p);
+            if (q != p) b[s] = *(const vec *)(f + q);
+        }
+#pragma unroll
+        for (int s = 0; s < kStep; s++) {
+            if (!to[s] || !turned || !late[s]) continue;
+            float u[kW], w[kW];
+#pragma unroll
+            for (int e = 0; e < kW; e++) { u[e] = (float)a[s][e]; w[e] = (float)b[s][e]; }
+            if constexpr (VEC) {
+                if (half) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) turn_pair(u[e], w[e], cs[8 * item + e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        turn_pair(u[2 * e], u[2 * e + 1], cs[8 * item + e]);
+                        turn_pair(w[2 * e], w[2 * e + 1], cs[8 * item + 4 + e]);
+                    }
+                }
+            } else {
+                turn_pair(u[0], w[0], cs[item]);
+            }
+#pragma unroll
+            for (int e = 0; e < kW; e++) { a[s][e] = (T)u[e]; b[s][e] = (T)w[e]; }
+        }
+        if (m.in_place) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // every read of the step is done
+            __syncthreads();
+        }
+#pragma unroll
+        for (int s = 0; s < kStep; s++) {
+            if (!to[s]) continue;
+            *(vec *)(to[s] + p) = a[s];
+            if (q != p) *(vec *)(to[s] + q) = b[s];
+        }
+    }
+}
+
+// Drop, 3 of 3: row blockIdx.x's table, its released pages, its length.
+__global__ void __launch_bounds__(256) drop_write_kernel(const Cache c)
+{
+    const uint32_t i = blockIdx.x;
+    const Move m = c.moves[i];
+    if (!m.ok) return;
+    uint32_t *table = c.table + (size_t)m.row * c.ld;
+    const uint32_t now = pages_of(c, m.left), was = pages_of(c, m.len);
+    for (uint32_t j = (m.from >> c.shift) + threadIdx.x; j < was; j += 256) {
+        const uint32_t old = table[j], p = j < now ? new_page(c, m, i, j) : GS_KV_NONE;
+        if (p == old) continue;
+        if (old < c.n_pages) atomicSub(&c.ref[old], 1u);
+        if (p != GS_KV_NONE) c.ref[p] = 1;
+        table[j] = p;
+    }
+    if (threadIdx.x == 0) c.len[m.row] = m.left;
+}
+
+} // namespace gs
+
+namespace {
+
+size_t up4(size_t x) { return (x + 3) & ~(size_t)3; }
+
+gs::Cache device_cache(const gs_kv_cache *c)
+{
+    gs::Cache d = {};
+    d.k = (char *)c->k; d.v = (char *)c->v;
+    d.n_layers = c->n_layers; d.n_pages = c->n_pages; d.n_kv = c->n_kv; d.d = c->d; d.rows = c->rows; d.ld = c->ld_table;
+    d.shift = log2_of(c->page_size);
+    d.table = c->table; d.len = c->len; d.ref = c->ref;
+    uint32_t *w = c->ws;
+    d.list = w; w += up4(c->n_pages);
+    d.owner = w; w += up4(c->rows);
+    d.moves = (gs::Move *)w; w += (size_t)c->rows * (sizeof(gs::Move) / 4);
+    d.stage = w;
+    return d;
+}
+
+int check_call(const gs_kv_cache *c, size_t n)
+{
+    if (int rc = check_cache(c)) return rc;
+    if (!c->ws || ((uintptr_t)c->ws & 15u)) return GS_ERR_INVALID;
+    return n <= c->rows && n <= 65535 ? GS_OK : GS_ERR_INVALID;
+}
+
+int launched() { return hipGetLastError() == hipSuccess ? GS_OK : GS_ERR_HIP; }
+
+// Workgroups that share a row's data, so that a few rows fill the CUs (2048
+// workgroups of 256 threads are 8 per CU) and many rows have one each.
+unsigned shares(size_t n, size_t most)
+{
+    size_t s = (2048 + n - 1) / n;
+    if (s > most) s = most;
+    return (unsigned)(s ? s : 1);
+}
+
+} // namespace
+
+extern "C" {
+
+size_t gs_kv_workspace(const gs_kv_cache *c)
+{
+    if (check_cache(c)) return 0;
+    return up4(c->n_pages) + up4(c->rows) + (size_t)c->rows * (sizeof(gs::Move) / 4) + (size_t)c->rows * c->ld_table;
+}
+
+int gs_kv_reset(const gs_kv_cache *c, void *stream)
+{
+    if (int rc = check_call(c, 0)) return rc;
+    hipLaunchKernelGGL(gs::reset_kernel, dim3(1024), dim3(256), 0, (hipStream_t)stream, device_cache(c));
+    return launched();
+}
+
+int gs_kv_extend(const gs_kv_cache *c, const uint32_t *rows, size_t n, const uint32_t *add, uint32_t add_all,
+                 int32_t *status, void *stream)
+{
+    if (int rc = check_call(c, n)) return rc;
+    if (n == 0) return GS_OK;
+    hipLaunchKernelGGL(gs::extend_kernel, dim3(1), dim3(gs::kBook), 0, (hipStream_t)stream, device_cache(c), rows, (uint32_t)n,
+                       add, add_all, status);
+    return launched();
+}
+
+int gs_kv_fork(const gs_kv_cache *c, const uint32_t *src, const uint32_t *dst, size_t n, int32_t *status, void *stream)
+{
+    if (int rc = check_call(c, n)) return rc;
+    if (n == 0) return GS_OK;
+    if (!src || !dst) return GS_ERR_INVALID;
+    const gs::Cache d = device_cache(c);
+    hipStream_t st = (hipStream_t)stream;
+    const unsigned y = shares(n, (2 * (size_t)c->n_layers * c->n_kv + 3) / 4);
+    hipLaunchKernelGGL(gs::fork_plan_kernel, dim3(1), dim3(gs::kBook), 0, st, d, src, dst, (uint32_t)n, status);
+    hipLaunchKernelGGL(gs::fork_copy_kernel, dim3((unsigned)n, y), dim3(256), 0, st, d);
+    hipLaunchKernelGGL(gs::fork_write_kernel, dim3((unsigned)n), dim3(256), 0, st, d);
+    return launched();
+}
+
+int gs_kv_free(const gs_kv_cache *c, const uint32_t *rows, size_t n, void *stream)
+{
+    if (int rc = check_call(c, n)) return rc;
+    if (n == 0) return GS_OK;
+    if (!rows) return GS_ERR_INVALID;
+    hipLaunchKernelGGL(gs::free_kernel, dim3((unsigned)n), dim3(256), 0, (hipStream_t)stream, device_cache(c), rows);
+    return launched();
+}
+
+int gs_kv_drop(const gs_kv_cache *c, const uint32_t *rows, size_t n, const uint32_t *from, const uint32_t *to,
+               const gs_rope *rope, int32_t *status, void *stream)
+{
+    if (int rc = check_call(c, n)) return rc;
+    if (rope && rope->d != c->d) return GS_ERR_INVALID;
+    if (n == 0) return GS_OK;
+    if (!rows || !from || !to) return GS_ERR_INVALID;
+    const gs::Cache d = device_cache(c);
+    hipStream_t st = (hipStream_t)stream;
+    const size_t streams = 2 * (size_t)c->n_layers * c->n_kv;
+    const int rot = rope ? (int)rope->rot : 0, half = rope && rope->layout == GS_ROPE_HALF;
+    const uint64_t *turns = rope ? rope->turns : nullptr;
+    const dim3 grid((unsigned)streams, shares(n * streams, 64), (unsigned)n);
+    hipLaunchKernelGGL(gs::drop_plan_kernel, dim3(1), dim3(gs::kBook), 0, st, d, rows, (uint32_t)n, from, to, status);
+    const bool f16 = c->type == GS_TYPE_F16;
+    // (a part that is not whole vectors of pairs goes pair by pair)
+    if (rot % 16 == 0) {
+        if (f16) hipLaunchKernelGGL((gs::drop_move_kernel<_Float16, true>), grid, dim3(256), 0, st, d, turns, rot, half);
+        else hipLaunchKernelGGL((gs::drop_move_kernel<__bf16, true>), grid, dim3(256), 0, st, d, turns, rot, half);
+    } else {
+        if (f16) hipLaunchKernelGGL((gs::drop_move_kernel<_Float16, false>), grid, dim3(256), 0, st, d, turns, rot, half);
+        else hipLaunchKernelGGL((gs::drop_move_kernel<__bf16, false>), grid, dim3(256), 0, st, d, turns, rot, half);
+    }
+    hipLaunchKernelGGL(gs::drop_write_kernel, dim3((unsigned)n), dim3(256), 0, st, d);
+    return launched();
+}
+
+} // extern "C"

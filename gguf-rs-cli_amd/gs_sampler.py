@@ -50,6 +50,12 @@ EXPORTS = [
     # include/gs_tokens.h
     "gs_vocab_create", "gs_vocab_destroy", "gs_vocab_find", "gs_token_decode", "gs_tokens_decode",
     "gs_chat_template_detect", "gs_stop_tokens",
+    # include/gs_rope.h
+    "gs_rope_create", "gs_rope_destroy", "gs_rope_apply",
+    # include/gs_cache.h
+    "gs_kv_workspace", "gs_kv_reset", "gs_kv_extend", "gs_kv_fork", "gs_kv_free", "gs_kv_drop", "gs_kv_append",
+    # include/gs_attn.h
+    "gs_attn_workspace", "gs_attn",
 ]
 
 
@@ -79,6 +85,45 @@ class DecodeCtx(ctypes.Structure):
                 ("generated", ctypes.c_void_p), ("ld_generated", ctypes.c_size_t), ("next", ctypes.c_void_p),
                 ("u", ctypes.c_void_p), ("tokens", ctypes.c_void_p), ("status", ctypes.c_void_p),
                 ("n_active", ctypes.c_void_p)]
+
+
+class RopeParams(ctypes.Structure):
+    """gs_rope_params (include/gs_rope.h)."""
+    _fields_ = [("d", ctypes.c_uint32), ("rot", ctypes.c_uint32), ("layout", ctypes.c_uint32),
+                ("scaling", ctypes.c_uint32), ("base", ctypes.c_double), ("factor", ctypes.c_double),
+                ("context", ctypes.c_uint32), ("beta_fast", ctypes.c_double), ("beta_slow", ctypes.c_double),
+                ("gain", ctypes.c_double), ("divisors", ctypes.c_void_p)]
+
+
+class GsKVCache(ctypes.Structure):
+    """gs_kv_cache (include/gs_cache.h)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("type", ctypes.c_uint32),
+                ("n_layers", ctypes.c_uint32), ("n_pages", ctypes.c_uint32), ("n_kv", ctypes.c_uint32),
+                ("page_size", ctypes.c_uint32), ("d", ctypes.c_uint32), ("rows", ctypes.c_uint32),
+                ("ld_table", ctypes.c_uint32), ("table", ctypes.c_void_p), ("len", ctypes.c_void_p),
+                ("ref", ctypes.c_void_p), ("ws", ctypes.c_void_p)]
+
+
+class GsKVBatch(ctypes.Structure):
+    """gs_kv_batch (include/gs_cache.h)."""
+    _fields_ = [("n", ctypes.c_uint32), ("n_tokens", ctypes.c_uint32), ("rows", ctypes.c_void_p),
+                ("start", ctypes.c_void_p)]
+
+
+class GsKVNew(ctypes.Structure):
+    """gs_kv_new (include/gs_cache.h)."""
+    _fields_ = [("type", ctypes.c_uint32), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("ld_k", ctypes.c_size_t),
+                ("ld_v", ctypes.c_size_t), ("q", ctypes.c_void_p), ("ld_q", ctypes.c_size_t),
+                ("q_out", ctypes.c_void_p), ("ld_q_out", ctypes.c_size_t), ("q_out_type", ctypes.c_uint32),
+                ("n_heads", ctypes.c_uint32)]
+
+
+class GsAttnArgs(ctypes.Structure):
+    """gs_attn_args (include/gs_attn.h)."""
+    _fields_ = [("type", ctypes.c_uint32), ("n_heads", ctypes.c_uint32), ("q", ctypes.c_void_p), ("ld_q", ctypes.c_size_t),
+                ("out", ctypes.c_void_p), ("ld_out", ctypes.c_size_t), ("scale", ctypes.c_float),
+                ("window", ctypes.c_uint32), ("max_q", ctypes.c_uint32), ("ws", ctypes.c_void_p),
+                ("ws_bytes", ctypes.c_size_t)]
 
 
 _lib = None
@@ -127,6 +172,19 @@ def load_library(path=LIB_PATH):
         "gs_tokens_decode": ([P, P, SZ, P, SZ, ctypes.POINTER(SZ)], I),
         "gs_chat_template_detect": ([P, ctypes.c_char_p, ctypes.POINTER(ctypes.c_uint32)], I),
         "gs_stop_tokens": ([P, ctypes.c_uint32, P, SZ, P, SZ, ctypes.POINTER(SZ)], I),
+        "gs_rope_create": ([ctypes.POINTER(RopeParams), ctypes.POINTER(P)], I),
+        "gs_rope_destroy": ([P], I),
+        "gs_rope_apply": ([P, ctypes.c_uint32, P, SZ, P, SZ, SZ, ctypes.c_uint32, P, P], I),
+        "gs_kv_workspace": ([ctypes.POINTER(GsKVCache)], SZ),
+        "gs_kv_reset": ([ctypes.POINTER(GsKVCache), P], I),
+        "gs_kv_extend": ([ctypes.POINTER(GsKVCache), P, SZ, P, ctypes.c_uint32, P, P], I),
+        "gs_kv_fork": ([ctypes.POINTER(GsKVCache), P, P, SZ, P, P], I),
+        "gs_kv_free": ([ctypes.POINTER(GsKVCache), P, SZ, P], I),
+        "gs_kv_drop": ([ctypes.POINTER(GsKVCache), P, SZ, P, P, P, P, P], I),
+        "gs_kv_append": ([ctypes.POINTER(GsKVCache), ctypes.c_uint32, ctypes.POINTER(GsKVBatch), P,
+                          ctypes.POINTER(GsKVNew), P], I),
+        "gs_attn_workspace": ([ctypes.POINTER(GsKVCache), ctypes.c_uint32], SZ),
+        "gs_attn": ([ctypes.POINTER(GsKVCache), ctypes.c_uint32, ctypes.POINTER(GsKVBatch), ctypes.POINTER(GsAttnArgs), P], I),
     }
     for name, (args, res) in sig.items():
         f = getattr(lib, name)
@@ -590,6 +648,221 @@ class Decoder:
         st = self.row_state()
         g = self.generated.cpu().numpy().view("<u4")
         return [g[b, :min(int(st["n_gen"][b]), g.shape[1])].copy() for b in range(self.B)]
+
+
+# ---- rotary positions and the paged cache (include/gs_rope.h, gs_cache.h) ------
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 30        # numbered as GgmlType
+ROPE_LAYOUTS = {"interleaved": 0, "half": 1}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "yarn": 2}
+KV_NONE = 0xFFFFFFFF
+_TYPES = {"torch.float32": TYPE_F32, "torch.float16": TYPE_F16, "torch.bfloat16": TYPE_BF16}
+
+
+def _type(x, what):
+    t = _TYPES.get(str(x.dtype))
+    if t is None:
+        raise TypeError("%s must be float32, float16 or bfloat16" % what)
+    return t
+
+
+def _heads(x, what, heads=None, d=None):
+    """(tokens, heads, d, values from token to token) of a [T, heads, d]
+    tensor on the device whose heads are contiguous."""
+    if x.dim() != 3 or not x.is_cuda:
+        raise TypeError("%s must be a [tokens, heads, d] tensor on the device" % what)
+    T, h, n = x.shape
+    if (heads is not None and h != heads) or (d is not None and n != d):
+        raise ValueError("%s has heads of another number or size" % what)
+    if (n > 1 and x.stride(2) != 1) or (h > 1 and x.stride(1) != n):
+        raise TypeError("the heads of %s must be contiguous" % what)
+    return T, h, n, (x.stride(0) if T > 1 else h * n)
+
+
+def _words(x, what, n=None):
+    """A contiguous device tensor of 4-byte integers (of n values), or None."""
+    if x is None:
+        return None
+    if not getattr(x, "is_cuda", False) or x.element_size() != 4 or x.is_floating_point() or not x.is_contiguous():
+        raise TypeError("%s must be a contiguous tensor of 4-byte integers on the device" % what)
+    if n is not None and x.numel() != n:
+        raise ValueError("%s must have %d values" % (what, n))
+    return x.data_ptr()
+
+
+class Rope:
+    """The plan of a rotation (include/gs_rope.h): the first `rot` values of
+    heads of d, in the "interleaved" or the "half" layout, with the scaling
+    "none", "linear" or "yarn" (`factor`, and for YaRN the trained `context`)
+    and the divisors of a rope_freqs tensor."""
+
+    def __init__(self, d, rot=None, layout="half", base=10000.0, scaling="none", factor=1.0, context=0, beta_fast=0.0,
+                 beta_slow=0.0, gain=0.0, divisors=None):
+        import numpy as np
+        self._lib = load_library()
+        self._h = None
+        rot = d if rot is None else rot
+        div = None
+        if divisors is not None:
+            div = np.ascontiguousarray(np.asarray(divisors, dtype=np.float32))
+            if div.size != rot // 2:
+                raise ValueError("divisors must have rot / 2 values")
+        p = RopeParams(d, rot, ROPE_LAYOUTS[layout], ROPE_SCALINGS[scaling], base, factor, context, beta_fast,
+                       beta_slow, gain, None if div is None else div.ctypes.data)
+        h = ctypes.c_void_p()
+        _check(self._lib.gs_rope_create(ctypes.byref(p), ctypes.byref(h)), "gs_rope_create")
+        self._h = h
+        self.d, self.rot = d, rot
+
+    def apply(self, x, pos, out=None, stream=None):
+        """x [T, heads, d] turned to positions pos [T] (4-byte integers), to
+        `out` (None: in place)."""
+        out = x if out is None else out
+        T, heads, d, ld = _heads(x, "x", d=self.d)
+        T2, _, _, ld_out = _heads(out, "out", heads, d)
+        if T2 != T or out.dtype != x.dtype:
+            raise ValueError("out must be as x")
+        _check(self._lib.gs_rope_apply(self._h, _type(x, "x"), x.data_ptr(), ld, out.data_ptr(), ld_out, T, heads,
+                                       _words(pos, "pos", T), _stream_handle(stream)), "gs_rope_apply")
+        return out
+
+    def close(self):
+        if self._h:
+            self._lib.gs_rope_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class KVCache:
+    """The paged cache of keys and values (include/gs_cache.h) over tensors on
+    the device: k, v [layers, pages, kv heads, page, d] in float16 or bfloat16,
+    table [rows, pages of a row], len [rows] and ref [pages] of 4-byte
+    integers (-1 in the table: no page).  KVCache.empty allocates them.  Row
+    numbers and other arguments of the calls are device tensors of 4-byte
+    integers; every call is stream-ordered and asynchronous."""
+
+    def __init__(self, k, v, table, len, ref):
+        import torch
+        self._lib = load_library()
+        if k.dim() != 5 or v.shape != k.shape or v.dtype != k.dtype or not k.is_contiguous() or not v.is_contiguous():
+            raise ValueError("k and v must be contiguous [layers, pages, heads, page, d] tensors alike")
+        if table.dim() != 2 or len.dim() != 1 or table.shape[0] != len.shape[0] or ref.numel() != k.shape[1]:
+            raise ValueError("table must be [rows, pages of a row], len [rows], ref [pages]")
+        for x, what in ((table, "table"), (len, "len"), (ref, "ref")):
+            _words(x, what)
+        self.k, self.v, self.table, self.len, self.ref = k, v, table, len, ref
+        self.layers, self.pages, self.kv, self.page, self.d = k.shape
+        self.rows, ld = table.shape
+        self.type = _type(k, "k")
+        self.c = GsKVCache(k.data_ptr(), v.data_ptr(), self.type, self.layers, self.pages, self.kv, self.page, self.d,
+                           self.rows, ld, table.data_ptr(), len.data_ptr(), ref.data_ptr(), None)
+        self._c = ctypes.byref(self.c)
+        words = self._lib.gs_kv_workspace(self._c)
+        if not words:
+            raise SamplerError(GS_ERR_UNSUPPORTED, "gs_kv_workspace")
+        self.ws = torch.empty(words, dtype=torch.int32, device=k.device)
+        self.c.ws = self.ws.data_ptr()
+        self._attn_ws = {}
+
+    @classmethod
+    def empty(cls, layers, pages, kv, d, rows, max_len, page=16, dtype=None, device="cuda"):
+        """A new cache: every row empty, every page free."""
+        import torch
+        dtype = torch.float16 if dtype is None else dtype
+        shape = (layers, pages, kv, page, d)
+        i32 = dict(dtype=torch.int32, device=device)
+        c = cls(torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device),
+                torch.empty((rows, -(-max_len // page)), **i32), torch.empty(rows, **i32), torch.empty(pages, **i32))
+        c.reset()
+        return c
+
+    def reset(self, stream=None):
+        _check(self._lib.gs_kv_reset(self._c, _stream_handle(stream)), "gs_kv_reset")
+
+    def extend(self, add, rows=None, status=None, stream=None):
+        """Room for new tokens: `add` for each of `rows` (None: every row), a
+        number or a tensor of one per row."""
+        n = self.rows if rows is None else rows.numel()
+        each = isinstance(add, int)
+        _check(self._lib.gs_kv_extend(self._c, _words(rows, "rows"), n, None if each else _words(add, "add", n),
+                                      add if each else 0, _words(status, "status", n), _stream_handle(stream)),
+               "gs_kv_extend")
+
+    def fork(self, src, dst, status=None, stream=None):
+        """Rows dst become copies of rows src, sharing their full pages (-1: empty)."""
+        n = dst.numel()
+        _check(self._lib.gs_kv_fork(self._c, _words(src, "src", n), _words(dst, "dst"), n, _words(status, "status", n),
+                                    _stream_handle(stream)), "gs_kv_fork")
+
+    def free(self, rows, stream=None):
+        _check(self._lib.gs_kv_free(self._c, _words(rows, "rows"), rows.numel(), _stream_handle(stream)), "gs_kv_free")
+
+    def drop(self, start, end, rows, rope=None, status=None, stream=None):
+        """Tokens start .. end - 1 of each of `rows` leave it (gs_kv_drop); with
+        `rope` the keys after them are turned back to their new positions."""
+        n = rows.numel()
+        _check(self._lib.gs_kv_drop(self._c, _words(rows, "rows"), n, _words(start, "start", n), _words(end, "end", n),
+                                    None if rope is None else rope._h, _words(status, "status", n),
+                                    _stream_handle(stream)), "gs_kv_drop")
+
+    def _batch(self, T, rows, q_start):
+        if q_start is None:
+            n = T
+        else:
+            n = q_start.numel() - 1
+        return GsKVBatch(n, T, _words(rows, "rows", n), _words(q_start, "q_start"))
+
+    def append(self, layer, k, v, q=None, q_out=None, rope=None, rows=None, q_start=None, stream=None):
+        """The newest tokens' keys and values [T, kv heads, d] (float32 or the
+        cache's type) to their pages, keys turned to their positions by
+        `rope`; q [T, heads, d] turned to q_out (None: in place).  One token
+        for each of `rows` (None: row i), or those from q_start[i] to
+        q_start[i + 1]."""
+        T, _, _, ld_k = _heads(k, "k", self.kv, self.d)
+        Tv, _, _, ld_v = _heads(v, "v", self.kv, self.d)
+        if Tv != T or v.dtype != k.dtype:
+            raise ValueError("v must be as k")
+        x = GsKVNew(_type(k, "k"), k.data_ptr(), v.data_ptr(), ld_k, ld_v, None, 0, None, 0, 0, 0)
+        if q is not None:
+            q_out = q if q_out is None else q_out
+            Tq, heads, _, ld_q = _heads(q, "q", d=self.d)
+            To, _, _, ld_o = _heads(q_out, "q_out", heads, self.d)
+            if Tq != T or To != T or q.dtype != k.dtype:
+                raise ValueError("q must have k's tokens and type, q_out q's heads")
+            x.q, x.ld_q, x.q_out, x.ld_q_out = q.data_ptr(), ld_q, q_out.data_ptr(), ld_o
+            x.q_out_type, x.n_heads = _type(q_out, "q_out"), heads
+        b = self._batch(T, rows, q_start)
+        _check(self._lib.gs_kv_append(self._c, layer, ctypes.byref(b), None if rope is None else rope._h,
+                                      ctypes.byref(x), _stream_handle(stream)), "gs_kv_append")
+
+    def attend(self, layer, q, out=None, rows=None, q_start=None, scale=0.0, window=0, max_q=0, stream=None):
+        """Causal attention of the rows' newest tokens (as append takes them) over
+        the rows' pages: q and out [T, heads, d] (float32 or the cache's type;
+        out None: a new tensor).  window: how many positions back a token
+        sees, itself included (0: all).  max_q: the most tokens of one
+        sequence, if the caller knows it."""
+        import torch
+        T, heads, _, ld_q = _heads(q, "q", d=self.d)
+        out = torch.empty((T, heads, self.d), dtype=q.dtype, device=q.device) if out is None else out
+        To, _, _, ld_o = _heads(out, "out", heads, self.d)
+        if To != T or out.dtype != q.dtype:
+            raise ValueError("out must be as q")
+        st = _stream_handle(stream)
+        ws = self._attn_ws.get((st, heads))         # calls on one stream do not overlap
+        if ws is None:
+            n = self._lib.gs_attn_workspace(self._c, heads)
+            if not n:
+                raise SamplerError(GS_ERR_INVALID, "gs_attn_workspace")
+            ws = self._attn_ws[st, heads] = torch.empty(n, dtype=torch.uint8, device=q.device)
+        b = self._batch(T, rows, q_start)
+        a = GsAttnArgs(_type(q, "q"), heads, q.data_ptr(), ld_q, out.data_ptr(), ld_o, scale, window, max_q, ws.data_ptr(),
+                       ws.numel())
+        _check(self._lib.gs_attn(self._c, layer, ctypes.byref(b), ctypes.byref(a), st), "gs_attn")
+        return out
 
 
 # ---- token text and stop set (include/gs_tokens.h) -----------------------------

@@ -38,7 +38,8 @@ struct AttnArgs {
     int shift;                      // log2 of the page size
     float scale;                    // of the scores, times log2(e)
     uint32_t window;                // (0xffffffff: none)
-    uint32_t n_wg;                  // runs
+    uint32_t n_wg;                  // runs, at most
+    uint32_t min_rows, max_rows;    // sequences with fewer or more query rows per head of keys are not this kernel's
     float *parts;                   // [2 n_wg][R][D + 2]: a run's cut units: the one it begins with, the one it ends with
     struct Cut *cuts;               // [n_wg]
 };
@@ -61,6 +62,7 @@ __device__ __forceinline__ Seq seq_of(const AttnArgs &a, uint32_t i)
     s.first = a.start ? min(a.start[i], a.n_tokens) : i;
     const uint32_t end = a.start ? min(a.start[i + 1], a.n_tokens) : i + 1;
     s.nq = end > s.first ? end - s.first : 0;
+    if (s.nq * a.group < a.min_rows || s.nq * a.group > a.max_rows) s.nq = 0;
     s.row = a.rows ? a.rows[i] : i;
     s.len = s.row < a.n_rows ? min(a.len[s.row], a.ld_table << a.shift) : 0;
     return s;
@@ -97,7 +99,8 @@ struct Run {
     uint64_t skip;
 };
 
-template <int R, int kTile, int kThreads> __device__ __forceinline__ Run run_of(const AttnArgs &a)
+// kLeast: tiles that a run has at least, if there are as many.
+template <int R, int kTile, int kThreads, int kLeast> __device__ __forceinline__ Run run_of(const AttnArgs &a, uint32_t g)
 {
     __shared__ uint64_t s_wave[kThreads / 64];
     __shared__ uint32_t s_seq;
@@ -123,8 +126,7 @@ template <int R, int kTile, int kThreads> __device__ __forceinline__ Run run_of(
         if (i < w) before += s_wave[i];
         r.total += s_wave[i];
     }
-    r.n_wg = (uint32_t)min((uint64_t)a.n_wg, r.total);
-    const uint32_t g = blockIdx.x;
+    r.n_wg = (uint32_t)min((uint64_t)a.n_wg, (r.total + kLeast - 1) / kLeast);
     if (g >= r.n_wg) { r.t0 = r.t1 = 0; r.seq = 0; r.skip = 0; return r; }
     r.t0 = r.total * g / r.n_wg;
     r.t1 = r.total * (g + 1) / r.n_wg;
@@ -186,7 +188,7 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(const AttnArgs a)
     __shared__ float s_o[4][16][D + 4];
     __shared__ float s_m[4][16], s_l[4][16];
 
-    Run run = run_of<R, kRowTile, 256>(a);
+    Run run = run_of<R, kRowTile, 256, 1>(a, blockIdx.x);
     if (threadIdx.x == 0 && blockIdx.x < a.n_wg) a.cuts[blockIdx.x].last = 0;
     if (run.t0 >= run.t1) return;
 
@@ -500,6 +502,310 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(const AttnArgs a)
     }
 }
 
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef short s4v __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ f16v mfma(h8 a, h8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f16v mfma(b8 a, b8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+
+// The shape of the kernel below for heads of D: waves, keys of a tile.
+template <int D> struct Chunk {
+    static constexpr int kWaves = D == 256 ? 4 : 8, kTile = D == 256 ? 32 : 64;
+    static constexpr int kRows = 32 * kWaves, kThreads = 64 * kWaves;
+};
+
+// Chunks of many query rows: what bounds it is the matrix cores and, beside
+// them, the exponentials.  A wave has 32 query rows, and all waves share the
+// tiles of K and V in LDS, two of each, so that the next tile's loads (through
+// registers) pass while this one is worked on: one barrier per tile.  The
+// products are S^T = K Q^T and O^T = V^T P^T again, 32 x 32 x 16: a lane has
+// the scores of query row lane & 31 for keys 8 x + 4 (lane >> 5) + y, x and
+// y < 4, of 32, and gives them back, rounded, as the second product's factor;
+// V^T's side takes the same keys by transposing reads of LDS, 4 keys of one
+// column each.  Rows of LDS are stored with their 16-byte pieces exchanged so
+// that neither reading order meets a bank twice.
+// The running maximum is raised only when a score passes it by 2^8, so the
+// sums are seldom scaled: the weights then reach 2^8, which f32 sums and the
+// type's range (f16: 2^7 is the lift here) take without loss.
+template <class T, int D>
+__global__ void __launch_bounds__(Chunk<D>::kThreads) attn_chunk_kernel(const AttnArgs a)
+{
+    constexpr int R = Chunk<D>::kRows, kTile = Chunk<D>::kTile, kThreads = Chunk<D>::kThreads;
+    constexpr int C = D / 8, KP = kTile * C / kThreads;         // 16-byte pieces of a row; pieces of a thread
+    constexpr int KT = kTile / 32, KS = D / 16, DT = D / 32;
+    constexpr float kUp = __is_same(T, _Float16) ? 7.0f : 0.0f, kSlack = 8.0f;
+    typedef typename Vec<T>::v8 v8;
+    __shared__ __align__(16) T s_k[2][kTile * D], s_v[2][kTile * D];
+    __shared__ uint64_t s_bad[3];                               // of this tile, the next, and one that is cleared
+
+    // runs that follow one another, which read the same keys, on one XCD
+    const uint32_t g8 = a.n_wg / 8, run_id = a.n_wg % 8 ? blockIdx.x : (blockIdx.x & 7) * g8 + (blockIdx.x >> 3);
+    Run run = run_of<R, kTile, kThreads, 4>(a, run_id);
+    if (threadIdx.x == 0) a.cuts[run_id].last = 0;
+    if (run.t0 >= run.t1) return;
+
+    const int lane = threadIdx.x & 63, hf = lane >> 5, col = lane & 31, l16 = lane & 15;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t slot = (1u << a.shift) - 1;
+    const size_t head = (size_t)a.d << a.shift;
+    const float scale = fabsf(a.scale);
+
+    // this thread's pieces of a tile: rows prow + KP.., piece pc, and their places in LDS
+    const int pc = threadIdx.x % C, prow = threadIdx.x / C;
+    constexpr int kStep = kThreads / C;                         // rows from piece to piece
+    auto swap_k = [](int row, int c) { return c ^ (row & (C < 16 ? C - 1 : 15)); };
+    auto swap_v = [](int row, int c) { return C == 8 ? c ^ (row >> 1 & 1) << 2 : c ^ (row & 3) << 2; };
+    const bool inside = 8 * pc < (int)a.d;
+
+    uint32_t si = run.seq;
+    Seq s = seq_of(a, si);
+    uint32_t per = tiles_of<R, kTile>(a, s);
+    uint64_t t = run.t0;
+    uint32_t kvh = (uint32_t)(run.skip / max(per, 1u)), skip = (uint32_t)(run.skip % max(per, 1u)), r0 = 0;
+    while (t < run.t1) {
+        const uint32_t rows = s.nq * a.group;
+        if (kvh == a.n_kv || rows == 0) {               // the next sequence
+            si++;
+            s = seq_of(a, si);
+            per = tiles_of<R, kTile>(a, s);
+            kvh = 0; r0 = 0; skip = 0;
+            continue;
+        }
+        const uint32_t r1 = min(r0 + R, rows);
+        const Span<kTile> span(a, s, r0, r1);
+        if (skip >= span.tiles) { skip -= span.tiles; r0 += R; continue; }
+        const uint32_t left = (uint32_t)min((uint64_t)(span.tiles - skip), run.t1 - t);
+        const int base = (int)s.len - (int)s.nq;        // position of the sequence's first token
+
+        // ---- queries: row col of the wave's 32, values 16 s + 8 hf ..
+        const uint32_t w0 = r0 + 32 * w;
+        const bool rows_here = w0 < r1;
+        const uint32_t mine = min(w0 + col, r1 - 1), tok = mine / a.group, hq = kvh * a.group + (mine - tok * a.group);
+        const int pos = base + (int)tok;
+        const int pos0 = base + (int)(min(w0, r1 - 1) / a.group), pos1 = base + (int)(min(w0 + 31, r1 - 1) / a.group);
+        v8 qf[KS];
+        const T *q = (const T *)a.q + (size_t)(s.first + tok) * a.ld_q + (size_t)hq * a.d;
+#pragma unroll
+        for (int c = 0; c < KS; c++) {
+            v8 x = {};
+            if (16 * c + 8 * hf < (int)a.d) x = *(const v8 *)(q + 16 * c + 8 * hf);
+            qf[c] = a.scale < 0.0f ? -x : x;
+        }
+
+        // ---- a tile's pieces
+        const uint32_t *table = a.table + (size_t)min(s.row, a.n_rows - 1) * a.ld_table;
+        const uint32_t last = span.hi > 0 ? span.hi - 1 : 0;
+        u4v kr[KP], vr[KP];
+        uint32_t id[KP];
+        auto pages = [&](uint32_t key0) {
+#pragma unroll
+            for (int i = 0; i < KP; i++) id[i] = table[min(key0 + prow + kStep * i, last) >> a.shift];
+        };
+        auto fetch = [&](uint32_t key0) {
+#pragma unroll
+            for (int i = 0; i < KP; i++) {
+                const uint32_t key = key0 + prow + kStep * i;
+                const size_t at = ((size_t)min(id[i], a.n_pages - 1) * a.n_kv + kvh) * head + (size_t)(key & slot) * a.d + 8 * pc;
+                kr[i] = vr[i] = u4v{0, 0, 0, 0};
+                if (inside) {
+                    kr[i] = *(const u4v *)((const T *)a.k + at);
+                    vr[i] = *(const u4v *)((const T *)a.v + at);
+                }
+            }
+        };
+        // Values of keys that no row of the unit sees are zeros, and so are
+        // those of keys that some rows only see if an infinity or a NaN is
+        // among them; s_bad says which (bit: the key of the tile).
+        auto put = [&](uint32_t key0, int b, int bs) {
+            const bool edge = key0 + kTile > (uint32_t)max(0, base + (int)(r0 / a.group) + 1) ||
+                              (int64_t)key0 < (int64_t)base + (r1 - 1) / a.group + 1 - (int64_t)a.window;
+            if (edge) {
+                uint64_t bad = 0;
+#pragma unroll
+                for (int i = 0; i < KP; i++) {
+                    const uint32_t row = prow + kStep * i, key = key0 + row;
+                    if (key >= span.hi || key < span.lo) vr[i] = u4v{0, 0, 0, 0};
+                    const uint64_t v = __ballot(not_finite<T>(vr[i]));
+                    constexpr uint64_t kMask = (1ull << C) - 1;
+                    if (v >> (lane / C * C) & kMask) { bad |= 1ull << row; vr[i] = u4v{0, 0, 0, 0}; }
+                }
+                if (bad) atomicOr((unsigned long long *)&s_bad[bs], (unsigned long long)bad);
+            }
+#pragma unroll
+            for (int i = 0; i < KP; i++) {
+                const int row = prow + kStep * i;
+                *(u4v *)&s_k[b][row * D + 8 * swap_k(row, pc)] = kr[i];
+                *(u4v *)&s_v[b][row * D + 8 * swap_v(row, pc)] = vr[i];
+            }
+        };
+
+        f16v o[DT];
+#pragma unroll
+        for (int c = 0; c < DT; c++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[c][i] = 0.0f;
+        float mx = -INFINITY, sum = 0.0f;
+
+        uint32_t key0 = (span.tile0 + skip) * kTile;
+        pages(key0);
+        fetch(key0);
+        pages(key0 + kTile);
+        __syncthreads();                                // (the last unit's tiles are read)
+        if (threadIdx.x < 3) s_bad[threadIdx.x] = 0;
+        __syncthreads();
+        put(key0, 0, 0);
+        __syncthreads();
+        int bs = 0;                                     // x % 3
+        for (uint32_t x = 0; x < left; x++, key0 += kTile) {
+            const int b = x & 1;
+            const bool more = x + 1 < left;
+            if (more) {
+                fetch(key0 + kTile);
+                pages(key0 + 2 * kTile);
+            }
+            if (rows_here && (int)key0 <= pos1 && (int64_t)key0 + kTile > (int64_t)pos0 + 1 - (int64_t)a.window) {
+                f16v z[KT];
+#pragma unroll
+                for (int y = 0; y < KT; y++) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) z[y][i] = 0.0f;
+#pragma unroll
+                    for (int c = 0; c < KS; c++) {
+                        const int row = 32 * y + col;
+                        const v8 kf = *(const v8 *)&s_k[b][row * D + 8 * swap_k(row, 2 * c + hf)];
+                        z[y] = mfma(kf, qf[c], z[y]);
+                    }
+                }
+                const bool edge = (int)(key0 + kTile) > pos0 + 1 || (int64_t)key0 < (int64_t)pos1 + 1 - (int64_t)a.window;
+                // the keys of z[y][i]: key0 + 32 y + 8 (i / 4) + 4 hf + i % 4
+                const int lo = (int)max((int64_t)0, (int64_t)pos + 1 - (int64_t)a.window);
+                if (edge) {
+#pragma unroll
+                    for (int y = 0; y < KT; y++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const int key = (int)key0 + 32 * y + 8 * (i >> 2) + 4 * hf + (i & 3);
+                            if (key > pos || key < lo) z[y][i] = -INFINITY;
+                        }
+                }
+                float top = z[0][0];
+#pragma unroll
+                for (int y = 0; y < KT; y++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) top = fmaxf(top, z[y][i]);
+                top = fmaxf(top, __shfl_xor(top, 32)) * scale;
+                if (__any(top > mx + kSlack)) {
+                    const float now = fmaxf(mx, top), by = __builtin_amdgcn_exp2f(mx - (now == -INFINITY ? 0.0f : now));
+                    mx = now;
+                    sum *= by;
+#pragma unroll
+                    for (int c = 0; c < DT; c++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) o[c][i] *= by;
+                }
+                const float ref = mx == -INFINITY ? 0.0f : mx - kUp;
+#pragma unroll
+                for (int y = 0; y < KT; y++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        z[y][i] = __builtin_amdgcn_exp2f(fmaf(z[y][i], scale, -ref));
+                        sum += z[y][i];
+                    }
+#pragma unroll
+                for (int c = 0; c < DT; c++)
+#pragma unroll
+                    for (int y = 0; y < 2 * KT; y++) {
+                        v8 pf;
+#pragma unroll
+                        for (int i = 0; i < 8; i++) pf[i] = (T)z[y >> 1][8 * (y & 1) + i];
+                        const int row = 16 * y + 4 * hf + (l16 >> 2), piece = 4 * c + 2 * (lane >> 4 & 1) + (l16 >> 1 & 1);
+                        union { s4v half[2]; v8 all; } u;
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            T *at = &s_v[b][(row + 8 * e) * D + 8 * swap_v(row + 8 * e, piece) + 4 * (l16 & 1)];
+                            u.half[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v *)at);
+                        }
+                        o[c] = mfma(u.all, pf, o[c]);
+                    }
+                // The values that were put aside count for the rows that see them.
+                for (uint64_t bad = s_bad[bs]; bad; bad &= bad - 1) {
+                    const int y = __ffsll((unsigned long long)bad) - 1;
+                    const uint32_t key = key0 + y;
+                    float wt = 0.0f;
+#pragma unroll
+                    for (int z0 = 0; z0 < KT; z0++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const float v = __shfl(z[z0][i], ((y >> 2 & 1) << 5) + col);
+                            if (z0 == y >> 5 && i == (y & 3) + 4 * (y >> 3 & 3)) wt = v;
+                        }
+                    if ((int)key > pos || (int)key < lo) continue;
+                    const uint32_t page = min(table[min(key, last) >> a.shift], a.n_pages - 1);
+                    const T *v = (const T *)a.v + ((size_t)page * a.n_kv + kvh) * head + (size_t)(key & slot) * a.d;
+#pragma unroll
+                    for (int c = 0; c < DT; c++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const int dv = 32 * c + 8 * (i >> 2) + 4 * hf + (i & 3);
+                            if (dv < (int)a.d) o[c][i] += wt * (float)v[dv];
+                        }
+                }
+            }
+            if (!more) break;
+            // (s_bad of the tile before this was read before the last barrier,
+            // and is written after the next)
+            const int next = bs == 2 ? 0 : bs + 1;
+            if (threadIdx.x == 0) s_bad[next == 2 ? 0 : next + 1] = 0;
+            put(key0 + kTile, b ^ 1, next);
+            bs = next;
+            __syncthreads();
+        }
+
+        // ---- the unit's rows, or its part
+        const bool whole = skip == 0 && left == span.tiles;
+        sum += __shfl_xor(sum, 32);
+        if (w0 + col < r1) {
+            if (whole) {
+                const float inv = pos < 0 ? 0.0f : 1.0f / sum;          // (no key: zeros)
+                T *to = (T *)a.out + (size_t)(s.first + tok) * a.ld_out + (size_t)hq * a.d;
+                typedef T v4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+                for (int c = 0; c < DT; c++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int dv = 32 * c + 8 * i + 4 * hf;
+                        if (dv < (int)a.d) {
+                            f4 y = {o[c][4 * i], o[c][4 * i + 1], o[c][4 * i + 2], o[c][4 * i + 3]};
+                            y *= inv;
+                            *(v4 *)(to + dv) = v4{(T)y[0], (T)y[1], (T)y[2], (T)y[3]};
+                        }
+                    }
+            } else {
+                float *part = a.parts + (size_t)(2 * run_id + (skip == 0)) * R * (D + 2);
+                const int rr = 32 * w + col;
+                if (hf == 0) { part[R * D + rr] = mx; part[R * D + R + rr] = sum; }
+#pragma unroll
+                for (int c = 0; c < DT; c++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        *(f4 *)(part + (size_t)rr * D + 32 * c + 8 * i + 4 * hf) =
+                            f4{o[c][4 * i], o[c][4 * i + 1], o[c][4 * i + 2], o[c][4 * i + 3]};
+            }
+        }
+        if (!whole && skip == 0 && threadIdx.x == 0) {
+            Cut c;
+            c.last = (uint32_t)(((t + span.tiles) * run.n_wg - 1) / run.total);
+            c.first_token = s.first; c.row0 = r0; c.rows = r1 - r0; c.kvh = kvh;
+            c.keyless = s.nq > s.len ? (s.nq - s.len) * a.group : 0;
+            a.cuts[run_id] = c;
+        }
+        t += left;
+        skip = 0;
+        r0 += R;
+        if (r0 >= rows) { r0 = 0; kvh++; }
+    }
+}
+
 // The parts of the unit that run blockIdx.x begins and another ends, in order:
 // a thread has 4 values of one row.
 template <class TO, int D, int R>
@@ -538,31 +844,56 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a)
 
 namespace {
 
-constexpr uint32_t kRuns = 512;         // two workgroups per CU
-constexpr int kMostRows = 64;
+constexpr uint32_t kRuns = 512;         // of the rows kernel: two workgroups per CU
+constexpr uint32_t kChunkRuns = 256;    // of the chunk kernel: one per CU
 
 int padded(uint32_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
 size_t cuts_bytes() { return kRuns * ((sizeof(gs::Cut) + 15) / 16 * 16); }
 
-template <class T, int D, int NT, bool F32> int rows_call(gs::AttnArgs &a, hipStream_t st)
+// Bytes of a kernel's parts with R rows in a unit.
+size_t parts_bytes(uint32_t runs, int R, int D) { return (size_t)2 * runs * R * (D + 2) * sizeof(float); }
+
+template <class TO, int D, int R> int join(const gs::AttnArgs &a, hipStream_t st)
 {
-    a.n_wg = kRuns;
-    hipLaunchKernelGGL((gs::attn_rows_kernel<T, D, NT, F32>), dim3(kRuns), dim3(256), 0, st, a);
-    using TO = std::conditional_t<F32, float, T>;
     constexpr int kRows = 256 / (D / 4);
-    hipLaunchKernelGGL((gs::attn_join_kernel<TO, D, 16 * NT>), dim3(kRuns, (16 * NT + kRows - 1) / kRows), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((gs::attn_join_kernel<TO, D, R>), dim3(a.n_wg, (R + kRows - 1) / kRows), dim3(256), 0, st, a);
     return hipGetLastError() == hipSuccess ? GS_OK : GS_ERR_HIP;
 }
 
+template <class T, int D, int NT, bool F32> int rows_call(gs::AttnArgs a, hipStream_t st)
+{
+    a.n_wg = kRuns;
+    hipLaunchKernelGGL((gs::attn_rows_kernel<T, D, NT, F32>), dim3(kRuns), dim3(256), 0, st, a);
+    return join<std::conditional_t<F32, float, T>, D, 16 * NT>(a, st);
+}
+
+template <class T, int D> int chunk_call(gs::AttnArgs a, hipStream_t st)
+{
+    a.n_wg = kChunkRuns;
+    hipLaunchKernelGGL((gs::attn_chunk_kernel<T, D>), dim3(kChunkRuns), dim3(gs::Chunk<D>::kThreads), 0, st, a);
+    return join<T, D, gs::Chunk<D>::kRows>(a, st);
+}
+
+// `rows`: the most query rows per head of keys that a sequence may have.
 template <class T, int D, bool F32> int by_rows(gs::AttnArgs &a, uint64_t rows, hipStream_t st)
 {
+    a.min_rows = 0;
+    a.max_rows = 0xffffffffu;
     if (rows <= 16) return rows_call<T, D, 1, F32>(a, st);
-    if constexpr (D == 256) return rows_call<T, D, 1, F32>(a, st);      // (two tiles of rows spill)
-    else if constexpr (F32) return rows_call<T, D, 2, F32>(a, st);
-    else {
-        if (rows <= 32) return rows_call<T, D, 2, F32>(a, st);
-        return rows_call<T, D, 4, F32>(a, st);
+    if constexpr (F32) {
+        if constexpr (D == 256) return rows_call<T, D, 1, F32>(a, st);      // (two tiles of rows spill)
+        else return rows_call<T, D, 2, F32>(a, st);
+    } else {
+        if constexpr (D != 256)
+            if (rows <= 32) return rows_call<T, D, 2, F32>(a, st);
+        // Sequences of a few rows go to the first kernel, the others to the second.
+        constexpr int kFew = D == 256 ? 16 : 32;
+        a.max_rows = kFew;
+        if (int rc = rows_call<T, D, kFew / 16, F32>(a, st)) return rc;
+        a.min_rows = kFew + 1;
+        a.max_rows = 0xffffffffu;
+        return chunk_call<T, D>(a, st);
     }
 }
 
@@ -582,7 +913,10 @@ extern "C" {
 size_t gs_attn_workspace(const gs_kv_cache *c, uint32_t n_heads)
 {
     if (check_cache(c) || n_heads == 0 || n_heads % c->n_kv) return 0;
-    return cuts_bytes() + (size_t)2 * kRuns * kMostRows * (padded(c->d) + 2) * sizeof(float);
+    // the larger of the two kernels': 32 rows in each of kRuns runs, or a chunk's in kChunkRuns
+    const int D = padded(c->d);
+    const size_t few = parts_bytes(kRuns, 32, D), many = parts_bytes(kChunkRuns, D == 256 ? gs::Chunk<256>::kRows : gs::Chunk<128>::kRows, D);
+    return cuts_bytes() + (few > many ? few : many);
 }
 
 int gs_attn(const gs_kv_cache *c, uint32_t layer, const gs_kv_batch *b, const gs_attn_args *x, void *stream)

@@ -90,33 +90,56 @@ template <int R, int kTile> __device__ __forceinline__ uint32_t tiles_of(const A
     return t;
 }
 
+// a / b, by 32-bit division where that is enough (as it is for any call that
+// fits the memory; 64 bits are several times as many instructions).
+__device__ __forceinline__ uint64_t quotient(uint64_t a, uint64_t b)
+{
+    return (a | b) >> 32 ? a / b : (uint32_t)a / (uint32_t)b;
+}
+
 // The run of this workgroup: its tiles [t0, t1) of `total`, the sequence the
 // first of them is in, and how many tiles of that sequence come before it.
-// Each thread counts a stretch of the sequences.
+// Run g has total / n_wg tiles, the first total % n_wg runs one more.
+// Each thread counts a stretch of the sequences, and the one that finds the
+// run's first leaves it in LDS.
 struct Run {
-    uint64_t t0, t1, total;
-    uint32_t n_wg, seq;
-    uint64_t skip;
+    uint64_t t0, t1, total, skip;
+    uint32_t n_wg, seq, per;        // per: tiles of the sequence and one head of keys
+    Seq s;
 };
+
+// The run that tile x is in.
+__device__ __forceinline__ uint32_t run_with(const Run &r, uint64_t x)
+{
+    const uint64_t q = quotient(r.total, r.n_wg), more = r.total - q * r.n_wg;
+    return (uint32_t)(x < more * (q + 1) ? quotient(x, q + 1) : more + quotient(x - more * (q + 1), q));
+}
 
 // kLeast: tiles that a run has at least, if there are as many.
 template <int R, int kTile, int kThreads, int kLeast> __device__ __forceinline__ Run run_of(const AttnArgs &a, uint32_t g)
 {
     __shared__ uint64_t s_wave[kThreads / 64];
-    __shared__ uint32_t s_seq;
-    __shared__ uint64_t s_skip;
+    __shared__ Run s_run;
     const uint32_t each = (a.n + kThreads - 1) / kThreads;
     const uint32_t i0 = min(threadIdx.x * each, a.n), i1 = min(i0 + each, a.n);
+    Seq s = {};
+    uint32_t per = 0;
     uint64_t mine = 0;
-    for (uint32_t i = i0; i < i1; i++) mine += (uint64_t)tiles_of<R, kTile>(a, seq_of(a, i)) * a.n_kv;
+    for (uint32_t i = i0; i < i1; i++) {
+        s = seq_of(a, i);
+        per = tiles_of<R, kTile>(a, s);
+        mine += (uint64_t)per * a.n_kv;
+    }
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     uint64_t x = mine;
+    if (a.n > each) {                       // (one sequence: the first thread has it)
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint64_t y = __shfl_up(x, o);
-        if (lane >= o) x += y;
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint64_t y = __shfl_up(x, o);
+            if (lane >= o) x += y;
+        }
     }
-    if (lane == 63) s_wave[w] = x;
+    if (lane == (a.n > each ? 63 : 0)) s_wave[w] = x;
     __syncthreads();
     uint64_t before = x - mine;
     Run r;
@@ -126,24 +149,26 @@ template <int R, int kTile, int kThreads, int kLeast> __device__ __forceinline__
         if (i < w) before += s_wave[i];
         r.total += s_wave[i];
     }
-    r.n_wg = (uint32_t)min((uint64_t)a.n_wg, (r.total + kLeast - 1) / kLeast);
-    if (g >= r.n_wg) { r.t0 = r.t1 = 0; r.seq = 0; r.skip = 0; return r; }
-    r.t0 = r.total * g / r.n_wg;
-    r.t1 = r.total * (g + 1) / r.n_wg;
-    if (r.t0 >= before && r.t0 < before + mine) {
+    const uint64_t most = quotient(r.total + kLeast - 1, kLeast);
+    r.n_wg = (uint32_t)min((uint64_t)a.n_wg, most);
+    if (g >= r.n_wg) { r.t0 = r.t1 = 0; return r; }
+    const uint64_t q = quotient(r.total, r.n_wg), more = r.total - q * r.n_wg;
+    r.t0 = g * q + min((uint64_t)g, more);
+    r.t1 = r.t0 + q + (g < more);
+    if (mine && r.t0 >= before && r.t0 < before + mine) {
         uint32_t i = i0;
-        for (;; i++) {
-            const uint64_t t = (uint64_t)tiles_of<R, kTile>(a, seq_of(a, i)) * a.n_kv;
-            if (r.t0 < before + t) break;
-            before += t;
-        }
-        s_seq = i;
-        s_skip = r.t0 - before;
+        if (each > 1)
+            for (;; i++) {
+                s = seq_of(a, i);
+                per = tiles_of<R, kTile>(a, s);
+                if (r.t0 < before + (uint64_t)per * a.n_kv) break;
+                before += (uint64_t)per * a.n_kv;
+            }
+        r.seq = i; r.skip = r.t0 - before; r.per = per; r.s = s;
+        s_run = r;
     }
     __syncthreads();
-    r.seq = s_seq;
-    r.skip = s_skip;
-    return r;
+    return s_run;
 }
 
 // An infinity or NaN among 8 values.
@@ -197,11 +222,10 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(const AttnArgs a)
     const uint32_t page = 1u << a.shift;
     const size_t head = (size_t)a.d << a.shift;         // values of a head's page
 
-    uint32_t si = run.seq;
-    Seq s = seq_of(a, si);
-    uint32_t per = tiles_of<R, kRowTile>(a, s);
+    uint32_t si = run.seq, per = run.per, r0 = 0;
+    Seq s = run.s;
     uint64_t t = run.t0;
-    uint32_t kvh = (uint32_t)(run.skip / max(per, 1u)), skip = (uint32_t)(run.skip % max(per, 1u)), r0 = 0;
+    uint32_t kvh = (uint32_t)quotient(run.skip, per), skip = (uint32_t)(run.skip - (uint64_t)kvh * per);
     while (t < run.t1) {
         const uint32_t rows = s.nq * a.group;
         if (kvh == a.n_kv || rows == 0) {               // the next sequence
@@ -490,7 +514,7 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(const AttnArgs a)
         }
         if (!whole && skip == 0 && threadIdx.x == 0) {
             Cut c;
-            c.last = (uint32_t)(((t + span.tiles) * run.n_wg - 1) / run.total);
+            c.last = run_with(run, t + span.tiles - 1);
             c.first_token = s.first; c.row0 = r0; c.rows = r1 - r0; c.kvh = kvh;
             c.keyless = s.nq > s.len ? (s.nq - s.len) * a.group : 0;
             a.cuts[blockIdx.x] = c;
@@ -557,11 +581,10 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads) attn_chunk_kernel(const At
     auto swap_v = [](int row, int c) { return C == 8 ? c ^ (row >> 1 & 1) << 2 : c ^ (row & 3) << 2; };
     const bool inside = 8 * pc < (int)a.d;
 
-    uint32_t si = run.seq;
-    Seq s = seq_of(a, si);
-    uint32_t per = tiles_of<R, kTile>(a, s);
+    uint32_t si = run.seq, per = run.per, r0 = 0;
+    Seq s = run.s;
     uint64_t t = run.t0;
-    uint32_t kvh = (uint32_t)(run.skip / max(per, 1u)), skip = (uint32_t)(run.skip % max(per, 1u)), r0 = 0;
+    uint32_t kvh = (uint32_t)quotient(run.skip, per), skip = (uint32_t)(run.skip - (uint64_t)kvh * per);
     while (t < run.t1) {
         const uint32_t rows = s.nq * a.group;
         if (kvh == a.n_kv || rows == 0) {               // the next sequence
@@ -694,9 +717,10 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads) attn_chunk_kernel(const At
 #pragma unroll
                     for (int i = 0; i < 16; i++) top = fmaxf(top, z[y][i]);
                 top = fmaxf(top, __shfl_xor(top, 32)) * scale;
-                if (__any(top > mx + kSlack)) {
-                    const float now = fmaxf(mx, top), by = __builtin_amdgcn_exp2f(mx - (now == -INFINITY ? 0.0f : now));
-                    mx = now;
+                const bool raise = top > mx + kSlack;           // (each row by itself: its bits do not depend on its neighbours)
+                if (__any(raise)) {
+                    const float by = raise ? __builtin_amdgcn_exp2f(mx - top) : 1.0f;
+                    mx = raise ? top : mx;
                     sum *= by;
 #pragma unroll
                     for (int c = 0; c < DT; c++)
@@ -794,7 +818,7 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads) attn_chunk_kernel(const At
         }
         if (!whole && skip == 0 && threadIdx.x == 0) {
             Cut c;
-            c.last = (uint32_t)(((t + span.tiles) * run.n_wg - 1) / run.total);
+            c.last = run_with(run, t + span.tiles - 1);
             c.first_token = s.first; c.row0 = r0; c.rows = r1 - r0; c.kvh = kvh;
             c.keyless = s.nq > s.len ? (s.nq - s.len) * a.group : 0;
             a.cuts[run_id] = c;
@@ -806,31 +830,54 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads) attn_chunk_kernel(const At
     }
 }
 
-// The parts of the unit that run blockIdx.x begins and another ends, in order:
-// a thread has 4 values of one row.
+// The parts of the unit that run blockIdx.x begins and another ends.  The
+// threads of a row (D / 4 of them, 4 values each) first share out its parts'
+// maximums and sums, up to kWide at a time, and then add the parts in order,
+// eight reads at a time: what bounds it is the chain of reads.
 template <class TO, int D, int R>
 __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a)
 {
     const Cut c = a.cuts[blockIdx.x];
     if (c.last == 0) return;
-    constexpr int kCols = D / 4, kRows = 256 / kCols;
-    const uint32_t rr = blockIdx.y * kRows + threadIdx.x / kCols, dv = 4 * (threadIdx.x % kCols);
-    if (rr >= c.rows || dv >= a.d) return;
+    constexpr int kCols = D / 4, kRows = 256 / kCols, kWide = kCols < 32 ? kCols : 32;
+    const uint32_t rr = blockIdx.y * kRows + threadIdx.x / kCols, dv = 4 * (threadIdx.x % kCols), j = threadIdx.x % kWide;
+    if (blockIdx.y * kRows >= c.rows) return;
+    const uint32_t row = min(rr, c.rows - 1);           // (the threads of a row past the unit's help no one)
     constexpr size_t kPart = (size_t)R * (D + 2);
-    const float *p0 = a.parts + (size_t)(2 * blockIdx.x + 1) * kPart, *p1 = a.parts + (size_t)(2 * blockIdx.x + 2) * kPart;
-    const uint32_t more = c.last - blockIdx.x;          // parts after the first, two slots apart
-    float top = p0[R * D + rr];
-    for (uint32_t i = 0; i < more; i++) top = fmaxf(top, p1[2 * i * kPart + R * D + rr]);
+    const uint32_t n = c.last - blockIdx.x + 1;         // part 0 is the run's second slot, the others their runs' first
+    const float *p0 = a.parts + (size_t)(2 * blockIdx.x) * kPart;
+    auto part = [&](uint32_t i) { return p0 + (i ? 2 * (size_t)i : 1) * kPart; };
+    float top = -INFINITY;
+    for (uint32_t i = j; i < n; i += kWide) top = fmaxf(top, part(i)[R * D + row]);
+#pragma unroll
+    for (int o = 1; o < kWide; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
     const float ref = top == -INFINITY ? 0.0f : top;
-    float by = __builtin_amdgcn_exp2f(p0[R * D + rr] - ref), total = by * p0[R * D + R + rr];
-    f4 x = *(const f4 *)(p0 + (size_t)rr * D + dv) * by;
-    for (uint32_t i = 0; i < more; i++) {
-        const float *p = p1 + 2 * i * kPart;
-        by = __builtin_amdgcn_exp2f(p[R * D + rr] - ref);
-        total += by * p[R * D + R + rr];
-        x += *(const f4 *)(p + (size_t)rr * D + dv) * by;
+    float total = 0.0f;
+    f4 x = {0, 0, 0, 0};
+    for (uint32_t i0 = 0; i0 < n; i0 += kWide) {
+        float by = 0.0f, add = 0.0f;
+        if (i0 + j < n) {
+            const float *p = part(i0 + j);
+            by = __builtin_amdgcn_exp2f(p[R * D + row] - ref);
+            add = by * p[R * D + R + row];
+        }
+        const uint32_t m = min(n - i0, (uint32_t)kWide);
+        for (uint32_t i = 0; i < m; i += 8) {
+            f4 y[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) y[e] = *(const f4 *)(part(i0 + min(i + e, m - 1)) + (size_t)row * D + dv);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float b = __shfl(by, (int)((threadIdx.x & 63 & ~(kWide - 1)) + ((i + e) & (kWide - 1))));
+                if (i + e < m) x += y[e] * b;
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < kWide; o <<= 1) add += __shfl_xor(add, o);
+        total += add;
     }
     const uint32_t r = c.row0 + rr, tok = r / a.group;
+    if (rr >= c.rows || dv >= a.d) return;
     x *= r < c.keyless ? 0.0f : 1.0f / total;
     const size_t to = (size_t)(c.first_token + tok) * a.ld_out + (size_t)(c.kvh * a.group + r - tok * a.group) * a.d + dv;
     if constexpr (sizeof(TO) == 4) *(f4 *)((float *)a.out + to) = x;

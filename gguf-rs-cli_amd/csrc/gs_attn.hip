@@ -203,8 +203,10 @@ constexpr int kRowTile = 128;           // keys of a tile: 32 for each wave
 // product i).  Four waves' sums meet in LDS at a unit's end.
 // F32: q in three parts of T whose sum is q (scaled by a power of two into
 // f16's range), and the weights too, so the products keep 24 bits.
-template <class T, int D, int NT, bool F32>
-__global__ void __launch_bounds__(256) attn_rows_kernel(const AttnArgs a)
+// FULL: heads of just D values (their strides are then constants, which takes
+// fewer registers and instructions).
+template <class T, int D, int NT, bool F32, bool FULL>
+__global__ void __launch_bounds__(256, D <= 128 && NT == 1 ? 2 : 1) attn_rows_kernel(const AttnArgs a)
 {
     constexpr int R = 16 * NT, NP = F32 ? 3 : 1, KS = D / 32;
     constexpr int CW = D >= 128 ? 8 : D / 16, NC = D / (16 * CW);       // values of a lane's V chunk, chunks
@@ -220,7 +222,8 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(const AttnArgs a)
     const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t page = 1u << a.shift;
-    const size_t head = (size_t)a.d << a.shift;         // values of a head's page
+    const uint32_t d = FULL ? D : a.d;
+    const size_t head = (size_t)d << a.shift;           // values of a head's page
 
     uint32_t si = run.seq, per = run.per, r0 = 0;
     Seq s = run.s;
@@ -240,6 +243,47 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(const AttnArgs a)
         if (skip >= span.tiles) { skip -= span.tiles; r0 += R; continue; }
         const uint32_t left = (uint32_t)min((uint64_t)(span.tiles - skip), run.t1 - t);
 
+        // ---- the keys.  Lane's K rows are in the page of key0 + 8 (m / 4), its V
+        // rows in that of key0 + 8 g; the pages' numbers are read a tile ahead
+        // of the rows (ahead of K, which is waited for before they are used).
+        const uint32_t *table = a.table + (size_t)min(s.row, a.n_rows - 1) * a.ld_table;
+        const uint32_t last = span.hi > 0 ? span.hi - 1 : 0;
+        auto page_of = [&](uint32_t key) { return table[min(key, last) >> a.shift]; };     // (the key is held to the unit's)
+        auto place = [&](uint32_t id) { return ((size_t)min(id, a.n_pages - 1) * a.n_kv + kvh) * head; };
+        v8 kf[2][KS];
+        vw vf[8][NC];
+        auto load_k = [&](uint32_t key0, uint32_t id) {
+            const T *p = (const T *)a.k + place(id);
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const T *row = p + (size_t)((key0 + 8 * (m >> 2) + 4 * x + (m & 3)) & (page - 1)) * d;
+#pragma unroll
+                for (int c = 0; c < KS; c++) {
+                    v8 y = {};
+                    if (32 * c + 8 * g < d) y = *(const v8 *)(row + 32 * c + 8 * g);
+                    kf[x][c] = y;
+                }
+            }
+        };
+        auto load_v = [&](uint32_t key0, uint32_t id) {
+            const T *p = (const T *)a.v + place(id);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const T *row = p + (size_t)((key0 + 8 * g + j) & (page - 1)) * d;
+#pragma unroll
+                for (int c = 0; c < NC; c++) {
+                    vw y = {};
+                    if (16 * CW * c + CW * m < d) y = *(const vw *)(row + 16 * CW * c + CW * m);
+                    vf[j][c] = y;
+                }
+            }
+        };
+        uint32_t key0 = (span.tile0 + skip) * kRowTile + 32 * w;
+        uint32_t kid = page_of(key0 + 8 * (m >> 2)), vid = page_of(key0 + 8 * g);
+        uint32_t kid1 = page_of(key0 + kRowTile + 8 * (m >> 2)), vid1 = page_of(key0 + kRowTile + 8 * g);
+        load_k(key0, kid);
+        load_v(key0, vid);
+
         // ---- queries: row r0 + 16 nt + m, values 32 s + 8 g .. + 7
         v8 qf[NT][NP][KS];
         float unscale[NT];
@@ -249,13 +293,13 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(const AttnArgs a)
             const uint32_t r = min(r0 + 16 * nt + m, r1 - 1);
             const uint32_t tok = r / a.group, h = kvh * a.group + (r - tok * a.group);
             pos[nt] = (int64_t)s.len - s.nq + tok;
-            const size_t at = (size_t)(s.first + tok) * a.ld_q + (size_t)h * a.d;
+            const size_t at = (size_t)(s.first + tok) * a.ld_q + (size_t)h * d;
             unscale[nt] = a.scale;
             if constexpr (F32) {
                 float x[KS][8], top = 0.0f;
 #pragma unroll
                 for (int c = 0; c < KS; c++) {
-                    if (32 * c + 8 * g < a.d) load8((const float *)a.q + at + 32 * c + 8 * g, x[c]);
+                    if (32 * c + 8 * g < d) load8((const float *)a.q + at + 32 * c + 8 * g, x[c]);
                     else
 #pragma unroll
                         for (int e = 0; e < 8; e++) x[c][e] = 0.0f;
@@ -283,47 +327,11 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(const AttnArgs a)
 #pragma unroll
                 for (int c = 0; c < KS; c++) {
                     v8 x = {};
-                    if (32 * c + 8 * g < a.d) x = *(const v8 *)((const T *)a.q + at + 32 * c + 8 * g);
+                    if (32 * c + 8 * g < d) x = *(const v8 *)((const T *)a.q + at + 32 * c + 8 * g);
                     qf[nt][0][c] = x;
                 }
             }
         }
-
-        // ---- the keys
-        const uint32_t *table = a.table + (size_t)min(s.row, a.n_rows - 1) * a.ld_table;
-        const uint32_t last = span.hi > 0 ? span.hi - 1 : 0;
-        auto place = [&](uint32_t key) {                // of a key's page for this head, in values; the key is held to the unit's
-            const uint32_t p = min(table[min(key, last) >> a.shift], a.n_pages - 1);
-            return ((size_t)p * a.n_kv + kvh) * head;
-        };
-        v8 kf[2][KS];
-        vw vf[8][NC];
-        auto load_k = [&](uint32_t key0) {
-            const T *p = (const T *)a.k + place(key0 + 8 * (m >> 2));
-#pragma unroll
-            for (int x = 0; x < 2; x++) {
-                const T *row = p + (size_t)((key0 + 8 * (m >> 2) + 4 * x + (m & 3)) & (page - 1)) * a.d;
-#pragma unroll
-                for (int c = 0; c < KS; c++) {
-                    v8 y = {};
-                    if (32 * c + 8 * g < a.d) y = *(const v8 *)(row + 32 * c + 8 * g);
-                    kf[x][c] = y;
-                }
-            }
-        };
-        auto load_v = [&](uint32_t key0) {
-            const T *p = (const T *)a.v + place(key0 + 8 * g);
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const T *row = p + (size_t)((key0 + 8 * g + j) & (page - 1)) * a.d;
-#pragma unroll
-                for (int c = 0; c < NC; c++) {
-                    vw y = {};
-                    if (16 * CW * c + CW * m < a.d) y = *(const vw *)(row + 16 * CW * c + CW * m);
-                    vf[j][c] = y;
-                }
-            }
-        };
 
         f4 o[NT][NC][CW];
         float mx[NT], sum[NT];
@@ -336,9 +344,6 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(const AttnArgs a)
 #pragma unroll
                 for (int i = 0; i < CW; i++) o[nt][c][i] = f4{0, 0, 0, 0};
         }
-        uint32_t key0 = (span.tile0 + skip) * kRowTile + 32 * w;
-        load_k(key0);
-        load_v(key0);
         for (uint32_t x = 0; x < left; x++, key0 += kRowTile) {
             // rows that see a part of the 32 keys only
             const bool edge = key0 + 32 > (uint32_t)max((int64_t)0, (int64_t)s.len - s.nq + r0 / a.group + 1) ||
@@ -355,7 +360,13 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(const AttnArgs a)
                         for (int c = 0; c < KS; c++) z = mfma(kf[y][c], qf[nt][q][c], z);
                     sc[nt][y] = z;
                 }
-            load_k(key0 + kRowTile);
+            const bool more = x + 1 < left;
+            if (more) {
+                kid = kid1; vid = vid1;
+                kid1 = page_of(key0 + 2 * kRowTile + 8 * (m >> 2));
+                vid1 = page_of(key0 + 2 * kRowTile + 8 * g);
+                load_k(key0 + kRowTile, kid);
+            }
 
             float p[NT][8];
 #pragma unroll
@@ -389,13 +400,17 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(const AttnArgs a)
                     for (int i = 0; i < CW; i++) o[nt][c][i] *= by;
             }
 
-            uint32_t bad = 0;               // keys 8 g + j of the edge with an infinity or a NaN, bit 8 g + j
+            // Values of keys that no row sees are zeros.  An infinity or a NaN of a
+            // key that only some rows see would reach the others as 0 * NaN: such
+            // keys (bit 8 g + j of `bad`) are left out of the product and come one
+            // by one after it, to the rows that see them.
+            uint32_t bad = 0;
             if (edge) {
-                const uint32_t see = span.hi;           // keys past these are no row's
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const uint32_t key = key0 + 8 * g + j;
-                    bool out = key >= see || key < span.lo, inf = false;
+                    const bool out = key >= span.hi || key < span.lo;
+                    bool inf = false;
 #pragma unroll
                     for (int c = 0; c < NC; c++) {
                         if (out) vf[j][c] = vw{};
@@ -407,23 +422,21 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(const AttnArgs a)
 #pragma unroll
                     for (int y = 0; y < 4; y++)
                         if (b >> (16 * y) & 0xffff) bad |= 1u << (8 * y + j);
-                    if (bad >> (8 * g + j) & 1)
-#pragma unroll
-                        for (int c = 0; c < NC; c++) vf[j][c] = vw{};
                 }
             }
+            v8 pf[NT][NP];
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                v8 pf[NP];
+            for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    pf[0][j] = (T)p[nt][j];
+                    pf[nt][0][j] = (T)p[nt][j];
                     if constexpr (F32) {
-                        const float y = p[nt][j] - (float)pf[0][j];
-                        pf[1][j] = (T)y;
-                        pf[2][j] = (T)(y - (float)pf[1][j]);
+                        const float y = p[nt][j] - (float)pf[nt][0][j];
+                        pf[nt][1][j] = (T)y;
+                        pf[nt][2][j] = (T)(y - (float)pf[nt][1][j]);
                     }
                 }
+            if (bad == 0) {
 #pragma unroll
                 for (int c = 0; c < NC; c++)
 #pragma unroll
@@ -432,34 +445,37 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(const AttnArgs a)
 #pragma unroll
                         for (int j = 0; j < 8; j++) x8[j] = vf[j][c][i];
 #pragma unroll
-                        for (int q = NP - 1; q >= 0; q--) o[nt][c][i] = mfma(x8, pf[q], o[nt][c][i]);
-                    }
-            }
-            // Those keys count for the rows that see them, and only for those.
-            for (; bad; bad &= bad - 1) {
-                const uint32_t y = __ffs(bad) - 1, key = key0 + y;
-                const T *row = (const T *)a.v + place(key) + (size_t)(key & (page - 1)) * a.d;
+                        for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    float wt = 0.0f;
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const float z = __shfl(p[nt][j], (y >> 3) * 16 + m);
-                        if (j == (int)(y & 7)) wt = z;
+                            for (int q = NP - 1; q >= 0; q--) o[nt][c][i] = mfma(x8, pf[nt][q], o[nt][c][i]);
                     }
-                    if ((int64_t)key > pos[nt] || (int64_t)key <= pos[nt] - (int64_t)a.window) continue;
+            } else {
+                uint32_t keep = ~bad;               // the keys of this pass
+                for (;;) {
+                    const int64_t key = (int64_t)key0 + __ffs(keep) - 1;
 #pragma unroll
                     for (int c = 0; c < NC; c++)
 #pragma unroll
-                        for (int i = 0; i < CW; i++)
+                        for (int i = 0; i < CW; i++) {
+                            v8 x8;
 #pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const uint32_t dv = 16 * CW * c + CW * (4 * g + e) + i;
-                                if (dv < a.d) o[nt][c][i][e] += wt * (float)row[dv];
+                            for (int j = 0; j < 8; j++) x8[j] = keep >> (8 * g + j) & 1 ? vf[j][c][i] : (T)0.0f;
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) {
+                                f4 y = o[nt][c][i];
+#pragma unroll
+                                for (int q = NP - 1; q >= 0; q--) y = mfma(x8, pf[nt][q], y);
+                                const bool sees = keep == ~bad || (key <= pos[nt] && key > pos[nt] - (int64_t)a.window);
+#pragma unroll
+                                for (int e = 0; e < 4; e++) o[nt][c][i][e] = sees ? y[e] : o[nt][c][i][e];
                             }
+                        }
+                    const uint32_t rest = keep == ~bad ? bad : bad & ~(keep | (keep - 1));
+                    if (rest == 0) break;
+                    keep = rest & -rest;
                 }
             }
-            load_v(key0 + kRowTile);
+            if (more) load_v(key0 + kRowTile, vid);
         }
 
         // ---- the waves' sums together; the unit's rows or its part
@@ -494,7 +510,7 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(const AttnArgs a)
             const int64_t at = (int64_t)s.len - s.nq + tok;
             const float inv = at < 0 ? 0.0f : 1.0f / total;             // (no key: zeros)
             if (!whole && c0 == 0) { part[R * D + 16 * nt + rr] = top; part[R * D + R + 16 * nt + rr] = total; }
-            const size_t to = (size_t)(s.first + tok) * a.ld_out + (size_t)(kvh * a.group + r - tok * a.group) * a.d;
+            const size_t to = (size_t)(s.first + tok) * a.ld_out + (size_t)(kvh * a.group + r - tok * a.group) * d;
 #pragma unroll
             for (int c = 0; c < D / 64; c++) {
                 const int dv = 64 * c + 4 * c0;
@@ -502,7 +518,7 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(const AttnArgs a)
 #pragma unroll
                 for (int y = 0; y < 4; y++) x += *(const f4 *)&s_o[y][rr][dv] * by[y];
                 if (!whole) *(f4 *)(part + (size_t)(16 * nt + rr) * D + dv) = x;
-                else if (dv < (int)a.d) {
+                else if (dv < (int)d) {
                     x *= inv;
                     if constexpr (F32) *(f4 *)((float *)a.out + to + dv) = x;
                     else {
@@ -551,7 +567,7 @@ template <int D> struct Chunk {
 // The running maximum is raised only when a score passes it by 2^8, so the
 // sums are seldom scaled: the weights then reach 2^8, which f32 sums and the
 // type's range (f16: 2^7 is the lift here) take without loss.
-template <class T, int D>
+template <class T, int D, bool FULL>
 __global__ void __launch_bounds__(Chunk<D>::kThreads) attn_chunk_kernel(const AttnArgs a)
 {
     constexpr int R = Chunk<D>::kRows, kTile = Chunk<D>::kTile, kThreads = Chunk<D>::kThreads;
@@ -571,7 +587,8 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads) attn_chunk_kernel(const At
     const int lane = threadIdx.x & 63, hf = lane >> 5, col = lane & 31, l16 = lane & 15;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t slot = (1u << a.shift) - 1;
-    const size_t head = (size_t)a.d << a.shift;
+    const uint32_t d = FULL ? D : a.d;
+    const size_t head = (size_t)d << a.shift;
     const float scale = fabsf(a.scale);
 
     // this thread's pieces of a tile: rows prow + KP.., piece pc, and their places in LDS
@@ -607,11 +624,11 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads) attn_chunk_kernel(const At
         const int pos = base + (int)tok;
         const int pos0 = base + (int)(min(w0, r1 - 1) / a.group), pos1 = base + (int)(min(w0 + 31, r1 - 1) / a.group);
         v8 qf[KS];
-        const T *q = (const T *)a.q + (size_t)(s.first + tok) * a.ld_q + (size_t)hq * a.d;
+        const T *q = (const T *)a.q + (size_t)(s.first + tok) * a.ld_q + (size_t)hq * d;
 #pragma unroll
         for (int c = 0; c < KS; c++) {
             v8 x = {};
-            if (16 * c + 8 * hf < (int)a.d) x = *(const v8 *)(q + 16 * c + 8 * hf);
+            if (16 * c + 8 * hf < (int)d) x = *(const v8 *)(q + 16 * c + 8 * hf);
             qf[c] = a.scale < 0.0f ? -x : x;
         }
 
@@ -628,7 +645,7 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads) attn_chunk_kernel(const At
 #pragma unroll
             for (int i = 0; i < KP; i++) {
                 const uint32_t key = key0 + prow + kStep * i;
-                const size_t at = ((size_t)min(id[i], a.n_pages - 1) * a.n_kv + kvh) * head + (size_t)(key & slot) * a.d + 8 * pc;
+                const size_t at = ((size_t)min(id[i], a.n_pages - 1) * a.n_kv + kvh) * head + (size_t)(key & slot) * d + 8 * pc;
                 kr[i] = vr[i] = u4v{0, 0, 0, 0};
                 if (inside) {
                     kr[i] = *(const u4v *)((const T *)a.k + at);
@@ -765,13 +782,13 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads) attn_chunk_kernel(const At
                         }
                     if ((int)key > pos || (int)key < lo) continue;
                     const uint32_t page = min(table[min(key, last) >> a.shift], a.n_pages - 1);
-                    const T *v = (const T *)a.v + ((size_t)page * a.n_kv + kvh) * head + (size_t)(key & slot) * a.d;
+                    const T *v = (const T *)a.v + ((size_t)page * a.n_kv + kvh) * head + (size_t)(key & slot) * d;
 #pragma unroll
                     for (int c = 0; c < DT; c++)
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
                             const int dv = 32 * c + 8 * (i >> 2) + 4 * hf + (i & 3);
-                            if (dv < (int)a.d) o[c][i] += wt * (float)v[dv];
+                            if (dv < (int)d) o[c][i] += wt * (float)v[dv];
                         }
                 }
             }
@@ -791,14 +808,14 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads) attn_chunk_kernel(const At
         if (w0 + col < r1) {
             if (whole) {
                 const float inv = pos < 0 ? 0.0f : 1.0f / sum;          // (no key: zeros)
-                T *to = (T *)a.out + (size_t)(s.first + tok) * a.ld_out + (size_t)hq * a.d;
+                T *to = (T *)a.out + (size_t)(s.first + tok) * a.ld_out + (size_t)hq * d;
                 typedef T v4 __attribute__((ext_vector_type(4)));
 #pragma unroll
                 for (int c = 0; c < DT; c++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const int dv = 32 * c + 8 * i + 4 * hf;
-                        if (dv < (int)a.d) {
+                        if (dv < (int)d) {
                             f4 y = {o[c][4 * i], o[c][4 * i + 1], o[c][4 * i + 2], o[c][4 * i + 3]};
                             y *= inv;
                             *(v4 *)(to + dv) = v4{(T)y[0], (T)y[1], (T)y[2], (T)y[3]};
@@ -911,14 +928,17 @@ template <class TO, int D, int R> int join(const gs::AttnArgs &a, hipStream_t st
 template <class T, int D, int NT, bool F32> int rows_call(gs::AttnArgs a, hipStream_t st)
 {
     a.n_wg = kRuns;
-    hipLaunchKernelGGL((gs::attn_rows_kernel<T, D, NT, F32>), dim3(kRuns), dim3(256), 0, st, a);
+    if (a.d == D) hipLaunchKernelGGL((gs::attn_rows_kernel<T, D, NT, F32, true>), dim3(kRuns), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((gs::attn_rows_kernel<T, D, NT, F32, false>), dim3(kRuns), dim3(256), 0, st, a);
     return join<std::conditional_t<F32, float, T>, D, 16 * NT>(a, st);
 }
 
 template <class T, int D> int chunk_call(gs::AttnArgs a, hipStream_t st)
 {
     a.n_wg = kChunkRuns;
-    hipLaunchKernelGGL((gs::attn_chunk_kernel<T, D>), dim3(kChunkRuns), dim3(gs::Chunk<D>::kThreads), 0, st, a);
+    const dim3 grid(kChunkRuns), block(gs::Chunk<D>::kThreads);
+    if (a.d == D) hipLaunchKernelGGL((gs::attn_chunk_kernel<T, D, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((gs::attn_chunk_kernel<T, D, false>), grid, block, 0, st, a);
     return join<T, D, gs::Chunk<D>::kRows>(a, st);
 }
 

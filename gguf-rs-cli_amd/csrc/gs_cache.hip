@@ -10,6 +10,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/gs_cache.h"
 #include "gs_cache.hpp"
 
@@ -17,6 +19,7 @@ namespace gs {
 
 constexpr int kBook = 1024;             // threads of the bookkeeping workgroup
 constexpr int kScan = 16;               // reference counts per thread and step of the search
+constexpr uint32_t kOwners = 8192;      // rows whose marks fit in LDS
 
 // One row of a fork or a drop, in ws.
 struct Move {
@@ -70,21 +73,52 @@ __device__ __forceinline__ uint32_t scan(uint32_t x, uint32_t &total)
 }
 
 // The free pages from `page` on, ascending, to list[found ..] until it has
-// `want`; both run on from call to call of one kernel.
+// `want`; both run on from call to call of one kernel.  A wave reads 64 counts
+// that lie together, kScan times 1024 apart, and the free ones of each such
+// read are counted by a ballot; the 256 counts are summed in order by wave 0.
 __device__ __forceinline__ void take(const Cache &c, uint32_t want, uint32_t &page, uint32_t &found)
 {
+    __shared__ uint32_t s_cnt[kScan * kBook / 64 + 1];
+    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     while (found < want && page < c.n_pages) {
-        const uint32_t p0 = page + threadIdx.x * kScan;
         uint32_t mask = 0;
 #pragma unroll
+        for (int i = 0; i < kScan; i++) {
+            const uint32_t p = page + i * kBook + threadIdx.x;
+            if (p < c.n_pages) mask |= (uint32_t)(c.ref[p] == 0) << i;
+        }
+        uint64_t free[kScan];
+#pragma unroll
+        for (int i = 0; i < kScan; i++) {
+            free[i] = __ballot(mask >> i & 1);
+            if (lane == 0) s_cnt[i * (kBook / 64) + w] = __popcll(free[i]);
+        }
+        __syncthreads();
+        if (w == 0) {
+            constexpr int kEach = kScan * kBook / 64 / 64;
+            uint32_t x[kEach], sum = 0;
+#pragma unroll
+            for (int i = 0; i < kEach; i++) { x[i] = s_cnt[lane * kEach + i]; sum += x[i]; }
+            uint32_t at = sum;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const uint32_t y = __shfl_up(at, o);
+                if ((int)lane >= o) at += y;
+            }
+            if (lane == 63) s_cnt[kScan * kBook / 64] = at;
+            at -= sum;
+#pragma unroll
+            for (int i = 0; i < kEach; i++) { s_cnt[lane * kEach + i] = at; at += x[i]; }
+        }
+        __syncthreads();
+#pragma unroll
         for (int i = 0; i < kScan; i++)
-            if (p0 + i < c.n_pages) mask |= (uint32_t)(c.ref[p0 + i] == 0) << i;
-        uint32_t total, at = found + scan(__popc(mask), total);
-        for (; mask; mask &= mask - 1) c.list[at++] = p0 + __ffs(mask) - 1;     // (at most n_pages in all)
-        found += total;
+            if (mask >> i & 1)          // (at most n_pages in all)
+                c.list[found + s_cnt[i * (kBook / 64) + w] + __popcll(free[i] & ((1ull << lane) - 1))] = page + i * kBook + threadIdx.x;
+        found += s_cnt[kScan * kBook / 64];
         page += kBook * kScan;
+        __syncthreads();
     }
-    __syncthreads();
 }
 
 __global__ void reset_kernel(const Cache c)
@@ -149,30 +183,39 @@ __global__ void __launch_bounds__(kBook) extend_kernel(const Cache c, const uint
     }
 }
 
-// Marks, for each row named, the first i that names it.  (Device-scope loads:
-// the marks are in L2.)
-__device__ __forceinline__ void claim(const Cache &c, const uint32_t *rows, uint32_t n)
+// Marks, for each row named, the first i that names it: in LDS, or for caches
+// of more than kOwners rows in ws.  (Device-scope accesses there: the marks
+// are in L2.)
+__device__ __forceinline__ void claim(const Cache &c, uint32_t *owner, const uint32_t *rows, uint32_t n)
 {
-    for (uint32_t i = threadIdx.x; i < n; i += kBook)
-        if (rows[i] < c.rows) __hip_atomic_store(&c.owner[rows[i]], GS_KV_NONE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __threadfence();
+    const bool local = c.rows <= kOwners;
+    for (uint32_t i = threadIdx.x; i < n; i += kBook) {
+        const uint32_t r = rows[i];
+        if (r >= c.rows) continue;
+        if (local) owner[r] = GS_KV_NONE;
+        else __hip_atomic_store(&c.owner[r], GS_KV_NONE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if (!local) __threadfence();
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < n; i += kBook)
-        if (rows[i] < c.rows) atomicMin(&c.owner[rows[i]], i);
-    __threadfence();
+    for (uint32_t i = threadIdx.x; i < n; i += kBook) {
+        const uint32_t r = rows[i];
+        if (r < c.rows) atomicMin(local ? &owner[r] : &c.owner[r], i);
+    }
+    if (!local) __threadfence();
     __syncthreads();
 }
 
-__device__ __forceinline__ bool claimed(const Cache &c, uint32_t row, uint32_t i)
+__device__ __forceinline__ bool claimed(const Cache &c, const uint32_t *owner, uint32_t row, uint32_t i)
 {
-    return __hip_atomic_load(&c.owner[row], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == i;
+    return (c.rows <= kOwners ? owner[row] : __hip_atomic_load(&c.owner[row], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) == i;
 }
 
 // Fork, 1 of 3: which pairs go ahead, and the page for each partial last page.
 __global__ void __launch_bounds__(kBook) fork_plan_kernel(const Cache c, const uint32_t *src, const uint32_t *dst, uint32_t n,
                                                           int32_t *status)
 {
-    claim(c, dst, n);
+    __shared__ uint32_t s_owner[kOwners];
+    claim(c, s_owner, dst, n);
     uint32_t page = 0, found = 0, given = 0;
     for (uint32_t i0 = 0; i0 < n; i0 += kBook) {
         const uint32_t i = i0 + threadIdx.x;
@@ -182,7 +225,7 @@ __global__ void __launch_bounds__(kBook) fork_plan_kernel(const Cache c, const u
         if (i < n) {
             m.row = dst[i];
             m.from = src[i];
-            if (m.row >= c.rows || (m.from >= c.rows && m.from != GS_KV_NONE) || !claimed(c, m.row, i)) rc = GS_ERR_INVALID;
+            if (m.row >= c.rows || (m.from >= c.rows && m.from != GS_KV_NONE) || !claimed(c, s_owner, m.row, i)) rc = GS_ERR_INVALID;
             else if (m.from != m.row) {
                 m.ok = 1;
                 m.old_len = row_len(c, m.row);
@@ -275,12 +318,14 @@ __global__ void __launch_bounds__(256) free_kernel(const Cache c, const uint32_t
 __global__ void __launch_bounds__(kBook) drop_plan_kernel(const Cache c, const uint32_t *rows, uint32_t n, const uint32_t *from,
                                                           const uint32_t *to, int32_t *status)
 {
-    claim(c, rows, n);
+    __shared__ uint32_t s_owner[kOwners];
+    claim(c, s_owner, rows, n);
+    constexpr int kPlan = 8;            // reads of 64 places that a wave has under way
     const uint32_t lane = threadIdx.x & 63;
     for (uint32_t i = threadIdx.x >> 6; i < n; i += kBook / 64) {
         Move m = {};
         m.row = rows[i];
-        m.ok = m.row < c.rows && claimed(c, m.row, i);
+        m.ok = m.row < c.rows && claimed(c, s_owner, m.row, i);
         uint32_t need = 0, written = 0;
         if (m.ok) {
             m.len = row_len(c, m.row);
@@ -288,16 +333,22 @@ __global__ void __launch_bounds__(kBook) drop_plan_kernel(const Cache c, const u
             m.left = m.len - (min(max(to[i], m.from), m.len) - m.from);
             const uint32_t first = m.from >> c.shift, now = pages_of(c, m.left);
             if (m.left < m.len) {
-                for (uint32_t j = first; j < now; j += 64) {
-                    bool fresh = false;
-                    if (j + lane < now) {
-                        const uint32_t p = c.table[(size_t)m.row * c.ld + j + lane];
-                        fresh = p < c.n_pages && c.ref[p] > 1;
+                const uint32_t *table = c.table + (size_t)m.row * c.ld;
+                for (uint32_t j = first; j < now; j += 64 * kPlan) {
+                    uint32_t p[kPlan], held[kPlan];
+#pragma unroll
+                    for (int e = 0; e < kPlan; e++) p[e] = j + 64 * e + lane < now ? table[j + 64 * e + lane] : GS_KV_NONE;
+#pragma unroll
+                    for (int e = 0; e < kPlan; e++) held[e] = p[e] < c.n_pages ? c.ref[p[e]] : 0;
+#pragma unroll
+                    for (int e = 0; e < kPlan; e++) {
+                        const bool fresh = held[e] > 1;
+                        const uint64_t b = __ballot(fresh);
+                        if (j + 64 * e + lane < now)
+                            c.stage[(size_t)i * c.ld + j + 64 * e + lane] =
+                                (need + __popcll(b & ((1ull << lane) - 1))) | (fresh ? 0x80000000u : 0u);
+                        need += __popcll(b);
                     }
-                    const uint64_t b = __ballot(fresh);
-                    if (j + lane < now)
-                        c.stage[(size_t)i * c.ld + j + lane] = (need + __popcll(b & ((1ull << lane) - 1))) | (fresh ? 0x80000000u : 0u);
-                    need += __popcll(b);
                 }
                 written = now > first ? now - first : 0;
             }
@@ -339,98 +390,79 @@ __device__ __forceinline__ uint32_t new_page(const Cache &c, const Move &m, uint
     return c.table[(size_t)m.row * c.ld + j];
 }
 
-// Drop, 2 of 3: the tokens move.  blockIdx.x: a stream (k or v, layer, head)
-// of row blockIdx.z; tokens go down in ascending order, kStep values of 16
-// bytes per thread and step, all read before any is written, so a workgroup
-// that has the stream alone may write over what it has read.  Rows all of
-// whose written pages are new are read from other pages than they are written
-// to, and their steps are shared by gridDim.y workgroups.
-// An item is 16 bytes of a token, or for turned keys two that belong together
-// (the pairs of the half layout; neighbours): a read, a write and little else,
-// bound by the traffic.
-template <class T, bool VEC>
-__global__ void __launch_bounds__(256) drop_move_kernel(const Cache c, const uint64_t *turns, int rot, int half)
-{
-    constexpr int kStep = 4;
-    const uint32_t i = blockIdx.z, stream = blockIdx.x;
-    const Move m = c.moves[i];
-    if (!m.ok) return;
-    const uint32_t slice = m.in_place ? 0 : blockIdx.y, slices = m.in_place ? 1 : gridDim.y;
-    if (slice != blockIdx.y) return;
-    const uint32_t h = stream % c.n_kv, l = stream / c.n_kv >> 1;
-    const bool keys = !(stream / c.n_kv & 1);
-    const uint32_t first = m.from >> c.shift, size = 1u << c.shift, gone = m.len - m.left;
-    // tokens before `from` move only where their page is a new one
-    const bool fresh = first < pages_of(c, m.left) && (c.stage[(size_t)i * c.ld + first] >> 31);
-    const uint32_t t0 = fresh ? first << c.shift : m.from;
-    const size_t head = (size_t)c.d << c.shift;
-    T *base = (T *)(keys ? c.k : c.v) + (size_t)l * c.n_pages * c.n_kv * head;
-    const uint32_t *table = c.table + (size_t)m.row * c.ld;
+// How a stream's values move: as they are or turned within vectors of 8 (the
+// interleaved layout); turned in pairs of vectors (the half layout); or value
+// by value, where the turned part is no whole number of such vectors.
+enum { kMoveVector, kMovePairs, kMoveValues };
 
-    const bool turn = keys && rot > 0;
-    const uint32_t pairs = rot >> 1;
-    // items of a token
-    const uint32_t nturn = !turn ? 0 : VEC ? rot / 16 : pairs, per = nturn + (VEC ? (c.d - (turn ? rot : 0)) / 8 : (c.d - (turn ? rot : 0)) / 2);
-    __shared__ float2 cs[128];
-    if (turn) {
-        for (uint32_t e = threadIdx.x; e < pairs; e += 256) cs[e] = turn_of(turns[e], -(int64_t)gone, 1.0f);
-        __syncthreads();
-    }
-    const uint32_t fit = 256 / per, each = fit ? fit : 1;                   // tokens of a step's round
-    const uint32_t tl = threadIdx.x / per, item = threadIdx.x - tl * per;   // (per <= 128)
-    const bool works = tl < each;
-    // the two vectors of an item
-    uint32_t p, q;
-    const bool turned = item < nturn;
-    if (VEC) {
-        p = turned ? (half ? 8 * item : 16 * item) : (turn ? rot : 0) + 8 * (item - nturn);
-        q = turned ? (half ? p + pairs : p + 8) : p;
-    } else {
-        p = turned && half ? item : 2 * item;
-        q = turned && half ? item + pairs : p + 1;
-    }
-    constexpr int kW = VEC ? 8 : 1;
+// The tokens of one stream (k or v, layer, head: `base`) of row i, kStep
+// rounds of 256 items at a time, where an item is a vector, two or a pair of
+// values of a token.  All of a step's reads come before its writes, and the
+// pages' numbers of the next step are read before both: the reads are what a
+// step waits for.
+template <class T, int MODE>
+__device__ __forceinline__ void move_stream(const Cache &c, const Move &m, uint32_t i, T *base, uint32_t h, int rot, bool interleaved,
+                                            const float2 *cs, uint32_t t0, uint32_t slice, uint32_t slices)
+{
+    constexpr int kStep = MODE == kMoveVector ? 8 : 4, kW = MODE == kMoveValues ? 1 : 8;
     typedef T vec __attribute__((ext_vector_type(kW)));
-    for (uint32_t t = t0 + slice * each * kStep; t < m.left; t += slices * each * kStep) {
-        vec a[kStep], b[kStep];
-        T *to[kStep];
-        bool late[kStep];
+    const uint32_t pairs = rot >> 1, size = 1u << c.shift, gone = m.len - m.left;
+    const uint32_t nturn = MODE == kMoveVector ? rot / 8 : MODE == kMovePairs ? rot / 16 : pairs;
+    const uint32_t per = nturn + (MODE == kMoveValues ? (c.d - rot) / 2 : (c.d - rot) / 8);     // items of a token, at most 128
+    const uint32_t each = 256 / per, tl = threadIdx.x / per, item = threadIdx.x - tl * per;      // tokens of a round; this thread's
+    const bool works = tl < each, turned = item < nturn;
+    uint32_t p, q;
+    if (MODE == kMoveVector) p = q = 8 * item;
+    else if (MODE == kMovePairs) { p = turned ? 8 * item : rot + 8 * (item - nturn); q = turned ? p + pairs : p; }
+    else { p = turned && !interleaved ? item : 2 * item; q = turned && !interleaved ? item + pairs : p + 1; }
+    const uint32_t *table = c.table + (size_t)m.row * c.ld;
+    const size_t head = (size_t)c.d << c.shift;
+
+    uint32_t to[kStep], from[kStep];            // pages
+    auto pages = [&](uint32_t t) {
 #pragma unroll
         for (int s = 0; s < kStep; s++) {
             const uint32_t x = t + s * each + tl;
-            to[s] = nullptr;
+            to[s] = from[s] = GS_KV_NONE;
             if (!works || x >= m.left) continue;
-            late[s] = x >= m.from;
-            const uint32_t y = late[s] ? x + gone : x;
-            const uint32_t np = new_page(c, m, i, x >> c.shift), op = table[y >> c.shift];
-            if (np >= c.n_pages || op >= c.n_pages) continue;
-            const T *f = base + ((size_t)op * c.n_kv + h) * head + (y & (size - 1)) * c.d;
-            to[s] = base + ((size_t)np * c.n_kv + h) * head + (x & (size - 1)) * c.d;
-            a[s] = *(const vec *)(f + p);
-            if (q != p) b[s] = *(const vec *)(f + q);
+            to[s] = new_page(c, m, i, x >> c.shift);
+            from[s] = table[(x >= m.from ? x + gone : x) >> c.shift];
         }
+    };
+    const uint32_t step = slices * each * kStep;
+    pages(t0 + slice * each * kStep);
+    for (uint32_t t = t0 + slice * each * kStep; t < m.left; t += step) {
+        vec a[kStep], b[kStep];
+        T *at[kStep];
 #pragma unroll
         for (int s = 0; s < kStep; s++) {
-            if (!to[s] || !turned || !late[s]) continue;
-            float u[kW], w[kW];
+            const uint32_t x = t + s * each + tl, y = x >= m.from ? x + gone : x;
+            at[s] = nullptr;
+            if (to[s] >= c.n_pages || from[s] >= c.n_pages) continue;
+            const T *f = base + ((size_t)from[s] * c.n_kv + h) * head + (y & (size - 1)) * c.d;
+            at[s] = base + ((size_t)to[s] * c.n_kv + h) * head + (x & (size - 1)) * c.d;
+            a[s] = *(const vec *)(f + p);
+            if (MODE == kMoveValues || (MODE == kMovePairs && turned)) b[s] = *(const vec *)(f + q);
+        }
+        pages(t + step);
 #pragma unroll
-            for (int e = 0; e < kW; e++) { u[e] = (float)a[s][e]; w[e] = (float)b[s][e]; }
-            if constexpr (VEC) {
-                if (half) {
+        for (int s = 0; s < kStep; s++) {
+            if (!at[s] || !turned || t + s * each + tl < m.from) continue;
+            if constexpr (MODE == kMoveVector) {
 #pragma unroll
-                    for (int e = 0; e < 8; e++) turn_pair(u[e], w[e], cs[8 * item + e]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        turn_pair(u[2 * e], u[2 * e + 1], cs[8 * item + e]);
-                        turn_pair(w[2 * e], w[2 * e + 1], cs[8 * item + 4 + e]);
-                    }
+                for (int e = 0; e < 4; e++) {
+                    float u = (float)a[s][2 * e], w = (float)a[s][2 * e + 1];
+                    turn_pair(u, w, cs[4 * item + e]);
+                    a[s][2 * e] = (T)u; a[s][2 * e + 1] = (T)w;
                 }
             } else {
-                turn_pair(u[0], w[0], cs[item]);
-            }
 #pragma unroll
-            for (int e = 0; e < kW; e++) { a[s][e] = (T)u[e]; b[s][e] = (T)w[e]; }
+                for (int e = 0; e < kW; e++) {
+                    float u = (float)a[s][e], w = (float)b[s][e];
+                    turn_pair(u, w, cs[kW * item + e]);
+                    a[s][e] = (T)u; b[s][e] = (T)w;
+                }
+            }
         }
         if (m.in_place) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // every read of the step is done
@@ -438,11 +470,42 @@ __global__ void __launch_bounds__(256) drop_move_kernel(const Cache c, const uin
         }
 #pragma unroll
         for (int s = 0; s < kStep; s++) {
-            if (!to[s]) continue;
-            *(vec *)(to[s] + p) = a[s];
-            if (q != p) *(vec *)(to[s] + q) = b[s];
+            if (!at[s]) continue;
+            *(vec *)(at[s] + p) = a[s];
+            if (MODE == kMoveValues || (MODE == kMovePairs && turned)) *(vec *)(at[s] + q) = b[s];
         }
     }
+}
+
+// Drop, 2 of 3: the tokens move.  blockIdx.x: a stream of row blockIdx.z.
+// Tokens go down in ascending order and a step's reads are all done before its
+// writes, so a workgroup that has the stream alone may write over what it has
+// read.  Rows all of whose written pages are new are read from other pages
+// than they are written to, and their steps are shared by gridDim.y
+// workgroups.
+// MODE: of keys that are turned.
+template <class T, int MODE>
+__global__ void __launch_bounds__(256) drop_move_kernel(const Cache c, const uint64_t *turns, int rot, int interleaved)
+{
+    __shared__ float2 cs[128];
+    const uint32_t i = blockIdx.z, stream = blockIdx.x;
+    const Move m = c.moves[i];
+    if (!m.ok || (m.in_place && blockIdx.y)) return;
+    const uint32_t slice = blockIdx.y, slices = m.in_place ? 1 : gridDim.y;
+    const uint32_t h = stream % c.n_kv, l = stream / c.n_kv >> 1;
+    const bool keys = !(stream / c.n_kv & 1);
+    // tokens before `from` move only where their page is a new one
+    const uint32_t first = m.from >> c.shift;
+    const bool fresh = first < pages_of(c, m.left) && (c.stage[(size_t)i * c.ld + first] >> 31);
+    const uint32_t t0 = fresh ? first << c.shift : m.from;
+    T *base = (T *)(keys ? c.k : c.v) + (size_t)l * c.n_pages * c.n_kv * ((size_t)c.d << c.shift);
+    if (!keys || rot == 0) {
+        move_stream<T, kMoveVector>(c, m, i, base, h, 0, true, cs, t0, slice, slices);
+        return;
+    }
+    for (uint32_t e = threadIdx.x; e < (uint32_t)rot >> 1; e += 256) cs[e] = turn_of(turns[e], (int64_t)m.left - m.len, 1.0f);
+    __syncthreads();
+    move_stream<T, MODE>(c, m, i, base, h, rot, interleaved, cs, t0, slice, slices);
 }
 
 // Drop, 3 of 3: row blockIdx.x's table, its released pages, its length.
@@ -562,19 +625,21 @@ int gs_kv_drop(const gs_kv_cache *c, const uint32_t *rows, size_t n, const uint3
     const gs::Cache d = device_cache(c);
     hipStream_t st = (hipStream_t)stream;
     const size_t streams = 2 * (size_t)c->n_layers * c->n_kv;
-    const int rot = rope ? (int)rope->rot : 0, half = rope && rope->layout == GS_ROPE_HALF;
+    const int rot = rope ? (int)rope->rot : 0;
+    const bool inter = rope && rope->layout == GS_ROPE_INTERLEAVED;
     const uint64_t *turns = rope ? rope->turns : nullptr;
     const dim3 grid((unsigned)streams, shares(n * streams, 64), (unsigned)n);
     hipLaunchKernelGGL(gs::drop_plan_kernel, dim3(1), dim3(gs::kBook), 0, st, d, rows, (uint32_t)n, from, to, status);
-    const bool f16 = c->type == GS_TYPE_F16;
-    // (a part that is not whole vectors of pairs goes pair by pair)
-    if (rot % 16 == 0) {
-        if (f16) hipLaunchKernelGGL((gs::drop_move_kernel<_Float16, true>), grid, dim3(256), 0, st, d, turns, rot, half);
-        else hipLaunchKernelGGL((gs::drop_move_kernel<__bf16, true>), grid, dim3(256), 0, st, d, turns, rot, half);
-    } else {
-        if (f16) hipLaunchKernelGGL((gs::drop_move_kernel<_Float16, false>), grid, dim3(256), 0, st, d, turns, rot, half);
-        else hipLaunchKernelGGL((gs::drop_move_kernel<__bf16, false>), grid, dim3(256), 0, st, d, turns, rot, half);
-    }
+    auto move = [&](auto t, auto mode) {
+        hipLaunchKernelGGL((gs::drop_move_kernel<decltype(t), decltype(mode)::value>), grid, dim3(256), 0, st, d, turns, rot, inter);
+    };
+    auto typed = [&](auto mode) {
+        if (c->type == GS_TYPE_F16) move(_Float16(), mode);
+        else move(__bf16(), mode);
+    };
+    if (rot == 0 || (inter && rot % 8 == 0)) typed(std::integral_constant<int, gs::kMoveVector>());
+    else if (!inter && rot % 16 == 0) typed(std::integral_constant<int, gs::kMovePairs>());
+    else typed(std::integral_constant<int, gs::kMoveValues>());
     hipLaunchKernelGGL(gs::drop_write_kernel, dim3((unsigned)n), dim3(256), 0, st, d);
     return launched();
 }

@@ -31,7 +31,7 @@ struct RopeArgs {
     uint32_t n, n_rows, ld_table, n_pages;
     int shift;                          // log2 of the page size
     void *kc, *vc;                      // the layer's pages
-    // work items: 16 turned values or 8 others (two of each in the pair form)
+    // work items: a vector of 8 values, or two that the half layout turns together (in the pair form two values)
     int turned, per_head, per_v;        // items of a head that are turned, all of its items, those of a head of v
     int tokens;                         // of a workgroup
     uint32_t by_head, by_token, by_v, by_vtoken;   // 2^32 / (per_head, items of a token, per_v, items of v of a token), up
@@ -42,13 +42,14 @@ __device__ __forceinline__ uint32_t quotient(uint32_t n, uint32_t d, uint32_t m)
 
 // Each value is read once and written once; a token's angles are computed once
 // by its workgroup and serve all heads from LDS.  What bounds it is the
-// traffic, so the item of a thread is 16 values (two vectors of 8, the pairs
-// of the half layout or 16 neighbours), and a workgroup has enough of them.
-// VEC: the pair form otherwise, for heads, parts or strides that are not
-// multiples of the vectors.
+// traffic, so neighbouring threads have neighbouring vectors of 8 values (for
+// the half layout's turned values two each, rot / 2 apart), and two such items
+// at a time.  VEC: the pair form otherwise, for heads, parts or strides that
+// are not multiples of the vectors.
 template <class TI, class TO, class TC, bool VEC>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a)
 {
+    constexpr int kItems = 2, kW = VEC ? 8 : 1;
     __shared__ float2 cs[kRopeTokens * 256];
     __shared__ int64_t place[kRopeTokens];      // of a token's slot in a head's pages, in slots; -1: not written
     const int t0 = blockIdx.x * a.tokens, nt = min(a.tokens, a.n_tokens - t0);
@@ -87,52 +88,75 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a)
     }
     __syncthreads();
 
+    // kItems items of a thread at a time: their reads are under way together
     const int heads = a.n_heads + a.n_kv;
-    const uint32_t per_token = heads * a.per_head;
-    for (uint32_t i = blockIdx.y * kRopeThreads + threadIdx.x; i < nt * per_token; i += gridDim.y * kRopeThreads) {
-        const uint32_t t = quotient(i, per_token, a.by_token), r = i - t * per_token;
-        const uint32_t h = quotient(r, a.per_head, a.by_head), j = r - h * a.per_head;
-        const size_t token = t0 + t;
-        const bool isq = (int)h < a.n_heads;
-        const TI *x = isq ? (const TI *)a.q + token * a.ld_q + (size_t)h * a.d
-                          : (const TI *)a.k + token * a.ld_k + (size_t)(h - a.n_heads) * a.d;
-        const int64_t at = isq ? 0 : place[t];
-        TO *yq = (TO *)a.q_out + token * a.ld_out + (size_t)h * a.d;
-        TC *yk = (TC *)a.kc + (h - a.n_heads) * head + at * a.d;
-        if (at < 0) continue;
-        const float2 *c = cs + t * 256;
-        if constexpr (VEC) {
-            if ((int)j < a.turned) {
-                const int p = a.half ? 8 * j : 16 * j, q = a.half ? p + pairs : p + 8;
-                float u[8], w[8];
-                load8(x + p, u);
-                load8(x + q, w);
-                if (a.half) {
+    const uint32_t per_token = heads * a.per_head, step = gridDim.y * kRopeThreads;
+    for (uint32_t i0 = blockIdx.y * kRopeThreads + threadIdx.x; i0 < nt * per_token; i0 += kItems * step) {
+        float u[kItems][kW], w[kItems][kW];
+        int p[kItems], q[kItems];
+        uint32_t cj[kItems];                // the item's first angle
+        TO *yq[kItems];
+        TC *yk[kItems];
+        bool live[kItems], turned[kItems];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) turn_pair(u[e], w[e], c[8 * j + e]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        turn_pair(u[2 * e], u[2 * e + 1], c[8 * j + e]);
-                        turn_pair(w[2 * e], w[2 * e + 1], c[8 * j + 4 + e]);
-                    }
-                }
-                if (isq) { store8(yq + p, u); store8(yq + q, w); }
-                else { store8(yk + p, u); store8(yk + q, w); }
+        for (int s = 0; s < kItems; s++) {
+            const uint32_t i = i0 + s * step;
+            live[s] = i < nt * per_token;
+            if (!live[s]) continue;
+            const uint32_t t = quotient(i, per_token, a.by_token), r = i - t * per_token;
+            const uint32_t h = quotient(r, a.per_head, a.by_head), j = r - h * a.per_head;
+            const size_t token = t0 + t;
+            const bool isq = (int)h < a.n_heads;
+            const TI *x = isq ? (const TI *)a.q + token * a.ld_q + (size_t)h * a.d
+                              : (const TI *)a.k + token * a.ld_k + (size_t)(h - a.n_heads) * a.d;
+            const int64_t at = isq ? 0 : place[t];
+            yq[s] = isq ? (TO *)a.q_out + token * a.ld_out + (size_t)h * a.d : nullptr;
+            yk[s] = (TC *)a.kc + (h - a.n_heads) * head + at * a.d;
+            live[s] = at >= 0;
+            if (!live[s]) continue;
+            turned[s] = (int)j < a.turned;
+            if constexpr (VEC) {
+                // one vector of 8, or for pairs of the half layout two
+                cj[s] = t * 256 + (a.half ? 8 : 4) * j;
+                p[s] = q[s] = turned[s] ? 8 * j : a.rot + 8 * (j - a.turned);
+                if (turned[s] && a.half) q[s] += pairs;
+                load8(x + p[s], u[s]);
+                if (q[s] != p[s]) load8(x + q[s], w[s]);
             } else {
-                const int p = a.rot + 8 * (j - a.turned);
-                float u[8];
-                load8(x + p, u);
-                if (isq) store8(yq + p, u);
-                else store8(yk + p, u);
+                cj[s] = t * 256 + j;
+                p[s] = turned[s] && a.half ? j : 2 * j;
+                q[s] = turned[s] && a.half ? j + pairs : 2 * j + 1;
+                u[s][0] = (float)x[p[s]];
+                w[s][0] = (float)x[q[s]];
             }
-        } else {
-            const bool turned = (int)j < a.turned;
-            const int p = !turned || !a.half ? 2 * j : j, q = !turned || !a.half ? p + 1 : p + pairs;
-            float u = (float)x[p], w = (float)x[q];
-            if (turned) turn_pair(u, w, c[j]);
-            if (isq) { yq[p] = (TO)u; yq[q] = (TO)w; }
-            else { yk[p] = (TC)u; yk[q] = (TC)w; }
+        }
+#pragma unroll
+        for (int s = 0; s < kItems; s++) {
+            if (!live[s]) continue;
+            const float2 *c = cs + cj[s];
+            if (turned[s]) {
+                if constexpr (VEC) {
+                    if (a.half) {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) turn_pair(u[s][e], w[s][e], c[e]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) turn_pair(u[s][2 * e], u[s][2 * e + 1], c[e]);
+                    }
+                } else turn_pair(u[s][0], w[s][0], c[0]);
+            }
+            if constexpr (VEC) {
+                if (yq[s]) {
+                    store8(yq[s] + p[s], u[s]);
+                    if (q[s] != p[s]) store8(yq[s] + q[s], w[s]);
+                } else {
+                    store8(yk[s] + p[s], u[s]);
+                    if (q[s] != p[s]) store8(yk[s] + q[s], w[s]);
+                }
+            } else {
+                if (yq[s]) { yq[s][p[s]] = (TO)u[s][0]; yq[s][q[s]] = (TO)w[s][0]; }
+                else { yk[s][p[s]] = (TC)u[s][0]; yk[s][q[s]] = (TC)w[s][0]; }
+            }
         }
     }
     if (a.n_kv == 0) return;
@@ -180,7 +204,7 @@ template <class Fn> int with_type(uint32_t type, Fn f)
 template <class TI, class TO, class TC>
 int launch(RopeArgs &a, bool vec, hipStream_t st)
 {
-    a.turned = vec ? a.rot / 16 : a.rot / 2;
+    a.turned = !vec ? a.rot / 2 : a.half ? a.rot / 16 : a.rot / 8;
     a.per_head = a.turned + (vec ? (a.d - a.rot) / 8 : (a.d - a.rot) / 2);
     a.per_v = vec ? a.d / 8 : a.d / 2;
     const uint64_t per_token = (uint64_t)(a.n_heads + a.n_kv) * a.per_head, items = per_token + (uint64_t)a.n_kv * a.per_v;
@@ -301,7 +325,7 @@ int gs_rope_apply(const gs_rope *r, uint32_t type, const void *x, size_t ld_x, v
     a.n_heads = (int)n_heads;
     a.n_tokens = (int)n_tokens;
     a.pos = pos;
-    const bool vec = r->rot % 16 == 0 && r->d % 8 == 0 && vectors(x, ld_x, type) && vectors(out, ld_out, type);
+    const bool vec = r->rot % (a.half ? 16 : 8) == 0 && r->d % 8 == 0 && vectors(x, ld_x, type) && vectors(out, ld_out, type);
     return with_type(type, [&](auto t) { return launch<decltype(t), decltype(t), _Float16>(a, vec, (hipStream_t)stream); });
 }
 
@@ -324,7 +348,7 @@ int gs_kv_append(const gs_kv_cache *c, uint32_t layer, const gs_kv_batch *b, con
     a.k = x->k; a.ld_k = x->ld_k;
     a.v = x->v; a.ld_v = x->ld_v;
     a.n_kv = (int)c->n_kv;
-    bool vec = a.rot % 16 == 0 && vectors(x->k, x->ld_k, x->type) && vectors(x->v, x->ld_v, x->type);
+    bool vec = a.rot % (a.half ? 16 : 8) == 0 && vectors(x->k, x->ld_k, x->type) && vectors(x->v, x->ld_v, x->type);
     if (x->q) {
         const size_t q = (size_t)x->n_heads * c->d;
         if (x->n_heads == 0 || !x->q_out || x->ld_q < q || x->ld_q_out < q) return GS_ERR_INVALID;

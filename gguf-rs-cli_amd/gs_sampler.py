@@ -655,11 +655,21 @@ TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 30        # numbered as GgmlType
 ROPE_LAYOUTS = {"interleaved": 0, "half": 1}
 ROPE_SCALINGS = {"none": 0, "linear": 1, "yarn": 2}
 KV_NONE = 0xFFFFFFFF
-_TYPES = {"torch.float32": TYPE_F32, "torch.float16": TYPE_F16, "torch.bfloat16": TYPE_BF16}
+_DT = None
+
+
+def _dtypes():
+    """torch's value types and what they are here, and its 4-byte integers."""
+    global _DT
+    if _DT is None:
+        import torch
+        _DT = ({torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}, (torch.int32, torch.uint32),
+               getattr(torch._C, "_cuda_getCurrentRawStream", None))
+    return _DT
 
 
 def _type(x, what):
-    t = _TYPES.get(str(x.dtype))
+    t = _dtypes()[0].get(x.dtype)
     if t is None:
         raise TypeError("%s must be float32, float16 or bfloat16" % what)
     return t
@@ -668,25 +678,37 @@ def _type(x, what):
 def _heads(x, what, heads=None, d=None):
     """(tokens, heads, d, values from token to token) of a [T, heads, d]
     tensor on the device whose heads are contiguous."""
-    if x.dim() != 3 or not x.is_cuda:
+    shape = x.shape
+    if len(shape) != 3 or not x.is_cuda:
         raise TypeError("%s must be a [tokens, heads, d] tensor on the device" % what)
-    T, h, n = x.shape
+    T, h, n = shape
     if (heads is not None and h != heads) or (d is not None and n != d):
         raise ValueError("%s has heads of another number or size" % what)
-    if (n > 1 and x.stride(2) != 1) or (h > 1 and x.stride(1) != n):
+    st, sh, sn = x.stride()
+    if (n > 1 and sn != 1) or (h > 1 and sh != n):
         raise TypeError("the heads of %s must be contiguous" % what)
-    return T, h, n, (x.stride(0) if T > 1 else h * n)
+    return T, h, n, (st if T > 1 else h * n)
 
 
 def _words(x, what, n=None):
-    """A contiguous device tensor of 4-byte integers (of n values), or None."""
+    """The address of a contiguous device tensor of 4-byte integers (of n values), or None."""
     if x is None:
         return None
-    if not getattr(x, "is_cuda", False) or x.element_size() != 4 or x.is_floating_point() or not x.is_contiguous():
+    if not getattr(x, "is_cuda", False) or x.dtype not in _dtypes()[1] or not x.is_contiguous():
         raise TypeError("%s must be a contiguous tensor of 4-byte integers on the device" % what)
     if n is not None and x.numel() != n:
         raise ValueError("%s must have %d values" % (what, n))
     return x.data_ptr()
+
+
+def _stream_of(x, stream):
+    """The HIP stream of a call on tensor x: `stream`, or the one that torch
+    works on now (_stream_handle, without a Stream object on the way)."""
+    if stream is None:
+        raw = _dtypes()[2]
+        if raw is not None:
+            return raw(x.get_device())
+    return _stream_handle(stream)
 
 
 class Rope:
@@ -722,7 +744,7 @@ class Rope:
         if T2 != T or out.dtype != x.dtype:
             raise ValueError("out must be as x")
         _check(self._lib.gs_rope_apply(self._h, _type(x, "x"), x.data_ptr(), ld, out.data_ptr(), ld_out, T, heads,
-                                       _words(pos, "pos", T), _stream_handle(stream)), "gs_rope_apply")
+                                       _words(pos, "pos", T), _stream_of(x, stream)), "gs_rope_apply")
         return out
 
     def close(self):
@@ -781,7 +803,7 @@ class KVCache:
         return c
 
     def reset(self, stream=None):
-        _check(self._lib.gs_kv_reset(self._c, _stream_handle(stream)), "gs_kv_reset")
+        _check(self._lib.gs_kv_reset(self._c, _stream_of(self.k, stream)), "gs_kv_reset")
 
     def extend(self, add, rows=None, status=None, stream=None):
         """Room for new tokens: `add` for each of `rows` (None: every row), a
@@ -789,17 +811,17 @@ class KVCache:
         n = self.rows if rows is None else rows.numel()
         each = isinstance(add, int)
         _check(self._lib.gs_kv_extend(self._c, _words(rows, "rows"), n, None if each else _words(add, "add", n),
-                                      add if each else 0, _words(status, "status", n), _stream_handle(stream)),
+                                      add if each else 0, _words(status, "status", n), _stream_of(self.k, stream)),
                "gs_kv_extend")
 
     def fork(self, src, dst, status=None, stream=None):
         """Rows dst become copies of rows src, sharing their full pages (-1: empty)."""
         n = dst.numel()
         _check(self._lib.gs_kv_fork(self._c, _words(src, "src", n), _words(dst, "dst"), n, _words(status, "status", n),
-                                    _stream_handle(stream)), "gs_kv_fork")
+                                    _stream_of(self.k, stream)), "gs_kv_fork")
 
     def free(self, rows, stream=None):
-        _check(self._lib.gs_kv_free(self._c, _words(rows, "rows"), rows.numel(), _stream_handle(stream)), "gs_kv_free")
+        _check(self._lib.gs_kv_free(self._c, _words(rows, "rows"), rows.numel(), _stream_of(self.k, stream)), "gs_kv_free")
 
     def drop(self, start, end, rows, rope=None, status=None, stream=None):
         """Tokens start .. end - 1 of each of `rows` leave it (gs_kv_drop); with
@@ -807,7 +829,7 @@ class KVCache:
         n = rows.numel()
         _check(self._lib.gs_kv_drop(self._c, _words(rows, "rows"), n, _words(start, "start", n), _words(end, "end", n),
                                     None if rope is None else rope._h, _words(status, "status", n),
-                                    _stream_handle(stream)), "gs_kv_drop")
+                                    _stream_of(self.k, stream)), "gs_kv_drop")
 
     def _batch(self, T, rows, q_start):
         if q_start is None:
@@ -837,7 +859,7 @@ class KVCache:
             x.q_out_type, x.n_heads = _type(q_out, "q_out"), heads
         b = self._batch(T, rows, q_start)
         _check(self._lib.gs_kv_append(self._c, layer, ctypes.byref(b), None if rope is None else rope._h,
-                                      ctypes.byref(x), _stream_handle(stream)), "gs_kv_append")
+                                      ctypes.byref(x), _stream_of(self.k, stream)), "gs_kv_append")
 
     def attend(self, layer, q, out=None, rows=None, q_start=None, scale=0.0, window=0, max_q=0, stream=None):
         """Causal attention of the rows' newest tokens (as append takes them) over
@@ -851,7 +873,7 @@ class KVCache:
         To, _, _, ld_o = _heads(out, "out", heads, self.d)
         if To != T or out.dtype != q.dtype:
             raise ValueError("out must be as q")
-        st = _stream_handle(stream)
+        st = _stream_of(self.k, stream)
         ws = self._attn_ws.get((st, heads))         # calls on one stream do not overlap
         if ws is None:
             n = self._lib.gs_attn_workspace(self._c, heads)

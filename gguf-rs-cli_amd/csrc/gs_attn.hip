@@ -68,6 +68,14 @@ __device__ __forceinline__ Seq seq_of(const AttnArgs &a, uint32_t i)
     return s;
 }
 
+// The same value in a scalar register, where all lanes have it.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ uint64_t uniform(uint64_t x)
+{
+    return (uint64_t)uniform((uint32_t)(x >> 32)) << 32 | uniform((uint32_t)x);
+}
+__device__ __forceinline__ Seq uniform(const Seq &s) { return Seq{uniform(s.row), uniform(s.len), uniform(s.first), uniform(s.nq)}; }
+
 // The keys that rows r0 .. r1 - 1 of a sequence see, [lo, hi), and the first
 // tile; `tiles` is at least 1, so that rows without keys are written too.
 template <int kTile> struct Span {
@@ -82,13 +90,56 @@ template <int kTile> struct Span {
     }
 };
 
-template <int R, int kTile> __device__ __forceinline__ uint32_t tiles_of(const AttnArgs &a, const Seq &s)
-{
-    uint32_t t = 0;
-    const uint32_t rows = s.nq * a.group;
-    for (uint32_t r = 0; r < rows; r += R) t += Span<kTile>(a, s, r, min(r + R, rows)).tiles;
-    return t;
-}
+// How a kernel deals its work: R rows in a unit, kTile keys in a tile, and a
+// unit's beginning and end (its queries, the first keys' way, its rows' way
+// out), which are dealt as kSetup tiles before its first.
+template <int R_, int kTile_, int kSetup_> struct Deal {
+    static constexpr int R = R_, kTile = kTile_, kSetup = kSetup_;
+    // Tiles of the unit of rows r ..
+    static __device__ __forceinline__ uint32_t unit(const AttnArgs &a, const Seq &s, uint32_t r)
+    {
+        return Span<kTile>(a, s, r, min(r + R, s.nq * a.group)).tiles + kSetup;
+    }
+    // Tiles of a sequence and one head of keys, counted by a thread ..
+    static __device__ __forceinline__ uint32_t count(const AttnArgs &a, const Seq &s)
+    {
+        uint32_t t = 0;
+        for (uint32_t r = 0; r < s.nq * a.group; r += R) t += unit(a, s, r);
+        return t;
+    }
+    // .. and by a wave, its lanes side by side
+    static __device__ __forceinline__ uint32_t count_wave(const AttnArgs &a, const Seq &s)
+    {
+        uint32_t t = 0;
+        for (uint32_t r = (threadIdx.x & 63) * R; r < s.nq * a.group; r += 64 * R) t += unit(a, s, r);
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) t += __shfl_xor(t, o);
+        return t;
+    }
+    // The first row of the unit that tile `skip` of the sequence is in; skip
+    // becomes the tile's number in the unit.  (a wave)
+    static __device__ __forceinline__ uint32_t find(const AttnArgs &a, const Seq &s, uint32_t &skip)
+    {
+        const uint32_t rows = s.nq * a.group, lane = threadIdx.x & 63;
+        if (rows <= R) return 0;
+        for (uint32_t r = 0;; r += 64 * R) {
+            const uint32_t mine = r + lane * R < rows ? unit(a, s, r + lane * R) : 0;
+            uint32_t sum = mine;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const uint32_t y = __shfl_up(sum, o);
+                if (lane >= o) sum += y;
+            }
+            const uint64_t past = __ballot(sum > skip);
+            if (past) {
+                const int at = __ffsll((unsigned long long)past) - 1;
+                skip -= uniform(__shfl(sum - mine, at));
+                return r + at * R;
+            }
+            skip -= uniform(__shfl(sum, 63));
+        }
+    }
+};
 
 // a / b, by 32-bit division where that is enough (as it is for any call that
 // fits the memory; 64 bits are several times as many instructions).
@@ -116,21 +167,38 @@ __device__ __forceinline__ uint32_t run_with(const Run &r, uint64_t x)
 }
 
 // kLeast: tiles that a run has at least, if there are as many.
-template <int R, int kTile, int kThreads, int kLeast> __device__ __forceinline__ Run run_of(const AttnArgs &a, uint32_t g)
+template <class D, int kThreads, int kLeast> __device__ __forceinline__ Run run_of(const AttnArgs &a, uint32_t g)
 {
-    __shared__ uint64_t s_wave[kThreads / 64];
+    constexpr uint32_t kWaves = kThreads / 64, kShort = 32;     // up to kShort sequences are counted by waves: theirs may be long
+    __shared__ uint64_t s_wave[kWaves];
+    __shared__ uint32_t s_per[kShort];
+    __shared__ Seq s_seq[kShort];
     __shared__ Run s_run;
     const uint32_t each = (a.n + kThreads - 1) / kThreads;
     const uint32_t i0 = min(threadIdx.x * each, a.n), i1 = min(i0 + each, a.n);
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     Seq s = {};
     uint32_t per = 0;
     uint64_t mine = 0;
-    for (uint32_t i = i0; i < i1; i++) {
-        s = seq_of(a, i);
-        per = tiles_of<R, kTile>(a, s);
-        mine += (uint64_t)per * a.n_kv;
+    if (a.n <= kShort) {
+        for (uint32_t i = w; i < a.n; i += kWaves) {
+            s = seq_of(a, i);
+            per = D::count_wave(a, s);
+            if (lane == 0) { s_per[i] = per; s_seq[i] = s; }
+        }
+        __syncthreads();
+        if (threadIdx.x < a.n) {
+            s = s_seq[threadIdx.x];
+            per = s_per[threadIdx.x];
+            mine = (uint64_t)per * a.n_kv;
+        }
+    } else {
+        for (uint32_t i = i0; i < i1; i++) {
+            s = seq_of(a, i);
+            per = D::count(a, s);
+            mine += (uint64_t)per * a.n_kv;
+        }
     }
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     uint64_t x = mine;
     if (a.n > each) {                       // (one sequence: the first thread has it)
 #pragma unroll
@@ -145,13 +213,13 @@ template <int R, int kTile, int kThreads, int kLeast> __device__ __forceinline__
     Run r;
     r.total = 0;
 #pragma unroll
-    for (int i = 0; i < kThreads / 64; i++) {
+    for (int i = 0; i < (int)kWaves; i++) {
         if (i < w) before += s_wave[i];
         r.total += s_wave[i];
     }
     const uint64_t most = quotient(r.total + kLeast - 1, kLeast);
     r.n_wg = (uint32_t)min((uint64_t)a.n_wg, most);
-    if (g >= r.n_wg) { r.t0 = r.t1 = 0; return r; }
+    if (g >= uniform(r.n_wg)) { r.t0 = r.t1 = 0; return r; }
     const uint64_t q = quotient(r.total, r.n_wg), more = r.total - q * r.n_wg;
     r.t0 = g * q + min((uint64_t)g, more);
     r.t1 = r.t0 + q + (g < more);
@@ -160,7 +228,7 @@ template <int R, int kTile, int kThreads, int kLeast> __device__ __forceinline__
         if (each > 1)
             for (;; i++) {
                 s = seq_of(a, i);
-                per = tiles_of<R, kTile>(a, s);
+                per = D::count(a, s);
                 if (r.t0 < before + (uint64_t)per * a.n_kv) break;
                 before += (uint64_t)per * a.n_kv;
             }
@@ -168,7 +236,8 @@ template <int R, int kTile, int kThreads, int kLeast> __device__ __forceinline__
         s_run = r;
     }
     __syncthreads();
-    return s_run;
+    const Run u = s_run;
+    return Run{uniform(u.t0), uniform(u.t1), uniform(u.total), uniform(u.skip), uniform(u.n_wg), uniform(u.seq), uniform(u.per), uniform(u.s)};
 }
 
 // An infinity or NaN among 8 values.
@@ -215,7 +284,8 @@ __global__ void __launch_bounds__(256, D <= 128 && NT == 1 ? 2 : 1) attn_rows_ke
     __shared__ float s_o[4][16][D + 4];
     __shared__ float s_m[4][16], s_l[4][16];
 
-    Run run = run_of<R, kRowTile, 256, 1>(a, blockIdx.x);
+    using Dealt = Deal<R, kRowTile, 1>;
+    Run run = run_of<Dealt, 256, 1>(a, blockIdx.x);
     if (threadIdx.x == 0 && blockIdx.x < a.n_wg) a.cuts[blockIdx.x].last = 0;
     if (run.t0 >= run.t1) return;
 
@@ -225,23 +295,27 @@ __global__ void __launch_bounds__(256, D <= 128 && NT == 1 ? 2 : 1) attn_rows_ke
     const uint32_t d = FULL ? D : a.d;
     const size_t head = (size_t)d << a.shift;           // values of a head's page
 
-    uint32_t si = run.seq, per = run.per, r0 = 0;
+    uint32_t si = run.seq, r0;
+    const uint32_t per = run.per;
     Seq s = run.s;
     uint64_t t = run.t0;
     uint32_t kvh = (uint32_t)quotient(run.skip, per), skip = (uint32_t)(run.skip - (uint64_t)kvh * per);
+    r0 = Dealt::find(a, s, skip);
     while (t < run.t1) {
         const uint32_t rows = s.nq * a.group;
         if (kvh == a.n_kv || rows == 0) {               // the next sequence
-            si++;
-            s = seq_of(a, si);
-            per = tiles_of<R, kRowTile>(a, s);
-            kvh = 0; r0 = 0; skip = 0;
+            s = uniform(seq_of(a, ++si));
+            kvh = 0; r0 = 0;
             continue;
         }
         const uint32_t r1 = min(r0 + R, rows);
         const Span<kRowTile> span(a, s, r0, r1);
-        if (skip >= span.tiles) { skip -= span.tiles; r0 += R; continue; }
-        const uint32_t left = (uint32_t)min((uint64_t)(span.tiles - skip), run.t1 - t);
+        // the run's part of the unit, tiles first .. first + left - 1
+        const uint32_t dealt = span.tiles + Dealt::kSetup, part_of = (uint32_t)min((uint64_t)(dealt - skip), run.t1 - t);
+        const uint32_t first = max(skip, (uint32_t)Dealt::kSetup) - Dealt::kSetup;
+        const uint32_t left = max(skip + part_of, (uint32_t)Dealt::kSetup) - Dealt::kSetup - first;
+        if (left == 0) break;                           // (its setup only: the next run begins it)
+        const uint64_t end = t - skip + dealt;
 
         // ---- the keys.  Lane's K rows are in the page of key0 + 8 (m / 4), its V
         // rows in that of key0 + 8 g; the pages' numbers are read a tile ahead
@@ -278,7 +352,7 @@ __global__ void __launch_bounds__(256, D <= 128 && NT == 1 ? 2 : 1) attn_rows_ke
                 }
             }
         };
-        uint32_t key0 = (span.tile0 + skip) * kRowTile + 32 * w;
+        uint32_t key0 = (span.tile0 + first) * kRowTile + 32 * w;
         uint32_t kid = page_of(key0 + 8 * (m >> 2)), vid = page_of(key0 + 8 * g);
         uint32_t kid1 = page_of(key0 + kRowTile + 8 * (m >> 2)), vid1 = page_of(key0 + kRowTile + 8 * g);
         load_k(key0, kid);
@@ -422,6 +496,9 @@ __global__ void __launch_bounds__(256, D <= 128 && NT == 1 ? 2 : 1) attn_rows_ke
 #pragma unroll
                     for (int y = 0; y < 4; y++)
                         if (b >> (16 * y) & 0xffff) bad |= 1u << (8 * y + j);
+                    if (bad >> (8 * g + j) & 1)
+#pragma unroll
+                        for (int c = 0; c < NC; c++) vf[j][c] = vw{};
                 }
             }
             v8 pf[NT][NP];
@@ -436,51 +513,47 @@ __global__ void __launch_bounds__(256, D <= 128 && NT == 1 ? 2 : 1) attn_rows_ke
                         pf[nt][2][j] = (T)(y - (float)pf[nt][1][j]);
                     }
                 }
-            if (bad == 0) {
 #pragma unroll
-                for (int c = 0; c < NC; c++)
+            for (int c = 0; c < NC; c++)
 #pragma unroll
-                    for (int i = 0; i < CW; i++) {
-                        v8 x8;
+                for (int i = 0; i < CW; i++) {
+                    v8 x8;
 #pragma unroll
-                        for (int j = 0; j < 8; j++) x8[j] = vf[j][c][i];
+                    for (int j = 0; j < 8; j++) x8[j] = vf[j][c][i];
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++)
+                    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                            for (int q = NP - 1; q >= 0; q--) o[nt][c][i] = mfma(x8, pf[nt][q], o[nt][c][i]);
-                    }
-            } else {
-                uint32_t keep = ~bad;               // the keys of this pass
-                for (;;) {
-                    const int64_t key = (int64_t)key0 + __ffs(keep) - 1;
+                        for (int q = NP - 1; q >= 0; q--) o[nt][c][i] = mfma(x8, pf[nt][q], o[nt][c][i]);
+                }
+            for (; bad; bad &= bad - 1) {
+                const uint32_t y = __ffs(bad) - 1;
+                const int64_t key = (int64_t)key0 + y;
+                const T *row = (const T *)a.v + place(page_of(key0 + y)) + (size_t)((key0 + y) & (page - 1)) * d;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    float wt = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        if (j == (int)(y & 7)) wt = p[nt][j];
+                    wt = __shfl(wt, (y >> 3) * 16 + m);         // (the lane that has the key)
+                    if (key > pos[nt] || key <= pos[nt] - (int64_t)a.window) continue;
 #pragma unroll
                     for (int c = 0; c < NC; c++)
 #pragma unroll
-                        for (int i = 0; i < CW; i++) {
-                            v8 x8;
+                        for (int i = 0; i < CW; i++)
 #pragma unroll
-                            for (int j = 0; j < 8; j++) x8[j] = keep >> (8 * g + j) & 1 ? vf[j][c][i] : (T)0.0f;
-#pragma unroll
-                            for (int nt = 0; nt < NT; nt++) {
-                                f4 y = o[nt][c][i];
-#pragma unroll
-                                for (int q = NP - 1; q >= 0; q--) y = mfma(x8, pf[nt][q], y);
-                                const bool sees = keep == ~bad || (key <= pos[nt] && key > pos[nt] - (int64_t)a.window);
-#pragma unroll
-                                for (int e = 0; e < 4; e++) o[nt][c][i][e] = sees ? y[e] : o[nt][c][i][e];
+                            for (int e = 0; e < 4; e++) {
+                                const uint32_t dv = 16 * CW * c + CW * (4 * g + e) + i;
+                                if (dv < d) o[nt][c][i][e] += wt * (float)row[dv];
                             }
-                        }
-                    const uint32_t rest = keep == ~bad ? bad : bad & ~(keep | (keep - 1));
-                    if (rest == 0) break;
-                    keep = rest & -rest;
                 }
             }
             if (more) load_v(key0 + kRowTile, vid);
         }
 
         // ---- the waves' sums together; the unit's rows or its part
-        const bool whole = skip == 0 && left == span.tiles;
-        float *part = a.parts + (size_t)(2 * blockIdx.x + (skip == 0)) * R * (D + 2);
+        const bool whole = left == span.tiles;
+        float *part = a.parts + (size_t)(2 * blockIdx.x + (first == 0)) * R * (D + 2);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
             float l = sum[nt];
@@ -528,14 +601,14 @@ __global__ void __launch_bounds__(256, D <= 128 && NT == 1 ? 2 : 1) attn_rows_ke
                 }
             }
         }
-        if (!whole && skip == 0 && threadIdx.x == 0) {
+        if (!whole && first == 0 && threadIdx.x == 0) {
             Cut c;
-            c.last = run_with(run, t + span.tiles - 1);
+            c.last = run_with(run, end - 1);
             c.first_token = s.first; c.row0 = r0; c.rows = r1 - r0; c.kvh = kvh;
             c.keyless = s.nq > s.len ? (s.nq - s.len) * a.group : 0;
             a.cuts[blockIdx.x] = c;
         }
-        t += left;
+        t += part_of;
         skip = 0;
         r0 += R;
         if (r0 >= rows) { r0 = 0; kvh++; }
@@ -548,11 +621,19 @@ typedef short s4v __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ f16v mfma(h8 a, h8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f16v mfma(b8 a, b8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 
+// The largest of a lane's value and that of the lane 32 away.
+__device__ __forceinline__ float max_halves(float x)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 // The shape of the kernel below for heads of D: waves, keys of a tile.
 template <int D> struct Chunk {
     static constexpr int kWaves = D == 256 ? 4 : 8, kTile = D == 256 ? 32 : 64;
     static constexpr int kRows = 32 * kWaves, kThreads = 64 * kWaves;
 };
+constexpr int kChunkRuns = 256;         // one workgroup per CU
 
 // Chunks of many query rows: what bounds it is the matrix cores and, beside
 // them, the exponentials.  A wave has 32 query rows, and all waves share the
@@ -568,7 +649,7 @@ template <int D> struct Chunk {
 // sums are seldom scaled: the weights then reach 2^8, which f32 sums and the
 // type's range (f16: 2^7 is the lift here) take without loss.
 template <class T, int D, bool FULL>
-__global__ void __launch_bounds__(Chunk<D>::kThreads) attn_chunk_kernel(const AttnArgs a)
+__global__ void __launch_bounds__(Chunk<D>::kThreads, D == 256 ? 1 : 2) attn_chunk_kernel(const AttnArgs a)
 {
     constexpr int R = Chunk<D>::kRows, kTile = Chunk<D>::kTile, kThreads = Chunk<D>::kThreads;
     constexpr int C = D / 8, KP = kTile * C / kThreads;         // 16-byte pieces of a row; pieces of a thread
@@ -580,7 +661,8 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads) attn_chunk_kernel(const At
 
     // runs that follow one another, which read the same keys, on one XCD
     const uint32_t g8 = a.n_wg / 8, run_id = a.n_wg % 8 ? blockIdx.x : (blockIdx.x & 7) * g8 + (blockIdx.x >> 3);
-    Run run = run_of<R, kTile, kThreads, 4>(a, run_id);
+    using Dealt = Deal<R, kTile, 3>;
+    Run run = run_of<Dealt, kThreads, 4>(a, run_id);
     if (threadIdx.x == 0) a.cuts[run_id].last = 0;
     if (run.t0 >= run.t1) return;
 
@@ -598,23 +680,27 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads) attn_chunk_kernel(const At
     auto swap_v = [](int row, int c) { return C == 8 ? c ^ (row >> 1 & 1) << 2 : c ^ (row & 3) << 2; };
     const bool inside = 8 * pc < (int)a.d;
 
-    uint32_t si = run.seq, per = run.per, r0 = 0;
+    uint32_t si = run.seq, r0;
+    const uint32_t per = run.per;
     Seq s = run.s;
     uint64_t t = run.t0;
     uint32_t kvh = (uint32_t)quotient(run.skip, per), skip = (uint32_t)(run.skip - (uint64_t)kvh * per);
+    r0 = Dealt::find(a, s, skip);
     while (t < run.t1) {
         const uint32_t rows = s.nq * a.group;
         if (kvh == a.n_kv || rows == 0) {               // the next sequence
-            si++;
-            s = seq_of(a, si);
-            per = tiles_of<R, kTile>(a, s);
-            kvh = 0; r0 = 0; skip = 0;
+            s = uniform(seq_of(a, ++si));
+            kvh = 0; r0 = 0;
             continue;
         }
         const uint32_t r1 = min(r0 + R, rows);
         const Span<kTile> span(a, s, r0, r1);
-        if (skip >= span.tiles) { skip -= span.tiles; r0 += R; continue; }
-        const uint32_t left = (uint32_t)min((uint64_t)(span.tiles - skip), run.t1 - t);
+        // the run's part of the unit, tiles first .. first + left - 1
+        const uint32_t dealt = span.tiles + Dealt::kSetup, part_of = (uint32_t)min((uint64_t)(dealt - skip), run.t1 - t);
+        const uint32_t first = max(skip, (uint32_t)Dealt::kSetup) - Dealt::kSetup;
+        const uint32_t left = max(skip + part_of, (uint32_t)Dealt::kSetup) - Dealt::kSetup - first;
+        if (left == 0) break;                           // (its setup only: the next run begins it)
+        const uint64_t end = t - skip + dealt;
         const int base = (int)s.len - (int)s.nq;        // position of the sequence's first token
 
         // ---- queries: row col of the wave's 32, values 16 s + 8 hf ..
@@ -622,15 +708,11 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads) attn_chunk_kernel(const At
         const bool rows_here = w0 < r1;
         const uint32_t mine = min(w0 + col, r1 - 1), tok = mine / a.group, hq = kvh * a.group + (mine - tok * a.group);
         const int pos = base + (int)tok;
+        // the wave's first and last row: positions, and the first keys they see
         const int pos0 = base + (int)(min(w0, r1 - 1) / a.group), pos1 = base + (int)(min(w0 + 31, r1 - 1) / a.group);
-        v8 qf[KS];
-        const T *q = (const T *)a.q + (size_t)(s.first + tok) * a.ld_q + (size_t)hq * d;
-#pragma unroll
-        for (int c = 0; c < KS; c++) {
-            v8 x = {};
-            if (16 * c + 8 * hf < (int)d) x = *(const v8 *)(q + 16 * c + 8 * hf);
-            qf[c] = a.scale < 0.0f ? -x : x;
-        }
+        auto first_of = [&](int p) { return (int)max((int64_t)0, (int64_t)p + 1 - (int64_t)a.window); };
+        const int lo = first_of(pos), lo0 = first_of(pos0), lo1 = first_of(pos1);
+        const int unit_pos0 = base + (int)(r0 / a.group), unit_lo1 = first_of(base + (int)((r1 - 1) / a.group));
 
         // ---- a tile's pieces
         const uint32_t *table = a.table + (size_t)min(s.row, a.n_rows - 1) * a.ld_table;
@@ -657,9 +739,7 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads) attn_chunk_kernel(const At
         // those of keys that some rows only see if an infinity or a NaN is
         // among them; s_bad says which (bit: the key of the tile).
         auto put = [&](uint32_t key0, int b, int bs) {
-            const bool edge = key0 + kTile > (uint32_t)max(0, base + (int)(r0 / a.group) + 1) ||
-                              (int64_t)key0 < (int64_t)base + (r1 - 1) / a.group + 1 - (int64_t)a.window;
-            if (edge) {
+            if ((int)key0 + kTile > unit_pos0 + 1 || (int)key0 < unit_lo1) {
                 uint64_t bad = 0;
 #pragma unroll
                 for (int i = 0; i < KP; i++) {
@@ -686,8 +766,17 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads) attn_chunk_kernel(const At
             for (int i = 0; i < 16; i++) o[c][i] = 0.0f;
         float mx = -INFINITY, sum = 0.0f;
 
-        uint32_t key0 = (span.tile0 + skip) * kTile;
+        uint32_t key0 = (span.tile0 + first) * kTile;
         pages(key0);
+        v8 qf[KS];
+        const T *q = (const T *)a.q + (size_t)(s.first + tok) * a.ld_q + (size_t)hq * d;
+#pragma unroll
+        for (int c = 0; c < KS; c++) {
+            v8 x = {};
+            if (16 * c + 8 * hf < (int)d) x = *(const v8 *)(q + 16 * c + 8 * hf);
+            qf[c] = a.scale < 0.0f ? -x : x;
+        }
+
         fetch(key0);
         pages(key0 + kTile);
         __syncthreads();                                // (the last unit's tiles are read)
@@ -703,86 +792,150 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads) attn_chunk_kernel(const At
                 fetch(key0 + kTile);
                 pages(key0 + 2 * kTile);
             }
-            if (rows_here && (int)key0 <= pos1 && (int64_t)key0 + kTile > (int64_t)pos0 + 1 - (int64_t)a.window) {
+            if (rows_here && (int)key0 <= pos1 && (int)key0 + kTile > lo0) {
+                // Each group of reads from LDS is under way while the products of
+                // the group before it run; the compiler would put every read
+                // right before its use.
+                constexpr int kGroup = 4, kGroups = KS / kGroup, kCols = DT < 4 ? DT : 4;
                 f16v z[KT];
+                v8 pf[KT][2], kf[2][kGroup], vf[2][kCols];
+                auto read_k = [&](int y, int gr) {      // 32 keys, 64 values
 #pragma unroll
-                for (int y = 0; y < KT; y++) {
+                    for (int c = 0; c < kGroup; c++)
+                        kf[(y * kGroups + gr) & 1][c] = *(const v8 *)&s_k[b][(32 * y + col) * D + 8 * swap_k(col, 2 * (gr * kGroup + c) + hf)];
+                };
+                constexpr int kParts = DT / kCols;      // of a step of 16 keys
+                auto read_v = [&](int x) {              // 16 keys, 32 kCols values
+                    const int y = x / kParts, c0 = x % kParts * kCols;
 #pragma unroll
-                    for (int i = 0; i < 16; i++) z[y][i] = 0.0f;
+                    for (int c = 0; c < kCols; c++) {
+                        const int row = 4 * hf + (l16 >> 2), piece = 4 * (c0 + c) + 2 * (lane >> 4 & 1) + (l16 >> 1 & 1);
+                        union { s4v half[2]; v8 all; } u;
 #pragma unroll
-                    for (int c = 0; c < KS; c++) {
-                        const int row = 32 * y + col;
-                        const v8 kf = *(const v8 *)&s_k[b][row * D + 8 * swap_k(row, 2 * c + hf)];
-                        z[y] = mfma(kf, qf[c], z[y]);
+                        for (int e = 0; e < 2; e++) {
+                            T *at = &s_v[b][(16 * y + row + 8 * e) * D + 8 * swap_v(row, piece) + 4 * (l16 & 1)];
+                            u.half[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v *)at);
+                        }
+                        vf[x & 1][c] = u.all;
                     }
-                }
-                const bool edge = (int)(key0 + kTile) > pos0 + 1 || (int64_t)key0 < (int64_t)pos1 + 1 - (int64_t)a.window;
-                // the keys of z[y][i]: key0 + 32 y + 8 (i / 4) + 4 hf + i % 4
-                const int lo = (int)max((int64_t)0, (int64_t)pos + 1 - (int64_t)a.window);
-                if (edge) {
+                };
+                auto score = [&](int y, int gr) {       // the products of a group
 #pragma unroll
-                    for (int y = 0; y < KT; y++)
+                    for (int c = 0; c < kGroup; c++) z[y] = mfma(kf[(y * kGroups + gr) & 1][c], qf[gr * kGroup + c], z[y]);
+                };
+                float by = 1.0f;
+                bool moved = false;
+                // the maximum over 32 keys: z[y][i] is key 32 y + 8 (i / 4) + 4 hf + i % 4
+                const bool edge = (int)key0 + kTile > pos0 + 1 || (int)key0 < lo1;
+                auto raise = [&](int y) {
+                    if (edge) {
+                        const int up = pos - (int)key0 - 4 * hf - 32 * y, down = lo - (int)key0 - 4 * hf - 32 * y;
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
-                            const int key = (int)key0 + 32 * y + 8 * (i >> 2) + 4 * hf + (i & 3);
-                            if (key > pos || key < lo) z[y][i] = -INFINITY;
+                            const int key = 8 * (i >> 2) + (i & 3);
+                            if (key > up || key < down) z[y][i] = -INFINITY;
                         }
-                }
-                float top = z[0][0];
+                    }
+                    float top = z[y][0];
 #pragma unroll
-                for (int y = 0; y < KT; y++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) top = fmaxf(top, z[y][i]);
-                top = fmaxf(top, __shfl_xor(top, 32)) * scale;
-                const bool raise = top > mx + kSlack;           // (each row by itself: its bits do not depend on its neighbours)
-                if (__any(raise)) {
-                    const float by = raise ? __builtin_amdgcn_exp2f(mx - top) : 1.0f;
-                    mx = raise ? top : mx;
-                    sum *= by;
+                    for (int i = 1; i < 16; i++) top = fmaxf(top, z[y][i]);
+                    top = max_halves(top) * scale;
+                    const bool up = top > mx + kSlack;  // (each row by itself: its bits do not depend on its neighbours)
+                    moved = __any(up);
+                    if (moved) {
+                        by = up ? __builtin_amdgcn_exp2f(mx - top) : 1.0f;
+                        mx = up ? top : mx;
+                        sum *= by;
+                    }
+                };
+                auto scale_o = [&] {
 #pragma unroll
                     for (int c = 0; c < DT; c++)
 #pragma unroll
                         for (int i = 0; i < 16; i++) o[c][i] *= by;
-                }
-                const float ref = mx == -INFINITY ? 0.0f : mx - kUp;
+                };
+                float ref;
+                auto weigh = [&](int y, int i0, int n) {        // the weights of n of the 16 scores, and their sum
+#pragma unroll
+                    for (int i = i0; i < i0 + n; i++) {
+                        const float x = __builtin_amdgcn_exp2f(fmaf(z[y][i], scale, -ref));
+                        sum += x;
+                        pf[y][i >> 3][i & 7] = (T)x;
+                    }
+                };
+                auto hold = [&](int y) {                // (computed here: else they are put off past the branch that follows)
+                    asm volatile("" : "+v"(pf[y][0]), "+v"(pf[y][1]), "+v"(sum));
+                };
 #pragma unroll
                 for (int y = 0; y < KT; y++)
 #pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        z[y][i] = __builtin_amdgcn_exp2f(fmaf(z[y][i], scale, -ref));
-                        sum += z[y][i];
+                    for (int i = 0; i < 16; i++) z[y][i] = 0.0f;
+                read_k(0, 0);
+#pragma unroll
+                for (int gr = 0; gr < kGroups; gr++) {
+                    if (gr + 1 < kGroups) read_k(0, gr + 1);
+                    else if (KT > 1) read_k(1, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                    score(0, gr);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                read_v(0);
+                raise(0);
+                if (moved) scale_o();
+                ref = mx == -INFINITY ? 0.0f : mx - kUp;
+                if constexpr (KT > 1) {
+                    // the second 32 keys' scores while the first's exponentials run
+#pragma unroll
+                    for (int gr = 0; gr < kGroups; gr++) {
+                        if (gr + 1 < kGroups) read_k(1, gr + 1);
+                        score(1, gr);
+                        weigh(0, gr * 16 / kGroups, 16 / kGroups);
                     }
 #pragma unroll
-                for (int c = 0; c < DT; c++)
-#pragma unroll
-                    for (int y = 0; y < 2 * KT; y++) {
-                        v8 pf;
-#pragma unroll
-                        for (int i = 0; i < 8; i++) pf[i] = (T)z[y >> 1][8 * (y & 1) + i];
-                        const int row = 16 * y + 4 * hf + (l16 >> 2), piece = 4 * c + 2 * (lane >> 4 & 1) + (l16 >> 1 & 1);
-                        union { s4v half[2]; v8 all; } u;
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            T *at = &s_v[b][(row + 8 * e) * D + 8 * swap_v(row + 8 * e, piece) + 4 * (l16 & 1)];
-                            u.half[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v *)at);
-                        }
-                        o[c] = mfma(u.all, pf, o[c]);
+                    for (int i = 0; i < 4 * kGroups; i++) {
+                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x002, 56 / (4 * kGroups), 0);
                     }
+                    hold(0);
+                    raise(1);
+                    ref = mx == -INFINITY ? 0.0f : mx - kUp;
+                    // and the first's values while the second's run
+#pragma unroll
+                    for (int x = 0; x < 2 * kParts; x++) {
+                        read_v(x + 1);
+#pragma unroll
+                        for (int c = 0; c < kCols; c++) o[x % kParts * kCols + c] = mfma(vf[x & 1][c], pf[0][x / kParts], o[x % kParts * kCols + c]);
+                        weigh(1, 16 / (2 * kParts) * x, 16 / (2 * kParts));
+                    }
+#pragma unroll
+                    for (int i = 0; i < 2 * DT; i++) {
+                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x002, 56 / (2 * DT), 0);
+                    }
+                    hold(1);
+                    if (moved) scale_o();
+                } else weigh(0, 0, 16);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int x = 2 * kParts * (KT - 1); x < 2 * kParts * KT; x++) {
+                    if (x + 1 < 2 * kParts * KT) read_v(x + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int c = 0; c < kCols; c++)
+                        o[x % kParts * kCols + c] = mfma(vf[x & 1][c], pf[KT - 1][x / kParts & 1], o[x % kParts * kCols + c]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
                 // The values that were put aside count for the rows that see them.
                 for (uint64_t bad = s_bad[bs]; bad; bad &= bad - 1) {
-                    const int y = __ffsll((unsigned long long)bad) - 1;
-                    const uint32_t key = key0 + y;
+                    const int y = __ffsll((unsigned long long)bad) - 1, at = 16 * (y >> 5) + (y & 3) + 4 * (y >> 3 & 3);   // (of the lane's weights)
+                    const uint32_t page = min(table[min(key0 + y, last) >> a.shift], a.n_pages - 1);
+                    const T *v = (const T *)a.v + ((size_t)page * a.n_kv + kvh) * head + (size_t)((key0 + y) & slot) * d;
                     float wt = 0.0f;
 #pragma unroll
-                    for (int z0 = 0; z0 < KT; z0++)
-#pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const float v = __shfl(z[z0][i], ((y >> 2 & 1) << 5) + col);
-                            if (z0 == y >> 5 && i == (y & 3) + 4 * (y >> 3 & 3)) wt = v;
-                        }
-                    if ((int)key > pos || (int)key < lo) continue;
-                    const uint32_t page = min(table[min(key, last) >> a.shift], a.n_pages - 1);
-                    const T *v = (const T *)a.v + ((size_t)page * a.n_kv + kvh) * head + (size_t)(key & slot) * d;
+                    for (int i = 0; i < 16 * KT; i++)
+                        if (i == at) wt = (float)pf[i >> 4][i >> 3 & 1][i & 7];
+                    wt = __shfl(wt, ((y >> 2 & 1) << 5) + col);         // (the half that has the key)
+                    if ((int)key0 + y > pos || (int)key0 + y < lo) continue;
 #pragma unroll
                     for (int c = 0; c < DT; c++)
 #pragma unroll
@@ -803,7 +956,7 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads) attn_chunk_kernel(const At
         }
 
         // ---- the unit's rows, or its part
-        const bool whole = skip == 0 && left == span.tiles;
+        const bool whole = left == span.tiles;
         sum += __shfl_xor(sum, 32);
         if (w0 + col < r1) {
             if (whole) {
@@ -822,7 +975,7 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads) attn_chunk_kernel(const At
                         }
                     }
             } else {
-                float *part = a.parts + (size_t)(2 * run_id + (skip == 0)) * R * (D + 2);
+                float *part = a.parts + (size_t)(2 * run_id + (first == 0)) * R * (D + 2);
                 const int rr = 32 * w + col;
                 if (hf == 0) { part[R * D + rr] = mx; part[R * D + R + rr] = sum; }
 #pragma unroll
@@ -833,14 +986,14 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads) attn_chunk_kernel(const At
                             f4{o[c][4 * i], o[c][4 * i + 1], o[c][4 * i + 2], o[c][4 * i + 3]};
             }
         }
-        if (!whole && skip == 0 && threadIdx.x == 0) {
+        if (!whole && first == 0 && threadIdx.x == 0) {
             Cut c;
-            c.last = run_with(run, t + span.tiles - 1);
+            c.last = run_with(run, end - 1);
             c.first_token = s.first; c.row0 = r0; c.rows = r1 - r0; c.kvh = kvh;
             c.keyless = s.nq > s.len ? (s.nq - s.len) * a.group : 0;
             a.cuts[run_id] = c;
         }
-        t += left;
+        t += part_of;
         skip = 0;
         r0 += R;
         if (r0 >= rows) { r0 = 0; kvh++; }
@@ -909,7 +1062,6 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a)
 namespace {
 
 constexpr uint32_t kRuns = 512;         // of the rows kernel: two workgroups per CU
-constexpr uint32_t kChunkRuns = 256;    // of the chunk kernel: one per CU
 
 int padded(uint32_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
@@ -935,8 +1087,8 @@ template <class T, int D, int NT, bool F32> int rows_call(gs::AttnArgs a, hipStr
 
 template <class T, int D> int chunk_call(gs::AttnArgs a, hipStream_t st)
 {
-    a.n_wg = kChunkRuns;
-    const dim3 grid(kChunkRuns), block(gs::Chunk<D>::kThreads);
+    a.n_wg = gs::kChunkRuns;
+    const dim3 grid(a.n_wg), block(gs::Chunk<D>::kThreads);
     if (a.d == D) hipLaunchKernelGGL((gs::attn_chunk_kernel<T, D, true>), grid, block, 0, st, a);
     else hipLaunchKernelGGL((gs::attn_chunk_kernel<T, D, false>), grid, block, 0, st, a);
     return join<T, D, gs::Chunk<D>::kRows>(a, st);
@@ -956,6 +1108,7 @@ template <class T, int D, bool F32> int by_rows(gs::AttnArgs &a, uint64_t rows, 
             if (rows <= 32) return rows_call<T, D, 2, F32>(a, st);
         // Sequences of a few rows go to the first kernel, the others to the second.
         constexpr int kFew = D == 256 ? 16 : 32;
+        if ((uint64_t)a.n_tokens * a.group == rows * a.n) return chunk_call<T, D>(a, st);      // (all of the same length, or the caller's most is wrong)
         a.max_rows = kFew;
         if (int rc = rows_call<T, D, kFew / 16, F32>(a, st)) return rc;
         a.min_rows = kFew + 1;
@@ -982,7 +1135,7 @@ size_t gs_attn_workspace(const gs_kv_cache *c, uint32_t n_heads)
     if (check_cache(c) || n_heads == 0 || n_heads % c->n_kv) return 0;
     // the larger of the two kernels': 32 rows in each of kRuns runs, or a chunk's in kChunkRuns
     const int D = padded(c->d);
-    const size_t few = parts_bytes(kRuns, 32, D), many = parts_bytes(kChunkRuns, D == 256 ? gs::Chunk<256>::kRows : gs::Chunk<128>::kRows, D);
+    const size_t few = parts_bytes(kRuns, 32, D), many = parts_bytes(gs::kChunkRuns, D == 256 ? gs::Chunk<256>::kRows : gs::Chunk<128>::kRows, D);
     return cuts_bytes() + (few > many ? few : many);
 }
 

@@ -628,10 +628,11 @@ __device__ __forceinline__ float max_halves(float x)
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// The shape of the kernel below for heads of D: waves, keys of a tile.
+// The shape of the kernel below for heads of D: eight waves of kM query rows
+// (heads of 256 take twice the registers of a row), keys of a tile.
 template <int D> struct Chunk {
-    static constexpr int kWaves = D == 256 ? 4 : 8, kTile = D == 256 ? 32 : 64;
-    static constexpr int kRows = 32 * kWaves, kThreads = 64 * kWaves;
+    static constexpr int kM = D == 256 ? 16 : 32, kTile = D == 256 ? 32 : 64;
+    static constexpr int kRows = 8 * kM, kThreads = 512;
 };
 constexpr int kChunkRuns = 256;         // one workgroup per CU
 
@@ -649,11 +650,14 @@ constexpr int kChunkRuns = 256;         // one workgroup per CU
 // sums are seldom scaled: the weights then reach 2^8, which f32 sums and the
 // type's range (f16: 2^7 is the lift here) take without loss.
 template <class T, int D, bool FULL>
-__global__ void __launch_bounds__(Chunk<D>::kThreads, D == 256 ? 1 : 2) attn_chunk_kernel(const AttnArgs a)
+__global__ void __launch_bounds__(Chunk<D>::kThreads, 2) attn_chunk_kernel(const AttnArgs a)
 {
     constexpr int R = Chunk<D>::kRows, kTile = Chunk<D>::kTile, kThreads = Chunk<D>::kThreads;
     constexpr int C = D / 8, KP = kTile * C / kThreads;         // 16-byte pieces of a row; pieces of a thread
-    constexpr int KT = kTile / 32, KS = D / 16, DT = D / 32;
+    constexpr int M = Chunk<D>::kM, KT = kTile / 32, DT = D / M;
+    constexpr int NA = M * M / 64, NZ = M / 2;                  // values of a lane: of a product, of the scores of 32 keys
+    constexpr int KF = D / 16;                                  // factors of 32 keys, of K and of V
+    using Acc = std::conditional_t<M == 32, f16v, f4>;
     constexpr float kUp = __is_same(T, _Float16) ? 7.0f : 0.0f, kSlack = 8.0f;
     typedef typename Vec<T>::v8 v8;
     __shared__ __align__(16) T s_k[2][kTile * D], s_v[2][kTile * D];
@@ -666,19 +670,22 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, D == 256 ? 1 : 2) attn_chu
     if (threadIdx.x == 0) a.cuts[run_id].last = 0;
     if (run.t0 >= run.t1) return;
 
-    const int lane = threadIdx.x & 63, hf = lane >> 5, col = lane & 31, l16 = lane & 15;
+    const int lane = threadIdx.x & 63, hg = lane / M, col = lane % M, l16 = lane & 15;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t slot = (1u << a.shift) - 1;
     const uint32_t d = FULL ? D : a.d;
     const size_t head = (size_t)d << a.shift;
     const float scale = fabsf(a.scale);
 
-    // this thread's pieces of a tile: rows prow + KP.., piece pc, and their places in LDS
+    // this thread's pieces of a tile: rows prow + kStep .., piece pc, and their places in LDS
     const int pc = threadIdx.x % C, prow = threadIdx.x / C;
     constexpr int kStep = kThreads / C;                         // rows from piece to piece
     auto swap_k = [](int row, int c) { return c ^ (row & (C < 16 ? C - 1 : 15)); };
-    auto swap_v = [](int row, int c) { return C == 8 ? c ^ (row >> 1 & 1) << 2 : c ^ (row & 3) << 2; };
-    const bool inside = 8 * pc < (int)a.d;
+    auto swap_v = [](int row, int c) { return C == 8 ? c ^ (row >> 1 & 1) << 2 : M == 32 ? c ^ (row & 3) << 2 : c ^ (row & 3) << 2 ^ (row >> 2 & 2); };
+    // What lane and place i stand for: a key of 32, a value of M
+    auto key_of = [&](int i) { return M == 32 ? 8 * (i >> 2) + 4 * hg + (i & 3) : 8 * hg + i; };
+    auto value_of = [&](int i) { return M == 32 ? 8 * (i >> 2) + 4 * hg + (i & 3) : 4 * hg + i; };
+    const bool inside = 8 * pc < (int)d;
 
     uint32_t si = run.seq, r0;
     const uint32_t per = run.per;
@@ -703,13 +710,13 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, D == 256 ? 1 : 2) attn_chu
         const uint64_t end = t - skip + dealt;
         const int base = (int)s.len - (int)s.nq;        // position of the sequence's first token
 
-        // ---- queries: row col of the wave's 32, values 16 s + 8 hf ..
-        const uint32_t w0 = r0 + 32 * w;
+        // ---- queries: row col of the wave's M
+        const uint32_t w0 = r0 + M * w;
         const bool rows_here = w0 < r1;
         const uint32_t mine = min(w0 + col, r1 - 1), tok = mine / a.group, hq = kvh * a.group + (mine - tok * a.group);
         const int pos = base + (int)tok;
         // the wave's first and last row: positions, and the first keys they see
-        const int pos0 = base + (int)(min(w0, r1 - 1) / a.group), pos1 = base + (int)(min(w0 + 31, r1 - 1) / a.group);
+        const int pos0 = base + (int)(min(w0, r1 - 1) / a.group), pos1 = base + (int)(min(w0 + M - 1, r1 - 1) / a.group);
         auto first_of = [&](int p) { return (int)max((int64_t)0, (int64_t)p + 1 - (int64_t)a.window); };
         const int lo = first_of(pos), lo0 = first_of(pos0), lo1 = first_of(pos1);
         const int unit_pos0 = base + (int)(r0 / a.group), unit_lo1 = first_of(base + (int)((r1 - 1) / a.group));
@@ -759,21 +766,22 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, D == 256 ? 1 : 2) attn_chu
             }
         };
 
-        f16v o[DT];
+        Acc o[DT];
 #pragma unroll
         for (int c = 0; c < DT; c++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) o[c][i] = 0.0f;
+            for (int i = 0; i < NA; i++) o[c][i] = 0.0f;
         float mx = -INFINITY, sum = 0.0f;
 
         uint32_t key0 = (span.tile0 + first) * kTile;
         pages(key0);
-        v8 qf[KS];
+        constexpr int QF = M == 32 ? KF : KF / 2, kWide = D / QF;       // factors of the queries, their values
+        v8 qf[QF];
         const T *q = (const T *)a.q + (size_t)(s.first + tok) * a.ld_q + (size_t)hq * d;
 #pragma unroll
-        for (int c = 0; c < KS; c++) {
+        for (int c = 0; c < QF; c++) {
             v8 x = {};
-            if (16 * c + 8 * hf < (int)d) x = *(const v8 *)(q + 16 * c + 8 * hf);
+            if (kWide * c + 8 * hg < (int)d) x = *(const v8 *)(q + kWide * c + 8 * hg);
             qf[c] = a.scale < 0.0f ? -x : x;
         }
 
@@ -796,50 +804,70 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, D == 256 ? 1 : 2) attn_chu
                 // Each group of reads from LDS is under way while the products of
                 // the group before it run; the compiler would put every read
                 // right before its use.
-                constexpr int kGroup = 4, kGroups = KS / kGroup, kCols = DT < 4 ? DT : 4;
-                f16v z[KT];
-                v8 pf[KT][2], kf[2][kGroup], vf[2][kCols];
-                auto read_k = [&](int y, int gr) {      // 32 keys, 64 values
+                constexpr int kGroups = KF / 4;         // of four factors
+                constexpr int NP = NZ / 8;
+                Acc z[KT][M == 32 ? 1 : 2];
+                v8 pf[KT][NP], kf[2][4], vf[2][4];
+                auto read_k = [&](int y, int gr) {      // of keys 32 y ..
 #pragma unroll
-                    for (int c = 0; c < kGroup; c++)
-                        kf[(y * kGroups + gr) & 1][c] = *(const v8 *)&s_k[b][(32 * y + col) * D + 8 * swap_k(col, 2 * (gr * kGroup + c) + hf)];
+                    for (int c = 0; c < 4; c++) {
+                        const int f = 4 * gr + c;
+                        const int row = M == 32 ? col : 8 * (col >> 2) + 4 * (f & 1) + (col & 3), piece = M == 32 ? 2 * f + hg : 4 * (f >> 1) + hg;
+                        kf[(y * kGroups + gr) & 1][c] = *(const v8 *)&s_k[b][(32 * y + row) * D + 8 * swap_k(row, piece)];
+                    }
                 };
-                constexpr int kParts = DT / kCols;      // of a step of 16 keys
-                auto read_v = [&](int x) {              // 16 keys, 32 kCols values
-                    const int y = x / kParts, c0 = x % kParts * kCols;
+                auto read_v = [&](int y, int gr) {
 #pragma unroll
-                    for (int c = 0; c < kCols; c++) {
-                        const int row = 4 * hf + (l16 >> 2), piece = 4 * (c0 + c) + 2 * (lane >> 4 & 1) + (l16 >> 1 & 1);
+                    for (int c = 0; c < 4; c++) {
+                        const int f = 4 * gr + c;       // M 32: 16 keys f / DT, values 32 (f % DT) ..; M 16: values 16 f ..
+                        const int row = (M == 32 ? 16 * (f / DT) + 4 * hg : 8 * hg) + (l16 >> 2);
+                        const int piece = M == 32 ? 4 * (f % DT) + 2 * (lane >> 4 & 1) + (l16 >> 1 & 1) : 2 * f + (l16 >> 1 & 1);
                         union { s4v half[2]; v8 all; } u;
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
-                            T *at = &s_v[b][(16 * y + row + 8 * e) * D + 8 * swap_v(row, piece) + 4 * (l16 & 1)];
+                            T *at = &s_v[b][(32 * y + row + (M == 32 ? 8 : 4) * e) * D + 8 * swap_v(row, piece) + 4 * (l16 & 1)];
                             u.half[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v *)at);
                         }
-                        vf[x & 1][c] = u.all;
+                        vf[(y * kGroups + gr) & 1][c] = u.all;
                     }
                 };
                 auto score = [&](int y, int gr) {       // the products of a group
 #pragma unroll
-                    for (int c = 0; c < kGroup; c++) z[y] = mfma(kf[(y * kGroups + gr) & 1][c], qf[gr * kGroup + c], z[y]);
+                    for (int c = 0; c < 4; c++) {
+                        const int f = 4 * gr + c, half = M == 32 ? 0 : f & 1;
+                        z[y][half] = mfma(kf[(y * kGroups + gr) & 1][c], qf[M == 32 ? f : f >> 1], z[y][half]);
+                    }
                 };
+                auto add_v = [&](int y, int gr) {
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        const int f = 4 * gr + c;
+                        o[f % DT] = mfma(vf[(y * kGroups + gr) & 1][c], pf[y][f / DT], o[f % DT]);
+                    }
+                };
+                auto score_of = [&](int y, int i) -> float { return z[y][i / NA][i % NA]; };
                 float by = 1.0f;
                 bool moved = false;
-                // the maximum over 32 keys: z[y][i] is key 32 y + 8 (i / 4) + 4 hf + i % 4
+                // the maximum over 32 keys
                 const bool edge = (int)key0 + kTile > pos0 + 1 || (int)key0 < lo1;
                 auto raise = [&](int y) {
                     if (edge) {
-                        const int up = pos - (int)key0 - 4 * hf - 32 * y, down = lo - (int)key0 - 4 * hf - 32 * y;
+                        const int up = pos - (int)key0 - 32 * y - key_of(0), down = lo - (int)key0 - 32 * y - key_of(0);
 #pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const int key = 8 * (i >> 2) + (i & 3);
-                            if (key > up || key < down) z[y][i] = -INFINITY;
+                        for (int i = 0; i < NZ; i++) {
+                            const int key = M == 32 ? 8 * (i >> 2) + (i & 3) : i;      // from the lane's first
+                            if (key > up || key < down) z[y][i / NA][i % NA] = -INFINITY;
                         }
                     }
-                    float top = z[y][0];
+                    float m[4];                         // (four short chains)
 #pragma unroll
-                    for (int i = 1; i < 16; i++) top = fmaxf(top, z[y][i]);
-                    top = max_halves(top) * scale;
+                    for (int i = 0; i < 4; i++) {
+                        m[i] = fmaxf(score_of(y, i), score_of(y, 4 + i));
+                        if constexpr (NZ == 16) m[i] = fmaxf(m[i], fmaxf(score_of(y, 8 + i), score_of(y, 12 + i)));
+                    }
+                    float top = max_halves(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
+                    if constexpr (M == 16) top = fmaxf(top, __shfl_xor(top, 16));
+                    top *= scale;
                     const bool up = top > mx + kSlack;  // (each row by itself: its bits do not depend on its neighbours)
                     moved = __any(up);
                     if (moved) {
@@ -852,24 +880,34 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, D == 256 ? 1 : 2) attn_chu
 #pragma unroll
                     for (int c = 0; c < DT; c++)
 #pragma unroll
-                        for (int i = 0; i < 16; i++) o[c][i] *= by;
+                        for (int i = 0; i < NA; i++) o[c][i] *= by;
                 };
                 float ref;
-                auto weigh = [&](int y, int i0, int n) {        // the weights of n of the 16 scores, and their sum
+                auto weigh = [&](int y, int i0, int n) {        // the weights of n scores, and their sum
 #pragma unroll
                     for (int i = i0; i < i0 + n; i++) {
-                        const float x = __builtin_amdgcn_exp2f(fmaf(z[y][i], scale, -ref));
+                        const float x = __builtin_amdgcn_exp2f(fmaf(score_of(y, i), scale, -ref));
                         sum += x;
                         pf[y][i >> 3][i & 7] = (T)x;
                     }
                 };
                 auto hold = [&](int y) {                // (computed here: else they are put off past the branch that follows)
-                    asm volatile("" : "+v"(pf[y][0]), "+v"(pf[y][1]), "+v"(sum));
+#pragma unroll
+                    for (int i = 0; i < NP; i++) asm volatile("" : "+v"(pf[y][i]));
+                    asm volatile("" : "+v"(sum));
+                };
+                // one product and its share of the exponentials in turn
+                auto in_turn = [&] {
+#pragma unroll
+                    for (int i = 0; i < KF; i++) {
+                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x002, NZ * 7 / 2 / KF, 0);
+                    }
                 };
 #pragma unroll
                 for (int y = 0; y < KT; y++)
 #pragma unroll
-                    for (int i = 0; i < 16; i++) z[y][i] = 0.0f;
+                    for (int i = 0; i < NZ; i++) z[y][i / NA][i % NA] = 0.0f;
                 read_k(0, 0);
 #pragma unroll
                 for (int gr = 0; gr < kGroups; gr++) {
@@ -879,7 +917,7 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, D == 256 ? 1 : 2) attn_chu
                     score(0, gr);
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                read_v(0);
+                read_v(0, 0);
                 raise(0);
                 if (moved) scale_o();
                 ref = mx == -INFINITY ? 0.0f : mx - kUp;
@@ -889,61 +927,54 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, D == 256 ? 1 : 2) attn_chu
                     for (int gr = 0; gr < kGroups; gr++) {
                         if (gr + 1 < kGroups) read_k(1, gr + 1);
                         score(1, gr);
-                        weigh(0, gr * 16 / kGroups, 16 / kGroups);
+                        weigh(0, gr * NZ / kGroups, NZ / kGroups);
                     }
-#pragma unroll
-                    for (int i = 0; i < 4 * kGroups; i++) {
-                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                        __builtin_amdgcn_sched_group_barrier(0x002, 56 / (4 * kGroups), 0);
-                    }
+                    in_turn();
                     hold(0);
                     raise(1);
                     ref = mx == -INFINITY ? 0.0f : mx - kUp;
                     // and the first's values while the second's run
 #pragma unroll
-                    for (int x = 0; x < 2 * kParts; x++) {
-                        read_v(x + 1);
-#pragma unroll
-                        for (int c = 0; c < kCols; c++) o[x % kParts * kCols + c] = mfma(vf[x & 1][c], pf[0][x / kParts], o[x % kParts * kCols + c]);
-                        weigh(1, 16 / (2 * kParts) * x, 16 / (2 * kParts));
+                    for (int gr = 0; gr < kGroups; gr++) {
+                        if (gr + 1 < kGroups) read_v(0, gr + 1);
+                        else read_v(1, 0);
+                        add_v(0, gr);
+                        weigh(1, gr * NZ / kGroups, NZ / kGroups);
                     }
-#pragma unroll
-                    for (int i = 0; i < 2 * DT; i++) {
-                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                        __builtin_amdgcn_sched_group_barrier(0x002, 56 / (2 * DT), 0);
-                    }
+                    in_turn();
                     hold(1);
                     if (moved) scale_o();
-                } else weigh(0, 0, 16);
+                } else weigh(0, 0, NZ);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int x = 2 * kParts * (KT - 1); x < 2 * kParts * KT; x++) {
-                    if (x + 1 < 2 * kParts * KT) read_v(x + 1);
+                for (int gr = 0; gr < kGroups; gr++) {
+                    if (gr + 1 < kGroups) read_v(KT - 1, gr + 1);
                     __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                    for (int c = 0; c < kCols; c++)
-                        o[x % kParts * kCols + c] = mfma(vf[x & 1][c], pf[KT - 1][x / kParts & 1], o[x % kParts * kCols + c]);
+                    add_v(KT - 1, gr);
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 // The values that were put aside count for the rows that see them.
-                for (uint64_t bad = s_bad[bs]; bad; bad &= bad - 1) {
-                    const int y = __ffsll((unsigned long long)bad) - 1, at = 16 * (y >> 5) + (y & 3) + 4 * (y >> 3 & 3);   // (of the lane's weights)
-                    const uint32_t page = min(table[min(key0 + y, last) >> a.shift], a.n_pages - 1);
-                    const T *v = (const T *)a.v + ((size_t)page * a.n_kv + kvh) * head + (size_t)((key0 + y) & slot) * d;
-                    float wt = 0.0f;
+                if ((int)key0 + kTile > unit_pos0 + 1 || (int)key0 < unit_lo1)
+                    for (uint64_t bad = s_bad[bs]; bad; bad &= bad - 1) {
+                        const int key = __ffsll((unsigned long long)bad) - 1, y = key & 31;
+                        // the place and the lane of its weight
+                        const int at = NZ * (key >> 5) + (M == 32 ? (y & 3) + 4 * (y >> 3) : y & 7), from = (M == 32 ? y >> 2 & 1 : y >> 3) * M + col;
+                        const uint32_t page = min(table[min(key0 + key, last) >> a.shift], a.n_pages - 1);
+                        const T *v = (const T *)a.v + ((size_t)page * a.n_kv + kvh) * head + (size_t)((key0 + key) & slot) * d;
+                        float wt = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 16 * KT; i++)
-                        if (i == at) wt = (float)pf[i >> 4][i >> 3 & 1][i & 7];
-                    wt = __shfl(wt, ((y >> 2 & 1) << 5) + col);         // (the half that has the key)
-                    if ((int)key0 + y > pos || (int)key0 + y < lo) continue;
+                        for (int i = 0; i < NZ * KT; i++)
+                            if (i == at) wt = (float)pf[i / NZ][i % NZ >> 3][i & 7];
+                        wt = __shfl(wt, from);
+                        if ((int)key0 + key > pos || (int)key0 + key < lo) continue;
 #pragma unroll
-                    for (int c = 0; c < DT; c++)
+                        for (int c = 0; c < DT; c++)
 #pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const int dv = 32 * c + 8 * (i >> 2) + 4 * hf + (i & 3);
-                            if (dv < (int)d) o[c][i] += wt * (float)v[dv];
-                        }
-                }
+                            for (int i = 0; i < NA; i++) {
+                                const int dv = M * c + value_of(i);
+                                if (dv < (int)d) o[c][i] += wt * (float)v[dv];
+                            }
+                    }
             }
             if (!more) break;
             // (s_bad of the tile before this was read before the last barrier,
@@ -958,6 +989,7 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, D == 256 ? 1 : 2) attn_chu
         // ---- the unit's rows, or its part
         const bool whole = left == span.tiles;
         sum += __shfl_xor(sum, 32);
+        if constexpr (M == 16) sum += __shfl_xor(sum, 16);
         if (w0 + col < r1) {
             if (whole) {
                 const float inv = pos < 0 ? 0.0f : 1.0f / sum;          // (no key: zeros)
@@ -966,8 +998,8 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, D == 256 ? 1 : 2) attn_chu
 #pragma unroll
                 for (int c = 0; c < DT; c++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int dv = 32 * c + 8 * i + 4 * hf;
+                    for (int i = 0; i < NA / 4; i++) {
+                        const int dv = M * c + value_of(4 * i);
                         if (dv < (int)d) {
                             f4 y = {o[c][4 * i], o[c][4 * i + 1], o[c][4 * i + 2], o[c][4 * i + 3]};
                             y *= inv;
@@ -976,13 +1008,13 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, D == 256 ? 1 : 2) attn_chu
                     }
             } else {
                 float *part = a.parts + (size_t)(2 * run_id + (first == 0)) * R * (D + 2);
-                const int rr = 32 * w + col;
-                if (hf == 0) { part[R * D + rr] = mx; part[R * D + R + rr] = sum; }
+                const int rr = M * w + col;
+                if (hg == 0) { part[R * D + rr] = mx; part[R * D + R + rr] = sum; }
 #pragma unroll
                 for (int c = 0; c < DT; c++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        *(f4 *)(part + (size_t)rr * D + 32 * c + 8 * i + 4 * hf) =
+                    for (int i = 0; i < NA / 4; i++)
+                        *(f4 *)(part + (size_t)rr * D + M * c + value_of(4 * i)) =
                             f4{o[c][4 * i], o[c][4 * i + 1], o[c][4 * i + 2], o[c][4 * i + 3]};
             }
         }

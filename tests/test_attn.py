@@ -195,6 +195,45 @@ def test_masked_values_do_not_count(gpu, torch, dtype, cache, news):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("d,H,kv", [(64, 4, 2), (80, 2, 1), (256, 6, 2)])
+@pytest.mark.parametrize("news,dtype", [([200, 40], "bfloat16"), ([3, 30], "float32")])
+def test_masked_values_of_other_heads(gpu, torch, d, H, kv, news, dtype):
+    """The same for the other sizes of heads, and with a window: values before
+    it and after a token leave its row as it is."""
+    lens, window = [500, 90], 60
+    c = build(gpu, torch, lens, kv, d, 16, "bfloat16", seed=7)
+    q = (torch.randn((sum(news), H, d), generator=torch.Generator("cuda").manual_seed(4), device="cuda")).to(getattr(torch, dtype))
+    start = starts(torch, news)
+    clean = c.attend(0, q, q_start=start, window=window)
+    at = {0: 440, 1: 70}
+    for r, t in at.items():
+        c.v[0, int(c.table[r, t // 16]), :, t % 16, d - 1] = math.nan
+        c.v[0, int(c.table[r, t // 16]), :, t % 16, 0] = math.inf
+    got = c.attend(0, q, q_start=start, window=window)
+    t = 0
+    for r, new in enumerate(news):
+        for i in range(new):
+            p = lens[r] - new + i
+            if p < at[r] or p - window >= at[r]:
+                assert torch.equal(got[t], clean[t]), (r, p)
+            else:
+                assert not bool(torch.isfinite(got[t][:, [0, d - 1]]).any()), (r, p)
+                assert bool(torch.isfinite(got[t][:, 1:d - 1]).all()), (r, p)
+            t += 1
+
+
+@pytest.mark.gpu
+def test_bits_do_not_depend_on_the_call(gpu, torch):
+    """A row's result over one run of its keys is the same bits whatever else is
+    in the call, as long as both fit one run."""
+    c = build(gpu, torch, [90, 60, 128], 2, 128, 16, "float16", seed=9)
+    q = torch.randn((3, 8, 128), generator=torch.Generator("cuda").manual_seed(5), device="cuda").half()
+    both = c.attend(0, q)
+    for r in range(3):
+        assert torch.equal(c.attend(0, q[r:r + 1], rows=words(torch, [r]))[0], both[r])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["float16", "float32"])
 def test_scores_far_apart(gpu, torch, dtype):
     """Weights over the whole range: one key far above the others, and rows

@@ -46,7 +46,8 @@ __device__ __forceinline__ uint32_t quotient(uint32_t n, uint32_t d, uint32_t m)
 // the half layout's turned values two each, rot / 2 apart), and two such items
 // at a time.  VEC: the pair form otherwise, for heads, parts or strides that
 // are not multiples of the vectors.
-template <class TI, class TO, class TC, bool VEC>
+// PAST: written past the caches.
+template <class TI, class TO, class TC, bool VEC, bool PAST>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a)
 {
     constexpr int kItems = 2, kW = VEC ? 8 : 1;
@@ -147,11 +148,11 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a)
             }
             if constexpr (VEC) {
                 if (yq[s]) {
-                    store8(yq[s] + p[s], u[s]);
-                    if (q[s] != p[s]) store8(yq[s] + q[s], w[s]);
+                    store8<PAST>(yq[s] + p[s], u[s]);
+                    if (q[s] != p[s]) store8<PAST>(yq[s] + q[s], w[s]);
                 } else {
-                    store8(yk[s] + p[s], u[s]);
-                    if (q[s] != p[s]) store8(yk[s] + q[s], w[s]);
+                    store8<PAST>(yk[s] + p[s], u[s]);
+                    if (q[s] != p[s]) store8<PAST>(yk[s] + q[s], w[s]);
                 }
             } else {
                 if (yq[s]) { yq[s][p[s]] = (TO)u[s][0]; yq[s][q[s]] = (TO)w[s][0]; }
@@ -170,7 +171,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a)
         if constexpr (VEC) {
             float u[8];
             load8(x + 8 * j, u);
-            store8(y + 8 * j, u);
+            store8<PAST>(y + 8 * j, u);
         } else {
             y[2 * j] = (TC)(float)x[2 * j];
             y[2 * j + 1] = (TC)(float)x[2 * j + 1];
@@ -222,8 +223,11 @@ int launch(RopeArgs &a, bool vec, hipStream_t st)
     a.by_token = over((uint32_t)per_token);
     a.by_v = over(a.per_v);
     a.by_vtoken = over(a.n_kv ? a.n_kv * a.per_v : 1);
-    if (vec) hipLaunchKernelGGL((gs::rope_kernel<TI, TO, TC, true>), dim3(blocks, y), dim3(gs::kRopeThreads), 0, st, a);
-    else hipLaunchKernelGGL((gs::rope_kernel<TI, TO, TC, false>), dim3(blocks, y), dim3(gs::kRopeThreads), 0, st, a);
+    const size_t written = (size_t)a.n_tokens * a.d * (a.n_heads * sizeof(TO) + 2 * a.n_kv * sizeof(TC));
+    const dim3 grid(blocks, y), block(gs::kRopeThreads);
+    if (!vec) hipLaunchKernelGGL((gs::rope_kernel<TI, TO, TC, false, false>), grid, block, 0, st, a);
+    else if (written > kPastCaches) hipLaunchKernelGGL((gs::rope_kernel<TI, TO, TC, true, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((gs::rope_kernel<TI, TO, TC, true, false>), grid, block, 0, st, a);
     return hipGetLastError() == hipSuccess ? GS_OK : GS_ERR_HIP;
 }
 

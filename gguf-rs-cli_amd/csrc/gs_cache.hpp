@@ -98,7 +98,7 @@ inline int check_cache(const gs_kv_cache *c)
     if (c->type != GS_TYPE_F16 && c->type != GS_TYPE_BF16) return GS_ERR_UNSUPPORTED;
     if (c->page_size < 16 || c->page_size > 1024 || (c->page_size & (c->page_size - 1))) return GS_ERR_UNSUPPORTED;
     if (c->d % 8 || c->d > GS_KV_MAX_HEAD) return GS_ERR_UNSUPPORTED;
-    if ((uint64_t)c->ld_table * c->page_size > 0x7fffffffull) return GS_ERR_UNSUPPORTED;
+    if ((uint64_t)c->ld_table * c->page_size > 1ull << 30) return GS_ERR_UNSUPPORTED;     // (positions are added to in 32 bits)
     if (c->n_kv > 4096 || c->n_layers > 65535 || c->n_pages > 0x7fffffffu || c->rows > 0x7fffffffu) return GS_ERR_UNSUPPORTED;
     return GS_OK;
 }

@@ -13,7 +13,9 @@
  *
  * All state is device memory that the caller owns, and every call is
  * asynchronous on its stream, allocates nothing and can be captured in a HIP
- * graph, as the calls of gs_decode.h.  Same status codes as gs_sampler.h.
+ * graph, as the calls of gs_decode.h.  Calls on one cache are ordered by the
+ * caller (one stream, or events between them): each reads what the last one
+ * wrote.  Same status codes as gs_sampler.h.
  */
 #ifndef GS_CACHE_H
 #define GS_CACHE_H
@@ -48,7 +50,7 @@ typedef struct gs_kv_cache {
     uint32_t page_size;     /* tokens of a page: a power of two, 16 to 1024 */
     uint32_t d;             /* values of a head: a multiple of 8, at most GS_KV_MAX_HEAD */
     uint32_t rows;
-    uint32_t ld_table;      /* most pages of a row; ld_table * page_size < 2^31 */
+    uint32_t ld_table;      /* most pages of a row; ld_table * page_size is at most 2^30 */
     uint32_t *table;        /* [rows][ld_table] */
     uint32_t *len;          /* [rows] tokens held */
     uint32_t *ref;          /* [n_pages] */

@@ -680,7 +680,7 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, 2) attn_chunk_kernel(const
     // this thread's pieces of a tile: rows prow + kStep .., piece pc, and their places in LDS
     const int pc = threadIdx.x % C, prow = threadIdx.x / C;
     constexpr int kStep = kThreads / C;                         // rows from piece to piece
-    auto swap_k = [](int row, int c) { return c ^ (row & (C < 16 ? C - 1 : 15)); };
+    auto swap_k = [](int row, int c) { return c ^ (M == 32 ? row & (C < 16 ? C - 1 : 15) : (row & 3) | (row >> 1 & 12)); };
     auto swap_v = [](int row, int c) { return C == 8 ? c ^ (row >> 1 & 1) << 2 : M == 32 ? c ^ (row & 3) << 2 : c ^ (row & 3) << 2 ^ (row >> 2 & 2); };
     // What lane and place i stand for: a key of 32, a value of M
     auto key_of = [&](int i) { return M == 32 ? 8 * (i >> 2) + 4 * hg + (i & 3) : 8 * hg + i; };

@@ -92,7 +92,10 @@ template <int kTile> struct Span {
 
 // How a kernel deals its work: R rows in a unit, kTile keys in a tile, and a
 // unit's beginning and end (its queries, the first keys' way, its rows' way
-// out), which are dealt as kSetup tiles before its first.
+// out), which are dealt as kSetup tiles before its first.  (us with 0, as it
+// is, twice as many: 16 prompts of 512, 28 / 4 heads of 128, kSetup 0, 3, 6:
+// 111, 92, 87; one of 2000, 32 / 8 heads, 3 and 6: 80, 84; 64 single tokens
+// over 1500, kSetup 0, 1, 2: 39.5, 39.2, 41.4.)
 template <int R_, int kTile_, int kSetup_> struct Deal {
     static constexpr int R = R_, kTile = kTile_, kSetup = kSetup_;
     // Tiles of the unit of rows r ..
@@ -166,7 +169,10 @@ __device__ __forceinline__ uint32_t run_with(const Run &r, uint64_t x)
     return (uint32_t)(x < more * (q + 1) ? quotient(x, q + 1) : more + quotient(x - more * (q + 1), q));
 }
 
-// kLeast: tiles that a run has at least, if there are as many.
+// kLeast: tiles that a run has at least, if there are as many: a shorter one
+// costs more to join than it saves.  (The chunk kernel, us with 4, 3, 2: 50
+// tokens over 4000, 32 / 8 heads of 128: 33.1, 32.7, 38.0; 300 over 300: 27.3,
+// 24.7, 24.7.)
 template <class D, int kThreads, int kLeast> __device__ __forceinline__ Run run_of(const AttnArgs &a, uint32_t g)
 {
     constexpr uint32_t kWaves = kThreads / 64, kShort = 32;     // up to kShort sequences are counted by waves: theirs may be long
@@ -270,6 +276,14 @@ constexpr int kRowTile = 128;           // keys of a tile: 32 for each wave
 // columns come from the 8 rows of V in a lane by a transposition of 8 x 8
 // values in registers (the value a lane's row m stands for is 8 m + i in
 // product i).  Four waves' sums meet in LDS at a unit's end.
+// The weights are rounded to T for the second product, as its factors have to
+// be: each is off by 2^-11 of itself (bf16: 2^-8) at most, without a common
+// direction, which is less than what the rounding of the result to T adds.
+// Their sum is of the unrounded ones, in f32.
+// Measured: 64 rows of 16000 tokens, 28 / 4 heads of 128, bf16: 353 us, 5.9
+// TB/s, what a read of this size reaches; one token over 4001: 10 us, of which
+// the empty launch, the search for the run's begin and three waits in a row
+// for memory (table, keys, values) are most.
 // F32: q in three parts of T whose sum is q (scaled by a power of two into
 // f16's range), and the weights too, so the products keep 24 bits.
 // FULL: heads of just D values (their strides are then constants, which takes
@@ -637,10 +651,11 @@ template <int D> struct Chunk {
 constexpr int kChunkRuns = 256;         // one workgroup per CU
 
 // Chunks of many query rows: what bounds it is the matrix cores and, beside
-// them, the exponentials.  A wave has 32 query rows, and all waves share the
+// them, the exponentials.  A wave has kM query rows, and all waves share the
 // tiles of K and V in LDS, two of each, so that the next tile's loads (through
 // registers) pass while this one is worked on: one barrier per tile.  The
-// products are S^T = K Q^T and O^T = V^T P^T again, 32 x 32 x 16: a lane has
+// products are S^T = K Q^T and O^T = V^T P^T again, 32 x 32 x 16 (heads of 256:
+// 16 x 16 x 32, as in the kernel above): a lane has
 // the scores of query row lane & 31 for keys 8 x + 4 (lane >> 5) + y, x and
 // y < 4, of 32, and gives them back, rounded, as the second product's factor;
 // V^T's side takes the same keys by transposing reads of LDS, 4 keys of one
@@ -648,7 +663,14 @@ constexpr int kChunkRuns = 256;         // one workgroup per CU
 // that neither reading order meets a bank twice.
 // The running maximum is raised only when a score passes it by 2^8, so the
 // sums are seldom scaled: the weights then reach 2^8, which f32 sums and the
-// type's range (f16: 2^7 is the lift here) take without loss.
+// type's range (f16: 2^7 is the lift here) take without loss.  They are rounded
+// to T as in the kernel above; the sum is of the unrounded ones.
+// Measured: four chunks of 2048 tokens over 8192, 32 / 8 heads of 128, f16: 710
+// to 880 TFLOP/s from card to card (a library product of 8192 x 8192 x 8192:
+// 1140), heads of 64 610, of 256 600 to 640.  No bank is met twice.  With 14 % fewer clocks per tile the
+// card lowered its frequency from 2.09 to 1.81 GHz and the time stayed: what
+// is left is power, of which each pass of keys and values through LDS for 32
+// rows is a part (64 rows of a wave do not fit its registers).
 template <class T, int D, bool FULL>
 __global__ void __launch_bounds__(Chunk<D>::kThreads, 2) attn_chunk_kernel(const AttnArgs a)
 {
@@ -666,7 +688,7 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, 2) attn_chunk_kernel(const
     // runs that follow one another, which read the same keys, on one XCD
     const uint32_t g8 = a.n_wg / 8, run_id = a.n_wg % 8 ? blockIdx.x : (blockIdx.x & 7) * g8 + (blockIdx.x >> 3);
     using Dealt = Deal<R, kTile, 3>;
-    Run run = run_of<Dealt, kThreads, 4>(a, run_id);
+    Run run = run_of<Dealt, kThreads, 3>(a, run_id);
     if (threadIdx.x == 0) a.cuts[run_id].last = 0;
     if (run.t0 >= run.t1) return;
 
@@ -1035,7 +1057,11 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, 2) attn_chunk_kernel(const
 // The parts of the unit that run blockIdx.x begins and another ends.  The
 // threads of a row (D / 4 of them, 4 values each) first share out its parts'
 // maximums and sums, up to kWide at a time, and then add the parts in order,
-// eight reads at a time: what bounds it is the chain of reads.
+// eight reads at a time: what bounds it is the chain of reads.  (One token over
+// 4001, 4 heads of keys: 4.7 us, an empty launch's 3.6 among them; four chunks
+// of 2048 over up to 8192: 18 us.  Joining in the first kernel by the last run
+// to come needs a release to the other XCDs by each run: 64 single tokens 206
+// us like this, 368 so.)
 template <class TO, int D, int R>
 __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a)
 {
@@ -1133,12 +1159,21 @@ template <class T, int D, bool F32> int by_rows(gs::AttnArgs &a, uint64_t rows, 
     a.max_rows = 0xffffffffu;
     if (rows <= 16) return rows_call<T, D, 1, F32>(a, st);
     if constexpr (F32) {
+        // f32 queries of any number go to the first kernel: its products are
+        // three for one, and four chunks of 512 tokens over 8192, 32 / 8 heads
+        // of 128, take 1250 us (640 TFLOP/s of products).
         if constexpr (D == 256) return rows_call<T, D, 1, F32>(a, st);      // (two tiles of rows spill)
         else return rows_call<T, D, 2, F32>(a, st);
     } else {
         if constexpr (D != 256)
             if (rows <= 32) return rows_call<T, D, 2, F32>(a, st);
-        // Sequences of a few rows go to the first kernel, the others to the second.
+        // Sequences of a few rows go to the first kernel, the others to the
+        // second.  (us, first and second; 64 sequences of 8000, 8 heads of keys:
+        // of 64, 32 rows: 184, 262; 48: 358, 289; of 128, 32 rows: 355, 378;
+        // 48: 697, 399; of 256, 16 rows: 687, 731; 24: 1361, 734.  Four of
+        // 4000, where the time is launches and waits: of 128, 16 rows: 23,
+        // 25; 32: 34, 26; of 256, 16: 42, 33: the lengths are on the device,
+        // so the rule is the large batch's.)
         constexpr int kFew = D == 256 ? 16 : 32;
         if ((uint64_t)a.n_tokens * a.group == rows * a.n) return chunk_call<T, D>(a, st);      // (all of the same length, or the caller's most is wrong)
         a.max_rows = kFew;

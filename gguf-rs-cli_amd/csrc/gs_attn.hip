@@ -266,6 +266,14 @@ template <class T> constexpr float kLift = __is_same(T, _Float16) ? 15.0f : 0.0f
 
 constexpr int kRowTile = 128;           // keys of a tile: 32 for each wave
 
+// Workgroups of the kernel below that a CU takes at a time, by their
+// registers, and so the runs that its work is dealt to: with twice as many the
+// second half begins when the first is done (us with 512 and 256 runs: 20
+// single tokens over 700 to 8192, 16 / 8 heads of 256, 88, 80; 16 sequences of
+// 8 over 500 to 4000, 32 / 8 heads of 128, 46, 35, and of 64, where two fit, 26,
+// 28).
+constexpr int rows_per_cu(int D, int NT) { return D == 64 || (D == 128 && NT == 1) ? 2 : 1; }
+
 // Up to 16 NT query rows against the keys, for single tokens and few of them:
 // what bounds it is the read of K and V, so each wave reads its 32 keys of a
 // tile straight to registers, once, K for the next tile while it works on
@@ -289,7 +297,7 @@ constexpr int kRowTile = 128;           // keys of a tile: 32 for each wave
 // FULL: heads of just D values (their strides are then constants, which takes
 // fewer registers and instructions).
 template <class T, int D, int NT, bool F32, bool FULL>
-__global__ void __launch_bounds__(256, D <= 128 && NT == 1 ? 2 : 1) attn_rows_kernel(const AttnArgs a)
+__global__ void __launch_bounds__(256, rows_per_cu(D, NT)) attn_rows_kernel(const AttnArgs a)
 {
     constexpr int R = 16 * NT, NP = F32 ? 3 : 1, KS = D / 32;
     constexpr int CW = D >= 128 ? 8 : D / 16, NC = D / (16 * CW);       // values of a lane's V chunk, chunks
@@ -1119,7 +1127,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a)
 
 namespace {
 
-constexpr uint32_t kRuns = 512;         // of the rows kernel: two workgroups per CU
+constexpr uint32_t kCUs = 256, kRuns = 2 * kCUs;        // runs at most
 
 int padded(uint32_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
@@ -1137,9 +1145,9 @@ template <class TO, int D, int R> int join(const gs::AttnArgs &a, hipStream_t st
 
 template <class T, int D, int NT, bool F32> int rows_call(gs::AttnArgs a, hipStream_t st)
 {
-    a.n_wg = kRuns;
-    if (a.d == D) hipLaunchKernelGGL((gs::attn_rows_kernel<T, D, NT, F32, true>), dim3(kRuns), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((gs::attn_rows_kernel<T, D, NT, F32, false>), dim3(kRuns), dim3(256), 0, st, a);
+    a.n_wg = kCUs * gs::rows_per_cu(D, NT);
+    if (a.d == D) hipLaunchKernelGGL((gs::attn_rows_kernel<T, D, NT, F32, true>), dim3(a.n_wg), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((gs::attn_rows_kernel<T, D, NT, F32, false>), dim3(a.n_wg), dim3(256), 0, st, a);
     return join<std::conditional_t<F32, float, T>, D, 16 * NT>(a, st);
 }
 

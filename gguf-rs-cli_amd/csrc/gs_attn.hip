@@ -1180,8 +1180,7 @@ template <class T, int D, bool F32> int by_rows(gs::AttnArgs &a, uint64_t rows, 
         // of 64, 32 rows: 184, 262; 48: 358, 289; of 128, 32 rows: 355, 378;
         // 48: 697, 399; of 256, 16 rows: 687, 731; 24: 1361, 734.  Four of
         // 4000, where the time is launches and waits: of 128, 16 rows: 23,
-        // 25; 32: 34, 26; of 256, 16: 42, 33: the lengths are on the device,
-        // so the rule is the large batch's.)
+        // 25; 32: 28, 26; of 256, 16: 35, 33.)
         constexpr int kFew = D == 256 ? 16 : 32;
         if ((uint64_t)a.n_tokens * a.group == rows * a.n) return chunk_call<T, D>(a, st);      // (all of the same length, or the caller's most is wrong)
         a.max_rows = kFew;

@@ -711,6 +711,21 @@ def _stream_of(x, stream):
     return _stream_handle(stream)
 
 
+def _empty_on(st, shape, dtype, like):
+    """A new tensor on like's device for work on the HIP stream st.  Memory that
+    torch's stream of the moment has freed may still be in use there: on
+    another stream the tensor comes from that one's memory."""
+    import torch
+    if st == _stream_of(like, None):
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    now = torch.cuda.current_stream(like.device)
+    on = torch.cuda.ExternalStream(st, like.device) if st else torch.cuda.default_stream(like.device)
+    with torch.cuda.stream(on):
+        x = torch.empty(shape, dtype=dtype, device=like.device)
+    x.record_stream(now)
+    return x
+
+
 class Rope:
     """The plan of a rotation (include/gs_rope.h): the first `rot` values of
     heads of d, in the "interleaved" or the "half" layout, with the scaling
@@ -869,17 +884,17 @@ class KVCache:
         sequence, if the caller knows it."""
         import torch
         T, heads, _, ld_q = _heads(q, "q", d=self.d)
-        out = torch.empty((T, heads, self.d), dtype=q.dtype, device=q.device) if out is None else out
+        st = _stream_of(self.k, stream)
+        out = _empty_on(st, (T, heads, self.d), q.dtype, q) if out is None else out
         To, _, _, ld_o = _heads(out, "out", heads, self.d)
         if To != T or out.dtype != q.dtype:
             raise ValueError("out must be as q")
-        st = _stream_of(self.k, stream)
         ws = self._attn_ws.get((st, heads))         # calls on one stream do not overlap
         if ws is None:
             n = self._lib.gs_attn_workspace(self._c, heads)
             if not n:
                 raise SamplerError(GS_ERR_INVALID, "gs_attn_workspace")
-            ws = self._attn_ws[st, heads] = torch.empty(n, dtype=torch.uint8, device=q.device)
+            ws = self._attn_ws[st, heads] = _empty_on(st, n, torch.uint8, q)
         b = self._batch(T, rows, q_start)
         a = GsAttnArgs(_type(q, "q"), heads, q.data_ptr(), ld_q, out.data_ptr(), ld_o, scale, window, max_q, ws.data_ptr(),
                        ws.numel())

@@ -361,3 +361,22 @@ def test_refusals_without_gpu():
     assert call(b=(65537, 65537, 4096, None)) == UNS
     assert call(b=(0, 0, None, 4096)) == gs.GS_OK
     assert lib.gs_attn(c, 0, None, None, None) == INV
+
+
+@pytest.mark.gpu
+def test_memory_of_another_stream(gpu, torch):
+    """What a call on a stream of its own allocates does not come from memory
+    that the stream of the moment has freed, where work may still use it."""
+    c = build(gpu, torch, [100, 31], 2, 64, 16, "float16", seed=9)
+    q = torch.randn((2, 4, 64), device="cuda")
+    here = c.attend(0, q)
+    n = next(iter(c._attn_ws.values())).numel()
+    torch.cuda.synchronize()
+    other = torch.cuda.Stream()
+    freed = [torch.empty(n, dtype=torch.uint8, device="cuda"), torch.empty_like(q)]
+    places = [x.data_ptr() for x in freed]
+    del freed
+    got = c.attend(0, q, stream=other)
+    torch.cuda.synchronize()
+    assert c._attn_ws[other.cuda_stream, 4].data_ptr() != places[0] and got.data_ptr() != places[1]
+    assert torch.equal(got, here)

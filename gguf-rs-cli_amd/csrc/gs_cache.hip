@@ -552,7 +552,7 @@ int check_call(const gs_kv_cache *c, size_t n)
 {
     if (int rc = check_cache(c)) return rc;
     if (!c->ws || ((uintptr_t)c->ws & 15u)) return GS_ERR_INVALID;
-    return n <= c->rows && n <= 65535 ? GS_OK : GS_ERR_INVALID;
+    return n <= c->rows && n <= 65535 ? GS_OK : GS_ERR_INVALID;     // (a grid's second and third sizes)
 }
 
 int launched() { return hipGetLastError() == hipSuccess ? GS_OK : GS_ERR_HIP; }
@@ -586,7 +586,8 @@ int gs_kv_reset(const gs_kv_cache *c, void *stream)
 int gs_kv_extend(const gs_kv_cache *c, const uint32_t *rows, size_t n, const uint32_t *add, uint32_t add_all,
                  int32_t *status, void *stream)
 {
-    if (int rc = check_call(c, n)) return rc;
+    if (int rc = check_call(c, 0)) return rc;
+    if (n > c->rows) return GS_ERR_INVALID;         // (one workgroup: any number of rows)
     if (n == 0) return GS_OK;
     hipLaunchKernelGGL(gs::extend_kernel, dim3(1), dim3(gs::kBook), 0, (hipStream_t)stream, device_cache(c), rows, (uint32_t)n,
                        add, add_all, status);

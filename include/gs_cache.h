@@ -60,6 +60,9 @@ typedef struct gs_kv_cache {
 /* Words of gs_kv_cache.ws (0 if the cache's sizes are out of range). */
 size_t gs_kv_workspace(const gs_kv_cache *c);
 
+/* The calls below take at most `rows` rows, and all but gs_kv_extend at most
+ * 65535. */
+
 /* Every row empty, every page free. */
 int gs_kv_reset(const gs_kv_cache *c, void *stream);
 

@@ -517,3 +517,16 @@ def test_refusals_without_gpu():
     assert append(type=30) == UNS                                         # not the cache's type
     assert append(type=1, q_out_type=0) == UNS
     assert append(b=(0, 0, None, 4096)) == gs.GS_OK
+
+
+@pytest.mark.gpu
+def test_extend_more_rows_than_a_grid_is_high(gpu, torch):
+    c = gpu.KVCache.empty(1, 70010, 1, 8, 70000, 32, page=16, dtype=torch.float16)
+    c.extend(3)
+    c.extend(2)
+    assert (c.len == 5).all() and (c.table[:, 1] == -1).all()
+    assert torch.equal(c.table[:, 0], torch.arange(70000, device="cuda", dtype=torch.int32))
+    assert c.ref.sum() == 70000 and (c.ref[70000:] == 0).all()
+    many = torch.zeros(65536, dtype=torch.int32, device="cuda")
+    with pytest.raises(gpu.SamplerError):
+        c.free(many)

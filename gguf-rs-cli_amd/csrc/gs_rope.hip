@@ -209,13 +209,14 @@ int launch(RopeArgs &a, bool vec, hipStream_t st)
     a.per_head = a.turned + (vec ? (a.d - a.rot) / 8 : (a.d - a.rot) / 2);
     a.per_v = vec ? a.d / 8 : a.d / 2;
     const uint64_t per_token = (uint64_t)(a.n_heads + a.n_kv) * a.per_head, items = per_token + (uint64_t)a.n_kv * a.per_v;
-    if (per_token > 65535) return GS_ERR_UNSUPPORTED;
+    if (per_token > 65535 || (uint64_t)a.n_kv * a.per_v > 65535) return GS_ERR_UNSUPPORTED;     // (quotient)
     // One token per workgroup until there are several workgroups per CU, then
     // four: with one, the angles and the places leave most lanes idle.  (us, one
     // and four, bf16: 1024 x 32 x 128 4.7, 6.4; 16384 x 32 x 128 40.6, 41.6; 16384
     // x 8 x 64 16.0, 8.5; 12001 x 32 x 96 28.8, 25.1; 4 x 2048 tokens written,
     // 16 / 2 heads of 64, 20.8, 11.4.)
-    // (quotient: 4 * 16384 * 16384 < 2^32)
+    // (quotient: values are twice the items of their keys at most, and
+    // 4 * 32768 * 32768 = 2^32)
     a.tokens = a.n_tokens >= 4096 && per_token <= 16384 ? gs::kRopeTokens : 1;
     const unsigned blocks = (a.n_tokens + a.tokens - 1) / a.tokens;
     // Few tokens: a token's items are spread over workgroups, each with one

@@ -530,3 +530,18 @@ def test_extend_more_rows_than_a_grid_is_high(gpu, torch):
     many = torch.zeros(65536, dtype=torch.int32, device="cuda")
     with pytest.raises(gpu.SamplerError):
         c.free(many)
+
+
+@pytest.mark.gpu
+def test_append_more_heads_than_counted(gpu, torch):
+    """Items of a token are counted in 16 bits: more of them are refused."""
+    for kv, fits in ((2047, True), (2048, False), (4095, False)):
+        c = gpu.KVCache.empty(1, 1, kv, 256, 1, 16, page=16, dtype=torch.float16)
+        c.extend(1)
+        k = torch.randn((1, kv, 256), device="cuda").half()
+        if fits:
+            c.append(0, k, k, rope=gpu.Rope(256, layout="half"))
+            assert torch.equal(c.v[0, 0, :, 0], k[0]) and torch.equal(c.k[0, 0, :, 0], k[0])
+        else:
+            with pytest.raises(gpu.SamplerError):
+                c.append(0, k, k, rope=gpu.Rope(256, layout="half"))

@@ -1062,7 +1062,7 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, 2) attn_chunk_kernel(const
     }
 }
 
-// The parts of the unit that run blockIdx.x begins and another ends.  The
+// The parts of the unit that run g begins and another ends.  The
 // threads of a row (D / 4 of them, 4 values each) first share out its parts'
 // maximums and sums, up to kWide at a time, and then add the parts in order,
 // eight reads at a time: what bounds it is the chain of reads.  (One token over
@@ -1070,18 +1070,17 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, 2) attn_chunk_kernel(const
 // of 2048 over up to 8192: 18 us.  Joining in the first kernel by the last run
 // to come needs a release to the other XCDs by each run: 64 single tokens 206
 // us like this, 368 so.)
-template <class TO, int D, int R>
-__global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a)
+template <class TO, int D, int R> __device__ __forceinline__ void join_unit(const AttnArgs &a, uint32_t g)
 {
-    const Cut c = a.cuts[blockIdx.x];
+    const Cut c = a.cuts[g];
     if (c.last == 0) return;
     constexpr int kCols = D / 4, kRows = 256 / kCols, kWide = kCols < 32 ? kCols : 32;
     const uint32_t rr = blockIdx.y * kRows + threadIdx.x / kCols, dv = 4 * (threadIdx.x % kCols), j = threadIdx.x % kWide;
     if (blockIdx.y * kRows >= c.rows) return;
     const uint32_t row = min(rr, c.rows - 1);           // (the threads of a row past the unit's help no one)
     constexpr size_t kPart = (size_t)R * (D + 2);
-    const uint32_t n = c.last - blockIdx.x + 1;         // part 0 is the run's second slot, the others their runs' first
-    const float *p0 = a.parts + (size_t)(2 * blockIdx.x) * kPart;
+    const uint32_t n = c.last - g + 1;                  // part 0 is the run's second slot, the others their runs' first
+    const float *p0 = a.parts + (size_t)(2 * g) * kPart;
     auto part = [&](uint32_t i) { return p0 + (i ? 2 * (size_t)i : 1) * kPart; };
     float top = -INFINITY;
     for (uint32_t i = j; i < n; i += kWide) top = fmaxf(top, part(i)[R * D + row]);
@@ -1123,6 +1122,19 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a)
     }
 }
 
+template <class TO, int D, int R>
+__global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) { join_unit<TO, D, R>(a, blockIdx.x); }
+
+// The parts of both kernels of a call that has sequences for each, in one
+// launch (a row of one token and one of 100, over up to 1000: 28.3 us with two,
+// 25.4; 24 rows over 700 to 8192, heads of 128: 220, 215).
+template <class TO, int D, int R, int R2>
+__global__ void __launch_bounds__(256) attn_join_both_kernel(const AttnArgs a, const AttnArgs b)
+{
+    if (blockIdx.x < a.n_wg) join_unit<TO, D, R>(a, blockIdx.x);
+    else join_unit<TO, D, R2>(b, blockIdx.x - a.n_wg);
+}
+
 } // namespace gs
 
 namespace {
@@ -1136,28 +1148,41 @@ size_t cuts_bytes() { return kRuns * ((sizeof(gs::Cut) + 15) / 16 * 16); }
 // Bytes of a kernel's parts with R rows in a unit.
 size_t parts_bytes(uint32_t runs, int R, int D) { return (size_t)2 * runs * R * (D + 2) * sizeof(float); }
 
+// Of the rows kernel's: 16 rows in each of kRuns runs, or 32 (of heads of 64 in
+// as many, of others in half of them).
+size_t few_bytes(int D) { return parts_bytes(kRuns, D == 64 ? 32 : 16, D); }
+
+template <int D, int R> dim3 join_grid(uint32_t runs)
+{
+    constexpr int kRows = 256 / (D / 4);        // of a workgroup
+    return dim3(runs, (R + kRows - 1) / kRows);
+}
+
 template <class TO, int D, int R> int join(const gs::AttnArgs &a, hipStream_t st)
 {
-    constexpr int kRows = 256 / (D / 4);
-    hipLaunchKernelGGL((gs::attn_join_kernel<TO, D, R>), dim3(a.n_wg, (R + kRows - 1) / kRows), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((gs::attn_join_kernel<TO, D, R>), (join_grid<D, R>(a.n_wg)), dim3(256), 0, st, a);
     return hipGetLastError() == hipSuccess ? GS_OK : GS_ERR_HIP;
 }
 
-template <class T, int D, int NT, bool F32> int rows_call(gs::AttnArgs a, hipStream_t st)
+template <class T, int D, int NT, bool F32> void rows_launch(gs::AttnArgs &a, hipStream_t st)
 {
     a.n_wg = kCUs * gs::rows_per_cu(D, NT);
     if (a.d == D) hipLaunchKernelGGL((gs::attn_rows_kernel<T, D, NT, F32, true>), dim3(a.n_wg), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((gs::attn_rows_kernel<T, D, NT, F32, false>), dim3(a.n_wg), dim3(256), 0, st, a);
+}
+
+template <class T, int D, int NT, bool F32> int rows_call(gs::AttnArgs &a, hipStream_t st)
+{
+    rows_launch<T, D, NT, F32>(a, st);
     return join<std::conditional_t<F32, float, T>, D, 16 * NT>(a, st);
 }
 
-template <class T, int D> int chunk_call(gs::AttnArgs a, hipStream_t st)
+template <class T, int D> void chunk_launch(gs::AttnArgs &a, hipStream_t st)
 {
     a.n_wg = gs::kChunkRuns;
     const dim3 grid(a.n_wg), block(gs::Chunk<D>::kThreads);
     if (a.d == D) hipLaunchKernelGGL((gs::attn_chunk_kernel<T, D, true>), grid, block, 0, st, a);
     else hipLaunchKernelGGL((gs::attn_chunk_kernel<T, D, false>), grid, block, 0, st, a);
-    return join<T, D, gs::Chunk<D>::kRows>(a, st);
 }
 
 // `rows`: the most query rows per head of keys that a sequence may have.
@@ -1182,12 +1207,20 @@ template <class T, int D, bool F32> int by_rows(gs::AttnArgs &a, uint64_t rows, 
         // 4000, where the time is launches and waits: of 128, 16 rows: 23,
         // 25; 32: 28, 26; of 256, 16: 35, 33.)
         constexpr int kFew = D == 256 ? 16 : 32;
-        if ((uint64_t)a.n_tokens * a.group == rows * a.n) return chunk_call<T, D>(a, st);      // (all of the same length, or the caller's most is wrong)
+        constexpr int R = gs::Chunk<D>::kRows;
+        if ((uint64_t)a.n_tokens * a.group == rows * a.n) {     // (all of the same length, or the caller's most is wrong)
+            chunk_launch<T, D>(a, st);
+            return join<T, D, R>(a, st);
+        }
+        gs::AttnArgs b = a;
+        b.cuts = (gs::Cut *)((char *)a.cuts + cuts_bytes());
+        b.parts = (float *)((char *)a.parts + few_bytes(D));
         a.max_rows = kFew;
-        if (int rc = rows_call<T, D, kFew / 16, F32>(a, st)) return rc;
-        a.min_rows = kFew + 1;
-        a.max_rows = 0xffffffffu;
-        return chunk_call<T, D>(a, st);
+        b.min_rows = kFew + 1;
+        rows_launch<T, D, kFew / 16, F32>(a, st);
+        chunk_launch<T, D>(b, st);
+        hipLaunchKernelGGL((gs::attn_join_both_kernel<T, D, kFew, R>), (join_grid<D, R>(a.n_wg + b.n_wg)), dim3(256), 0, st, a, b);
+        return hipGetLastError() == hipSuccess ? GS_OK : GS_ERR_HIP;
     }
 }
 
@@ -1207,10 +1240,8 @@ extern "C" {
 size_t gs_attn_workspace(const gs_kv_cache *c, uint32_t n_heads)
 {
     if (check_cache(c) || n_heads == 0 || n_heads % c->n_kv) return 0;
-    // the larger of the two kernels': 32 rows in each of kRuns runs, or a chunk's in kChunkRuns
     const int D = padded(c->d);
-    const size_t few = parts_bytes(kRuns, 32, D), many = parts_bytes(gs::kChunkRuns, D == 256 ? gs::Chunk<256>::kRows : gs::Chunk<128>::kRows, D);
-    return cuts_bytes() + (few > many ? few : many);
+    return 2 * cuts_bytes() + few_bytes(D) + parts_bytes(gs::kChunkRuns, D == 256 ? gs::Chunk<256>::kRows : gs::Chunk<128>::kRows, D);
 }
 
 int gs_attn(const gs_kv_cache *c, uint32_t layer, const gs_kv_batch *b, const gs_attn_args *x, void *stream)
@@ -1239,7 +1270,7 @@ int gs_attn(const gs_kv_cache *c, uint32_t layer, const gs_kv_batch *b, const gs
     a.scale = (float)((x->scale == 0.0f ? 1.0 / sqrt((double)c->d) : (double)x->scale) * M_LOG2E);
     a.window = x->window ? x->window : 0xffffffffu;
     a.cuts = (gs::Cut *)x->ws;
-    a.parts = (float *)((char *)x->ws + cuts_bytes());
+    a.parts = (float *)((char *)x->ws + 2 * cuts_bytes());
     const uint32_t most = !b->start ? 1 : x->max_q && x->max_q < b->n_tokens ? x->max_q : b->n_tokens;
     const uint64_t rows = (uint64_t)most * a.group;
     hipStream_t st = (hipStream_t)stream;

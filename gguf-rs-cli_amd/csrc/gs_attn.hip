@@ -984,6 +984,9 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, 2) attn_chunk_kernel(const
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 // The values that were put aside count for the rows that see them.
+                // (The first 32 keys' weights are those to the maximum before the
+                // second raise, which has scaled the sums since.)
+                const float since = KT > 1 && moved ? by : 1.0f;
                 if ((int)key0 + kTile > unit_pos0 + 1 || (int)key0 < unit_lo1)
                     for (uint64_t bad = s_bad[bs]; bad; bad &= bad - 1) {
                         const int key = __ffsll((unsigned long long)bad) - 1, y = key & 31;
@@ -996,6 +999,7 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, 2) attn_chunk_kernel(const
                         for (int i = 0; i < NZ * KT; i++)
                             if (i == at) wt = (float)pf[i / NZ][i % NZ >> 3][i & 7];
                         wt = __shfl(wt, from);
+                        if (key < 32) wt *= since;
                         if ((int)key0 + key > pos || (int)key0 + key < lo) continue;
 #pragma unroll
                         for (int c = 0; c < DT; c++)

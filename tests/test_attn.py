@@ -195,6 +195,37 @@ def test_masked_values_do_not_count(gpu, torch, dtype, cache, news):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("news", [3, 190])
+def test_values_beside_an_infinity(gpu, torch, dtype, d, news):
+    """A key whose value has an infinity, in tiles that only some rows see whole,
+    and after it in the same tile a key whose score is 2^12 of weight and more
+    above all before it: the other values of the rows that see both are the
+    formula's."""
+    lens, H, kv, page = [333, 262], 4, 2, 16
+    c = build(gpu, torch, lens, kv, d, page, dtype, seed=11)
+    for r, n in enumerate(lens):
+        for key, big in ((n - 70, 0), (n - 40, 1), (n - 12, 0), (n - 3, 1)):
+            at = (0, int(c.table[r, key // page]), slice(None), key % page)
+            if big:
+                c.k[at][:, 0] = 24.0 if key == n - 3 else 12.0
+            else:
+                c.v[at][:, 7] = math.inf if key == n - 12 else -math.inf
+    q = torch.randn((2 * news, H, d), generator=torch.Generator("cuda").manual_seed(6), device="cuda")
+    q[:, :, 0] = math.sqrt(d)                           # the large keys score 12 and 24
+    q = q.to(getattr(torch, dtype))
+    got = c.attend(0, q, q_start=starts(torch, [news, news]), max_q=news).double().cpu().numpy()
+    with np.errstate(invalid="ignore"):
+        out, tol = want(c, 0, q, [0, 1], [news, news])
+        seen = ~np.isfinite(out)
+        assert seen.any() and not seen[..., :7].any() and not seen[..., 8:].any()
+        assert not np.isfinite(got[seen]).any()
+        bad = ~seen & ~(np.abs(got - out) <= tol)
+    assert not bad.any(), np.argwhere(bad)[:5]
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("d,H,kv", [(64, 4, 2), (80, 2, 1), (256, 6, 2)])
 @pytest.mark.parametrize("news,dtype", [([200, 40], "bfloat16"), ([3, 30], "float32")])
 def test_masked_values_of_other_heads(gpu, torch, d, H, kv, news, dtype):

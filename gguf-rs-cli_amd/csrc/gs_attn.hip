@@ -573,6 +573,51 @@ __global__ void __launch_bounds__(256, rows_per_cu(D, NT)) attn_rows_kernel(cons
             if (more) load_v(key0 + kRowTile, vid);
         }
 
+        // Row r over the wave's keys by the vector units, from the unsplit query
+        // and weights, with 64 lanes beside one another along the head; to s_m,
+        // s_l and s_o as the products leave them.  A row whose query is not
+        // finite, or that has met a NaN, is NaN and costs no more than that.
+        auto alone = [&](uint32_t r) {
+            constexpr int E = D / 64;
+            const uint32_t tok = r / a.group, h = kvh * a.group + (r - tok * a.group), rr = (r - r0) & 15;
+            const int64_t at = (int64_t)s.len - s.nq + tok;
+            const size_t qa = (size_t)(s.first + tok) * a.ld_q + (size_t)h * d;
+            float q[E], y[E], top = -INFINITY, l = 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const uint32_t dv = 64 * e + lane;
+                y[e] = 0.0f;
+                q[e] = 0.0f;
+                if (dv < d) q[e] = F32 ? ((const float *)a.q)[qa + dv] : (float)((const T *)a.q)[qa + dv];
+                l = fmaf(q[e], 0.0f, l);
+            }
+            if (__any(!(l == 0.0f))) return;
+            for (uint32_t x = 0; x < 32 * left && l == l; x++) {
+                const uint32_t key = (span.tile0 + first + x / 32) * kRowTile + 32 * w + x % 32;
+                if ((int64_t)key > at || (int64_t)key <= at - (int64_t)a.window) continue;
+                const size_t from = place(page_of(key)) + (size_t)(key & (page - 1)) * d;
+                float dot = 0.0f;
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    if (64 * e + lane < d) dot += q[e] * (float)((const T *)a.k)[from + 64 * e + lane];
+#pragma unroll
+                for (int o = 1; o < 64; o <<= 1) dot += __shfl_xor(dot, o);
+                dot *= a.scale;
+                const float up = fmaxf(top, dot), ref = up == -INFINITY ? 0.0f : up, by = __builtin_amdgcn_exp2f(top - ref);
+                const float wt = __builtin_amdgcn_exp2f(dot - ref + kLift<T>);
+                top = up;
+                l = l * by + wt;
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    y[e] *= by;
+                    if (64 * e + lane < d) y[e] += wt * (float)((const T *)a.v)[from + 64 * e + lane];
+                }
+            }
+            if (lane == 0) { s_m[w][rr] = top; s_l[w][rr] = l; }
+#pragma unroll
+            for (int e = 0; e < E; e++) s_o[w][rr][64 * e + lane] = y[e];
+        };
+
         // ---- the waves' sums together; the unit's rows or its part
         const bool whole = left == span.tiles;
         float *part = a.parts + (size_t)(2 * blockIdx.x + (first == 0)) * R * (D + 2);
@@ -581,6 +626,19 @@ __global__ void __launch_bounds__(256, rows_per_cu(D, NT)) attn_rows_kernel(cons
             float l = sum[nt];
             l += __shfl_xor(l, 16);
             l += __shfl_xor(l, 32);
+            // A sum that is no finite number may be so by an infinity that met the
+            // parts of a query or a weight (inf - inf, 0 inf) where the formula
+            // has -inf or inf: such rows are computed again without parts.
+            float off = l * 0.0f;
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int i = 0; i < CW; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) off = fmaf(o[nt][c][i][e], 0.0f, off);
+            uint64_t again = __ballot(!(off == 0.0f));
+            again = (again | again >> 32);
+            again = (again | again >> 16) & 0xffff;
             __syncthreads();
             if (g == 0) { s_m[w][m] = mx[nt]; s_l[w][m] = l; }
 #pragma unroll
@@ -591,6 +649,10 @@ __global__ void __launch_bounds__(256, rows_per_cu(D, NT)) attn_rows_kernel(cons
                     for (int i = 0; i < CW; i += 4)
                         *(f4 *)&s_o[w][m][16 * CW * c + CW * (4 * g + e) + i] =
                             f4{o[nt][c][i][e], o[nt][c][i + 1][e], o[nt][c][i + 2][e], o[nt][c][i + 3][e]};
+            for (; again; again &= again - 1) {
+                const uint32_t r = r0 + 16 * nt + __ffsll((unsigned long long)again) - 1;
+                if (r < r1) alone(r);
+            }
             __syncthreads();
             const uint32_t rr = threadIdx.x >> 4, r = r0 + 16 * nt + rr, c0 = threadIdx.x & 15;
             if (r >= r1) continue;

@@ -226,6 +226,43 @@ def test_values_beside_an_infinity(gpu, torch, dtype, d, news):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,cache", [("float32", "float16"), ("float32", "bfloat16"), ("float16", "float16"),
+                                         ("bfloat16", "bfloat16")])
+@pytest.mark.parametrize("d,H,kv", [(64, 4, 2), (80, 20, 1), (128, 6, 2), (256, 2, 1)])
+@pytest.mark.parametrize("news", [1, 5, 90])
+def test_infinities_that_all_rows_see(gpu, torch, dtype, cache, d, H, kv, news):
+    """A key that scores -inf has the weight 0 and the rest is the formula's; a
+    value with an infinity gives infinities of its sign in its place, not NaN.
+    Row 1 has a key that scores +inf: no number."""
+    lens, page = [420, 300], 16
+    c = build(gpu, torch, lens, kv, d, page, cache, seed=13)
+    put = lambda x, r, key, at, value: x[0, int(c.table[r, key // page]), :, key % page].__setitem__((slice(None), at), value)  # noqa: E731
+    put(c.k, 0, 20, 5, -math.inf)
+    put(c.k, 0, 163, 5, -math.inf)
+    put(c.v, 0, 40, 9, math.inf)
+    put(c.v, 0, 150, 11, -math.inf)
+    put(c.k, 1, 10, 5, math.inf)
+    q = torch.randn((2 * news, H, d), generator=torch.Generator("cuda").manual_seed(7), device="cuda")
+    q[:, :, 5] = q[:, :, 5].abs() + 0.1
+    q = q.to(getattr(torch, dtype))
+    got = c.attend(0, q, q_start=starts(torch, [news, news])).double().cpu().numpy()
+    assert np.isnan(got[news:]).all()
+    assert (got[:news, :, 9] == np.inf).all() and (got[:news, :, 11] == -np.inf).all()
+    rest = np.delete(np.arange(d), [9, 11])
+    # the same without the two keys' part in the scores' error
+    small = build(gpu, torch, lens, kv, d, page, cache, seed=13)
+    keep = [t for t in range(lens[0]) if t not in (20, 163)]
+    k, v = small.k[0].clone(), small.v[0].clone()
+    for t, f in enumerate(keep):
+        for x, y in ((small.k, k), (small.v, v)):
+            x[0, int(small.table[0, t // page]), :, t % page] = y[int(small.table[0, f // page]), :, f % page]
+    small.len[0] = len(keep)
+    out, tol = want(small, 0, q[:news], [0], [news])
+    bad = ~(np.abs(got[:news] - out) <= tol)[..., rest]
+    assert not bad.any(), np.argwhere(bad)[:5]
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("d,H,kv", [(64, 4, 2), (80, 2, 1), (256, 6, 2)])
 @pytest.mark.parametrize("news,dtype", [([200, 40], "bfloat16"), ([3, 30], "float32")])
 def test_masked_values_of_other_heads(gpu, torch, d, H, kv, news, dtype):

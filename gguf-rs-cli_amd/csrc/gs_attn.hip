@@ -284,10 +284,12 @@ constexpr int rows_per_cu(int D, int NT) { return D == 64 || (D == 128 && NT == 
 // columns come from the 8 rows of V in a lane by a transposition of 8 x 8
 // values in registers (the value a lane's row m stands for is 8 m + i in
 // product i).  Four waves' sums meet in LDS at a unit's end.
-// The weights are rounded to T for the second product, as its factors have to
-// be: each is off by 2^-11 of itself (bf16: 2^-8) at most, without a common
-// direction, which is less than what the rounding of the result to T adds.
-// Their sum is of the unrounded ones, in f32.
+// The second product's factors are of T: a weight goes in as two of them, its
+// rounding and the rest, which hold 22 bits of it (bf16: 16), one product more
+// where the matrix cores have the time.  (us with one and two: 64 rows of 16000,
+// 28 / 4 heads of 128, bf16, 356, 357; 4 tokens each, 64 / 8 heads, 699, 711; 64
+// over 1000 to 32768 206 and 206, there the outputs' relative distance to 32-bit
+// weights' 6.8e-4 and 4e-5.)  Their sum is in f32.
 // Measured: 64 rows of 16000 tokens, 28 / 4 heads of 128, bf16: 353 us, 5.9
 // TB/s, what a read of this size reaches; one token over 4001: 10 us, of which
 // the empty launch, the search for the run's begin and three waits in a row
@@ -299,7 +301,7 @@ constexpr int rows_per_cu(int D, int NT) { return D == 64 || (D == 128 && NT == 
 template <class T, int D, int NT, bool F32, bool FULL>
 __global__ void __launch_bounds__(256, rows_per_cu(D, NT)) attn_rows_kernel(const AttnArgs a)
 {
-    constexpr int R = 16 * NT, NP = F32 ? 3 : 1, KS = D / 32;
+    constexpr int R = 16 * NT, NP = F32 ? 3 : 1, NW = F32 ? 3 : 2, KS = D / 32;
     constexpr int CW = D >= 128 ? 8 : D / 16, NC = D / (16 * CW);       // values of a lane's V chunk, chunks
     typedef typename Vec<T>::v8 v8;
     typedef T vw __attribute__((ext_vector_type(CW)));
@@ -523,17 +525,15 @@ __global__ void __launch_bounds__(256, rows_per_cu(D, NT)) attn_rows_kernel(cons
                         for (int c = 0; c < NC; c++) vf[j][c] = vw{};
                 }
             }
-            v8 pf[NT][NP];
+            v8 pf[NT][NW];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     pf[nt][0][j] = (T)p[nt][j];
-                    if constexpr (F32) {
-                        const float y = p[nt][j] - (float)pf[nt][0][j];
-                        pf[nt][1][j] = (T)y;
-                        pf[nt][2][j] = (T)(y - (float)pf[nt][1][j]);
-                    }
+                    const float y = p[nt][j] - (float)pf[nt][0][j];
+                    pf[nt][1][j] = (T)y;
+                    if constexpr (F32) pf[nt][2][j] = (T)(y - (float)pf[nt][1][j]);
                 }
 #pragma unroll
             for (int c = 0; c < NC; c++)
@@ -545,7 +545,7 @@ __global__ void __launch_bounds__(256, rows_per_cu(D, NT)) attn_rows_kernel(cons
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                        for (int q = NP - 1; q >= 0; q--) o[nt][c][i] = mfma(x8, pf[nt][q], o[nt][c][i]);
+                        for (int q = NW - 1; q >= 0; q--) o[nt][c][i] = mfma(x8, pf[nt][q], o[nt][c][i]);
                 }
             for (; bad; bad &= bad - 1) {
                 const uint32_t y = __ffs(bad) - 1;
@@ -733,8 +733,13 @@ constexpr int kChunkRuns = 256;         // one workgroup per CU
 // that neither reading order meets a bank twice.
 // The running maximum is raised only when a score passes it by 2^8, so the
 // sums are seldom scaled: the weights then reach 2^8, which f32 sums and the
-// type's range (f16: 2^7 is the lift here) take without loss.  They are rounded
-// to T as in the kernel above; the sum is of the unrounded ones.
+// type's range (f16: 2^7 is the lift here) take without loss.  Each is rounded to
+// T once, off by 2^-11 of itself (bf16: 2^-8) at most and without a common
+// direction; the sum is of the unrounded ones.  A second part, as in the kernel
+// above, would cost a quarter: 4 x 2048 over 8192, 32 / 8 heads of 128, f16, 1292
+// -> 1641 us; one chunk of 8192, bf16, 664 -> 827.  Without it the relative error
+// of the output, most of it the result's own rounding, is 2.16e-4 for 2.09e-4
+// (f16) and, in a call of chunks and single tokens, 1.74e-3 for 1.66e-3 (bf16).
 // Measured: four chunks of 2048 tokens over 8192, 32 / 8 heads of 128, f16: 710
 // to 880 TFLOP/s from card to card (a library product of 8192 x 8192 x 8192:
 // 1140), heads of 64 610, of 256 600 to 640.  No bank is met twice.  With 14 % fewer clocks per tile the

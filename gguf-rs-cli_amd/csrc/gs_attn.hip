@@ -103,17 +103,18 @@ template <int R_, int kTile_, int kSetup_> struct Deal {
     {
         return Span<kTile>(a, s, r, min(r + R, s.nq * a.group)).tiles + kSetup;
     }
-    // Tiles of a sequence and one head of keys, counted by a thread ..
-    static __device__ __forceinline__ uint32_t count(const AttnArgs &a, const Seq &s)
+    // Tiles of a sequence and one head of keys (a chunk of 66000 tokens over 2^23
+    // has more than 2^32 of 16 rows), counted by a thread ..
+    static __device__ __forceinline__ uint64_t count(const AttnArgs &a, const Seq &s)
     {
-        uint32_t t = 0;
+        uint64_t t = 0;
         for (uint32_t r = 0; r < s.nq * a.group; r += R) t += unit(a, s, r);
         return t;
     }
     // .. and by a wave, its lanes side by side
-    static __device__ __forceinline__ uint32_t count_wave(const AttnArgs &a, const Seq &s)
+    static __device__ __forceinline__ uint64_t count_wave(const AttnArgs &a, const Seq &s)
     {
-        uint32_t t = 0;
+        uint64_t t = 0;
         for (uint32_t r = (threadIdx.x & 63) * R; r < s.nq * a.group; r += 64 * R) t += unit(a, s, r);
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) t += __shfl_xor(t, o);
@@ -121,7 +122,7 @@ template <int R_, int kTile_, int kSetup_> struct Deal {
     }
     // The first row of the unit that tile `skip` of the sequence is in; skip
     // becomes the tile's number in the unit.  (a wave)
-    static __device__ __forceinline__ uint32_t find(const AttnArgs &a, const Seq &s, uint32_t &skip)
+    static __device__ __forceinline__ uint32_t find(const AttnArgs &a, const Seq &s, uint64_t &skip)
     {
         const uint32_t rows = s.nq * a.group, lane = threadIdx.x & 63;
         if (rows <= R) return 0;
@@ -157,8 +158,8 @@ __device__ __forceinline__ uint64_t quotient(uint64_t a, uint64_t b)
 // Each thread counts a stretch of the sequences, and the one that finds the
 // run's first leaves it in LDS.
 struct Run {
-    uint64_t t0, t1, total, skip;
-    uint32_t n_wg, seq, per;        // per: tiles of the sequence and one head of keys
+    uint64_t t0, t1, total, skip, per;  // per: tiles of the sequence and one head of keys
+    uint32_t n_wg, seq;
     Seq s;
 };
 
@@ -177,15 +178,14 @@ template <class D, int kThreads, int kLeast> __device__ __forceinline__ Run run_
 {
     constexpr uint32_t kWaves = kThreads / 64, kShort = 32;     // up to kShort sequences are counted by waves: theirs may be long
     __shared__ uint64_t s_wave[kWaves];
-    __shared__ uint32_t s_per[kShort];
+    __shared__ uint64_t s_per[kShort];
     __shared__ Seq s_seq[kShort];
     __shared__ Run s_run;
     const uint32_t each = (a.n + kThreads - 1) / kThreads;
     const uint32_t i0 = min(threadIdx.x * each, a.n), i1 = min(i0 + each, a.n);
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     Seq s = {};
-    uint32_t per = 0;
-    uint64_t mine = 0;
+    uint64_t per = 0, mine = 0;
     if (a.n <= kShort) {
         for (uint32_t i = w; i < a.n; i += kWaves) {
             s = seq_of(a, i);
@@ -196,13 +196,13 @@ template <class D, int kThreads, int kLeast> __device__ __forceinline__ Run run_
         if (threadIdx.x < a.n) {
             s = s_seq[threadIdx.x];
             per = s_per[threadIdx.x];
-            mine = (uint64_t)per * a.n_kv;
+            mine = per * a.n_kv;
         }
     } else {
         for (uint32_t i = i0; i < i1; i++) {
             s = seq_of(a, i);
             per = D::count(a, s);
-            mine += (uint64_t)per * a.n_kv;
+            mine += per * a.n_kv;
         }
     }
     uint64_t x = mine;
@@ -235,15 +235,15 @@ template <class D, int kThreads, int kLeast> __device__ __forceinline__ Run run_
             for (;; i++) {
                 s = seq_of(a, i);
                 per = D::count(a, s);
-                if (r.t0 < before + (uint64_t)per * a.n_kv) break;
-                before += (uint64_t)per * a.n_kv;
+                if (r.t0 < before + per * a.n_kv) break;
+                before += per * a.n_kv;
             }
         r.seq = i; r.skip = r.t0 - before; r.per = per; r.s = s;
         s_run = r;
     }
     __syncthreads();
     const Run u = s_run;
-    return Run{uniform(u.t0), uniform(u.t1), uniform(u.total), uniform(u.skip), uniform(u.n_wg), uniform(u.seq), uniform(u.per), uniform(u.s)};
+    return Run{uniform(u.t0), uniform(u.t1), uniform(u.total), uniform(u.skip), uniform(u.per), uniform(u.n_wg), uniform(u.seq), uniform(u.s)};
 }
 
 // An infinity or NaN among 8 values.
@@ -320,11 +320,12 @@ __global__ void __launch_bounds__(256, rows_per_cu(D, NT)) attn_rows_kernel(cons
     const size_t head = (size_t)d << a.shift;           // values of a head's page
 
     uint32_t si = run.seq, r0;
-    const uint32_t per = run.per;
     Seq s = run.s;
     uint64_t t = run.t0;
-    uint32_t kvh = (uint32_t)quotient(run.skip, per), skip = (uint32_t)(run.skip - (uint64_t)kvh * per);
-    r0 = Dealt::find(a, s, skip);
+    uint32_t kvh = (uint32_t)quotient(run.skip, run.per);
+    uint64_t before = run.skip - kvh * run.per;
+    r0 = Dealt::find(a, s, before);
+    uint32_t skip = (uint32_t)before;
     while (t < run.t1) {
         const uint32_t rows = s.nq * a.group;
         if (kvh == a.n_kv || rows == 0) {               // the next sequence
@@ -785,11 +786,12 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, 2) attn_chunk_kernel(const
     const bool inside = 8 * pc < (int)d;
 
     uint32_t si = run.seq, r0;
-    const uint32_t per = run.per;
     Seq s = run.s;
     uint64_t t = run.t0;
-    uint32_t kvh = (uint32_t)quotient(run.skip, per), skip = (uint32_t)(run.skip - (uint64_t)kvh * per);
-    r0 = Dealt::find(a, s, skip);
+    uint32_t kvh = (uint32_t)quotient(run.skip, run.per);
+    uint64_t before = run.skip - kvh * run.per;
+    r0 = Dealt::find(a, s, before);
+    uint32_t skip = (uint32_t)before;
     while (t < run.t1) {
         const uint32_t rows = s.nq * a.group;
         if (kvh == a.n_kv || rows == 0) {               // the next sequence

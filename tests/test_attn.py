@@ -375,6 +375,22 @@ def test_a_far_page(gpu, torch):
 
 
 @pytest.mark.gpu
+def test_more_tiles_than_32_bits_count(gpu, torch):
+    """66000 tokens over 2^23: 4.3e9 tiles of 16 rows and 128 keys in one
+    sequence.  Keys of zeros weigh all alike, so every row is the values' mean."""
+    n, news, page, d = 1 << 23, 66000, 1024, 8
+    c = gpu.KVCache.empty(1, n // page, 1, d, 1, n, page=page, dtype=torch.bfloat16)
+    c.k.zero_()
+    c.v.fill_(1.0)
+    c.table[0] = torch.arange(n // page, dtype=torch.int32, device="cuda")
+    c.len.fill_(n)
+    q = torch.randn((news, 16, d), device="cuda").bfloat16()
+    out = torch.full_like(q, 99.0)
+    c.attend(0, q, out, q_start=starts(torch, [news]), max_q=1)
+    assert bool((out == 1.0).all())
+
+
+@pytest.mark.gpu
 def test_many_sequences(gpu, torch):
     rng = np.random.default_rng(12)
     lens = rng.integers(0, 90, 700).tolist()

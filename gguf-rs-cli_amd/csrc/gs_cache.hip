@@ -641,6 +641,7 @@ int gs_kv_drop(const gs_kv_cache *c, const uint32_t *rows, size_t n, const uint3
     const gs::Cache d = device_cache(c);
     hipStream_t st = (hipStream_t)stream;
     const size_t streams = 2 * (size_t)c->n_layers * c->n_kv;
+    if (streams * 256 > 0xffffffffull) return GS_ERR_UNSUPPORTED;       // (a grid's threads side by side)
     const int rot = rope ? (int)rope->rot : 0;
     const bool inter = rope && rope->layout == GS_ROPE_INTERLEAVED;
     const uint64_t *turns = rope ? rope->turns : nullptr;

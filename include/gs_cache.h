@@ -103,7 +103,7 @@ int gs_kv_free(const gs_kv_cache *c, const uint32_t *rows, size_t n, void *strea
  * replaced by a new one (lowest-numbered free pages, in the order of i, then
  * of their place), others are written in place; pages that are no longer
  * needed are released.  status[i] as of gs_kv_extend, GS_ERR_INVALID also for
- * a row that an earlier i has. */
+ * a row that an earlier i has.  At most 2^23 - 1 layers times heads. */
 int gs_kv_drop(const gs_kv_cache *c, const uint32_t *rows, size_t n, const uint32_t *from, const uint32_t *to,
                const gs_rope *rope, int32_t *status, void *stream);
 

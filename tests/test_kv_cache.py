@@ -545,3 +545,14 @@ def test_append_more_heads_than_counted(gpu, torch):
         else:
             with pytest.raises(gpu.SamplerError):
                 c.append(0, k, k, rope=gpu.Rope(256, layout="half"))
+
+
+def test_drop_of_more_streams_than_a_grid_is_wide():
+    """Refused before anything is launched: the row's table would be written
+    without its tokens having moved."""
+    import gs_sampler as gs
+    lib = gs.load_library()
+    for layers, kv in ((2048, 4096), (65535, 4096), (2049, 4095)):
+        c = fake(gs, n_layers=layers, n_kv=kv)
+        assert lib.gs_kv_drop(c, 4096, 1, 4096, 4096, None, None, None) == gs.GS_ERR_UNSUPPORTED
+        assert lib.gs_kv_drop(c, None, 0, None, None, None, None, None) == gs.GS_OK

@@ -34,6 +34,7 @@ struct RopeArgs {
     // work items: a vector of 8 values, or two that the half layout turns together (in the pair form two values)
     int turned, per_head, per_v;        // items of a head that are turned, all of its items, those of a head of v
     int tokens;                         // of a workgroup
+    int first;                          // token of the launch
     uint32_t by_head, by_token, by_v, by_vtoken;   // 2^32 / (per_head, items of a token, per_v, items of v of a token), up
 };
 
@@ -56,7 +57,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a)
     constexpr int kItems = 2, kW = VEC ? 8 : 1;
     __shared__ float2 cs[kRopeTokens * 256];
     __shared__ int64_t place[kRopeTokens];      // of a token's slot in a head's pages, in slots; -1: not written
-    const int t0 = blockIdx.x * a.tokens, nt = min(a.tokens, a.n_tokens - t0);
+    const int t0 = a.first + blockIdx.x * a.tokens, nt = min(a.tokens, a.n_tokens - t0);
     const int pairs = a.rot >> 1;
     const size_t head = ((size_t)1 << a.shift) * a.d;
 
@@ -221,7 +222,7 @@ int launch(RopeArgs &a, bool vec, hipStream_t st)
     // (quotient: values are twice the items of their keys at most, and
     // 4 * 32768 * 32768 = 2^32)
     a.tokens = a.n_tokens >= 4096 && per_token <= 16384 ? gs::kRopeTokens : 1;
-    const unsigned blocks = (a.n_tokens + a.tokens - 1) / a.tokens;
+    const unsigned blocks = ((unsigned)a.n_tokens + a.tokens - 1) / a.tokens;
     // Few tokens: a token's items are spread over workgroups, each with one
     // round of them; the angles are computed by each.  (One token of 128 heads
     // of 256: 3.0 us, by one workgroup 8.8; of 32 heads of 128 either way 2.6.)
@@ -232,10 +233,15 @@ int launch(RopeArgs &a, bool vec, hipStream_t st)
     a.by_v = over(a.per_v);
     a.by_vtoken = over(a.n_kv ? a.n_kv * a.per_v : 1);
     const size_t written = (size_t)a.n_tokens * a.d * (a.n_heads * sizeof(TO) + 2 * a.n_kv * sizeof(TC));
-    const dim3 grid(blocks, y), block(gs::kRopeThreads);
-    if (!vec) hipLaunchKernelGGL((gs::rope_kernel<TI, TO, TC, false, false>), grid, block, 0, st, a);
-    else if (written > kPastCaches) hipLaunchKernelGGL((gs::rope_kernel<TI, TO, TC, true, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((gs::rope_kernel<TI, TO, TC, true, false>), grid, block, 0, st, a);
+    // (a grid has less than 2^32 threads side by side)
+    constexpr unsigned kMost = 1u << 23;
+    for (unsigned done = 0; done < blocks; done += kMost) {
+        a.first = (int)(done * a.tokens);
+        const dim3 grid(blocks - done < kMost ? blocks - done : kMost, y), block(gs::kRopeThreads);
+        if (!vec) hipLaunchKernelGGL((gs::rope_kernel<TI, TO, TC, false, false>), grid, block, 0, st, a);
+        else if (written > kPastCaches) hipLaunchKernelGGL((gs::rope_kernel<TI, TO, TC, true, true>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((gs::rope_kernel<TI, TO, TC, true, false>), grid, block, 0, st, a);
+    }
     return hipGetLastError() == hipSuccess ? GS_OK : GS_ERR_HIP;
 }
 

@@ -185,3 +185,20 @@ def test_refusals(gpu, torch):
         rope.apply(x, pos.long())
     with pytest.raises(TypeError):
         rope.apply(x.double(), pos)
+
+
+@pytest.mark.gpu
+def test_more_tokens_than_a_grid_is_wide(gpu, torch):
+    """Over 2^24 workgroups of four tokens."""
+    T, H, d, dtype = 70000003, 1, 2, "bfloat16"
+    rope = gpu.Rope(d, layout="half")
+    x = torch.ones((T, H, d), dtype=getattr(torch, dtype), device="cuda")
+    x[:, 0, 1] = 0.0
+    pos = torch.arange(T, dtype=torch.int32, device="cuda")
+    out = rope.apply(x, pos, out=torch.full_like(x, 99.0))
+    for at in (slice(0, 1000), slice(T // 2, T // 2 + 1000), slice(T - 1000, T)):
+        a, p = x[at].double().cpu().numpy(), pos[at].cpu().numpy()
+        f, gain = frequencies(d, 10000.0)
+        want, mag = turned(a, p, f, gain, "half")
+        assert (np.abs(out[at].double().cpu().numpy() - want) <= bound(want, mag, dtype) + 1e-8 * mag).all()
+    assert float(out.float().abs().max()) < 1.01

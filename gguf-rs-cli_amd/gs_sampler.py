@@ -726,6 +726,15 @@ def _empty_on(st, shape, dtype, like):
     return x
 
 
+def _turn(rope):
+    """The handle of a rotation, or None for none; a closed one is no rotation to go without."""
+    if rope is None:
+        return None
+    if not rope._h:
+        raise ValueError("the rotation is closed")
+    return rope._h
+
+
 class Rope:
     """The plan of a rotation (include/gs_rope.h): the first `rot` values of
     heads of d, in the "interleaved" or the "half" layout, with the scaling
@@ -758,7 +767,7 @@ class Rope:
         T2, _, _, ld_out = _heads(out, "out", heads, d)
         if T2 != T or out.dtype != x.dtype:
             raise ValueError("out must be as x")
-        _check(self._lib.gs_rope_apply(self._h, _type(x, "x"), x.data_ptr(), ld, out.data_ptr(), ld_out, T, heads,
+        _check(self._lib.gs_rope_apply(_turn(self), _type(x, "x"), x.data_ptr(), ld, out.data_ptr(), ld_out, T, heads,
                                        _words(pos, "pos", T), _stream_of(x, stream)), "gs_rope_apply")
         return out
 
@@ -841,9 +850,9 @@ class KVCache:
     def drop(self, start, end, rows, rope=None, status=None, stream=None):
         """Tokens start .. end - 1 of each of `rows` leave it (gs_kv_drop); with
         `rope` the keys after them are turned back to their new positions."""
-        n = rows.numel()
+        n, turn = rows.numel(), _turn(rope)
         _check(self._lib.gs_kv_drop(self._c, _words(rows, "rows"), n, _words(start, "start", n), _words(end, "end", n),
-                                    None if rope is None else rope._h, _words(status, "status", n),
+                                    turn, _words(status, "status", n),
                                     _stream_of(self.k, stream)), "gs_kv_drop")
 
     def _batch(self, T, rows, q_start):
@@ -859,6 +868,7 @@ class KVCache:
         `rope`; q [T, heads, d] turned to q_out (None: in place).  One token
         for each of `rows` (None: row i), or those from q_start[i] to
         q_start[i + 1]."""
+        turn = _turn(rope)
         T, _, _, ld_k = _heads(k, "k", self.kv, self.d)
         Tv, _, _, ld_v = _heads(v, "v", self.kv, self.d)
         if Tv != T or v.dtype != k.dtype:
@@ -873,8 +883,8 @@ class KVCache:
             x.q, x.ld_q, x.q_out, x.ld_q_out = q.data_ptr(), ld_q, q_out.data_ptr(), ld_o
             x.q_out_type, x.n_heads = _type(q_out, "q_out"), heads
         b = self._batch(T, rows, q_start)
-        _check(self._lib.gs_kv_append(self._c, layer, ctypes.byref(b), None if rope is None else rope._h,
-                                      ctypes.byref(x), _stream_of(self.k, stream)), "gs_kv_append")
+        _check(self._lib.gs_kv_append(self._c, layer, ctypes.byref(b), turn, ctypes.byref(x), _stream_of(self.k, stream)),
+               "gs_kv_append")
 
     def attend(self, layer, q, out=None, rows=None, q_start=None, scale=0.0, window=0, max_q=0, stream=None):
         """Causal attention of the rows' newest tokens (as append takes them) over

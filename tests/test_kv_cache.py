@@ -556,3 +556,35 @@ def test_drop_of_more_streams_than_a_grid_is_wide():
         c = fake(gs, n_layers=layers, n_kv=kv)
         assert lib.gs_kv_drop(c, 4096, 1, 4096, 4096, None, None, None) == gs.GS_ERR_UNSUPPORTED
         assert lib.gs_kv_drop(c, None, 0, None, None, None, None, None) == gs.GS_OK
+
+
+def test_a_closed_rotation_is_refused_without_gpu():
+    """It has no handle, and no handle means no rotation to the library."""
+    import gs_sampler as gs
+
+    class Rows:
+        def numel(self):
+            return 1
+
+    rope, cache = gs.Rope.__new__(gs.Rope), gs.KVCache.__new__(gs.KVCache)
+    rope._h, cache._lib = None, None                              # (nothing can be called)
+    for call in (lambda: cache.append(0, None, None, rope=rope), lambda: cache.drop(None, None, Rows(), rope=rope)):
+        with pytest.raises(ValueError):
+            call()
+
+
+@pytest.mark.gpu
+def test_a_closed_rotation_writes_nothing(gpu, torch):
+    c, m = make(gpu, torch)
+    rows = words(torch, [1])
+    c.extend(40, rows=rows)
+    m.extend([1], [40])
+    rope = gpu.Rope(64)
+    rope.close()
+    k = torch.randn((1, 2, 64), device="cuda")
+    pos = words(torch, [3])
+    for call in (lambda: c.append(0, k, k, rope=rope, rows=rows), lambda: c.drop(pos, words(torch, [9]), rows, rope=rope),
+                 lambda: rope.apply(k, pos)):
+        with pytest.raises(ValueError):
+            call()
+    m.check(c)

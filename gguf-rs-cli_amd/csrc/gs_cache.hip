@@ -635,7 +635,7 @@ int gs_kv_drop(const gs_kv_cache *c, const uint32_t *rows, size_t n, const uint3
                const gs_rope *rope, int32_t *status, void *stream)
 {
     if (int rc = check_call(c, n)) return rc;
-    if (rope && rope->d != c->d) return GS_ERR_INVALID;
+    if (rope && (rope->d != c->d || !is_here(rope))) return GS_ERR_INVALID;
     if (n == 0) return GS_OK;
     if (!rows || !from || !to) return GS_ERR_INVALID;
     const gs::Cache d = device_cache(c);

@@ -103,6 +103,13 @@ inline int check_cache(const gs_kv_cache *c)
     return GS_OK;
 }
 
+// A plan's turns are memory of the device it was made on.
+inline bool is_here(const gs_rope *r)
+{
+    int device;
+    return hipGetDevice(&device) == hipSuccess && device == r->device;
+}
+
 inline int check_batch(const gs_kv_cache *c, const gs_kv_batch *b)
 {
     if (!b) return GS_ERR_INVALID;

@@ -333,6 +333,7 @@ int gs_rope_apply(const gs_rope *r, uint32_t type, const void *x, size_t ld_x, v
     if (!x || !out || !pos) return GS_ERR_INVALID;
     if (ld_x < (size_t)n_heads * r->d || ld_out < (size_t)n_heads * r->d) return GS_ERR_INVALID;
     if (x == out && ld_x != ld_out) return GS_ERR_INVALID;
+    if (!is_here(r)) return GS_ERR_INVALID;
     if (((uintptr_t)x | (uintptr_t)out) % bytes_of(type)) return GS_ERR_INVALID;
     if (n_tokens > 0x3fffffff) return GS_ERR_UNSUPPORTED;
     RopeArgs a = {};
@@ -353,7 +354,7 @@ int gs_kv_append(const gs_kv_cache *c, uint32_t layer, const gs_kv_batch *b, con
     if (int rc = check_cache(c)) return rc;
     if (int rc = check_batch(c, b)) return rc;
     if (!x || layer >= c->n_layers) return GS_ERR_INVALID;
-    if (rope && rope->d != c->d) return GS_ERR_INVALID;
+    if (rope && (rope->d != c->d || !is_here(rope))) return GS_ERR_INVALID;
     if (x->type != GS_TYPE_F32 && x->type != c->type) return GS_ERR_UNSUPPORTED;
     if (x->q && x->q_out_type != x->type && x->q_out_type != c->type) return GS_ERR_UNSUPPORTED;
     if (b->n_tokens == 0) return GS_OK;

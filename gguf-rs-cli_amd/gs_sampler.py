@@ -659,55 +659,75 @@ _DT = None
 
 
 def _dtypes():
-    """torch's value types and what they are here, and its 4-byte integers."""
+    """torch's value types and what they are here, its 4-byte integers, the
+    current stream's handle without an object on the way, and the current
+    device's number (None: there is one device)."""
     global _DT
     if _DT is None:
         import torch
         _DT = ({torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}, (torch.int32, torch.uint32),
-               getattr(torch._C, "_cuda_getCurrentRawStream", None))
+               getattr(torch._C, "_cuda_getCurrentRawStream", None),
+               torch.cuda.current_device if torch.cuda.device_count() > 1 else None)
     return _DT
 
 
 def _type(x, what):
-    t = _dtypes()[0].get(x.dtype)
-    if t is None:
-        raise TypeError("%s must be float32, float16 or bfloat16" % what)
-    return t
+    try:
+        return (_DT or _dtypes())[0][x.dtype]
+    except KeyError:
+        raise TypeError("%s must be float32, float16 or bfloat16" % what) from None
 
 
-def _heads(x, what, heads=None, d=None):
+def _call(dev, f, what, *args):
+    """f(*args) of the library, with the tensors' device dev the current one."""
+    now = (_DT or _dtypes())[3]
+    if now is None or now() == dev:
+        _check(f(*args), what)
+    else:
+        import torch
+        with torch.cuda.device(dev):
+            _check(f(*args), what)
+
+
+def _heads(x, what, dev, heads=None, d=None):
     """(tokens, heads, d, values from token to token) of a [T, heads, d]
-    tensor on the device whose heads are contiguous."""
+    tensor on device dev whose heads are contiguous."""
     shape = x.shape
-    if len(shape) != 3 or not x.is_cuda:
+    if len(shape) != 3 or x.get_device() != dev or dev < 0:
         raise TypeError("%s must be a [tokens, heads, d] tensor on the device" % what)
     T, h, n = shape
     if (heads is not None and h != heads) or (d is not None and n != d):
         raise ValueError("%s has heads of another number or size" % what)
+    if x.is_contiguous():
+        return T, h, n, h * n
     st, sh, sn = x.stride()
     if (n > 1 and sn != 1) or (h > 1 and sh != n):
         raise TypeError("the heads of %s must be contiguous" % what)
     return T, h, n, (st if T > 1 else h * n)
 
 
-def _words(x, what, n=None):
-    """The address of a contiguous device tensor of 4-byte integers (of n values), or None."""
+def _words(x, what, dev, n=None):
+    """The address of a contiguous tensor of 4-byte integers (n of them) on device dev, or None."""
     if x is None:
         return None
-    if not getattr(x, "is_cuda", False) or x.dtype not in _dtypes()[1] or not x.is_contiguous():
+    try:
+        wrong = x.get_device() != dev or x.dtype not in (_DT or _dtypes())[1] or not x.is_contiguous()
+    except AttributeError:
+        wrong = True
+    if wrong or dev < 0:
         raise TypeError("%s must be a contiguous tensor of 4-byte integers on the device" % what)
     if n is not None and x.numel() != n:
         raise ValueError("%s must have %d values" % (what, n))
     return x.data_ptr()
 
 
-def _stream_of(x, stream):
-    """The HIP stream of a call on tensor x: `stream`, or the one that torch
-    works on now (_stream_handle, without a Stream object on the way)."""
+def _stream_of(dev, stream):
+    """The HIP stream of a call on device dev: `stream`, or the one that torch
+    works on there now (_stream_handle, without a Stream object on the way)."""
     if stream is None:
-        raw = _dtypes()[2]
+        raw = (_DT or _dtypes())[2]
         if raw is not None:
-            return raw(x.get_device())
+            return raw(dev)
     return _stream_handle(stream)
 
 
@@ -716,7 +736,7 @@ def _empty_on(st, shape, dtype, like):
     torch's stream of the moment has freed may still be in use there: on
     another stream the tensor comes from that one's memory."""
     import torch
-    if st == _stream_of(like, None):
+    if st == _stream_of(like.get_device(), None):
         return torch.empty(shape, dtype=dtype, device=like.device)
     now = torch.cuda.current_stream(like.device)
     on = torch.cuda.ExternalStream(st, like.device) if st else torch.cuda.default_stream(like.device)
@@ -762,13 +782,13 @@ class Rope:
     def apply(self, x, pos, out=None, stream=None):
         """x [T, heads, d] turned to positions pos [T] (4-byte integers), to
         `out` (None: in place)."""
-        out = x if out is None else out
-        T, heads, d, ld = _heads(x, "x", d=self.d)
-        T2, _, _, ld_out = _heads(out, "out", heads, d)
+        out, dev = x if out is None else out, x.get_device()
+        T, heads, d, ld = _heads(x, "x", dev, d=self.d)
+        T2, _, _, ld_out = _heads(out, "out", dev, heads, d)
         if T2 != T or out.dtype != x.dtype:
             raise ValueError("out must be as x")
-        _check(self._lib.gs_rope_apply(_turn(self), _type(x, "x"), x.data_ptr(), ld, out.data_ptr(), ld_out, T, heads,
-                                       _words(pos, "pos", T), _stream_of(x, stream)), "gs_rope_apply")
+        _call(dev, self._lib.gs_rope_apply, "gs_rope_apply", _turn(self), _type(x, "x"), x.data_ptr(), ld, out.data_ptr(), ld_out,
+              T, heads, _words(pos, "pos", dev, T), _stream_of(dev, stream))
         return out
 
     def close(self):
@@ -798,8 +818,11 @@ class KVCache:
             raise ValueError("k and v must be contiguous [layers, pages, heads, page, d] tensors alike")
         if table.dim() != 2 or len.dim() != 1 or table.shape[0] != len.shape[0] or ref.numel() != k.shape[1]:
             raise ValueError("table must be [rows, pages of a row], len [rows], ref [pages]")
+        self.dev = k.get_device()
+        if self.dev < 0 or v.get_device() != self.dev:
+            raise TypeError("k and v must be on one device")
         for x, what in ((table, "table"), (len, "len"), (ref, "ref")):
-            _words(x, what)
+            _words(x, what, self.dev)
         self.k, self.v, self.table, self.len, self.ref = k, v, table, len, ref
         self.layers, self.pages, self.kv, self.page, self.d = k.shape
         self.rows, ld = table.shape
@@ -827,40 +850,41 @@ class KVCache:
         return c
 
     def reset(self, stream=None):
-        _check(self._lib.gs_kv_reset(self._c, _stream_of(self.k, stream)), "gs_kv_reset")
+        _call(self.dev, self._lib.gs_kv_reset, "gs_kv_reset", self._c, _stream_of(self.dev, stream))
 
     def extend(self, add, rows=None, status=None, stream=None):
         """Room for new tokens: `add` for each of `rows` (None: every row), a
         number or a tensor of one per row."""
-        n = self.rows if rows is None else rows.numel()
+        n, dev = self.rows if rows is None else rows.numel(), self.dev
         each = isinstance(add, int)
-        _check(self._lib.gs_kv_extend(self._c, _words(rows, "rows"), n, None if each else _words(add, "add", n),
-                                      add if each else 0, _words(status, "status", n), _stream_of(self.k, stream)),
-               "gs_kv_extend")
+        _call(dev, self._lib.gs_kv_extend, "gs_kv_extend", self._c, _words(rows, "rows", dev), n,
+              None if each else _words(add, "add", dev, n), add if each else 0, _words(status, "status", dev, n),
+              _stream_of(self.dev, stream))
 
     def fork(self, src, dst, status=None, stream=None):
         """Rows dst become copies of rows src, sharing their full pages (-1: empty)."""
-        n = dst.numel()
-        _check(self._lib.gs_kv_fork(self._c, _words(src, "src", n), _words(dst, "dst"), n, _words(status, "status", n),
-                                    _stream_of(self.k, stream)), "gs_kv_fork")
+        n, dev = dst.numel(), self.dev
+        _call(dev, self._lib.gs_kv_fork, "gs_kv_fork", self._c, _words(src, "src", dev, n), _words(dst, "dst", dev), n,
+              _words(status, "status", dev, n), _stream_of(self.dev, stream))
 
     def free(self, rows, stream=None):
-        _check(self._lib.gs_kv_free(self._c, _words(rows, "rows"), rows.numel(), _stream_of(self.k, stream)), "gs_kv_free")
+        _call(self.dev, self._lib.gs_kv_free, "gs_kv_free", self._c, _words(rows, "rows", self.dev), rows.numel(),
+              _stream_of(self.dev, stream))
 
     def drop(self, start, end, rows, rope=None, status=None, stream=None):
         """Tokens start .. end - 1 of each of `rows` leave it (gs_kv_drop); with
         `rope` the keys after them are turned back to their new positions."""
-        n, turn = rows.numel(), _turn(rope)
-        _check(self._lib.gs_kv_drop(self._c, _words(rows, "rows"), n, _words(start, "start", n), _words(end, "end", n),
-                                    turn, _words(status, "status", n),
-                                    _stream_of(self.k, stream)), "gs_kv_drop")
+        turn = _turn(rope)
+        n, dev = rows.numel(), self.dev
+        _call(dev, self._lib.gs_kv_drop, "gs_kv_drop", self._c, _words(rows, "rows", dev), n, _words(start, "start", dev, n),
+              _words(end, "end", dev, n), turn, _words(status, "status", dev, n), _stream_of(self.dev, stream))
 
     def _batch(self, T, rows, q_start):
         if q_start is None:
             n = T
         else:
             n = q_start.numel() - 1
-        return GsKVBatch(n, T, _words(rows, "rows", n), _words(q_start, "q_start"))
+        return GsKVBatch(n, T, _words(rows, "rows", self.dev, n), _words(q_start, "q_start", self.dev))
 
     def append(self, layer, k, v, q=None, q_out=None, rope=None, rows=None, q_start=None, stream=None):
         """The newest tokens' keys and values [T, kv heads, d] (float32 or the
@@ -868,23 +892,23 @@ class KVCache:
         `rope`; q [T, heads, d] turned to q_out (None: in place).  One token
         for each of `rows` (None: row i), or those from q_start[i] to
         q_start[i + 1]."""
-        turn = _turn(rope)
-        T, _, _, ld_k = _heads(k, "k", self.kv, self.d)
-        Tv, _, _, ld_v = _heads(v, "v", self.kv, self.d)
+        turn, dev = _turn(rope), self.dev
+        T, _, _, ld_k = _heads(k, "k", dev, self.kv, self.d)
+        Tv, _, _, ld_v = _heads(v, "v", dev, self.kv, self.d)
         if Tv != T or v.dtype != k.dtype:
             raise ValueError("v must be as k")
         x = GsKVNew(_type(k, "k"), k.data_ptr(), v.data_ptr(), ld_k, ld_v, None, 0, None, 0, 0, 0)
         if q is not None:
             q_out = q if q_out is None else q_out
-            Tq, heads, _, ld_q = _heads(q, "q", d=self.d)
-            To, _, _, ld_o = _heads(q_out, "q_out", heads, self.d)
+            Tq, heads, _, ld_q = _heads(q, "q", dev, d=self.d)
+            To, _, _, ld_o = _heads(q_out, "q_out", dev, heads, self.d)
             if Tq != T or To != T or q.dtype != k.dtype:
                 raise ValueError("q must have k's tokens and type, q_out q's heads")
             x.q, x.ld_q, x.q_out, x.ld_q_out = q.data_ptr(), ld_q, q_out.data_ptr(), ld_o
             x.q_out_type, x.n_heads = _type(q_out, "q_out"), heads
         b = self._batch(T, rows, q_start)
-        _check(self._lib.gs_kv_append(self._c, layer, ctypes.byref(b), turn, ctypes.byref(x), _stream_of(self.k, stream)),
-               "gs_kv_append")
+        _call(dev, self._lib.gs_kv_append, "gs_kv_append", self._c, layer, ctypes.byref(b), turn, ctypes.byref(x),
+              _stream_of(self.dev, stream))
 
     def attend(self, layer, q, out=None, rows=None, q_start=None, scale=0.0, window=0, max_q=0, stream=None):
         """Causal attention of the rows' newest tokens (as append takes them) over
@@ -893,10 +917,10 @@ class KVCache:
         sees, itself included (0: all).  max_q: the most tokens of one
         sequence, if the caller knows it."""
         import torch
-        T, heads, _, ld_q = _heads(q, "q", d=self.d)
-        st = _stream_of(self.k, stream)
+        T, heads, _, ld_q = _heads(q, "q", self.dev, d=self.d)
+        st = _stream_of(self.dev, stream)
         out = _empty_on(st, (T, heads, self.d), q.dtype, q) if out is None else out
-        To, _, _, ld_o = _heads(out, "out", heads, self.d)
+        To, _, _, ld_o = _heads(out, "out", self.dev, heads, self.d)
         if To != T or out.dtype != q.dtype:
             raise ValueError("out must be as q")
         ws = self._attn_ws.get((st, heads))         # calls on one stream do not overlap
@@ -908,7 +932,7 @@ class KVCache:
         b = self._batch(T, rows, q_start)
         a = GsAttnArgs(_type(q, "q"), heads, q.data_ptr(), ld_q, out.data_ptr(), ld_o, scale, window, max_q, ws.data_ptr(),
                        ws.numel())
-        _check(self._lib.gs_attn(self._c, layer, ctypes.byref(b), ctypes.byref(a), st), "gs_attn")
+        _call(self.dev, self._lib.gs_attn, "gs_attn", self._c, layer, ctypes.byref(b), ctypes.byref(a), st)
         return out
 
 

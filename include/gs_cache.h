@@ -11,7 +11,7 @@
  * range of tokens leaves a row without a second run of the prompt
  * (gs_kv_drop).
  *
- * All state is device memory that the caller owns, and every call is
+ * All state is memory of the current HIP device that the caller owns, and every call is
  * asynchronous on its stream, allocates nothing and can be captured in a HIP
  * graph, as the calls of gs_decode.h.  Calls on one cache are ordered by the
  * caller (one stream, or events between them): each reads what the last one

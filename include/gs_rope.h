@@ -56,7 +56,7 @@ typedef struct gs_rope_params {
 typedef struct gs_rope gs_rope;
 
 /* The plan: each pair's turns per position as a 64-bit fraction, on the
- * current HIP device.  A position's turns are then an integer product whose
+ * current HIP device (calls with it on another one are GS_ERR_INVALID).  A position's turns are then an integer product whose
  * whole turns fall off by themselves: angles are as exact at position 2^31 as
  * at 1, where p f_i in f32 is off by p 2^-25 radians.  Synchronous. */
 int gs_rope_create(const gs_rope_params *p, gs_rope **out);

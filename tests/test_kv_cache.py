@@ -588,3 +588,78 @@ def test_a_closed_rotation_writes_nothing(gpu, torch):
         with pytest.raises(ValueError):
             call()
     m.check(c)
+
+
+@pytest.mark.gpu
+def test_tensors_of_other_devices_are_refused(gpu, torch):
+    c = gpu.KVCache.empty(1, 4, 2, 64, 2, 32, page=16)
+    for i in range(5):
+        x = [c.k, c.v, c.table, c.len, c.ref]
+        x[i] = x[i].cpu()
+        with pytest.raises(TypeError):
+            gpu.KVCache(*x)
+    c.extend(1)
+    k, q, pos = torch.randn((2, 2, 64), device="cuda"), torch.randn((2, 4, 64), device="cuda"), words(torch, [0, 1])
+    for call in (lambda: c.append(0, k, k.cpu()), lambda: c.append(0, k, k, q=q, q_out=q.cpu()), lambda: c.attend(0, q, q.cpu()),
+                 lambda: c.append(0, k, k, rows=pos.cpu()), lambda: c.drop(pos, pos.cpu(), pos),
+                 lambda: gpu.Rope(64).apply(k, pos, out=k.cpu()), lambda: gpu.Rope(64).apply(k.cpu(), pos)):
+        with pytest.raises(TypeError):
+            call()
+
+
+@pytest.mark.gpu
+def test_calls_make_the_tensors_device_current(gpu, torch, monkeypatch):
+    """With another device current, which is only said here."""
+    c, m = make(gpu, torch)
+    rope, k, q, rows = gpu.Rope(64), torch.randn((1, 2, 64), device="cuda"), torch.randn((1, 4, 64), device="cuda"), words(torch, [1])
+    out, status, to = torch.empty_like(q), words(torch, [7]), words(torch, [2])
+    c.attend(0, q, out, rows=rows)
+    on = []
+
+    class Device:
+        def __init__(self, device):
+            on.append(device)
+
+        def __enter__(self):
+            pass
+
+        def __exit__(self, *a):
+            pass
+
+    dt = gpu._dtypes()
+    monkeypatch.setattr(gpu, "_DT", dt[:3] + (lambda: 1,))
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    for call in (lambda: c.extend(20, rows=rows), lambda: c.append(0, k, k, q=q, q_out=out, rope=rope, rows=rows),
+                 lambda: c.attend(0, q, out, rows=rows), lambda: c.fork(rows, to, status=status), lambda: rope.apply(q, rows, out=out),
+                 lambda: c.drop(rows, to, rows, rope=rope), lambda: c.free(to), lambda: c.reset()):
+        call()
+        assert on == [0]
+        on.clear()
+    assert status.cpu().tolist() == [0]
+
+
+@pytest.mark.gpu
+def test_a_rotation_of_another_device_is_refused(gpu, torch):
+    """A copy of a plan (struct gs_rope of csrc/gs_cache.hpp) that says device 1."""
+    class Plan(ctypes.Structure):
+        _fields_ = [("d", ctypes.c_uint32), ("rot", ctypes.c_uint32), ("layout", ctypes.c_uint32), ("gain", ctypes.c_float),
+                    ("device", ctypes.c_int), ("turns", ctypes.c_void_p)]
+
+    c, m = make(gpu, torch)
+    rows = words(torch, [1])
+    c.extend(40, rows=rows)
+    m.extend([1], [40])
+    rope = gpu.Rope(64)
+    k, pos = torch.randn((1, 2, 64), device="cuda"), words(torch, [3])
+    keep, plan = rope._h, Plan.from_buffer_copy(Plan.from_address(rope._h.value))
+    assert (plan.d, plan.rot, plan.layout, plan.device) == (64, 64, 1, torch.cuda.current_device())
+    plan.device += 1
+    rope._h = ctypes.c_void_p(ctypes.addressof(plan))
+    try:
+        for call in (lambda: c.append(0, k, k, rope=rope, rows=rows), lambda: c.drop(pos, words(torch, [9]), rows, rope=rope),
+                     lambda: rope.apply(k, pos)):
+            with pytest.raises(gpu.SamplerError):
+                call()
+    finally:
+        rope._h = keep
+    m.check(c)

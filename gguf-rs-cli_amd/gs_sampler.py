@@ -915,7 +915,11 @@ class KVCache:
         the rows' pages: q and out [T, heads, d] (float32 or the cache's type;
         out None: a new tensor).  window: how many positions back a token
         sees, itself included (0: all).  max_q: the most tokens of one
-        sequence, if the caller knows it."""
+        sequence, if the caller knows it.
+        The cache keeps a workspace of 43 to 85 MB for each stream that attend
+        was called on.  A captured graph uses that of the stream it was captured
+        on, wherever it is replayed: replays of such graphs, and calls on that
+        stream, must not overlap."""
         import torch
         T, heads, _, ld_q = _heads(q, "q", self.dev, d=self.d)
         st = _stream_of(self.dev, stream)
@@ -928,7 +932,9 @@ class KVCache:
             n = self._lib.gs_attn_workspace(self._c, heads)
             if not n:
                 raise SamplerError(GS_ERR_INVALID, "gs_attn_workspace")
-            ws = self._attn_ws[st, heads] = _empty_on(st, n, torch.uint8, q)
+            # (its size depends on the heads' values, not on their number)
+            ws = next((w for (s, _), w in self._attn_ws.items() if s == st and w.numel() >= n), None)
+            ws = self._attn_ws[st, heads] = _empty_on(st, n, torch.uint8, q) if ws is None else ws
         b = self._batch(T, rows, q_start)
         a = GsAttnArgs(_type(q, "q"), heads, q.data_ptr(), ld_q, out.data_ptr(), ld_o, scale, window, max_q, ws.data_ptr(),
                        ws.numel())

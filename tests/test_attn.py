@@ -479,3 +479,19 @@ def test_memory_of_another_stream(gpu, torch):
     torch.cuda.synchronize()
     assert c._attn_ws[other.cuda_stream, 4].data_ptr() != places[0] and got.data_ptr() != places[1]
     assert torch.equal(got, here)
+
+
+@pytest.mark.gpu
+def test_one_workspace_of_a_stream(gpu, torch):
+    """Calls of other numbers of heads share it; another stream has its own."""
+    c = build(gpu, torch, [100, 31], 2, 64, 16, "float16", seed=9)
+    q = torch.randn((2, 8, 64), device="cuda")
+    for heads in (2, 8, 4):
+        check(c.attend(0, q[:, :heads]), want(c, 0, q[:, :heads], [0, 1], [1, 1]))
+    assert len({w.data_ptr() for w in c._attn_ws.values()}) == 1
+    here = c.attend(0, q)
+    torch.cuda.synchronize()
+    other = torch.cuda.Stream()
+    got = c.attend(0, q, stream=other)
+    torch.cuda.synchronize()
+    assert torch.equal(got, here) and len({w.data_ptr() for w in c._attn_ws.values()}) == 2

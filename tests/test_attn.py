@@ -332,6 +332,25 @@ def test_scores_far_apart(gpu, torch, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("d", [64, 80, 128, 256])
+def test_scores_far_apart_in_chunks(gpu, torch, dtype, d):
+    """The same for chunks: the largest scores first, in the middle of a tile,
+    late after many tiles and last; scales given by the caller, also below 0."""
+    lens, news = [1500, 700, 333], [150, 300, 333]
+    c = build(gpu, torch, lens, 1, d, 16, dtype, seed=4)
+    for r, t, f in ((0, 3, 5.0), (0, 37, 9.0), (0, 1400, 12.0), (0, 1499, 14.0), (1, 450, 10.0), (1, 699, 9.0), (2, 0, 12.0), (2, 300, 6.0)):
+        c.k[0, int(c.table[r, t // 16]), 0, t % 16] *= f
+    q = (torch.randn((sum(news), 2, d), generator=torch.Generator("cuda").manual_seed(8), device="cuda") * 2).to(getattr(torch, dtype))
+    start = starts(torch, news)
+    for scale in (0.0, 0.3, -0.05, -1.0 / math.sqrt(d)):
+        check(c.attend(0, q, q_start=start, max_q=333, scale=scale),
+              want(c, 0, q, [0, 1, 2], news, scale=float(np.float32(scale)) or None))
+    check(c.attend(0, q, q_start=start, max_q=333, scale=-0.2, window=70),
+          want(c, 0, q, [0, 1, 2], news, scale=float(np.float32(-0.2)), window=70))
+
+
+@pytest.mark.gpu
 def test_queries_of_any_size(gpu, torch):
     """f32 queries beyond f16's range, and small ones."""
     c = build(gpu, torch, [300], 1, 64, 16, "float16", seed=5)

@@ -122,3 +122,86 @@ def test_generate_past_the_context(example, torch):
         assert torch.equal(ref, m.cache.ref)
         assert m.cache.len.cpu().tolist()[:3] == [0, 0, 0] and int(m.cache.len.max()) <= 192
     assert runs[0] == runs[1] and all(len(r) == 120 for r in runs[0])
+
+
+class Dense:
+    """One conversation in 64 bits: keys before their rotation and values of
+    each layer, and what happens to them."""
+
+    def __init__(self, model):
+        c, self.m = model.cfg, model
+        h, d, H, kv = c["hidden"], c["d"], c["heads"], c["kv"]
+        shapes = dict(qkv=((H + 2 * kv) * d, h), o=(h, H * d), gate=(c["ffn"], h), up=(c["ffn"], h), down=(h, c["ffn"]))
+        self.w = [{n: matrix(b[n], *s) for n, s in shapes.items()} for b in model.blocks]
+        self.head = matrix(model.head_blocks, c["vocab"], h)
+        self.embed = model.embed.double().cpu().numpy()
+        self.k = [np.empty((0, kv, d)) for _ in self.w]
+        self.v = [np.empty((0, kv, d)) for _ in self.w]
+
+    def turn(self, x, first):
+        """x [n, heads, d] at positions first ..: as complex numbers."""
+        d = self.m.cfg["d"]
+        ang = (first + np.arange(len(x)))[:, None] * self.m.cfg["base"] ** (-2.0 * np.arange(d // 2) / d)
+        z = (x[..., :d // 2] + 1j * x[..., d // 2:]) * np.exp(1j * ang)[:, None]
+        return np.concatenate([z.real, z.imag], -1)
+
+    def add(self, tokens):
+        """The logits after the last of them."""
+        c = self.m.cfg
+        d, H, kv, n = c["d"], c["heads"], c["kv"], len(tokens)
+        norm = lambda x: x / np.sqrt((x * x).mean(-1, keepdims=True) + 1e-6)  # noqa: E731
+        x = self.embed[np.array(tokens)]
+        for i, w in enumerate(self.w):
+            y = (norm(x) @ w["qkv"].T).reshape(n, -1, d)
+            held = len(self.k[i])
+            self.k[i], self.v[i] = np.concatenate([self.k[i], y[:, H:H + kv]]), np.concatenate([self.v[i], y[:, H + kv:]])
+            q, k = self.turn(y[:, :H], held), self.turn(self.k[i], 0)
+            a = np.empty((n, H, d))
+            for t in range(n):
+                for j in range(H):
+                    s = k[:held + t + 1, j * kv // H] @ q[t, j] / np.sqrt(d)
+                    e = np.exp(s - s.max())
+                    a[t, j] = e / e.sum() @ self.v[i][:held + t + 1, j * kv // H]
+            x = x + a.reshape(n, -1) @ w["o"].T
+            y = norm(x)
+            g = y @ w["gate"].T
+            x = x + (g / (1 + np.exp(-g)) * (y @ w["up"].T)) @ w["down"].T
+        return self.head @ norm(x[-1])
+
+    def drop(self, start, end):
+        self.k, self.v = ([np.delete(x, slice(start, end), 0) for x in y] for y in (self.k, self.v))
+
+
+@pytest.mark.gpu
+def test_tokens_after_a_drop(example, torch):
+    """Rows that own their pages and rows that share them lose tokens, twice, and
+    go on: the logits of a model that moves its own keys and values.  A drop
+    rounds the moved keys once more: 3 effects per layer in place of 2, and 4
+    after the second, of two layers: 16 x 2^-11 of the norm."""
+    rng = np.random.default_rng(5)
+    m = example.PagedModel(example.SMALL, 4, 48)
+    seqs = [rng.integers(0, 4096, k).tolist() for k in (150, 61)]
+    dense = [Dense(m) for _ in seqs]
+    for x, s in zip(dense, seqs):
+        x.add(s)
+    rows = example.words([0, 1])
+    m.cache.extend(example.words([150, 61]), rows=rows)
+    m.forward(example.words(sum(seqs, [])), rows, example.words([0, 150, 211]), 150)
+    m.cache.fork(example.words([0]), example.words([3]))        # row 0's full pages are shared now, row 1's are its own
+    for cut, new in (([(8, 77), (5, 6)], 3), ([(0, 20), (30, 63)], 2)):
+        m.cache.drop(example.words([a for a, _ in cut]), example.words([b for _, b in cut]), rows, rope=m.rope)
+        for x, (a, b) in zip(dense, cut):
+            x.drop(a, b)
+        for _ in range(new):
+            tokens = rng.integers(0, 4096, 2).tolist()
+            m.cache.extend(1, rows=rows)
+            got = logits_of(m, m.forward(example.words(tokens), rows), torch)
+            for g, x, t in zip(got, dense, tokens):
+                want = x.add([t])
+                assert np.linalg.norm(g - want) <= 16 * 2.0 ** -11 * np.linalg.norm(want)
+    # the fork still holds all of its tokens
+    m.cache.extend(1, rows=example.words([3]))
+    whole = seqs[0] + [7]
+    got = logits_of(m, m.forward(example.words([7]), example.words([3])), torch)
+    assert near(got[0], dense_logits(m, np.array(whole)))
+    assert [len(x.k[0]) for x in dense] == m.cache.len.cpu().tolist()[:2]

@@ -857,6 +857,8 @@ class KVCache:
         number or a tensor of one per row."""
         n, dev = self.rows if rows is None else rows.numel(), self.dev
         each = isinstance(add, int)
+        if each and not 0 <= add <= 0xFFFFFFFF:
+            raise ValueError("add must be a number of tokens")
         _call(dev, self._lib.gs_kv_extend, "gs_kv_extend", self._c, _words(rows, "rows", dev), n,
               None if each else _words(add, "add", dev, n), add if each else 0, _words(status, "status", dev, n),
               _stream_of(self.dev, stream))

@@ -663,3 +663,13 @@ def test_a_rotation_of_another_device_is_refused(gpu, torch):
     finally:
         rope._h = keep
     m.check(c)
+
+
+def test_extend_by_no_number_of_tokens_without_gpu():
+    """A C uint32 would take them modulo 2^32."""
+    import gs_sampler as gs
+    cache = gs.KVCache.__new__(gs.KVCache)
+    cache.rows, cache.dev, cache._lib = 1, 0, None                # (nothing can be called)
+    for add in (-1, 1 << 32, (1 << 32) + 5):
+        with pytest.raises(ValueError):
+            cache.extend(add)

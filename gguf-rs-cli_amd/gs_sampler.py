@@ -923,6 +923,8 @@ class KVCache:
         on, wherever it is replayed: replays of such graphs, and calls on that
         stream, must not overlap."""
         import torch
+        if not 0 <= window <= 0xFFFFFFFF:
+            raise ValueError("window must be a number of positions")
         T, heads, _, ld_q = _heads(q, "q", self.dev, d=self.d)
         st = _stream_of(self.dev, stream)
         out = _empty_on(st, (T, heads, self.d), q.dtype, q) if out is None else out

@@ -514,3 +514,13 @@ def test_one_workspace_of_a_stream(gpu, torch):
     got = c.attend(0, q, stream=other)
     torch.cuda.synchronize()
     assert torch.equal(got, here) and len({w.data_ptr() for w in c._attn_ws.values()}) == 2
+
+
+def test_a_window_that_is_no_number_of_positions_without_gpu():
+    """A C uint32 would take it modulo 2^32: 2^32 + 5 as 5, -1 as none."""
+    import gs_sampler as gs
+    cache = gs.KVCache.__new__(gs.KVCache)
+    cache.dev = cache.d = 0                                             # (nothing can be called)
+    for window in (-1, (1 << 32) + 5):
+        with pytest.raises(ValueError):
+            cache.attend(0, None, window=window)

@@ -284,12 +284,14 @@ constexpr int rows_per_cu(int D, int NT) { return D == 64 || (D == 128 && NT == 
 // columns come from the 8 rows of V in a lane by a transposition of 8 x 8
 // values in registers (the value a lane's row m stands for is 8 m + i in
 // product i).  Four waves' sums meet in LDS at a unit's end.
-// The second product's factors are of T: a weight goes in as two of them, its
-// rounding and the rest, which hold 22 bits of it (bf16: 16), one product more
-// where the matrix cores have the time.  (us with one and two: 64 rows of 16000,
-// 28 / 4 heads of 128, bf16, 356, 357; 4 tokens each, 64 / 8 heads, 699, 711; 64
-// over 1000 to 32768 206 and 206, there the outputs' relative distance to 32-bit
-// weights' 6.8e-4 and 4e-5.)  Their sum is in f32.
+// The second product's factors are of T.  A bf16 weight goes in as two of them,
+// its rounding and the rest, 16 bits together, one product more where the matrix
+// cores have the time; an f16 weight is rounded once, off by 2^-11 of itself at
+// most and without a common direction, a quarter of what the rounding
+// of the result adds.  (us with one and two: 64 single tokens over 1000 to 32768,
+// bf16, 206, 206, the outputs' relative distance to 32-bit weights' 6.8e-4, 4e-5;
+// 64 sequences of 8 over 8000, 32 / 8 heads of 64, bf16 182, 185, f16 184, 194;
+// of 128, bf16 364, 367, f16 362, 370.)  Their sum is of the unrounded ones, in f32.
 // Measured: 64 rows of 16000 tokens, 28 / 4 heads of 128, bf16: 353 us, 5.9
 // TB/s, what a read of this size reaches; one token over 4001: 10 us, of which
 // the empty launch, the search for the run's begin and three waits in a row
@@ -301,7 +303,7 @@ constexpr int rows_per_cu(int D, int NT) { return D == 64 || (D == 128 && NT == 
 template <class T, int D, int NT, bool F32, bool FULL>
 __global__ void __launch_bounds__(256, rows_per_cu(D, NT)) attn_rows_kernel(const AttnArgs a)
 {
-    constexpr int R = 16 * NT, NP = F32 ? 3 : 1, NW = F32 ? 3 : 2, KS = D / 32;
+    constexpr int R = 16 * NT, NP = F32 ? 3 : 1, NW = F32 ? 3 : __is_same(T, __bf16) ? 2 : 1, KS = D / 32;
     constexpr int CW = D >= 128 ? 8 : D / 16, NC = D / (16 * CW);       // values of a lane's V chunk, chunks
     typedef typename Vec<T>::v8 v8;
     typedef T vw __attribute__((ext_vector_type(CW)));
@@ -533,7 +535,7 @@ __global__ void __launch_bounds__(256, rows_per_cu(D, NT)) attn_rows_kernel(cons
                 for (int j = 0; j < 8; j++) {
                     pf[nt][0][j] = (T)p[nt][j];
                     const float y = p[nt][j] - (float)pf[nt][0][j];
-                    pf[nt][1][j] = (T)y;
+                    if constexpr (NW > 1) pf[nt][1][j] = (T)y;
                     if constexpr (F32) pf[nt][2][j] = (T)(y - (float)pf[nt][1][j]);
                 }
 #pragma unroll
@@ -544,9 +546,9 @@ __global__ void __launch_bounds__(256, rows_per_cu(D, NT)) attn_rows_kernel(cons
 #pragma unroll
                     for (int j = 0; j < 8; j++) x8[j] = vf[j][c][i];
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
+                    for (int q = NW - 1; q >= 0; q--)           // (neighbours do not wait for one another)
 #pragma unroll
-                        for (int q = NW - 1; q >= 0; q--) o[nt][c][i] = mfma(x8, pf[nt][q], o[nt][c][i]);
+                        for (int nt = 0; nt < NT; nt++) o[nt][c][i] = mfma(x8, pf[nt][q], o[nt][c][i]);
                 }
             for (; bad; bad &= bad - 1) {
                 const uint32_t y = __ffs(bad) - 1;
@@ -650,7 +652,7 @@ __global__ void __launch_bounds__(256, rows_per_cu(D, NT)) attn_rows_kernel(cons
                     for (int i = 0; i < CW; i += 4)
                         *(f4 *)&s_o[w][m][16 * CW * c + CW * (4 * g + e) + i] =
                             f4{o[nt][c][i][e], o[nt][c][i + 1][e], o[nt][c][i + 2][e], o[nt][c][i + 3][e]};
-            for (; again; again &= again - 1) {
+            for (; __builtin_expect(again != 0, 0); again &= again - 1) {
                 const uint32_t r = r0 + 16 * nt + __ffsll((unsigned long long)again) - 1;
                 if (r < r1) alone(r);
             }

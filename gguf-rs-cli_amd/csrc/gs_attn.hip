@@ -287,15 +287,15 @@ constexpr int rows_per_cu(int D, int NT) { return D == 64 || (D == 128 && NT == 
 // The second product's factors are of T.  A bf16 weight goes in as two of them,
 // its rounding and the rest, 16 bits together, one product more where the matrix
 // cores have the time; an f16 weight is rounded once, off by 2^-11 of itself at
-// most and without a common direction, a quarter of what the rounding
-// of the result adds.  (us with one and two: 64 single tokens over 1000 to 32768,
+// most and without a common direction, a quarter of what the rounding of the
+// result adds.  (us with one and two: 64 single tokens over 1000 to 32768,
 // bf16, 206, 206, the outputs' relative distance to 32-bit weights' 6.8e-4, 4e-5;
 // 64 sequences of 8 over 8000, 32 / 8 heads of 64, bf16 182, 185, f16 184, 194;
 // of 128, bf16 364, 367, f16 362, 370.)  Their sum is of the unrounded ones, in f32.
-// Measured: 64 rows of 16000 tokens, 28 / 4 heads of 128, bf16: 353 us, 5.9
-// TB/s, what a read of this size reaches; one token over 4001: 10 us, of which
-// the empty launch, the search for the run's begin and three waits in a row
-// for memory (table, keys, values) are most.
+// Measured: 64 rows of 16000 tokens, 28 / 4 heads of 128, bf16: 357 us, 5.9
+// TB/s, what a read of this size reaches; one token over 4001, f32: 9.7 us of
+// kernel, most of them the search for the run's begin and three waits in a row
+// for memory (table, keys, values).
 // F32: q in three parts of T whose sum is q (scaled by a power of two into
 // f16's range), and the weights too, so the products keep 24 bits.
 // FULL: heads of just D values (their strides are then constants, which takes
@@ -743,12 +743,12 @@ constexpr int kChunkRuns = 256;         // one workgroup per CU
 // -> 1641 us; one chunk of 8192, bf16, 664 -> 827.  Without it the relative error
 // of the output, most of it the result's own rounding, is 2.16e-4 for 2.09e-4
 // (f16) and, in a call of chunks and single tokens, 1.74e-3 for 1.66e-3 (bf16).
-// Measured: four chunks of 2048 tokens over 8192, 32 / 8 heads of 128, f16: 710
-// to 880 TFLOP/s from card to card (a library product of 8192 x 8192 x 8192:
-// 1140), heads of 64 610, of 256 600 to 640.  No bank is met twice.  With 14 % fewer clocks per tile the
-// card lowered its frequency from 2.09 to 1.81 GHz and the time stayed: what
-// is left is power, of which each pass of keys and values through LDS for 32
-// rows is a part (64 rows of a wave do not fit its registers).
+// Measured: four chunks of 2048 tokens over 8192, 32 / 8 heads of 128, f16: 740
+// TFLOP/s, one chunk of 1024 over 32768, bf16: 850 (a library product of 8192 x
+// 8192 x 8192: 1140 and 1200), heads of 64 620, of 256 660.  No bank is met twice;
+// vector issue is half of the clocks, the matrix cores two fifths.  Each pass of
+// keys and values through LDS serves 32 rows of a wave (64 do not fit its
+// registers).
 template <class T, int D, bool FULL>
 __global__ void __launch_bounds__(Chunk<D>::kThreads, 2) attn_chunk_kernel(const AttnArgs a)
 {
@@ -1140,9 +1140,9 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, 2) attn_chunk_kernel(const
 // The parts of the unit that run g begins and another ends.  The
 // threads of a row (D / 4 of them, 4 values each) first share out its parts'
 // maximums and sums, up to kWide at a time, and then add the parts in order,
-// eight reads at a time: what bounds it is the chain of reads.  (One token over
-// 4001, 4 heads of keys: 4.7 us, an empty launch's 3.6 among them; four chunks
-// of 2048 over up to 8192: 18 us.  Joining in the first kernel by the last run
+// eight reads at a time: what bounds it is the chain of reads.  (Of kernel: one
+// token over 4001, 4 heads of keys: 5.1 us; four chunks of 2048 over up to 8192:
+// 18 us.  Joining in the first kernel by the last run
 // to come needs a release to the other XCDs by each run: 64 single tokens 206
 // us like this, 368 so.)
 template <class TO, int D, int R> __device__ __forceinline__ void join_unit(const AttnArgs &a, uint32_t g)
@@ -1269,18 +1269,18 @@ template <class T, int D, bool F32> int by_rows(gs::AttnArgs &a, uint64_t rows, 
     if constexpr (F32) {
         // f32 queries of any number go to the first kernel: its products are
         // three for one, and four chunks of 512 tokens over 8192, 32 / 8 heads
-        // of 128, take 1250 us (640 TFLOP/s of products).
+        // of 128, take 1230 us (650 TFLOP/s of products; a bf16 cache: 1130).
         if constexpr (D == 256) return rows_call<T, D, 1, F32>(a, st);      // (two tiles of rows spill)
         else return rows_call<T, D, 2, F32>(a, st);
     } else {
         if constexpr (D != 256)
             if (rows <= 32) return rows_call<T, D, 2, F32>(a, st);
         // Sequences of a few rows go to the first kernel, the others to the
-        // second.  (us, first and second; 64 sequences of 8000, 8 heads of keys:
-        // of 64, 32 rows: 184, 262; 48: 358, 289; of 128, 32 rows: 355, 378;
-        // 48: 697, 399; of 256, 16 rows: 687, 731; 24: 1361, 734.  Four of
-        // 4000, where the time is launches and waits: of 128, 16 rows: 23,
-        // 25; 32: 28, 26; of 256, 16: 35, 33.)
+        // second.  (us, first and second, f16 as bf16; 64 sequences of 8000, 8
+        // heads of keys: of 64, 32 rows: 195, 267; 48: 371, 282; of 128, 32
+        // rows: 367, 381; 48: 719, 411; of 256, 16 rows: 692, 735; 24: 1364,
+        // 738.  Four of 4000, where the time is launches and waits: of 128, 16
+        // rows: 24, 25; 32: 30, 26; of 256, 16: 35, 33.)
         constexpr int kFew = D == 256 ? 16 : 32;
         constexpr int R = gs::Chunk<D>::kRows;
         if ((uint64_t)a.n_tokens * a.group == rows * a.n) {     // (all of the same length, or the caller's most is wrong)

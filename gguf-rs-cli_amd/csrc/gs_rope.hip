@@ -49,8 +49,8 @@ __device__ __forceinline__ uint32_t quotient(uint32_t n, uint32_t d, uint32_t m)
 // are not multiples of the vectors.
 // PAST: written past the caches.
 // Measured: 12001 x 32 x 96, bf16, 148 MB: 24.6 us, 6.0 TB/s; the new tokens of
-// one layer, 4 x 2048 x (32 + 2 x 8) x 128, f16, 201 MB: 33.6 us, 6.0 TB/s; one
-// token 2.3 to 3.2 us, an empty launch 2.2.
+// one layer, 4 x 2048 x (32 + 2 x 8) x 128, f16, 201 MB: 34 us, 5.9 TB/s; one
+// token 2.3 to 3.1 us of kernel (one that reads a word and ends: 1.3).
 template <class TI, class TO, class TC, bool VEC, bool PAST>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a)
 {

@@ -284,14 +284,15 @@ constexpr int rows_per_cu(int D, int NT) { return D == 64 || (D == 128 && NT == 
 // columns come from the 8 rows of V in a lane by a transposition of 8 x 8
 // values in registers (the value a lane's row m stands for is 8 m + i in
 // product i).  Four waves' sums meet in LDS at a unit's end.
-// The second product's factors are of T.  A bf16 weight goes in as two of them,
-// its rounding and the rest, 16 bits together, one product more where the matrix
-// cores have the time; an f16 weight is rounded once, off by 2^-11 of itself at
-// most and without a common direction, a quarter of what the rounding of the
-// result adds.  (us with one and two: 64 single tokens over 1000 to 32768,
-// bf16, 206, 206, the outputs' relative distance to 32-bit weights' 6.8e-4, 4e-5;
-// 64 sequences of 8 over 8000, 32 / 8 heads of 64, bf16 182, 185, f16 184, 194;
-// of 128, bf16 364, 367, f16 362, 370.)  Their sum is of the unrounded ones, in f32.
+// The second product's factors are of T.  With up to 16 rows a bf16 weight goes in
+// as two of them, its rounding and the rest, 16 bits together: one product more,
+// where the matrix cores have the time.  Others are rounded once, off by 2^-11 of
+// themselves (bf16: 2^-8) at most and without a common direction, a quarter of
+// what the rounding of the result adds.  (us with one and two: 64 single tokens
+// over 1000 to 32768, bf16, 206, 206, the outputs' relative distance to 32-bit
+// weights' 6.8e-4, 4e-5; 64 sequences of 8 over 8000, 32 rows of 32 / 8 heads of
+// 128, bf16 390, 419; of 64, f16 184, 194.)  Their sum is of the unrounded ones,
+// in f32.
 // Measured: 64 rows of 16000 tokens, 28 / 4 heads of 128, bf16: 357 us, 5.9
 // TB/s, what a read of this size reaches; one token over 4001, f32: 9.7 us of
 // kernel, most of them the search for the run's begin and three waits in a row
@@ -303,7 +304,7 @@ constexpr int rows_per_cu(int D, int NT) { return D == 64 || (D == 128 && NT == 
 template <class T, int D, int NT, bool F32, bool FULL>
 __global__ void __launch_bounds__(256, rows_per_cu(D, NT)) attn_rows_kernel(const AttnArgs a)
 {
-    constexpr int R = 16 * NT, NP = F32 ? 3 : 1, NW = F32 ? 3 : __is_same(T, __bf16) ? 2 : 1, KS = D / 32;
+    constexpr int R = 16 * NT, NP = F32 ? 3 : 1, NW = F32 ? 3 : __is_same(T, __bf16) && NT == 1 ? 2 : 1, KS = D / 32;
     constexpr int CW = D >= 128 ? 8 : D / 16, NC = D / (16 * CW);       // values of a lane's V chunk, chunks
     typedef typename Vec<T>::v8 v8;
     typedef T vw __attribute__((ext_vector_type(CW)));
@@ -1276,11 +1277,11 @@ template <class T, int D, bool F32> int by_rows(gs::AttnArgs &a, uint64_t rows, 
         if constexpr (D != 256)
             if (rows <= 32) return rows_call<T, D, 2, F32>(a, st);
         // Sequences of a few rows go to the first kernel, the others to the
-        // second.  (us, first and second, f16 as bf16; 64 sequences of 8000, 8
-        // heads of keys: of 64, 32 rows: 195, 267; 48: 371, 282; of 128, 32
-        // rows: 367, 381; 48: 719, 411; of 256, 16 rows: 692, 735; 24: 1364,
-        // 738.  Four of 4000, where the time is launches and waits: of 128, 16
-        // rows: 24, 25; 32: 30, 26; of 256, 16: 35, 33.)
+        // second.  (us, first and second, f16; 64 sequences of 8000, 8 heads of
+        // keys: of 64, 32 rows: 204, 295; 48: 367, 287; of 128, 32 rows: 362,
+        // 384; 48: 713, 425; of 256, 16 rows: 688, 736; 24: 1366, 739.  Four of
+        // 4000, where the time is launches and waits: of 128, 16 rows: 23, 25;
+        // 32: 30, 26; of 256, 16: 35, 33.)
         constexpr int kFew = D == 256 ? 16 : 32;
         constexpr int R = gs::Chunk<D>::kRows;
         if ((uint64_t)a.n_tokens * a.group == rows * a.n) {     // (all of the same length, or the caller's most is wrong)

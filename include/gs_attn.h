@@ -48,9 +48,9 @@ size_t gs_attn_workspace(const gs_kv_cache *c, uint32_t n_heads);
  * both factors of a product in one type.  With F32 q, q and the weights go
  * through them in three parts of the cache's type, which hold 24 bits.  With q
  * of the cache's type the weights are rounded to that type once, but BF16 weights
- * of sequences with at most 32 rows of queries per head of keys (16 for heads of
- * more than 128) go in two parts, 16 bits.  Two calls with the same arguments
- * give the same bits.  Asynchronous on `stream`. */
+ * go in two parts, 16 bits, in calls whose sequences have at most 16 rows of
+ * queries per head of keys, as single tokens mostly are.  Two calls with the
+ * same arguments give the same bits.  Asynchronous on `stream`. */
 int gs_attn(const gs_kv_cache *c, uint32_t layer, const gs_kv_batch *b, const gs_attn_args *a, void *stream);
 
 #ifdef __cplusplus

@@ -127,15 +127,17 @@ def test_single_tokens(gpu, torch, lens, H, kv, d, page, dtype, cache, window):
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
 @pytest.mark.parametrize("d,H,kv,news", [(64, 8, 2, 1), (64, 8, 2, 8), (128, 16, 1, 1), (128, 8, 8, 1), (128, 28, 4, 4), (256, 8, 2, 3)])
 def test_weights_of_few_rows(gpu, torch, dtype, d, H, kv, news):
-    """16-bit queries.  A bf16 weight reaches the values in two parts, off by 2^-16
-    of itself at most, which twice the 32-bit form's (keys / 32 + 64) 2^-23
-    covers; besides, the result's own rounding.  An f16 weight is rounded once."""
+    """16-bit queries.  With up to 16 rows per head of keys a bf16 weight reaches
+    the values in two parts, off by 2^-16 of itself at most, which twice the
+    32-bit form's (keys / 32 + 64) 2^-23 covers; besides, the result's own
+    rounding.  Other weights are rounded once."""
     lens = [700, 33, 260]
     c = build(gpu, torch, lens, kv, d, 16, dtype, seed=15)
     q = torch.randn((3 * news, H, d), generator=torch.Generator("cuda").manual_seed(10), device="cuda").to(getattr(torch, dtype))
     got = c.attend(0, q, q_start=starts(torch, [news] * 3), max_q=news)
     out, tol = want(c, 0, q.float(), [0, 1, 2], [news] * 3)
-    check(got, (out, 3 * tol + U[dtype] * np.abs(out)) if dtype == "bfloat16" else want(c, 0, q, [0, 1, 2], [news] * 3))
+    two = dtype == "bfloat16" and H // kv * news <= 16
+    check(got, (out, 3 * tol + U[dtype] * np.abs(out)) if two else want(c, 0, q, [0, 1, 2], [news] * 3))
 
 
 CHUNKS = [  # lengths, new tokens, heads, kv, d, page, type, cache, window

@@ -1,5 +1,5 @@
 // gs_cache.hip -- the pages of the cache of keys and values: rows grow, are
-// forked, freed and lose tokens (include/gs_cache.h).
+// forked, freed, lose tokens and are cut to a budget (include/gs_cache.h).
 //
 // The bookkeeping is whole numbers in a fixed order, so a call's result does
 // not depend on timing: pages are counted over the rows by a scan, taken from
@@ -23,12 +23,21 @@ constexpr uint32_t kOwners = 8192;      // rows whose marks fit in LDS
 
 // One row of a fork or a drop, in ws.
 struct Move {
-    uint32_t row, from;         // fork: dst, src (GS_KV_NONE: none); drop: the row, its first token that leaves
+    uint32_t row, from;         // fork: dst, src (GS_KV_NONE: none); drop, eviction: the row, its first token that leaves
     uint32_t len, left;         // tokens before and after
     uint32_t old_len;           // fork: tokens of dst before
     uint32_t base;              // its first new page in the list
     uint32_t ok;                // 0: leave the row as it is
-    uint32_t in_place;          // drop: a written page keeps its place
+    uint32_t in_place;          // drop, eviction: a written page keeps its place
+};
+
+// Where the tokens of an eviction were: place x of row i of the call has
+// token list[i * ld + x] after it.  Ascending, and never below x.
+struct Stays {
+    uint32_t *list;
+    size_t ld;
+    float *mass;                // [rows][ld_mass]
+    size_t ld_mass;
 };
 
 struct Cache {
@@ -323,22 +332,29 @@ __global__ void __launch_bounds__(256) free_kernel(const Cache c, const uint32_t
 // that others hold too.  A wave counts a row's pages; stage[i][j] is the
 // number of new pages before place j, with the top bit where j gets one.  (One
 // row of 512 pages or 16 of up to 94: 6.7 us, a chain of reads.)
+// EVICT: what leaves is in moves already (evict_select_kernel).
+template <bool EVICT>
 __global__ void __launch_bounds__(kBook) drop_plan_kernel(const Cache c, const uint32_t *rows, uint32_t n, const uint32_t *from,
                                                           const uint32_t *to, int32_t *status)
 {
-    __shared__ uint32_t s_owner[kOwners];
-    claim(c, s_owner, rows, n);
+    __shared__ uint32_t s_owner[EVICT ? 1 : kOwners];
+    if constexpr (!EVICT) claim(c, s_owner, rows, n);
     constexpr int kPlan = 8;            // reads of 64 places that a wave has under way
     const uint32_t lane = threadIdx.x & 63;
     for (uint32_t i = threadIdx.x >> 6; i < n; i += kBook / 64) {
         Move m = {};
-        m.row = rows[i];
-        m.ok = m.row < c.rows && claimed(c, s_owner, m.row, i);
+        if constexpr (EVICT) m = c.moves[i];
+        else {
+            m.row = rows[i];
+            m.ok = m.row < c.rows && claimed(c, s_owner, m.row, i);
+        }
         uint32_t need = 0, written = 0;
         if (m.ok) {
-            m.len = row_len(c, m.row);
-            m.from = min(from[i], m.len);
-            m.left = m.len - (min(max(to[i], m.from), m.len) - m.from);
+            if constexpr (!EVICT) {
+                m.len = row_len(c, m.row);
+                m.from = min(from[i], m.len);
+                m.left = m.len - (min(max(to[i], m.from), m.len) - m.from);
+            }
             const uint32_t first = m.from >> c.shift, now = pages_of(c, m.left);
             if (m.left < m.len) {
                 const uint32_t *table = c.table + (size_t)m.row * c.ld;
@@ -408,10 +424,12 @@ enum { kMoveVector, kMovePairs, kMoveValues };
 // values of a token.  All of a step's reads come before its writes, and the
 // pages' numbers of the next step are read before both: the reads are what a
 // step waits for.  Both go past the caches (2048 of 8192 tokens, 681 MB moved:
-// 185 -> 178 us).
-template <class T, int MODE>
+// 185 -> 178 us).  EVICT: the tokens come from where `from_list` says, and each
+// is turned by its own way.
+template <class T, int MODE, bool EVICT>
 __device__ __forceinline__ void move_stream(const Cache &c, const Move &m, uint32_t i, T *base, uint32_t h, int rot, bool interleaved,
-                                            const float2 *cs, uint32_t t0, uint32_t slice, uint32_t slices)
+                                            const float2 *cs, uint32_t t0, uint32_t slice, uint32_t slices, const uint32_t *from_list,
+                                            const uint64_t *turns)
 {
     constexpr int kStep = MODE == kMoveVector ? 8 : 4, kW = MODE == kMoveValues ? 1 : 8;
     typedef T vec __attribute__((ext_vector_type(kW)));
@@ -427,15 +445,23 @@ __device__ __forceinline__ void move_stream(const Cache &c, const Move &m, uint3
     const uint32_t *table = c.table + (size_t)m.row * c.ld;
     const size_t head = (size_t)c.d << c.shift;
 
-    uint32_t to[kStep], from[kStep];            // pages
+    uint64_t by_turns[EVICT ? kW : 1];          // of this thread's pairs
+    if constexpr (EVICT) {
+        const int at = MODE == kMoveVector ? 4 * item : kW * item;
+#pragma unroll
+        for (int e = 0; e < (MODE == kMoveVector ? 4 : kW); e++) by_turns[e] = works && turned ? turns[at + e] : 0;
+    }
+    uint32_t to[kStep], from[kStep], was[kStep];        // pages, and tokens of the row before
     auto pages = [&](uint32_t t) {
 #pragma unroll
         for (int s = 0; s < kStep; s++) {
             const uint32_t x = t + s * each + tl;
             to[s] = from[s] = GS_KV_NONE;
+            was[s] = 0;
             if (!works || x >= m.left) continue;
             to[s] = new_page(c, m, i, x >> c.shift);
-            from[s] = table[(x >= m.from ? x + gone : x) >> c.shift];
+            was[s] = x < m.from ? x : EVICT ? from_list[x] : x + gone;
+            from[s] = table[was[s] >> c.shift];
         }
     };
     const uint32_t step = slices * each * kStep;
@@ -443,9 +469,11 @@ __device__ __forceinline__ void move_stream(const Cache &c, const Move &m, uint3
     for (uint32_t t = t0 + slice * each * kStep; t < m.left; t += step) {
         vec a[kStep], b[kStep];
         T *at[kStep];
+        uint32_t way[kStep];
 #pragma unroll
         for (int s = 0; s < kStep; s++) {
-            const uint32_t x = t + s * each + tl, y = x >= m.from ? x + gone : x;
+            const uint32_t x = t + s * each + tl, y = EVICT ? was[s] : x >= m.from ? x + gone : x;
+            if constexpr (EVICT) way[s] = y - x;
             at[s] = nullptr;
             if (to[s] >= c.n_pages || from[s] >= c.n_pages) continue;
             const T *f = base + ((size_t)from[s] * c.n_kv + h) * head + (y & (size - 1)) * c.d;
@@ -457,18 +485,19 @@ __device__ __forceinline__ void move_stream(const Cache &c, const Move &m, uint3
 #pragma unroll
         for (int s = 0; s < kStep; s++) {
             if (!at[s] || !turned || t + s * each + tl < m.from) continue;
+            auto turn = [&](int pair, int e) { return EVICT ? turn_of(by_turns[EVICT ? e : 0], -(int64_t)way[s], 1.0f) : cs[pair]; };
             if constexpr (MODE == kMoveVector) {
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     float u = (float)a[s][2 * e], w = (float)a[s][2 * e + 1];
-                    turn_pair(u, w, cs[4 * item + e]);
+                    turn_pair(u, w, turn(4 * item + e, e));
                     a[s][2 * e] = (T)u; a[s][2 * e + 1] = (T)w;
                 }
             } else {
 #pragma unroll
                 for (int e = 0; e < kW; e++) {
                     float u = (float)a[s][e], w = (float)b[s][e];
-                    turn_pair(u, w, cs[kW * item + e]);
+                    turn_pair(u, w, turn(kW * item + e, e));
                     a[s][e] = (T)u; b[s][e] = (T)w;
                 }
             }
@@ -496,8 +525,8 @@ __device__ __forceinline__ void move_stream(const Cache &c, const Move &m, uint3
 // TB/s (a copy: 5.15); in place, by one workgroup per stream, 3.5 TB/s with 224
 // streams and 4.6 with 2048.
 // MODE: of keys that are turned.
-template <class T, int MODE>
-__global__ void __launch_bounds__(256) drop_move_kernel(const Cache c, const uint64_t *turns, int rot, int interleaved)
+template <class T, int MODE, bool EVICT>
+__global__ void __launch_bounds__(256) drop_move_kernel(const Cache c, const uint64_t *turns, int rot, int interleaved, const Stays e)
 {
     __shared__ float2 cs[128];
     const uint32_t i = blockIdx.z, stream = blockIdx.x;
@@ -511,25 +540,52 @@ __global__ void __launch_bounds__(256) drop_move_kernel(const Cache c, const uin
     const bool fresh = first < pages_of(c, m.left) && (c.stage[(size_t)i * c.ld + first] >> 31);
     const uint32_t t0 = fresh ? first << c.shift : m.from;
     T *base = (T *)(keys ? c.k : c.v) + (size_t)l * c.n_pages * c.n_kv * ((size_t)c.d << c.shift);
+    const uint32_t *list = EVICT ? e.list + i * e.ld : nullptr;
     if (!keys || rot == 0) {
-        move_stream<T, kMoveVector>(c, m, i, base, h, 0, true, cs, t0, slice, slices);
+        move_stream<T, kMoveVector, EVICT>(c, m, i, base, h, 0, true, cs, t0, slice, slices, list, turns);
         return;
     }
-    for (uint32_t e = threadIdx.x; e < (uint32_t)rot >> 1; e += 256) cs[e] = turn_of(turns[e], (int64_t)m.left - m.len, 1.0f);
-    __syncthreads();
-    move_stream<T, MODE>(c, m, i, base, h, rot, interleaved, cs, t0, slice, slices);
+    if constexpr (!EVICT) {
+        for (uint32_t e = threadIdx.x; e < (uint32_t)rot >> 1; e += 256) cs[e] = turn_of(turns[e], (int64_t)m.left - m.len, 1.0f);
+        __syncthreads();
+    }
+    move_stream<T, MODE, EVICT>(c, m, i, base, h, rot, interleaved, cs, t0, slice, slices, list, turns);
 }
 
 // Drop, 3 of 3: row blockIdx.x's table, its released pages, its length.  (4.7
-// us: words only.)
-__global__ void __launch_bounds__(256) drop_write_kernel(const Cache c)
+// us: words only.)  EVICT: its weights too, kEach times 1024 at a time: they go
+// down in ascending order, and all of a step are read before one is written.
+template <bool EVICT> __global__ void __launch_bounds__(EVICT ? 1024 : 256) drop_write_kernel(const Cache c, const Stays e)
 {
+    constexpr uint32_t kThreads = EVICT ? 1024 : 256;
     const uint32_t i = blockIdx.x;
     const Move m = c.moves[i];
     if (!m.ok) return;
+    if constexpr (EVICT) {
+        constexpr int kEach = 8;
+        float *mass = e.mass + m.row * e.ld_mass;
+        const uint32_t *list = e.list + i * e.ld;
+        for (uint32_t x0 = m.from; x0 < m.left; x0 += kEach * kThreads) {
+            float w[kEach];
+#pragma unroll
+            for (int k = 0; k < kEach; k++) {
+                const uint32_t x = x0 + k * kThreads + threadIdx.x;
+                w[k] = x < m.left ? mass[list[x]] : 0.0f;
+            }
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < kEach; k++) {
+                const uint32_t x = x0 + k * kThreads + threadIdx.x;
+                if (x < m.left) mass[x] = w[k];
+            }
+        }
+        __syncthreads();            // (the last step's reads are done)
+        for (uint32_t x = m.left + threadIdx.x; x < m.len; x += kThreads) mass[x] = 0.0f;
+    }
     uint32_t *table = c.table + (size_t)m.row * c.ld;
     const uint32_t now = pages_of(c, m.left), was = pages_of(c, m.len);
-    for (uint32_t j = (m.from >> c.shift) + threadIdx.x; j < was; j += 256) {
+    for (uint32_t j = (m.from >> c.shift) + threadIdx.x; j < was; j += kThreads) {
         const uint32_t old = table[j], p = j < now ? new_page(c, m, i, j) : GS_KV_NONE;
         if (p == old) continue;
         if (old < c.n_pages) atomicSub(&c.ref[old], 1u);
@@ -537,6 +593,118 @@ __global__ void __launch_bounds__(256) drop_write_kernel(const Cache c)
         table[j] = p;
     }
     if (threadIdx.x == 0) c.len[m.row] = m.left;
+}
+
+// A weight as a whole number that grows with it: NaN above all, -0 as 0.
+__device__ __forceinline__ uint32_t rank_of(float x)
+{
+    const uint32_t u = __float_as_uint(x);
+    if ((u << 1) > 0xff000000u) return 0xffffffffu;
+    if ((u << 1) == 0) return 0x80000000u;
+    return u >> 31 ? ~u : u | 0x80000000u;
+}
+
+// Eviction, 1 of 4: which tokens of row rows[blockIdx.x] stay.  Of the tokens
+// between the first and the newest the k of greatest weight: the rank of the
+// k-th is found 8 bits at a time, by counting the weights that share the bits
+// found so far; then one pass over the row writes the tokens above it, and the
+// lowest of those that have it, to the list.
+__global__ void __launch_bounds__(kBook) evict_select_kernel(const Cache c, const uint32_t *rows, const uint32_t *budget,
+                                                             uint32_t budget_all, uint32_t first, uint32_t recent, const Stays e)
+{
+    constexpr int kEach = 4;            // tokens of a thread in a step of the last pass
+    __shared__ uint32_t s_count[256], s_bin, s_above, s_from;
+    const uint32_t i = blockIdx.x, row = rows[i];
+    bool again = row >= c.rows;         // (a row that an earlier i has counts there)
+    for (uint32_t j = threadIdx.x; j < i; j += kBook) again |= rows[j] == row;
+    again = __syncthreads_or(again);
+    Move m = {};
+    m.row = row;
+    if (again) {
+        if (threadIdx.x == 0) c.moves[i] = m;
+        return;
+    }
+    m.ok = 1;
+    m.len = row_len(c, row);
+    m.left = min(m.len, budget ? budget[i] : budget_all);
+    m.from = m.left;
+    if (m.left == m.len) {
+        if (threadIdx.x == 0) c.moves[i] = m;
+        return;
+    }
+    const float *mass = e.mass + row * e.ld_mass;
+    uint32_t *list = e.list + i * e.ld;
+    const uint32_t tail = m.len - min(recent, m.left), head = min(first, m.left - (m.len - tail));
+    uint32_t want = m.left - head - (m.len - tail);     // of head .. tail - 1, which are more
+    uint32_t rank = 0, known = 0;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        if (threadIdx.x < 256) s_count[threadIdx.x] = 0;
+        __syncthreads();
+        for (uint32_t t = head + threadIdx.x; t < tail; t += kBook) {
+            const uint32_t r = rank_of(mass[t]);
+            if ((r & known) == rank) atomicAdd(&s_count[r >> shift & 255], 1u);
+        }
+        __syncthreads();
+        if (threadIdx.x < 64) {         // four counts a lane, from the greatest down
+            uint32_t x[4], sum = 0;
+#pragma unroll
+            for (int k = 0; k < 4; k++) { x[k] = s_count[255 - (4 * threadIdx.x + k)]; sum += x[k]; }
+            uint32_t upto = sum;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const uint32_t y = __shfl_up(upto, o);
+                if ((int)threadIdx.x >= o) upto += y;
+            }
+            uint32_t above = upto - sum;
+            // (want 0: the first bin, none of which is taken)
+            const bool mine = want == 0 ? threadIdx.x == 0 : above < want && want <= upto;
+            if (mine) {
+                int k = 0;
+                if (want)
+                    while (above + x[k & 3] < want && k < 3) above += x[k++ & 3];
+                s_bin = 255 - (4 * threadIdx.x + k);
+                s_above = above;
+            }
+        }
+        __syncthreads();
+        rank |= s_bin << shift;
+        known |= 255u << shift;
+        want -= s_above;
+    }
+    // those of rank `rank`: the lowest `want` stay
+    if (threadIdx.x == 0) s_from = m.left;
+    uint32_t sure = 0, even = 0;        // before this step's tokens: that stay, and that have that rank
+    for (uint32_t t0 = 0; t0 < m.len; t0 += kBook * kEach) {
+        uint32_t above = 0, same = 0;   // bits
+#pragma unroll
+        for (int k = 0; k < kEach; k++) {
+            const uint32_t t = t0 + threadIdx.x * kEach + k;
+            if (t >= m.len) break;
+            if (t < head || t >= tail) above |= 1u << k;
+            else {
+                const uint32_t r = rank_of(mass[t]);
+                above |= (uint32_t)(r > rank) << k;
+                same |= (uint32_t)(r == rank) << k;
+            }
+        }
+        uint32_t total;
+        const uint32_t before = scan(__popc(above) | __popc(same) << 16, total);
+        uint32_t a = sure + (before & 0xffff), b = even + (before >> 16);
+#pragma unroll
+        for (int k = 0; k < kEach; k++) {
+            const uint32_t t = t0 + threadIdx.x * kEach + k;
+            const bool stays = above >> k & 1 || (same >> k & 1 && b < want);
+            if (stays) list[a + min(b, want)] = t;
+            else if (t < m.len) atomicMin(&s_from, t);
+            a += above >> k & 1;
+            b += same >> k & 1;
+        }
+        sure += total & 0xffff;
+        even += total >> 16;
+    }
+    __syncthreads();
+    m.from = s_from;
+    if (threadIdx.x == 0) c.moves[i] = m;
 }
 
 } // namespace gs
@@ -576,6 +744,33 @@ unsigned shares(size_t n, size_t all, size_t most)
     size_t s = (all + n - 1) / n;
     if (s > most) s = most;
     return (unsigned)(s ? s : 1);
+}
+
+// (a grid's threads side by side are counted in 32 bits)
+bool too_many_streams(const gs_kv_cache *c) { return 2 * (size_t)c->n_layers * c->n_kv * 256 > 0xffffffffull; }
+
+// The tokens of a drop or an eviction to their places.
+template <bool EVICT>
+void move_tokens(const gs_kv_cache *c, const gs::Cache &d, size_t n, const gs_rope *rope, const gs::Stays &e, hipStream_t st)
+{
+    const size_t streams = 2 * (size_t)c->n_layers * c->n_kv;
+    const int rot = rope ? (int)rope->rot : 0;
+    const bool inter = rope && rope->layout == GS_ROPE_INTERLEAVED;
+    const uint64_t *turns = rope ? rope->turns : nullptr;
+    // Several times as many workgroups as run at a time even out rows of unlike
+    // lengths (16 rows of 2500 to 6000 tokens, us: 2048 workgroups 669, 4096
+    // 611, 8192 586, 16384 567).
+    const dim3 grid((unsigned)streams, shares(n * streams, 16384, 64), (unsigned)n);
+    auto move = [&](auto t, auto mode) {
+        hipLaunchKernelGGL((gs::drop_move_kernel<decltype(t), decltype(mode)::value, EVICT>), grid, dim3(256), 0, st, d, turns, rot, inter, e);
+    };
+    auto typed = [&](auto mode) {
+        if (c->type == GS_TYPE_F16) move(_Float16(), mode);
+        else move(__bf16(), mode);
+    };
+    if (rot == 0 || (inter && rot % 8 == 0)) typed(std::integral_constant<int, gs::kMoveVector>());
+    else if (!inter && rot % 16 == 0) typed(std::integral_constant<int, gs::kMovePairs>());
+    else typed(std::integral_constant<int, gs::kMoveValues>());
 }
 
 } // namespace
@@ -639,29 +834,43 @@ int gs_kv_drop(const gs_kv_cache *c, const uint32_t *rows, size_t n, const uint3
     if (rope && (rope->d != c->d || !is_here(rope))) return GS_ERR_INVALID;
     if (n == 0) return GS_OK;
     if (!rows || !from || !to) return GS_ERR_INVALID;
+    if (too_many_streams(c)) return GS_ERR_UNSUPPORTED;
     const gs::Cache d = device_cache(c);
     hipStream_t st = (hipStream_t)stream;
-    const size_t streams = 2 * (size_t)c->n_layers * c->n_kv;
-    if (streams * 256 > 0xffffffffull) return GS_ERR_UNSUPPORTED;       // (a grid's threads side by side)
-    const int rot = rope ? (int)rope->rot : 0;
-    const bool inter = rope && rope->layout == GS_ROPE_INTERLEAVED;
-    const uint64_t *turns = rope ? rope->turns : nullptr;
-    // Several times as many workgroups as run at a time even out rows of unlike
-    // lengths (16 rows of 2500 to 6000 tokens, us: 2048 workgroups 669, 4096
-    // 611, 8192 586, 16384 567).
-    const dim3 grid((unsigned)streams, shares(n * streams, 16384, 64), (unsigned)n);
-    hipLaunchKernelGGL(gs::drop_plan_kernel, dim3(1), dim3(gs::kBook), 0, st, d, rows, (uint32_t)n, from, to, status);
-    auto move = [&](auto t, auto mode) {
-        hipLaunchKernelGGL((gs::drop_move_kernel<decltype(t), decltype(mode)::value>), grid, dim3(256), 0, st, d, turns, rot, inter);
-    };
-    auto typed = [&](auto mode) {
-        if (c->type == GS_TYPE_F16) move(_Float16(), mode);
-        else move(__bf16(), mode);
-    };
-    if (rot == 0 || (inter && rot % 8 == 0)) typed(std::integral_constant<int, gs::kMoveVector>());
-    else if (!inter && rot % 16 == 0) typed(std::integral_constant<int, gs::kMovePairs>());
-    else typed(std::integral_constant<int, gs::kMoveValues>());
-    hipLaunchKernelGGL(gs::drop_write_kernel, dim3((unsigned)n), dim3(256), 0, st, d);
+    hipLaunchKernelGGL(gs::drop_plan_kernel<false>, dim3(1), dim3(gs::kBook), 0, st, d, rows, (uint32_t)n, from, to, status);
+    move_tokens<false>(c, d, n, rope, gs::Stays(), st);
+    hipLaunchKernelGGL(gs::drop_write_kernel<false>, dim3((unsigned)n), dim3(256), 0, st, d, gs::Stays());
+    return launched();
+}
+
+size_t gs_kv_evict_workspace(const gs_kv_cache *c, size_t n, uint32_t budget)
+{
+    if (check_cache(c) || n > c->rows || n > 65535) return 0;
+    const size_t most = (size_t)c->ld_table * c->page_size;
+    return ((n ? n : 1) * up4(budget && budget < most ? budget : most)) * 4;
+}
+
+int gs_kv_evict(const gs_kv_cache *c, const gs_kv_evict_args *x, void *stream)
+{
+    if (!x) return GS_ERR_INVALID;
+    if (int rc = check_call(c, x->n)) return rc;
+    if (x->rope && (x->rope->d != c->d || !is_here(x->rope))) return GS_ERR_INVALID;
+    if (x->n == 0) return GS_OK;
+    const size_t most = (size_t)c->ld_table * c->page_size;
+    if (!x->rows || !x->mass || ((uintptr_t)x->mass & 3u) || x->ld_mass < most) return GS_ERR_INVALID;
+    if (x->ld_mass > (size_t)1 << 40) return GS_ERR_UNSUPPORTED;
+    const uint32_t all = x->budget ? 0 : x->budget_all;
+    if (!x->ws || ((uintptr_t)x->ws & 15u) || x->ws_bytes < gs_kv_evict_workspace(c, x->n, all)) return GS_ERR_INVALID;
+    if (too_many_streams(c)) return GS_ERR_UNSUPPORTED;
+    const gs::Cache d = device_cache(c);
+    const gs::Stays e = {(uint32_t *)x->ws, up4(all && all < most ? all : most), x->mass, x->ld_mass};
+    hipStream_t st = (hipStream_t)stream;
+    hipLaunchKernelGGL(gs::evict_select_kernel, dim3((unsigned)x->n), dim3(gs::kBook), 0, st, d, x->rows, x->budget, x->budget_all,
+                       x->first, x->recent, e);
+    hipLaunchKernelGGL(gs::drop_plan_kernel<true>, dim3(1), dim3(gs::kBook), 0, st, d, x->rows, (uint32_t)x->n,
+                       (const uint32_t *)nullptr, (const uint32_t *)nullptr, x->status);
+    move_tokens<true>(c, d, x->n, x->rope, e, st);
+    hipLaunchKernelGGL(gs::drop_write_kernel<true>, dim3((unsigned)x->n), dim3(1024), 0, st, d, e);
     return launched();
 }
 

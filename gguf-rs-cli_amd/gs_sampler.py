@@ -54,6 +54,7 @@ EXPORTS = [
     "gs_rope_create", "gs_rope_destroy", "gs_rope_apply",
     # include/gs_cache.h
     "gs_kv_workspace", "gs_kv_reset", "gs_kv_extend", "gs_kv_fork", "gs_kv_free", "gs_kv_drop", "gs_kv_append",
+    "gs_kv_evict_workspace", "gs_kv_evict",
     # include/gs_attn.h
     "gs_attn_workspace", "gs_attn",
 ]
@@ -126,6 +127,13 @@ class GsAttnArgs(ctypes.Structure):
                 ("ws_bytes", ctypes.c_size_t)]
 
 
+class GsKVEvictArgs(ctypes.Structure):
+    """gs_kv_evict_args: include/gs_cache.h."""
+    _fields_ = [("rows", ctypes.c_void_p), ("n", ctypes.c_size_t), ("budget", ctypes.c_void_p), ("budget_all", ctypes.c_uint32),
+                ("first", ctypes.c_uint32), ("recent", ctypes.c_uint32), ("mass", ctypes.c_void_p), ("ld_mass", ctypes.c_size_t),
+                ("rope", ctypes.c_void_p), ("status", ctypes.c_void_p), ("ws", ctypes.c_void_p), ("ws_bytes", ctypes.c_size_t)]
+
+
 _lib = None
 
 
@@ -181,6 +189,8 @@ def load_library(path=LIB_PATH):
         "gs_kv_fork": ([ctypes.POINTER(GsKVCache), P, P, SZ, P, P], I),
         "gs_kv_free": ([ctypes.POINTER(GsKVCache), P, SZ, P], I),
         "gs_kv_drop": ([ctypes.POINTER(GsKVCache), P, SZ, P, P, P, P, P], I),
+        "gs_kv_evict_workspace": ([ctypes.POINTER(GsKVCache), SZ, ctypes.c_uint32], SZ),
+        "gs_kv_evict": ([ctypes.POINTER(GsKVCache), ctypes.POINTER(GsKVEvictArgs), P], I),
         "gs_kv_append": ([ctypes.POINTER(GsKVCache), ctypes.c_uint32, ctypes.POINTER(GsKVBatch), P,
                           ctypes.POINTER(GsKVNew), P], I),
         "gs_attn_workspace": ([ctypes.POINTER(GsKVCache), ctypes.c_uint32], SZ),
@@ -836,6 +846,7 @@ class KVCache:
         self.ws = torch.empty(words, dtype=torch.int32, device=k.device)
         self.c.ws = self.ws.data_ptr()
         self._attn_ws = {}
+        self._more_ws = {}
 
     @classmethod
     def empty(cls, layers, pages, kv, d, rows, max_len, page=16, dtype=None, device="cuda"):
@@ -880,6 +891,57 @@ class KVCache:
         n, dev = rows.numel(), self.dev
         _call(dev, self._lib.gs_kv_drop, "gs_kv_drop", self._c, _words(rows, "rows", dev), n, _words(start, "start", dev, n),
               _words(end, "end", dev, n), turn, _words(status, "status", dev, n), _stream_of(self.dev, stream))
+
+    def mass(self):
+        """A new tensor for the weights that weigh() adds up and evict() goes by:
+        [rows, most tokens of a row] float32, zeros.  Its rows go with the
+        cache's: after fork, mass[dst] = mass[src] is the caller's to do."""
+        import torch
+        return torch.zeros((self.rows, self.table.shape[1] * self.page), device=self.k.device)
+
+    def _mass(self, mass):
+        """Values from row to row of a tensor as mass() makes it."""
+        import torch
+        if mass.dtype != torch.float32 or mass.dim() != 2 or mass.get_device() != self.dev or mass.stride(1) != 1:
+            raise TypeError("mass must be a [rows, tokens] tensor of float32 on the cache's device")
+        if mass.shape[0] != self.rows or mass.shape[1] < self.table.shape[1] * self.page:
+            raise ValueError("mass must have the cache's rows and room for the most tokens of each")
+        if mass.stride(0) < mass.shape[1] and self.rows > 1:
+            raise TypeError("the rows of mass must not overlap")
+        return mass.stride(0) if self.rows > 1 else mass.shape[1]
+
+    def evict(self, mass, budget, rows, first=0, recent=0, rope=None, status=None, stream=None):
+        """Each of `rows` that holds more than `budget` tokens (a number, or a
+        tensor of one per row) keeps its newest `recent`, its `first` ones and
+        those of greatest weight between (gs_kv_evict); they move down, their
+        weights in `mass` with them, and with `rope` keys are turned back as
+        far as they move.
+        The cache keeps a workspace of 4 bytes for each token that may stay for
+        each stream that evict was called on, as attend does."""
+        turn, dev = _turn(rope), self.dev
+        n, ld = rows.numel(), self._mass(mass)
+        each = isinstance(budget, int)
+        for x, what in ((budget if each else 0, "budget"), (first, "first"), (recent, "recent")):
+            if not 0 <= x <= 0xFFFFFFFF:
+                raise ValueError("%s must be a number of tokens" % what)
+        st = _stream_of(dev, stream)
+        most = budget if each else 0
+        ws = self._workspace("evict", st, self._lib.gs_kv_evict_workspace(self._c, n, most), mass)
+        x = GsKVEvictArgs(_words(rows, "rows", dev), n, None if each else _words(budget, "budget", dev, n), most, first, recent,
+                          mass.data_ptr(), ld, turn, _words(status, "status", dev, n), ws.data_ptr(), ws.numel())
+        _call(dev, self._lib.gs_kv_evict, "gs_kv_evict", self._c, ctypes.byref(x), st)
+
+    def _workspace(self, what, st, n, like):
+        """A workspace of n bytes for the calls of one kind on the stream st,
+        where they do not overlap.  Larger ones come beside those that captured
+        graphs may hold, and are at least twice their size."""
+        import torch
+        if not n:
+            raise SamplerError(GS_ERR_INVALID, what)
+        held = self._more_ws.setdefault((what, st), [])
+        if not held or held[-1].numel() < n:
+            held.append(_empty_on(st, max(n, 2 * held[-1].numel() if held else 0), torch.uint8, like))
+        return held[-1]
 
     def _batch(self, T, rows, q_start):
         if q_start is None:

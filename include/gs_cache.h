@@ -1,6 +1,7 @@
 /*
  * gs_cache.h -- C ABI of the paged cache of keys and values, and of what
- * happens to its pages: rows grow, are forked, freed, and lose tokens.
+ * happens to its pages: rows grow, are forked, freed, lose tokens, and are cut
+ * to a budget.
  *
  * gguf-rs-cli keeps one contiguous f32 cache per layer and writes one position
  * of it per token (the kv_write shader, dispatched at src/gpu/mod.rs:458-466);
@@ -106,6 +107,38 @@ int gs_kv_free(const gs_kv_cache *c, const uint32_t *rows, size_t n, void *strea
  * a row that an earlier i has.  At most 2^23 - 1 layers times heads. */
 int gs_kv_drop(const gs_kv_cache *c, const uint32_t *rows, size_t n, const uint32_t *from, const uint32_t *to,
                const gs_rope *rope, int32_t *status, void *stream);
+
+/* Rows that hold more tokens than their budget are cut to it: of row rows[i]
+ * stay its newest `recent` tokens, its first `first` ones, and of those between
+ * the ones of greatest weight, as many as the budget has left (budgets below
+ * first + recent: the newest come first).  Of equal weights the lowest token
+ * stays; NaN is more than any number.  Weights are mass[row * ld_mass + token],
+ * which gs_attn_weigh adds up.  Those that stay keep their order and move down
+ * to places 0 .. budget - 1, their weights with them (those of the places
+ * behind, up to the old length, become 0); with `rope` keys are turned back by as
+ * many positions as they move (the gain is not applied again).  Pages, rounding
+ * and status[i] as of gs_kv_drop; a row with an error is as before.
+ * At most 2^23 - 1 layers times heads.  Device memory, but for the struct. */
+typedef struct gs_kv_evict_args {
+    const uint32_t *rows;   /* [n] */
+    size_t n;
+    const uint32_t *budget; /* [n] tokens, or NULL: budget_all for each */
+    uint32_t budget_all;
+    uint32_t first, recent;
+    float *mass;            /* [rows][ld_mass] */
+    size_t ld_mass;         /* at least ld_table * page_size */
+    const gs_rope *rope;    /* or NULL */
+    int32_t *status;        /* [n], or NULL */
+    void *ws;               /* [gs_kv_evict_workspace] bytes, 16-byte aligned */
+    size_t ws_bytes;
+} gs_kv_evict_args;
+
+/* Bytes of workspace of an eviction of n rows with budgets of at most `budget`
+ * (the budget_all of the call; 0, or where `budget` is given: any).  0 if the
+ * sizes are out of range.  No value is kept in it from call to call. */
+size_t gs_kv_evict_workspace(const gs_kv_cache *c, size_t n, uint32_t budget);
+
+int gs_kv_evict(const gs_kv_cache *c, const gs_kv_evict_args *x, void *stream);
 
 /* The sequences of a call of gs_kv_append or gs_attn, device pointers: the
  * newest tokens of n rows, one row after the other.  Sequence i has the tokens

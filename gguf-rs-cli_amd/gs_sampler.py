@@ -56,7 +56,7 @@ EXPORTS = [
     "gs_kv_workspace", "gs_kv_reset", "gs_kv_extend", "gs_kv_fork", "gs_kv_free", "gs_kv_drop", "gs_kv_append",
     "gs_kv_evict_workspace", "gs_kv_evict",
     # include/gs_attn.h
-    "gs_attn_workspace", "gs_attn",
+    "gs_attn_workspace", "gs_attn", "gs_attn_lse", "gs_attn_shared", "gs_attn_shared_workspace",
 ]
 
 
@@ -195,6 +195,10 @@ def load_library(path=LIB_PATH):
                           ctypes.POINTER(GsKVNew), P], I),
         "gs_attn_workspace": ([ctypes.POINTER(GsKVCache), ctypes.c_uint32], SZ),
         "gs_attn": ([ctypes.POINTER(GsKVCache), ctypes.c_uint32, ctypes.POINTER(GsKVBatch), ctypes.POINTER(GsAttnArgs), P], I),
+        "gs_attn_lse": ([ctypes.POINTER(GsKVCache), ctypes.c_uint32, ctypes.POINTER(GsKVBatch), ctypes.POINTER(GsAttnArgs), P, P], I),
+        "gs_attn_shared": ([ctypes.POINTER(GsKVCache), ctypes.c_uint32, ctypes.POINTER(GsKVBatch), P, ctypes.c_uint32,
+                            ctypes.POINTER(GsAttnArgs), P, P], I),
+        "gs_attn_shared_workspace": ([ctypes.POINTER(GsKVCache)] + 4 * [ctypes.c_uint32], SZ),
     }
     for name, (args, res) in sig.items():
         f = getattr(lib, name)
@@ -974,12 +978,24 @@ class KVCache:
         _call(dev, self._lib.gs_kv_append, "gs_kv_append", self._c, layer, ctypes.byref(b), turn, ctypes.byref(x),
               _stream_of(self.dev, stream))
 
-    def attend(self, layer, q, out=None, rows=None, q_start=None, scale=0.0, window=0, max_q=0, stream=None):
+    def _lse(self, lse, T, heads):
+        """The address of a contiguous [T, heads] float32 tensor, or None."""
+        import torch
+        if lse is None:
+            return None
+        if lse.dtype != torch.float32 or lse.get_device() != self.dev or not lse.is_contiguous():
+            raise TypeError("lse must be a contiguous tensor of float32 on the cache's device")
+        if lse.shape != (T, heads):
+            raise ValueError("lse must be [tokens, heads]")
+        return lse.data_ptr()
+
+    def attend(self, layer, q, out=None, rows=None, q_start=None, scale=0.0, window=0, max_q=0, stream=None, lse=None):
         """Causal attention of the rows' newest tokens (as append takes them) over
         the rows' pages: q and out [T, heads, d] (float32 or the cache's type;
         out None: a new tensor).  window: how many positions back a token
         sees, itself included (0: all).  max_q: the most tokens of one
-        sequence, if the caller knows it.
+        sequence, if the caller knows it.  lse [T, heads] float32: gets the
+        logarithm of each softmax's sum, which weigh() takes.
         The cache keeps a workspace of 43 to 85 MB for each stream that attend
         was called on.  A captured graph uses that of the stream it was captured
         on, wherever it is replayed: replays of such graphs, and calls on that
@@ -1004,7 +1020,34 @@ class KVCache:
         b = self._batch(T, rows, q_start)
         a = GsAttnArgs(_type(q, "q"), heads, q.data_ptr(), ld_q, out.data_ptr(), ld_o, scale, window, max_q, ws.data_ptr(),
                        ws.numel())
-        _call(self.dev, self._lib.gs_attn, "gs_attn", self._c, layer, ctypes.byref(b), ctypes.byref(a), st)
+        _call(self.dev, self._lib.gs_attn_lse, "gs_attn", self._c, layer, ctypes.byref(b), ctypes.byref(a), self._lse(lse, T, heads), st)
+        return out
+
+    def attend_shared(self, layer, q, families, out=None, rows=None, q_start=None, scale=0.0, window=0, max_q=0, stream=None, lse=None):
+        """attend() of sequences that come in families: sequences families[j] to
+        families[j + 1] - 1 of the call, whose rows begin with the same pages,
+        as fork() leaves them.  A family's common pages are read once, not once
+        for each row; the result is attend()'s whatever the rows hold.
+        The cache keeps a workspace of 43 to 85 MB and 8 d + 24 bytes for each
+        token and head for each stream that attend_shared was called on, as
+        attend does."""
+        if not 0 <= window <= 0xFFFFFFFF:
+            raise ValueError("window must be a number of positions")
+        T, heads, _, ld_q = _heads(q, "q", self.dev, d=self.d)
+        st = _stream_of(self.dev, stream)
+        out = _empty_on(st, (T, heads, self.d), q.dtype, q) if out is None else out
+        To, _, _, ld_o = _heads(out, "out", self.dev, heads, self.d)
+        if To != T or out.dtype != q.dtype:
+            raise ValueError("out must be as q")
+        b = self._batch(T, rows, q_start)
+        m = families.numel() - 1
+        if m < 1:
+            raise ValueError("families must have the begin of each and the end of the last")
+        ws = self._workspace("attend_shared", st, self._lib.gs_attn_shared_workspace(self._c, heads, b.n, m, T), q)
+        a = GsAttnArgs(_type(q, "q"), heads, q.data_ptr(), ld_q, out.data_ptr(), ld_o, scale, window, max_q, ws.data_ptr(),
+                       ws.numel())
+        _call(self.dev, self._lib.gs_attn_shared, "gs_attn_shared", self._c, layer, ctypes.byref(b),
+              _words(families, "families", self.dev), m, ctypes.byref(a), self._lse(lse, T, heads), st)
         return out
 
 

@@ -53,6 +53,27 @@ size_t gs_attn_workspace(const gs_kv_cache *c, uint32_t n_heads);
  * same arguments give the same bits.  Asynchronous on `stream`. */
 int gs_attn(const gs_kv_cache *c, uint32_t layer, const gs_kv_batch *b, const gs_attn_args *a, void *stream);
 
+/* gs_attn that also leaves, for each token and head, the logarithm of its
+ * softmax's sum: lse[t * n_heads + h] = log(sum over j of exp(scale * (q . k_j))),
+ * -inf where the token sees no key (NULL: none). */
+int gs_attn_lse(const gs_kv_cache *c, uint32_t layer, const gs_kv_batch *b, const gs_attn_args *a, float *lse, void *stream);
+
+/* gs_attn_lse for a batch whose sequences come in families: sequences
+ * families[j] .. families[j + 1] - 1 of the batch, j < n_families, whose rows begin
+ * with the same pages, as gs_kv_fork leaves them.  The pages that all rows of a
+ * family have in common are read once for the family, with the queries of all
+ * its sequences; results are those of gs_attn, whatever the rows hold.
+ * `families` [n_families + 1] is device memory, ascending; sequences before the
+ * first or after the last family are by themselves.  The workspace is larger
+ * and grows with the tokens: gs_attn_shared_workspace bytes.
+ * 16-bit queries: weights are rounded to the cache's type once. */
+int gs_attn_shared(const gs_kv_cache *c, uint32_t layer, const gs_kv_batch *b, const uint32_t *families, uint32_t n_families,
+                   const gs_attn_args *a, float *lse, void *stream);
+
+/* Bytes of gs_attn_args.ws of a call of gs_attn_shared with up to n sequences,
+ * n_families families and n_tokens tokens (0 if the sizes are out of range). */
+size_t gs_attn_shared_workspace(const gs_kv_cache *c, uint32_t n_heads, uint32_t n, uint32_t n_families, uint32_t n_tokens);
+
 #ifdef __cplusplus
 }
 #endif

@@ -28,7 +28,7 @@ PEAK_HBM_GBS = 8000.0   # MI355X HBM3E
 
 # Sources of the operators beside the sampler, the projection and the decode
 # step: none of the profiled kernels is built from them.
-OTHER_SOURCES = ("gs_rope.hip", "gs_cache.hip", "gs_cache.hpp", "gs_attn.hip", "gs_attn.hpp", "gs_shared.hip")
+OTHER_SOURCES = ("gs_rope.hip", "gs_cache.hip", "gs_cache.hpp", "gs_attn.hip", "gs_attn.hpp", "gs_shared.hip", "gs_weigh.hip")
 
 
 def sources_digest():

@@ -26,7 +26,7 @@ HIP_FLAGS = [
     "-mllvm", "-amdgpu-function-calls=false",
     "-Wall", "-Wno-unused-function",
 ]
-SOURCES = ["gs_kernels.hip", "gs_api.cpp", "gs_gemv.hip", "gs_decode.hip", "gs_tokens.cpp", "gs_rope.hip", "gs_cache.hip", "gs_attn.hip", "gs_shared.hip"]
+SOURCES = ["gs_kernels.hip", "gs_api.cpp", "gs_gemv.hip", "gs_decode.hip", "gs_tokens.cpp", "gs_rope.hip", "gs_cache.hip", "gs_attn.hip", "gs_shared.hip", "gs_weigh.hip"]
 
 
 def _run(cmd, cwd=None):

@@ -56,7 +56,7 @@ EXPORTS = [
     "gs_kv_workspace", "gs_kv_reset", "gs_kv_extend", "gs_kv_fork", "gs_kv_free", "gs_kv_drop", "gs_kv_append",
     "gs_kv_evict_workspace", "gs_kv_evict",
     # include/gs_attn.h
-    "gs_attn_workspace", "gs_attn", "gs_attn_lse", "gs_attn_shared", "gs_attn_shared_workspace",
+    "gs_attn_workspace", "gs_attn", "gs_attn_lse", "gs_attn_shared", "gs_attn_shared_workspace", "gs_attn_weigh",
 ]
 
 
@@ -125,6 +125,13 @@ class GsAttnArgs(ctypes.Structure):
                 ("out", ctypes.c_void_p), ("ld_out", ctypes.c_size_t), ("scale", ctypes.c_float),
                 ("window", ctypes.c_uint32), ("max_q", ctypes.c_uint32), ("ws", ctypes.c_void_p),
                 ("ws_bytes", ctypes.c_size_t)]
+
+
+class GsWeighArgs(ctypes.Structure):
+    """gs_weigh_args: include/gs_attn.h."""
+    _fields_ = [("type", ctypes.c_uint32), ("n_heads", ctypes.c_uint32), ("q", ctypes.c_void_p), ("ld_q", ctypes.c_size_t),
+                ("lse", ctypes.c_void_p), ("mass", ctypes.c_void_p), ("ld_mass", ctypes.c_size_t), ("keep", ctypes.c_float),
+                ("scale", ctypes.c_float), ("window", ctypes.c_uint32), ("max_q", ctypes.c_uint32)]
 
 
 class GsKVEvictArgs(ctypes.Structure):
@@ -198,6 +205,7 @@ def load_library(path=LIB_PATH):
         "gs_attn_lse": ([ctypes.POINTER(GsKVCache), ctypes.c_uint32, ctypes.POINTER(GsKVBatch), ctypes.POINTER(GsAttnArgs), P, P], I),
         "gs_attn_shared": ([ctypes.POINTER(GsKVCache), ctypes.c_uint32, ctypes.POINTER(GsKVBatch), P, ctypes.c_uint32,
                             ctypes.POINTER(GsAttnArgs), P, P], I),
+        "gs_attn_weigh": ([ctypes.POINTER(GsKVCache), ctypes.c_uint32, ctypes.POINTER(GsKVBatch), ctypes.POINTER(GsWeighArgs), P], I),
         "gs_attn_shared_workspace": ([ctypes.POINTER(GsKVCache)] + 4 * [ctypes.c_uint32], SZ),
     }
     for name, (args, res) in sig.items():
@@ -1049,6 +1057,24 @@ class KVCache:
         _call(self.dev, self._lib.gs_attn_shared, "gs_attn_shared", self._c, layer, ctypes.byref(b),
               _words(families, "families", self.dev), m, ctypes.byref(a), self._lse(lse, T, heads), st)
         return out
+
+
+    def weigh(self, layer, q, lse, mass, rows=None, q_start=None, scale=0.0, window=0, max_q=0, keep=1.0, stream=None):
+        """The weight that each token of the rows gets from their newest ones in
+        this layer, summed over those and the heads, is added to `keep` times
+        `mass` (as mass() makes it; 0: begins anew).  q, rows, q_start, scale,
+        window as attend() had them, lse [T, heads] as it left it."""
+        if not 0 <= window <= 0xFFFFFFFF:
+            raise ValueError("window must be a number of positions")
+        T, heads, _, ld_q = _heads(q, "q", self.dev, d=self.d)
+        if lse is None:
+            raise TypeError("lse must be given")
+        ld = self._mass(mass)
+        b = self._batch(T, rows, q_start)
+        a = GsWeighArgs(_type(q, "q"), heads, q.data_ptr(), ld_q, self._lse(lse, T, heads), mass.data_ptr(), ld, keep, scale, window, max_q)
+        _call(self.dev, self._lib.gs_attn_weigh, "gs_attn_weigh", self._c, layer, ctypes.byref(b), ctypes.byref(a),
+              _stream_of(self.dev, stream))
+        return mass
 
 
 # ---- token text and stop set (include/gs_tokens.h) -----------------------------

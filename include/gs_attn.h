@@ -74,6 +74,33 @@ int gs_attn_shared(const gs_kv_cache *c, uint32_t layer, const gs_kv_batch *b, c
  * n_families families and n_tokens tokens (0 if the sizes are out of range). */
 size_t gs_attn_shared_workspace(const gs_kv_cache *c, uint32_t n_heads, uint32_t n, uint32_t n_families, uint32_t n_tokens);
 
+/* The weight that the tokens of a row get from the row's newest ones, summed over
+ * those and the heads, of one layer: for token j of the row r of sequence i of
+ * `b`, j < len[r],
+ *   mass[r][j] = keep * mass[r][j] + sum over t, h of exp(scale * (q_th . k_j) - lse_th),
+ * over the sequence's tokens t that see j (as in gs_attn) and all heads h.  lse
+ * is what gs_attn_lse or gs_attn_shared left for the same tokens.  Called for
+ * each layer with keep = 1 it adds the layers up; keep = 0 begins anew (what
+ * mass held does not count).  Of sequences of the same row the first counts;
+ * rows out of range are skipped.  What masked keys hold does not count. */
+typedef struct gs_weigh_args {
+    uint32_t type;          /* of q: the cache's, or GS_TYPE_F32 */
+    uint32_t n_heads;       /* a multiple of n_kv */
+    const void *q;          /* as in gs_attn_args */
+    size_t ld_q;
+    const float *lse;       /* [n_tokens][n_heads] */
+    float *mass;            /* [rows][ld_mass] */
+    size_t ld_mass;         /* at least ld_table * page_size */
+    float keep;
+    float scale;            /* 0: 1 / sqrt(d) */
+    uint32_t window;
+    uint32_t max_q;         /* the most tokens that a sequence has (0: n_tokens); a smaller number only costs time */
+} gs_weigh_args;
+
+/* Scores and sums are f32; f32 q goes through the matrix cores in three parts,
+ * as in gs_attn.  Two calls with the same arguments give the same bits. */
+int gs_attn_weigh(const gs_kv_cache *c, uint32_t layer, const gs_kv_batch *b, const gs_weigh_args *a, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -167,6 +167,7 @@ template <int kTile> struct Span {
 template <int R_, int kTile_, int kSetup_, class S> struct Deal {
     static constexpr int R = R_, kTile = kTile_, kSetup = kSetup_;
     using Work = S;
+    static __device__ __forceinline__ uint32_t heads(const AttnArgs &a) { return a.n_kv; }
     // Tiles of the unit of rows r ..
     static __device__ __forceinline__ uint32_t unit(const AttnArgs &a, const S &s, uint32_t r)
     {
@@ -243,7 +244,7 @@ template <class S> __device__ __forceinline__ uint32_t run_with(const Run<S> &r,
 // costs more to join than it saves.  (The chunk kernel, us with 4, 3, 2: 50
 // tokens over 4000, 32 / 8 heads of 128: 33.1, 32.7, 38.0; 300 over 300: 27.3,
 // 24.7, 24.7.)
-template <class D, int kThreads, int kLeast> __device__ __forceinline__ Run<typename D::Work> run_of(const AttnArgs &a, uint32_t g)
+template <class D, int kThreads, int kLeast, class A> __device__ __forceinline__ Run<typename D::Work> run_of(const A &a, uint32_t g)
 {
     using S = typename D::Work;
     constexpr uint32_t kWaves = kThreads / 64, kShort = 32;     // up to kShort sequences are counted by waves: theirs may be long
@@ -266,13 +267,13 @@ template <class D, int kThreads, int kLeast> __device__ __forceinline__ Run<type
         if (threadIdx.x < a.n) {
             s = s_seq[threadIdx.x];
             per = s_per[threadIdx.x];
-            mine = per * a.n_kv;
+            mine = per * D::heads(a);
         }
     } else {
         for (uint32_t i = i0; i < i1; i++) {
             s = work_of<S>(a, i);
             per = D::count(a, s);
-            mine += per * a.n_kv;
+            mine += per * D::heads(a);
         }
     }
     uint64_t x = mine;
@@ -305,8 +306,8 @@ template <class D, int kThreads, int kLeast> __device__ __forceinline__ Run<type
             for (;; i++) {
                 s = work_of<S>(a, i);
                 per = D::count(a, s);
-                if (r.t0 < before + per * a.n_kv) break;
-                before += per * a.n_kv;
+                if (r.t0 < before + per * D::heads(a)) break;
+                before += per * D::heads(a);
             }
         r.seq = i; r.skip = r.t0 - before; r.per = per; r.s = s;
         s_run = r;

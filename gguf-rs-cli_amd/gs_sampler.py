@@ -57,6 +57,7 @@ EXPORTS = [
     "gs_kv_evict_workspace", "gs_kv_evict",
     # include/gs_attn.h
     "gs_attn_workspace", "gs_attn", "gs_attn_lse", "gs_attn_shared", "gs_attn_shared_workspace", "gs_attn_weigh",
+    "gs_attn_weigh_workspace",
 ]
 
 
@@ -131,7 +132,8 @@ class GsWeighArgs(ctypes.Structure):
     """gs_weigh_args: include/gs_attn.h."""
     _fields_ = [("type", ctypes.c_uint32), ("n_heads", ctypes.c_uint32), ("q", ctypes.c_void_p), ("ld_q", ctypes.c_size_t),
                 ("lse", ctypes.c_void_p), ("mass", ctypes.c_void_p), ("ld_mass", ctypes.c_size_t), ("keep", ctypes.c_float),
-                ("scale", ctypes.c_float), ("window", ctypes.c_uint32), ("max_q", ctypes.c_uint32)]
+                ("scale", ctypes.c_float), ("window", ctypes.c_uint32), ("max_q", ctypes.c_uint32), ("ws", ctypes.c_void_p),
+                ("ws_bytes", ctypes.c_size_t)]
 
 
 class GsKVEvictArgs(ctypes.Structure):
@@ -205,6 +207,7 @@ def load_library(path=LIB_PATH):
         "gs_attn_lse": ([ctypes.POINTER(GsKVCache), ctypes.c_uint32, ctypes.POINTER(GsKVBatch), ctypes.POINTER(GsAttnArgs), P, P], I),
         "gs_attn_shared": ([ctypes.POINTER(GsKVCache), ctypes.c_uint32, ctypes.POINTER(GsKVBatch), P, ctypes.c_uint32,
                             ctypes.POINTER(GsAttnArgs), P, P], I),
+        "gs_attn_weigh_workspace": ([ctypes.POINTER(GsKVCache)], SZ),
         "gs_attn_weigh": ([ctypes.POINTER(GsKVCache), ctypes.c_uint32, ctypes.POINTER(GsKVBatch), ctypes.POINTER(GsWeighArgs), P], I),
         "gs_attn_shared_workspace": ([ctypes.POINTER(GsKVCache)] + 4 * [ctypes.c_uint32], SZ),
     }
@@ -1063,7 +1066,9 @@ class KVCache:
         """The weight that each token of the rows gets from their newest ones in
         this layer, summed over those and the heads, is added to `keep` times
         `mass` (as mass() makes it; 0: begins anew).  q, rows, q_start, scale,
-        window as attend() had them, lse [T, heads] as it left it."""
+        window as attend() had them, lse [T, heads] as it left it.
+        The cache keeps a workspace of 1 MB for each stream that weigh was
+        called on, as attend does."""
         if not 0 <= window <= 0xFFFFFFFF:
             raise ValueError("window must be a number of positions")
         T, heads, _, ld_q = _heads(q, "q", self.dev, d=self.d)
@@ -1071,9 +1076,11 @@ class KVCache:
             raise TypeError("lse must be given")
         ld = self._mass(mass)
         b = self._batch(T, rows, q_start)
-        a = GsWeighArgs(_type(q, "q"), heads, q.data_ptr(), ld_q, self._lse(lse, T, heads), mass.data_ptr(), ld, keep, scale, window, max_q)
-        _call(self.dev, self._lib.gs_attn_weigh, "gs_attn_weigh", self._c, layer, ctypes.byref(b), ctypes.byref(a),
-              _stream_of(self.dev, stream))
+        st = _stream_of(self.dev, stream)
+        ws = self._workspace("weigh", st, self._lib.gs_attn_weigh_workspace(self._c), mass)
+        a = GsWeighArgs(_type(q, "q"), heads, q.data_ptr(), ld_q, self._lse(lse, T, heads), mass.data_ptr(), ld, keep, scale, window,
+                        max_q, ws.data_ptr(), ws.numel())
+        _call(self.dev, self._lib.gs_attn_weigh, "gs_attn_weigh", self._c, layer, ctypes.byref(b), ctypes.byref(a), st)
         return mass
 
 

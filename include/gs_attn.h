@@ -95,7 +95,13 @@ typedef struct gs_weigh_args {
     float scale;            /* 0: 1 / sqrt(d) */
     uint32_t window;
     uint32_t max_q;         /* the most tokens that a sequence has (0: n_tokens); a smaller number only costs time */
+    void *ws;               /* [gs_attn_weigh_workspace] bytes, 16-byte aligned */
+    size_t ws_bytes;
 } gs_weigh_args;
+
+/* Bytes of workspace of any call (0 if the sizes are out of range).  No value is
+ * kept in it from call to call; calls that may overlap need one each. */
+size_t gs_attn_weigh_workspace(const gs_kv_cache *c);
 
 /* Scores and sums are f32; f32 q goes through the matrix cores in three parts,
  * as in gs_attn.  Two calls with the same arguments give the same bits. */

@@ -256,15 +256,18 @@ def test_refusals_without_gpu():
     lib = gs.load_library()
     INV, UNS = gs.GS_ERR_INVALID, gs.GS_ERR_UNSUPPORTED
     c = fake(gs)
+    ws = lib.gs_attn_weigh_workspace(c)
+    assert ws > 0 and lib.gs_attn_weigh_workspace(fake(gs, d=12)) == 0
 
     def call(layer=0, b=(1, 1, None, None), cache=c, **kw):
-        x = dict(type=1, n_heads=4, q=4096, ld_q=256, lse=4096, mass=4096, ld_mass=64, keep=1.0, scale=0.0, window=0, max_q=0)
+        x = dict(type=1, n_heads=4, q=4096, ld_q=256, lse=4096, mass=4096, ld_mass=64, keep=1.0, scale=0.0, window=0, max_q=0,
+                 ws=4096, ws_bytes=ws)
         x.update(kw)
         return lib.gs_attn_weigh(cache, layer, ctypes.byref(gs.GsKVBatch(*b)), ctypes.byref(gs.GsWeighArgs(**x)), None)
 
     for kw in (dict(layer=1), dict(n_heads=3), dict(n_heads=0), dict(q=None), dict(ld_q=255), dict(ld_q=260), dict(q=4104),
                dict(lse=None), dict(lse=4098), dict(mass=None), dict(mass=4097), dict(ld_mass=63), dict(scale=math.nan),
-               dict(keep=math.inf), dict(keep=math.nan), dict(b=(2, 1, None, None)), dict(b=(5, 5, None, None)),
+               dict(ws=None), dict(ws=4104), dict(ws_bytes=ws - 1), dict(keep=math.inf), dict(keep=math.nan), dict(b=(2, 1, None, None)), dict(b=(5, 5, None, None)),
                dict(cache=fake(gs, k=None))):
         assert call(**kw) == INV, kw
     assert call(type=30) == UNS and call(type=2) == UNS and call(ld_mass=(1 << 40) + 1) == UNS

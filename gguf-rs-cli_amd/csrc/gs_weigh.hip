@@ -88,7 +88,7 @@ __device__ __forceinline__ void base_of(const WeighArgs &x, float lse, float &n,
 {
     const float hi = lse * x.base, lo = fmaf(lse, x.base, -hi) + lse * x.base_rest;
     n = rintf(hi);
-    c = exp2f((n - hi) - lo);
+    c = __builtin_amdgcn_exp2f((n - hi) - lo);
     if (!(fabsf(hi) < INFINITY)) { n = lse; c = 1.0f; }
 }
 
@@ -244,10 +244,12 @@ __global__ void __launch_bounds__(256) weigh_few_kernel(const WeighArgs a)
     }
 }
 
-// The shape of the kernel below for heads of D: four waves of kMine keys.
-template <int D> struct Many {
-    static constexpr int kTiles = D == 256 ? 1 : 2, kMine = 32 * kTiles, kKeys = 4 * kMine;
-    static constexpr int kSetup = 2;                // the keys' way and the sums', dealt as tiles of rows
+// The shape of the kernel below for heads of D: four waves of kMine keys, tiles
+// of kRows query rows (in three parts twice as many would leave room for one
+// workgroup in a CU).
+template <int D, bool F32> struct Many {
+    static constexpr int kTiles = D == 256 ? 1 : 2, kMine = 32 * kTiles, kKeys = 4 * kMine, kRows = F32 ? 32 : 64;
+    static constexpr int kSetup = 1;                // the keys' way and the sums', dealt as tiles of rows
 };
 constexpr int kManyRuns = 512;                      // two workgroups per CU
 
@@ -259,15 +261,16 @@ struct Left {
 
 // How its work is dealt: of a sequence, a block of keys after the other, each
 // with all heads of keys one after the other, each with the rows that see one
-// of the block's keys, 32 at a time.
-template <int D> struct ManyDeal {
+// of the block's keys, kRows at a time.
+template <int D, bool F32> struct ManyDeal {
     using Work = WeighSeq;
-    static constexpr int kKeys = Many<D>::kKeys;
+    using M = Many<D, F32>;
+    static constexpr int kKeys = M::kKeys;
     static __device__ __forceinline__ uint32_t heads(const WeighArgs &a) { return a.n_kv; }
     static __device__ __forceinline__ uint32_t block(const WeighArgs &a, const WeighSeq &s, uint32_t tile)
     {
         const Seers r(a, s, tile * kKeys, kKeys);
-        return (r.r1 - r.r0 + 31) / 32 + Many<D>::kSetup;
+        return (r.r1 - r.r0 + M::kRows - 1) / M::kRows + M::kSetup;
     }
     static __device__ __forceinline__ uint64_t count(const WeighArgs &a, const WeighSeq &s)
     {
@@ -317,7 +320,7 @@ __device__ __forceinline__ void add_mass(const WeighArgs &a, uint32_t row, uint3
 }
 
 // For chunks of tokens what bounds it is the matrix cores and, beside them, the
-// exponentials.  A wave holds its keys of a head as factors, 32 rows of queries
+// exponentials.  A wave holds its keys of a head as factors, kRows rows of queries
 // at a time pass through LDS for all four waves (two tiles of them, so that the
 // next one's loads pass while this one is worked on), and a lane adds up the
 // weights of query row lane & 31 for the keys that its results of S^T = K Q^T,
@@ -325,20 +328,21 @@ __device__ __forceinline__ void add_mass(const WeighArgs &a, uint32_t row, uint3
 template <class T, int D, bool F32>
 __global__ void __launch_bounds__(256, F32 && D == 256 ? 1 : 2) weigh_many_kernel(const WeighArgs a)
 {
-    constexpr int KT = Many<D>::kTiles, kMine = Many<D>::kMine, kKeys = Many<D>::kKeys, kSetup = Many<D>::kSetup;
+    using M = Many<D, F32>;
+    constexpr int KT = M::kTiles, kMine = M::kMine, kKeys = M::kKeys, kSetup = M::kSetup, kRows = M::kRows, U = kRows / 32;
     constexpr int KF = D / 16, NP = F32 ? 3 : 1, C = D / 8, kEach = C / 8;      // factors; parts; 16-byte pieces of a row, of a thread
     typedef typename Vec<T>::v8 v8;
-    __shared__ __align__(16) T s_q[2][NP][32 * D];
-    __shared__ float s_n[2][32], s_c[2][32], s_u[2][32];
+    __shared__ __align__(16) T s_q[2][NP][kRows * D];
+    __shared__ float s_n[2][kRows], s_c[2][kRows], s_u[2][kRows];
     __shared__ float s_sum[kKeys];
-    using Dealt = ManyDeal<D>;
+    using Dealt = ManyDeal<D, F32>;
     const Run<WeighSeq> run = run_of<Dealt, 256, 4>(a, blockIdx.x);
     if (threadIdx.x == 0) a.left[blockIdx.x].last = 0;
     if (run.t0 >= run.t1) return;
 
     const int lane = threadIdx.x & 63, hg = lane >> 5, col = lane & 31;
     const uint32_t w = uniform(threadIdx.x >> 6);
-    const int prow = threadIdx.x >> 3, pc = threadIdx.x & 7;        // this thread's row of a tile of queries; its pieces pc + 8 i
+    const int prow = threadIdx.x >> 3, pc = threadIdx.x & 7;        // this thread's first row of a tile of queries (the others 32 apart); its pieces pc + 8 i
     const uint32_t slot = (1u << a.shift) - 1, d = a.d;
     const size_t head = (size_t)d << a.shift;
     auto place = [](int row, int c) { return c ^ (row & (C < 16 ? C - 1 : 15)); };
@@ -358,7 +362,7 @@ __global__ void __launch_bounds__(256, F32 && D == 256 ? 1 : 2) weigh_many_kerne
         }
         const uint32_t key0 = (keys.tile0 + b) * kKeys, w0 = key0 + kMine * w;
         const Seers rows(a, s, key0, kKeys);
-        const uint32_t per = (rows.r1 - rows.r0 + 31) / 32 + kSetup;
+        const uint32_t per = (rows.r1 - rows.r0 + kRows - 1) / kRows + kSetup;
         const uint64_t all = (uint64_t)per * a.n_kv, part = min(all - skip, run.t1 - t);
         const int base = (int)s.len - (int)s.nq;
         const uint32_t *table = a.table + (size_t)min(s.row, a.n_rows - 1) * a.ld_table;
@@ -400,64 +404,96 @@ __global__ void __launch_bounds__(256, F32 && D == 256 ? 1 : 2) weigh_many_kerne
                     kf[y][c] = z;
                 }
             }
-            // a tile of queries through registers to LDS
-            v8 qr[F32 ? 1 : kEach];
-            float fr[F32 ? kEach : 1][8], lse = 0.0f;
+            // A tile of queries through registers to LDS.  The bases of its rows are
+            // a wave's, another one's for each tile.
+            v8 qr[F32 ? 1 : U][F32 ? 1 : kEach];
+            float fr[F32 ? U : 1][F32 ? kEach : 1][8], lse = 0.0f;
+            auto row_of = [&](uint32_t r, uint32_t &tok, uint32_t &h) {     // (rows past the last are the last once more)
+                r = min(r, rows.r1 - 1);
+                tok = r / a.group;
+                h = r - tok * a.group;
+            };
+            // where a thread's rows are: from tile to tile by additions
+            const size_t step = (size_t)(kRows / a.group) * a.ld_q + (size_t)(kRows % a.group) * d, wrap = a.ld_q - (size_t)a.group * d;
+            size_t at[U];
+            uint32_t head_at[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                uint32_t tok;
+                row_of(rows.r0 + kRows * x0 + prow + 32 * u, tok, head_at[u]);
+                at[u] = (size_t)(s.first + tok) * a.ld_q + (size_t)(kvh * a.group + head_at[u]) * d;
+            }
             auto fetch = [&](uint32_t x) {
-                const uint32_t r = min(rows.r0 + 32 * x + prow, rows.r1 - 1), tok = r / a.group, h = kvh * a.group + (r - tok * a.group);
-                const size_t at = (size_t)(s.first + tok) * a.ld_q + (size_t)h * d;
-                if (pc == 0) lse = a.sums[(size_t)(s.first + tok) * a.n_kv * a.group + h];
+                const bool last = rows.r0 + kRows * (x + 1) > rows.r1;
 #pragma unroll
-                for (int i = 0; i < kEach; i++) {
-                    const int c = 8 * (pc + 8 * i);
-                    if constexpr (F32) {
-#pragma unroll
-                        for (int e = 0; e < 8; e++) fr[i][e] = 0.0f;
-                        if (c < (int)d) load8((const float *)a.q + at + c, fr[i]);
-                    } else {
-                        v8 z = {};
-                        if (c < (int)d) z = *(const v8 *)((const T *)a.q + at + c);
-                        qr[i] = z;
+                for (int u = 0; u < U; u++) {
+                    if (last && x > x0) {
+                        uint32_t tok, h;
+                        row_of(rows.r0 + kRows * x + prow + 32 * u, tok, h);
+                        at[u] = (size_t)(s.first + tok) * a.ld_q + (size_t)(kvh * a.group + h) * d;
                     }
+#pragma unroll
+                    for (int i = 0; i < kEach; i++) {
+                        const int c = 8 * (pc + 8 * i);
+                        if constexpr (F32) {
+#pragma unroll
+                            for (int e = 0; e < 8; e++) fr[u][i][e] = 0.0f;
+                            if (c < (int)d) load8((const float *)a.q + at[u] + c, fr[u][i]);
+                        } else {
+                            v8 z = {};
+                            if (c < (int)d) z = *(const v8 *)((const T *)a.q + at[u] + c);
+                            qr[u][i] = z;
+                        }
+                    }
+                    at[u] += step;
+                    head_at[u] += kRows % a.group;
+                    if (head_at[u] >= a.group) { head_at[u] -= a.group; at[u] += wrap; }
+                }
+                if (w == (x & 3) && lane < kRows) {
+                    uint32_t tok, h;
+                    row_of(rows.r0 + kRows * x + lane, tok, h);
+                    lse = a.sums[((size_t)(s.first + tok) * a.n_kv + kvh) * a.group + h];
                 }
             };
             auto put = [&](uint32_t x, int o) {
-                float unscale = a.scale;
-                if constexpr (F32) {
-                    float top = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < kEach; i++)
+                for (int u = 0; u < U; u++) {
+                    const int row = prow + 32 * u;
+                    if constexpr (F32) {
+                        float top = 0.0f;
 #pragma unroll
-                        for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(fr[i][e]));
+                        for (int i = 0; i < kEach; i++)
 #pragma unroll
-                    for (int k = 1; k < 8; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
-                    int ex = 0;
-                    if (__is_same(T, _Float16) && top > 0.0f && top < INFINITY) ex = 14 - ilogbf(top);
-                    unscale *= ldexpf(1.0f, -ex);
+                            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(fr[u][i][e]));
 #pragma unroll
-                    for (int i = 0; i < kEach; i++) {
-                        v8 p[3];
+                        for (int k = 1; k < 8; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
+                        int ex = 0;
+                        if (__is_same(T, _Float16) && top > 0.0f && top < INFINITY) ex = 14 - ilogbf(top);
+                        if (pc == 0) s_u[o][row] = a.scale * ldexpf(1.0f, -ex);
 #pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            const float y = ldexpf(fr[i][e], ex);
-                            p[0][e] = (T)y;
-                            const float y1 = y - (float)p[0][e];
-                            p[1][e] = (T)y1;
-                            p[2][e] = (T)(y1 - (float)p[1][e]);
+                        for (int i = 0; i < kEach; i++) {
+                            v8 p[3];
+#pragma unroll
+                            for (int e = 0; e < 8; e++) {
+                                const float y = ldexpf(fr[u][i][e], ex);
+                                p[0][e] = (T)y;
+                                const float y1 = y - (float)p[0][e];
+                                p[1][e] = (T)y1;
+                                p[2][e] = (T)(y1 - (float)p[1][e]);
+                            }
+#pragma unroll
+                            for (int q = 0; q < 3; q++) *(v8 *)&s_q[o][q % NP][row * D + 8 * place(row, pc + 8 * i)] = p[q];
                         }
+                    } else {
 #pragma unroll
-                        for (int q = 0; q < 3; q++) *(v8 *)&s_q[o][q % NP][prow * D + 8 * place(prow, pc + 8 * i)] = p[q];
+                        for (int i = 0; i < kEach; i++) *(v8 *)&s_q[o][0][row * D + 8 * place(row, pc + 8 * i)] = qr[u][i];
                     }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < kEach; i++) *(v8 *)&s_q[o][0][prow * D + 8 * place(prow, pc + 8 * i)] = qr[i];
                 }
-                if (pc == 0) {
+                if (w == (x & 3) && lane < kRows) {
                     float n, c;
                     base_of(a, lse, n, c);
-                    s_n[o][prow] = n;
-                    s_c[o][prow] = rows.r0 + 32 * x + prow < rows.r1 ? c : 0.0f;       // (rows past the last are the last once more)
-                    s_u[o][prow] = unscale;
+                    s_n[o][lane] = n;
+                    s_c[o][lane] = rows.r0 + kRows * x + lane < rows.r1 ? c : 0.0f;
                 }
             };
             fetch(x0);
@@ -468,49 +504,53 @@ __global__ void __launch_bounds__(256, F32 && D == 256 ? 1 : 2) weigh_many_kerne
                 const int o = (x - x0) & 1;
                 const bool more = x + 1 < x1;
                 if (more) fetch(x + 1);
-                // the tile's first and last positions
-                const uint32_t ra = rows.r0 + 32 * x, rb = min(ra + 31, rows.r1 - 1);
-                const int pa = base + (int)(ra / a.group), pb = base + (int)(rb / a.group);
-                if ((int)w0 <= pb && (int64_t)w0 + kMine > (int64_t)pa + 1 - (int64_t)a.window) {
-                    const float n = s_n[o][col], by = s_c[o][col], unscale = F32 ? s_u[o][col] : a.scale;
-                    const bool edge = (int)w0 + kMine > pa + 1 || (int64_t)w0 < (int64_t)pb + 1 - (int64_t)a.window;
-                    constexpr bool kAhead = NP == 1 && D < 256;         // all of a tile's factors at once (more do not fit the registers)
-                    v8 f[kAhead ? KF : 1];
-                    auto factor = [&](int q, int c) { return *(const v8 *)&s_q[o][q][col * D + 8 * place(col, 2 * c + hg)]; };
-                    if constexpr (kAhead)
+#pragma unroll 1
+                for (int u = 0; u < U; u++) {
+                    // 32 rows at a time: their first and last positions
+                    const uint32_t ra = rows.r0 + kRows * x + 32 * u, rb = min(ra + 31, rows.r1 - 1);
+                    if (ra >= rows.r1) break;
+                    const int pa = base + (int)(ra / a.group), pb = base + (int)(rb / a.group);
+                    if ((int)w0 <= pb && (int64_t)w0 + kMine > (int64_t)pa + 1 - (int64_t)a.window) {
+                        const float n = s_n[o][32 * u + col], by = s_c[o][32 * u + col], unscale = F32 ? s_u[o][32 * u + col] : a.scale;
+                        const bool edge = (int)w0 + kMine > pa + 1 || (int64_t)w0 < (int64_t)pb + 1 - (int64_t)a.window;
+                        constexpr bool kAhead = NP == 1 && D < 256;         // all of a tile's factors at once (more do not fit the registers)
+                        v8 f[kAhead ? KF : 1];
+                        auto factor = [&](int q, int c) { return *(const v8 *)&s_q[o][q][(32 * u + col) * D + 8 * place(col, 2 * c + hg)]; };
+                        if constexpr (kAhead)
 #pragma unroll
-                        for (int c = 0; c < KF; c++) f[c] = factor(0, c);
-                    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                    for (int y = 0; y < KT; y++) {
-                        // these scores while the last ones' exponentials run
-                        f16v z;
-#pragma unroll
-                        for (int i = 0; i < 16; i++) z[i] = 0.0f;
-                        constexpr int kAll = NP * KF, kTurn = kAll < 8 ? 4 : kAll < 16 ? 2 : 1;
-#pragma unroll
-                        for (int p = 0; p < kAll; p++) {            // (the small parts first)
-                            z = mfma(kf[y][p % KF], kAhead ? f[kAhead ? p : 0] : factor(NP - 1 - p / KF, p % KF), z);
-                            if (kTurn * p < 16) weigh(y ? y - 1 : KT - 1, kTurn * p, kTurn);
-                        }
-#pragma unroll
-                        for (int p = 0; p < kAll; p++) {
-                            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                            if (kTurn * p < 16) __builtin_amdgcn_sched_group_barrier(0x002, 2 * kTurn, 0);
-                        }
-#pragma unroll
-                        for (int i = 0; i < 16; i++) asm volatile("" : "+v"(sum[y ? y - 1 : KT - 1][i]));     // (here: else they are put off past the branch below)
+                            for (int c = 0; c < KF; c++) f[c] = factor(0, c);
                         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                        for (int i = 0; i < 16; i++) wait[i] = fmaf(z[i], unscale, -n);
-                        wait_by = by;
-                        if (edge) {
-                            const int pos = base + (int)(min(ra + col, rb) / a.group);
-                            const int up = pos - (int)w0 - 4 * hg, down = (int)max((int64_t)-1, (int64_t)pos + 1 - (int64_t)a.window - w0) - 4 * hg;
+                        for (int y = 0; y < KT; y++) {
+                            // these scores while the last ones' exponentials run
+                            f16v z;
 #pragma unroll
-                            for (int i = 0; i < 16; i++) {
-                                const int key = 32 * y + 8 * (i >> 2) + (i & 3);        // from the lane's first
-                                if (key > up || key < down) wait[i] = -INFINITY;
+                            for (int i = 0; i < 16; i++) z[i] = 0.0f;
+                            constexpr int kAll = NP * KF, kTurn = kAll < 8 ? 4 : kAll < 16 ? 2 : 1;
+#pragma unroll
+                            for (int p = 0; p < kAll; p++) {            // (the small parts first)
+                                z = mfma(kf[y][p % KF], kAhead ? f[kAhead ? p : 0] : factor(NP - 1 - p / KF, p % KF), z);
+                                if (kTurn * p < 16) weigh(y ? y - 1 : KT - 1, kTurn * p, kTurn);
+                            }
+#pragma unroll
+                            for (int p = 0; p < kAll; p++) {
+                                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                                if (kTurn * p < 16) __builtin_amdgcn_sched_group_barrier(0x002, 2 * kTurn, 0);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 16; i++) asm volatile("" : "+v"(sum[y ? y - 1 : KT - 1][i]));     // (here: else they are put off past the branch below)
+                            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                            for (int i = 0; i < 16; i++) wait[i] = fmaf(z[i], unscale, -n);
+                            wait_by = by;
+                            if (edge) {
+                                const int pos = base + (int)(min(ra + col, rb) / a.group);
+                                const int up = pos - (int)w0 - 4 * hg, down = (int)max((int64_t)-1, (int64_t)pos + 1 - (int64_t)a.window - w0) - 4 * hg;
+#pragma unroll
+                                for (int i = 0; i < 16; i++) {
+                                    const int key = 32 * y + 8 * (i >> 2) + (i & 3);        // from the lane's first
+                                    if (key > up || key < down) wait[i] = -INFINITY;
+                                }
                             }
                         }
                     }
@@ -543,7 +583,7 @@ __global__ void __launch_bounds__(256, F32 && D == 256 ? 1 : 2) weigh_many_kerne
                         tiles_of(kvh, x0, x1);
                         const uint32_t id = min(table[key >> a.shift], a.n_pages - 1);
                         const T *p = (const T *)a.k + ((size_t)id * a.n_kv + kvh) * head + (size_t)(key & slot) * d;
-                        for (uint32_t r = rows.r0 + 32 * x0 + lane; r < min(rows.r0 + 32 * x1, rows.r1); r += 64) {
+                        for (uint32_t r = rows.r0 + kRows * x0 + lane; r < min(rows.r0 + kRows * x1, rows.r1); r += 64) {
                             const uint32_t tok = r / a.group, h = kvh * a.group + (r - tok * a.group);
                             const int pos = base + (int)tok;
                             if ((int)key > pos || (int64_t)key <= (int64_t)pos - (int64_t)a.window) continue;
@@ -605,7 +645,7 @@ template <class T, int D, bool F32> void by_rows(gs::WeighArgs a, uint64_t rows,
     a.max_rows = 0xffffffffu;
     a.n_wg = gs::kManyRuns;
     hipLaunchKernelGGL((gs::weigh_many_kernel<T, D, F32>), dim3(a.n_wg), dim3(256), 0, st, a);
-    hipLaunchKernelGGL(gs::weigh_join_kernel, dim3(a.n_wg), dim3(256), 0, st, a, gs::Many<D>::kKeys);
+    hipLaunchKernelGGL(gs::weigh_join_kernel, dim3(a.n_wg), dim3(256), 0, st, a, gs::Many<D, F32>::kKeys);
 }
 
 template <class T, bool F32> void by_head(const gs::WeighArgs &a, uint64_t rows, hipStream_t st)
@@ -623,7 +663,7 @@ extern "C" {
 
 size_t gs_attn_weigh_workspace(const gs_kv_cache *c)
 {
-    return check_cache(c) ? 0 : kLeftBytes + (size_t)2 * gs::kManyRuns * gs::Many<128>::kKeys * sizeof(float);
+    return check_cache(c) ? 0 : kLeftBytes + (size_t)2 * gs::kManyRuns * gs::Many<128, false>::kKeys * sizeof(float);
 }
 
 int gs_attn_weigh(const gs_kv_cache *c, uint32_t layer, const gs_kv_batch *b, const gs_weigh_args *x, void *stream)

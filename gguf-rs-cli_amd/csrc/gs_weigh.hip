@@ -372,13 +372,18 @@ __global__ void __launch_bounds__(256, F32 && D == 256 ? 1 : 2) weigh_many_kerne
         for (int y = 0; y < KT; y++)
 #pragma unroll
             for (int i = 0; i < 16; i++) sum[y][i] = 0.0f;
-        // the last 32 keys' exponents and factors, whose exponentials are still to come
-        float wait[16], wait_by = 0.0f;
+        // the last rows' exponents and factors, whose exponentials are still to come
+        float wait[KT][16], wait_by = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; i++) wait[i] = -INFINITY;
-        auto weigh = [&](int y, int i0, int n) {
+        for (int y = 0; y < KT; y++)
 #pragma unroll
-            for (int i = i0; i < i0 + n; i++) sum[y][i] = fmaf(__builtin_amdgcn_exp2f(wait[i]), wait_by, sum[y][i]);
+            for (int i = 0; i < 16; i++) wait[y][i] = -INFINITY;
+        auto weigh = [&](int i0, int i1) {
+#pragma unroll
+            for (int i = i0; i < i1 && i < 16 * KT; i++) {
+                sum[i >> 4][i & 15] = fmaf(__builtin_amdgcn_exp2f(wait[i >> 4][i & 15]), wait_by, sum[i >> 4][i & 15]);
+                asm volatile("" : "+v"(sum[i >> 4][i & 15]));       // (here: else it is put off past the branch that follows)
+            }
         };
         const uint32_t kv0 = (uint32_t)quotient(skip, per), kv1 = (uint32_t)quotient(skip + part - 1, per);
         // tiles of rows x0 .. x1 - 1 of head kvh are this run's
@@ -513,45 +518,44 @@ __global__ void __launch_bounds__(256, F32 && D == 256 ? 1 : 2) weigh_many_kerne
                     if ((int)w0 <= pb && (int64_t)w0 + kMine > (int64_t)pa + 1 - (int64_t)a.window) {
                         const float n = s_n[o][32 * u + col], by = s_c[o][32 * u + col], unscale = F32 ? s_u[o][32 * u + col] : a.scale;
                         const bool edge = (int)w0 + kMine > pa + 1 || (int64_t)w0 < (int64_t)pb + 1 - (int64_t)a.window;
-                        constexpr bool kAhead = NP == 1 && D < 256;         // all of a tile's factors at once (more do not fit the registers)
-                        v8 f[kAhead ? KF : 1];
-                        auto factor = [&](int q, int c) { return *(const v8 *)&s_q[o][q][(32 * u + col) * D + 8 * place(col, 2 * c + hg)]; };
-                        if constexpr (kAhead)
+                        // these scores while the last ones' exponentials run; the factors
+                        // come from LDS kAhead products before theirs
+                        constexpr int kAll = NP * KF, kAhead = F32 ? 2 : 4, kTurn = (16 * KT + kAll - 1) / kAll;
+                        v8 f[kAhead];
+                        auto factor = [&](int p) {                          // (the small parts first)
+                            f[p % kAhead] = *(const v8 *)&s_q[o][NP - 1 - p / KF][(32 * u + col) * D + 8 * place(col, 2 * (p % KF) + hg)];
+                        };
+                        f16v z[KT];
 #pragma unroll
-                            for (int c = 0; c < KF; c++) f[c] = factor(0, c);
+                        for (int y = 0; y < KT; y++)
+#pragma unroll
+                            for (int i = 0; i < 16; i++) z[y][i] = 0.0f;
+#pragma unroll
+                        for (int p = 0; p < kAhead; p++) factor(p);
                         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                        for (int y = 0; y < KT; y++) {
-                            // these scores while the last ones' exponentials run
-                            f16v z;
+                        for (int p = 0; p < kAll; p++) {
 #pragma unroll
-                            for (int i = 0; i < 16; i++) z[i] = 0.0f;
-                            constexpr int kAll = NP * KF, kTurn = kAll < 8 ? 4 : kAll < 16 ? 2 : 1;
-#pragma unroll
-                            for (int p = 0; p < kAll; p++) {            // (the small parts first)
-                                z = mfma(kf[y][p % KF], kAhead ? f[kAhead ? p : 0] : factor(NP - 1 - p / KF, p % KF), z);
-                                if (kTurn * p < 16) weigh(y ? y - 1 : KT - 1, kTurn * p, kTurn);
-                            }
-#pragma unroll
-                            for (int p = 0; p < kAll; p++) {
-                                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                                if (kTurn * p < 16) __builtin_amdgcn_sched_group_barrier(0x002, 2 * kTurn, 0);
-                            }
-#pragma unroll
-                            for (int i = 0; i < 16; i++) asm volatile("" : "+v"(sum[y ? y - 1 : KT - 1][i]));     // (here: else they are put off past the branch below)
+                            for (int y = 0; y < KT; y++) z[y] = mfma(kf[y][p % KF], f[p % kAhead], z[y]);
+                            if (p + kAhead < kAll) factor(p + kAhead);
+                            weigh(kTurn * p, kTurn * (p + 1));
                             __builtin_amdgcn_sched_barrier(0);
+                        }
 #pragma unroll
-                            for (int i = 0; i < 16; i++) wait[i] = fmaf(z[i], unscale, -n);
-                            wait_by = by;
-                            if (edge) {
-                                const int pos = base + (int)(min(ra + col, rb) / a.group);
-                                const int up = pos - (int)w0 - 4 * hg, down = (int)max((int64_t)-1, (int64_t)pos + 1 - (int64_t)a.window - w0) - 4 * hg;
+                        for (int y = 0; y < KT; y++)
+#pragma unroll
+                            for (int i = 0; i < 16; i++) wait[y][i] = fmaf(z[y][i], unscale, -n);
+                        wait_by = by;
+                        if (edge) {
+                            const int pos = base + (int)(min(ra + col, rb) / a.group);
+                            const int up = pos - (int)w0 - 4 * hg, down = (int)max((int64_t)-1, (int64_t)pos + 1 - (int64_t)a.window - w0) - 4 * hg;
+#pragma unroll
+                            for (int y = 0; y < KT; y++)
 #pragma unroll
                                 for (int i = 0; i < 16; i++) {
                                     const int key = 32 * y + 8 * (i >> 2) + (i & 3);        // from the lane's first
-                                    if (key > up || key < down) wait[i] = -INFINITY;
+                                    if (key > up || key < down) wait[y][i] = -INFINITY;
                                 }
-                            }
                         }
                     }
                 }
@@ -560,7 +564,7 @@ __global__ void __launch_bounds__(256, F32 && D == 256 ? 1 : 2) weigh_many_kerne
             }
         }
 
-        weigh(KT - 1, 0, 16);
+        weigh(0, 16 * KT);
 
         // ---- the block's sums, or this run's part of them
 #pragma unroll

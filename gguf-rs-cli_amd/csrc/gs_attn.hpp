@@ -158,20 +158,36 @@ template <int kTile> struct Span {
     }
 };
 
+// a / b, by 32-bit division where that is enough (as it is for any call that
+// fits the memory; 64 bits are several times as many instructions).
+__device__ __forceinline__ uint64_t quotient(uint64_t a, uint64_t b)
+{
+    return (a | b) >> 32 ? a / b : (uint32_t)a / (uint32_t)b;
+}
+
 // How a kernel deals its work: R rows in a unit, kTile keys in a tile, and a
 // unit's beginning and end (its queries, the first keys' way, its rows' way
 // out), which are dealt as kSetup tiles before its first.  (us with 0, as it
 // is, twice as many: 16 prompts of 512, 28 / 4 heads of 128, kSetup 0, 3, 6:
 // 111, 92, 87; one of 2000, 32 / 8 heads, 3 and 6: 80, 84; 64 single tokens
 // over 1500, kSetup 0, 1, 2: 39.5, 39.2, 41.4.)
-template <int R_, int kTile_, int kSetup_, class S> struct Deal {
+// Where kBase is given, a tile is dealt as kBase pieces and one for each kM rows
+// that a wave has of it; a tile is the run's that its first piece is in.
+template <int R_, int kTile_, int kSetup_, class S, int kBase = 0, int kM = 1> struct Deal {
     static constexpr int R = R_, kTile = kTile_, kSetup = kSetup_;
     using Work = S;
+    static __device__ __forceinline__ uint32_t weight(uint32_t r0, uint32_t r1) { return kBase ? kBase + (r1 - r0 + kM - 1) / kM : 1; }
+    // The first tile of a unit whose pieces begin at or after `piece` of its beginning.
+    static __device__ __forceinline__ uint32_t tile_at(uint64_t piece, uint32_t weight)
+    {
+        return max((uint32_t)quotient(piece + weight - 1, weight), (uint32_t)kSetup) - kSetup;
+    }
     static __device__ __forceinline__ uint32_t heads(const AttnArgs &a) { return a.n_kv; }
     // Tiles of the unit of rows r ..
     static __device__ __forceinline__ uint32_t unit(const AttnArgs &a, const S &s, uint32_t r)
     {
-        return Span<kTile>(a, s, r, min(r + R, s.nq * a.group)).tiles + kSetup;
+        const uint32_t r1 = min(r + R, s.nq * a.group);
+        return (Span<kTile>(a, s, r, r1).tiles + kSetup) * weight(r, r1);       // (below 2^32: tiles of 32 keys, positions below 2^30)
     }
     // Tiles of a sequence and one head of keys (a chunk of 66000 tokens over 2^23
     // has more than 2^32 of 16 rows), counted by a thread ..
@@ -194,33 +210,27 @@ template <int R_, int kTile_, int kSetup_, class S> struct Deal {
     // becomes the tile's number in the unit.  (a wave)
     static __device__ __forceinline__ uint32_t find(const AttnArgs &a, const S &s, uint64_t &skip)
     {
+        using Sum = std::conditional_t<kBase == 0, uint32_t, uint64_t>;       // (of 64 units)
         const uint32_t rows = s.nq * a.group, lane = threadIdx.x & 63;
         if (rows <= R) return 0;
         for (uint32_t r = 0;; r += 64 * R) {
             const uint32_t mine = r + lane * R < rows ? unit(a, s, r + lane * R) : 0;
-            uint32_t sum = mine;
+            Sum sum = mine;
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
-                const uint32_t y = __shfl_up(sum, o);
+                const Sum y = __shfl_up(sum, o);
                 if (lane >= o) sum += y;
             }
             const uint64_t past = __ballot(sum > skip);
             if (past) {
                 const int at = __ffsll((unsigned long long)past) - 1;
-                skip -= uniform(__shfl(sum - mine, at));
+                skip -= uniform((Sum)__shfl((Sum)(sum - mine), at));
                 return r + at * R;
             }
-            skip -= uniform(__shfl(sum, 63));
+            skip -= uniform((Sum)__shfl(sum, 63));
         }
     }
 };
-
-// a / b, by 32-bit division where that is enough (as it is for any call that
-// fits the memory; 64 bits are several times as many instructions).
-__device__ __forceinline__ uint64_t quotient(uint64_t a, uint64_t b)
-{
-    return (a | b) >> 32 ? a / b : (uint32_t)a / (uint32_t)b;
-}
 
 // The run of this workgroup: its tiles [t0, t1) of `total`, the sequence the
 // first of them is in, and how many tiles of that sequence come before it.
@@ -844,6 +854,14 @@ __device__ __forceinline__ float max_halves(float x)
 template <int D> struct Chunk {
     static constexpr int kM = D == 256 ? 16 : 32, kTile = D == 256 ? 32 : 64;
     static constexpr int kRows = 8 * kM, kThreads = 512;
+    // What a tile costs beside its rows, in eighths of what 8 kM rows add, where
+    // units of many and of few rows are dealt together.  (us of a tile of 64 keys
+    // of heads of 128, 8 waves with rows, 6 and 1: 2.4, 2.1, 1.5; of 32 keys of 256,
+    // 8 and 1: 1.7, 1.3.  One family of 64 rows over 16000 tokens, 28 / 4 heads:
+    // 63 us, with tiles dealt alike 70.)
+    static constexpr int kBase = D == 256 ? 24 : 8;
+    // (a run is at least as long as the heaviest tile, also where two share little more than twice that)
+    static constexpr int kLeast = 3 * (kBase + 1) > 2 * (kBase + 8) ? 3 * (kBase + 1) : 2 * (kBase + 8);
 };
 constexpr int kChunkRuns = 256;         // one workgroup per CU
 
@@ -890,8 +908,8 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, 2) attn_chunk_kernel(const
     // runs that follow one another, which read the same keys, on one XCD
     const uint32_t g8 = a.n_wg / 8, run_id = a.n_wg % 8 ? blockIdx.x : (blockIdx.x & 7) * g8 + (blockIdx.x >> 3);
     using S = std::conditional_t<SHARED, Job, Seq>;
-    using Dealt = Deal<R, kTile, 3, S>;
-    Run<S> run = run_of<Dealt, kThreads, 3>(a, run_id);
+    using Dealt = Deal<R, kTile, 3, S, SHARED ? Chunk<D>::kBase : 0, M>;
+    Run<S> run = run_of<Dealt, kThreads, SHARED ? Chunk<D>::kLeast : 3>(a, run_id);
     if (!SHARED && threadIdx.x == 0) a.cuts[run_id].last = 0;
     if (run.t0 >= run.t1) return;
 
@@ -929,11 +947,17 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, 2) attn_chunk_kernel(const
         const uint32_t r1 = min(r0 + R, rows);
         const Span<kTile> span(a, s, r0, r1);
         // the run's part of the unit, tiles first .. first + left - 1
-        const uint32_t dealt = span.tiles + Dealt::kSetup, part_of = (uint32_t)min((uint64_t)(dealt - skip), run.t1 - t);
-        const uint32_t first = max(skip, (uint32_t)Dealt::kSetup) - Dealt::kSetup;
-        const uint32_t left = max(skip + part_of, (uint32_t)Dealt::kSetup) - Dealt::kSetup - first;
-        if (left == 0) break;                           // (its setup only: the next run begins it)
-        const uint64_t end = t - skip + dealt;
+        const uint32_t weight = Dealt::weight(r0, r1);
+        const uint32_t dealt = (span.tiles + Dealt::kSetup) * weight, part_of = (uint32_t)min((uint64_t)(dealt - skip), run.t1 - t);
+        const uint32_t first = Dealt::tile_at(skip, weight), left = Dealt::tile_at((uint64_t)skip + part_of, weight) - first;
+        if (left == 0) {                                // (its setup only: the next run begins it; or a piece of its last tile)
+            t += part_of;
+            skip = 0;
+            r0 += R;
+            if (r0 >= rows) { r0 = 0; kvh++; }
+            continue;
+        }
+        const uint64_t end = t - skip + dealt - (weight - 1);       // behind the last tile's first piece
         const int base = (int)s.len - (int)s.nq;        // position of the sequence's first token
 
         // ---- queries: row col of the wave's M

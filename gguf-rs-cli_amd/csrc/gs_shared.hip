@@ -21,86 +21,124 @@ namespace gs {
 constexpr int kPlan = 1024;
 
 // The jobs of family blockIdx.x and its sequences, and their tokens' positions.
-// The common keys are whole pages that every row's table has alike, and that all
-// of the family's new tokens come after.
+// The common keys are whole pages that the tables of all rows with new tokens
+// have alike, and that all of the family's new tokens come after.  What bounds
+// it is its chain of reads (begins, rows, lengths, tables), so the tables are
+// compared kTables pieces of 64 pages at a time.
 __global__ void __launch_bounds__(kPlan) shared_plan_kernel(const AttnArgs a, const uint32_t *families, uint32_t n, Job *jobs, int32_t *pos)
 {
-    __shared__ uint32_t s_pages;
+    constexpr int kTables = 16;
+    __shared__ uint32_t s_pages, s_first, s_end, s_lead, s_count, s_row[kPlan];
     __shared__ int32_t s_p0, s_p1;
     const uint32_t j = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     // (tokens of no sequence are left as they are)
     const size_t rows = (size_t)a.n_tokens * a.n_kv * a.group;
     for (size_t i = (size_t)j * kPlan + threadIdx.x; i < rows; i += (size_t)gridDim.x * kPlan) a.where[rows + i] = kDone;
-    auto bound = [&](uint32_t i) { return i < a.n_families ? min(families[i], n) : min(families[a.n_families], n); };
-    const uint32_t s0 = bound(j), s1 = max(bound(j + 1), s0);
-    auto sequence = [&](uint32_t i, Job &x) {
-        x = Job();
+    const uint32_t s0 = min(families[j], n), s1 = max(min(families[j + 1], n), s0);
+    auto sequence = [&](uint32_t i) {
+        Job x = {};
         x.first = a.start ? min(a.start[i], a.n_tokens) : i;
         const uint32_t end = a.start ? min(a.start[i + 1], a.n_tokens) : i + 1;
         x.nq = end > x.first ? end - x.first : 0;
         x.row = a.rows ? a.rows[i] : i;
         x.len = x.row < a.n_rows ? min(a.len[x.row], a.ld_table << a.shift) : 0;
         x.k1 = x.len;
+        return x;
     };
-    // pages before the earliest new token
-    if (threadIdx.x == 0) { s_pages = s1 - s0 > 1 ? a.ld_table : 0; s_p0 = 0x7fffffff; s_p1 = -1; }
-    __syncthreads();
-    for (uint32_t i = s0 + threadIdx.x; i < s1; i += kPlan) {
-        Job x;
-        sequence(i, x);
-        if (x.nq == 0) continue;
-        atomicMin(&s_pages, x.len > x.nq ? (x.len - x.nq) >> a.shift : 0);
-        atomicMin(&s_p0, (int32_t)(x.len - x.nq));
-        atomicMax(&s_p1, (int32_t)x.len - 1);
+    if (threadIdx.x == 0) {
+        s_pages = a.ld_table;
+        s_first = 0xffffffffu; s_end = 0; s_lead = 0xffffffffu; s_count = 0;
+        s_p0 = 0x7fffffff; s_p1 = -1;
     }
     __syncthreads();
-    // and alike in the tables of all rows that have new tokens
-    const uint32_t most = s_pages;
-    if (most) {
-        uint32_t lead = GS_KV_NONE, least = most;
-        for (uint32_t i = s0; i < s1 && lead == GS_KV_NONE; i++) {
-            Job x;
-            sequence(i, x);
-            if (x.nq) lead = x.row;
+    // the sequences with new tokens: how many, the first of them, their positions, pages before the earliest token
+    // (a wave's first, and then one atomic of each: 64 of them to one word take a microsecond)
+    if (s0 + 64 * w < s1) {
+        uint32_t pages = a.ld_table, first = 0xffffffffu, end = 0, before = 0xffffffffu, count = 0;
+        int32_t p0 = 0x7fffffff, p1 = -1;
+        for (uint32_t i = s0 + threadIdx.x; i < s1; i += kPlan) {
+            const Job x = sequence(i);
+            if (x.nq == 0) continue;
+            pages = min(pages, x.len > x.nq ? (x.len - x.nq) >> a.shift : 0);
+            p0 = min(p0, (int32_t)(x.len - x.nq));
+            p1 = max(p1, (int32_t)x.len - 1);
+            first = min(first, x.first);
+            end = max(end, x.first + x.nq);
+            before = min(before, i);
+            count++;
         }
-        const uint32_t *t0 = a.table + (size_t)lead * a.ld_table;       // (every row with new tokens is there: it has pages before them)
-        for (uint32_t i = s0 + w; i < s1; i += kPlan / 64) {
-            Job x;
-            sequence(i, x);
-            if (x.nq == 0 || x.row == lead) continue;
-            const uint32_t *t1 = a.table + (size_t)x.row * a.ld_table;
-            for (uint32_t p = 0; p < least; p += 64) {
-                const uint64_t other = __ballot(p + lane < least && t0[p + lane] != t1[p + lane]);
-                if (other) { least = p + __ffsll((unsigned long long)other) - 1; break; }
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            pages = min(pages, (uint32_t)__shfl_xor(pages, o));
+            p0 = min(p0, __shfl_xor(p0, o));
+            p1 = max(p1, __shfl_xor(p1, o));
+            first = min(first, (uint32_t)__shfl_xor(first, o));
+            end = max(end, (uint32_t)__shfl_xor(end, o));
+            before = min(before, (uint32_t)__shfl_xor(before, o));
+            count += __shfl_xor(count, o);
+        }
+        if (lane == 0) {
+            atomicMin(&s_pages, pages);
+            atomicMin(&s_p0, p0);
+            atomicMax(&s_p1, p1);
+            atomicMin(&s_first, first);
+            atomicMax(&s_end, end);
+            atomicMin(&s_lead, before);
+            atomicAdd(&s_count, count);
+        }
+    }
+    __syncthreads();
+    const uint32_t most = s_count > 1 ? s_pages : 0;
+    uint32_t lead = 0;
+    if (most) {
+        // (every row with new tokens is there: it has pages before them)
+        lead = a.rows ? a.rows[s_lead] : s_lead;
+        const uint32_t *t0 = a.table + (size_t)lead * a.ld_table;
+        const uint32_t pieces = (most + 63) / 64;
+        uint32_t least = most;
+        for (uint32_t i0 = s0; i0 < s1; i0 += kPlan) {          // the rows of up to kPlan sequences, `lead` for those without tokens
+            const uint32_t m = min(s1 - i0, (uint32_t)kPlan);
+            __syncthreads();
+            if (threadIdx.x < m) {
+                const Job y = sequence(i0 + threadIdx.x);
+                s_row[threadIdx.x] = y.nq ? y.row : lead;
+            }
+            __syncthreads();
+            const uint32_t all = m * pieces;                    // (below 2^30: a table has at most 2^26 places)
+            for (uint32_t x0 = w; x0 < all; x0 += kPlan / 64 * kTables) {
+                uint32_t p[kTables], mine[kTables], other[kTables];
+#pragma unroll
+                for (int e = 0; e < kTables; e++) {
+                    const uint32_t x = min(x0 + kPlan / 64 * e, all - 1), i = x / pieces;
+                    p[e] = min(64 * (x - i * pieces) + lane, most - 1);
+                    mine[e] = t0[p[e]];
+                    other[e] = a.table[(size_t)s_row[i] * a.ld_table + p[e]];
+                }
+#pragma unroll
+                for (int e = 0; e < kTables; e++)
+                    if (mine[e] != other[e]) least = min(least, p[e]);
             }
         }
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) least = min(least, (uint32_t)__shfl_xor(least, o));
+        __syncthreads();                    // (s_pages is read)
         if (lane == 0) atomicMin(&s_pages, least);
     }
     __syncthreads();
-    const uint32_t common = s_pages << a.shift;
-    auto write = [&](uint32_t i, uint32_t k0) {
-        Job x;
-        sequence(i, x);
+    const uint32_t common = most ? s_pages << a.shift : 0;
+    auto write = [&](uint32_t i, uint32_t k0) {         // (a wave)
+        Job x = sequence(i);
         x.k0 = k0;
-        jobs[a.n_families + i] = x;
-        for (uint32_t t = 0; t < x.nq; t++) pos[x.first + t] = (int32_t)x.len - (int32_t)x.nq + (int32_t)t;
+        if (lane == 0) jobs[a.n_families + i] = x;
+        for (uint32_t t = lane; t < x.nq; t += 64) pos[x.first + t] = (int32_t)x.len - (int32_t)x.nq + (int32_t)t;
     };
-    for (uint32_t i = s0 + threadIdx.x; i < s1; i += kPlan) write(i, common);
+    for (uint32_t i = s0 + w; i < s1; i += kPlan / 64) write(i, common);
     if (threadIdx.x == 0) {
         Job x = {};
-        if (common) {
-            Job y;
-            uint32_t first = a.n_tokens, end = 0;
-            for (uint32_t i = s0; i < s1; i++) {
-                sequence(i, y);
-                if (y.nq == 0) continue;
-                if (first == a.n_tokens) { first = y.first; x.row = y.row; }
-                end = y.first + y.nq;
-            }
-            x.first = first;
-            x.nq = end > first ? end - first : 0;
-        }
+        x.row = lead;
         x.len = kFamily;
+        x.first = common ? s_first : 0;
+        x.nq = common ? s_end - s_first : 0;
         x.k1 = common;
         x.p0 = s_p0;
         x.p1 = s_p1;
@@ -108,9 +146,9 @@ __global__ void __launch_bounds__(kPlan) shared_plan_kernel(const AttnArgs a, co
     }
     // sequences of no family
     if (j == 0)
-        for (uint32_t i = threadIdx.x; i < s0; i += kPlan) write(i, 0);
+        for (uint32_t i = w; i < s0; i += kPlan / 64) write(i, 0);
     if (j + 1 == a.n_families)
-        for (uint32_t i = s1 + threadIdx.x; i < n; i += kPlan) write(i, 0);
+        for (uint32_t i = s1 + w; i < n; i += kPlan / 64) write(i, 0);
 }
 
 // Where the parts of one of a row's jobs are.
@@ -271,35 +309,45 @@ template <class TO, int D, int R1, int R2> void join(const gs::AttnArgs &a, cons
 }
 
 // `own`, `family`: the most query rows per head of keys that a sequence, or a
-// family, may have.  a: the first kernel's arguments, b: the second's.
-template <class T, int D, bool F32> void by_rows(gs::AttnArgs &a, gs::AttnArgs &b, uint64_t family, hipStream_t st)
+// family, may have.  Jobs of few rows are the first kernel's, the others the
+// second's.
+template <class T, int D, int NT, bool F32> void few_and_many(gs::AttnArgs &a, gs::AttnArgs &b, uint64_t family, hipStream_t st)
 {
-    b.second = gs::kSecond;
-    if constexpr (F32) {
-        constexpr int NT = D == 256 ? 1 : 2;
-        rows_launch<T, D, NT, F32>(a, st);
-        join<float, D, 16 * NT, 16 * NT>(a, a, st);
-    } else {
-        constexpr int kFew = D == 256 ? 16 : 32;
-        if (family <= kFew) {
-            rows_launch<T, D, kFew / 16, F32>(a, st);
-            join<T, D, kFew, kFew>(a, a, st);
+    if constexpr (!F32)
+        if (family > 16 * NT) {
+            b.second = gs::kSecond;
+            // Few sequences' own keys do not fill a launch of their own.  (us with two
+            // kernels and with the second alone, heads of 128: one family of 8 rows
+            // over 1000 tokens and up to 50 of their own, 8 heads of keys, 37.5, 26.9;
+            // 4 of 8 over 2000, 40.2, 33.7; one of 64 over 4000, 52.4, 54.4; 8 of 32 over
+            // 2000, 4 heads of keys, 77.9, 89.4.  Heads of 256, one of 16 over 8000, 57.9,
+            // 41.7; 16 of 16 over 2000 and up to 1000, 293, 306.)
+            if ((uint64_t)(a.n - a.n_families) * a.n_kv > gs::kChunkRuns) {
+                a.max_rows = 16 * NT;
+                b.min_rows = 16 * NT + 1;
+                rows_launch<T, D, NT, F32>(a, st);
+            }
+            chunk_launch<T, D>(b, st);
+            join<T, D, 16 * NT, gs::Chunk<D>::kRows>(a, b, st);
             return;
         }
-        a.max_rows = kFew;
-        b.min_rows = kFew + 1;
-        rows_launch<T, D, kFew / 16, F32>(a, st);
-        chunk_launch<T, D>(b, st);
-        join<T, D, kFew, gs::Chunk<D>::kRows>(a, b, st);
-    }
+    rows_launch<T, D, NT, F32>(a, st);
+    join<std::conditional_t<F32, float, T>, D, 16 * NT, 16 * NT>(a, a, st);
 }
 
-template <class T, bool F32> void by_head(gs::AttnArgs &a, gs::AttnArgs &b, uint64_t family, hipStream_t st)
+template <class T, int D, bool F32> void by_rows(gs::AttnArgs &a, gs::AttnArgs &b, uint64_t own, uint64_t family, hipStream_t st)
+{
+    if constexpr (D == 256) few_and_many<T, D, 1, F32>(a, b, family, st);       // (two tiles of rows spill, or go to the second kernel)
+    else if ((F32 ? family : own) <= 16) few_and_many<T, D, 1, F32>(a, b, family, st);
+    else few_and_many<T, D, 2, F32>(a, b, family, st);
+}
+
+template <class T, bool F32> void by_head(gs::AttnArgs &a, gs::AttnArgs &b, uint64_t own, uint64_t family, hipStream_t st)
 {
     switch (padded(a.d)) {
-    case 64: return by_rows<T, 64, F32>(a, b, family, st);
-    case 128: return by_rows<T, 128, F32>(a, b, family, st);
-    default: return by_rows<T, 256, F32>(a, b, family, st);
+    case 64: return by_rows<T, 64, F32>(a, b, own, family, st);
+    case 128: return by_rows<T, 128, F32>(a, b, own, family, st);
+    default: return by_rows<T, 256, F32>(a, b, own, family, st);
     }
 }
 
@@ -340,10 +388,10 @@ int gs_attn_shared(const gs_kv_cache *c, uint32_t layer, const gs_kv_batch *b, c
     a.n = b->n + n_families;
     gs::AttnArgs a2 = a;
     a2.parts = (float *)(ws + p.parts2);
-    const uint64_t family = (uint64_t)b->n_tokens * a.group;
+    const uint64_t own = (uint64_t)most_tokens(b, x) * a.group, family = (uint64_t)b->n_tokens * a.group;
     const bool f16 = c->type == GS_TYPE_F16;
-    if (x->type == GS_TYPE_F32) f16 ? by_head<_Float16, true>(a, a2, family, st) : by_head<__bf16, true>(a, a2, family, st);
-    else f16 ? by_head<_Float16, false>(a, a2, family, st) : by_head<__bf16, false>(a, a2, family, st);
+    if (x->type == GS_TYPE_F32) f16 ? by_head<_Float16, true>(a, a2, own, family, st) : by_head<__bf16, true>(a, a2, own, family, st);
+    else f16 ? by_head<_Float16, false>(a, a2, own, family, st) : by_head<__bf16, false>(a, a2, own, family, st);
     return hipGetLastError() == hipSuccess ? GS_OK : GS_ERR_HIP;
 }
 

@@ -417,7 +417,26 @@ __device__ __forceinline__ uint32_t new_page(const Cache &c, const Move &m, uint
 // How a stream's values move: as they are or turned within vectors of 8 (the
 // interleaved layout); turned in pairs of vectors (the half layout); or value
 // by value, where the turned part is no whole number of such vectors.
-enum { kMoveVector, kMovePairs, kMoveValues };
+// kMoveWhole: an eviction's vectors that are not turned.
+enum { kMoveVector, kMovePairs, kMoveValues, kMoveWhole };
+
+// cos and sin of -way positions' angle, where each pair of each token has its
+// own: turn_of, in fewer instructions.  The high 32 bits of the product modulo
+// 2^64 are the fraction of a turn, off by 2^-32 at most; the nearest quarter turn
+// leaves an eighth either way, for which Taylor's series to the ninth and
+// eighth power are off by 2e-9 and 3e-8 before their roundings.  (32 rows of 1100 to
+// 2500 tokens cut to 1000, us of the move: 446 with turn_of, 384.)
+__device__ __forceinline__ float2 turn_back(uint64_t turns, uint32_t way)
+{
+    const uint32_t part = (uint32_t)(turns >> 32) * way + __umulhi((uint32_t)turns, way);
+    const uint32_t quarter = part + 0x20000000u;
+    const float x = (float)(int32_t)(part - (quarter & 0xc0000000u)) * 0x1p-32f, y = x * x;
+    const float s = x * fmaf(y, fmaf(y, fmaf(y, fmaf(y, 42.0586939f, -76.7058597f), 81.6052493f), -41.3417022f), 6.28318531f);
+    const float c = fmaf(y, fmaf(y, fmaf(y, fmaf(y, 60.2446414f, -85.4568172f), 64.9393940f), -19.7392088f), 1.0f);
+    const bool odd = quarter >> 30 & 1;
+    const uint32_t minus_c = (quarter ^ quarter << 1) & 0x80000000u, minus_s = ~quarter & 0x80000000u;
+    return make_float2(__uint_as_float(__float_as_uint(odd ? s : c) ^ minus_c), __uint_as_float(__float_as_uint(odd ? c : s) ^ minus_s));
+}
 
 // The tokens of one stream (k or v, layer, head: `base`) of row i, kStep
 // rounds of 256 items at a time, where an item is a vector, two or a pair of
@@ -431,22 +450,26 @@ __device__ __forceinline__ void move_stream(const Cache &c, const Move &m, uint3
                                             const float2 *cs, uint32_t t0, uint32_t slice, uint32_t slices, const uint32_t *from_list,
                                             const uint64_t *turns)
 {
-    constexpr int kStep = MODE == kMoveVector ? 8 : 4, kW = MODE == kMoveValues ? 1 : 8;
+    // (turning vectors of tokens that each have their own way, eight at a time, takes
+    // registers that cost more than they bring: 32 rows of 1100 to 2500 tokens to
+    // 1000, us of the call with eight and four: 413, 390)
+    constexpr bool kVector = MODE == kMoveVector || MODE == kMoveWhole;
+    constexpr int kStep = MODE == kMoveWhole || (MODE == kMoveVector && !EVICT) ? 8 : 4, kW = MODE == kMoveValues ? 1 : 8;
     typedef T vec __attribute__((ext_vector_type(kW)));
     const uint32_t pairs = rot >> 1, size = 1u << c.shift, gone = m.len - m.left;
-    const uint32_t nturn = MODE == kMoveVector ? rot / 8 : MODE == kMovePairs ? rot / 16 : pairs;
+    const uint32_t nturn = MODE == kMoveWhole ? 0 : MODE == kMoveVector ? rot / 8 : MODE == kMovePairs ? rot / 16 : pairs;
     const uint32_t per = nturn + (MODE == kMoveValues ? (c.d - rot) / 2 : (c.d - rot) / 8);     // items of a token, at most 128
     const uint32_t each = 256 / per, tl = threadIdx.x / per, item = threadIdx.x - tl * per;      // tokens of a round; this thread's
     const bool works = tl < each, turned = item < nturn;
     uint32_t p, q;
-    if (MODE == kMoveVector) p = q = 8 * item;
+    if (kVector) p = q = 8 * item;
     else if (MODE == kMovePairs) { p = turned ? 8 * item : rot + 8 * (item - nturn); q = turned ? p + pairs : p; }
     else { p = turned && !interleaved ? item : 2 * item; q = turned && !interleaved ? item + pairs : p + 1; }
     const uint32_t *table = c.table + (size_t)m.row * c.ld;
     const size_t head = (size_t)c.d << c.shift;
 
     uint64_t by_turns[EVICT ? kW : 1];          // of this thread's pairs
-    if constexpr (EVICT) {
+    if constexpr (EVICT && MODE != kMoveWhole) {
         const int at = MODE == kMoveVector ? 4 * item : kW * item;
 #pragma unroll
         for (int e = 0; e < (MODE == kMoveVector ? 4 : kW); e++) by_turns[e] = works && turned ? turns[at + e] : 0;
@@ -464,9 +487,15 @@ __device__ __forceinline__ void move_stream(const Cache &c, const Move &m, uint3
             from[s] = table[was[s] >> c.shift];
         }
     };
-    const uint32_t step = slices * each * kStep;
-    pages(t0 + slice * each * kStep);
-    for (uint32_t t = t0 + slice * each * kStep; t < m.left; t += step) {
+    if constexpr (EVICT) {                      // as many slices as end together
+        const uint32_t all = m.left - min(t0, m.left), one = each * kStep;
+        const uint32_t rounds = max((all + slices * one - 1) / (slices * one), 1u);
+        slices = max((all + rounds * one - 1) / (rounds * one), 1u);
+        if (slice >= slices) return;
+    }
+    const uint32_t step = slices * each * kStep, begin = t0 + slice * each * kStep;
+    pages(begin);
+    for (uint32_t t = begin; t < m.left; t += step) {
         vec a[kStep], b[kStep];
         T *at[kStep];
         uint32_t way[kStep];
@@ -484,8 +513,8 @@ __device__ __forceinline__ void move_stream(const Cache &c, const Move &m, uint3
         pages(t + step);
 #pragma unroll
         for (int s = 0; s < kStep; s++) {
-            if (!at[s] || !turned || t + s * each + tl < m.from) continue;
-            auto turn = [&](int pair, int e) { return EVICT ? turn_of(by_turns[EVICT ? e : 0], -(int64_t)way[s], 1.0f) : cs[pair]; };
+            if (MODE == kMoveWhole || !at[s] || !turned || t + s * each + tl < m.from) continue;
+            auto turn = [&](int pair, int e) { return EVICT ? turn_back(by_turns[EVICT ? e : 0], way[s]) : cs[pair]; };
             if constexpr (MODE == kMoveVector) {
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
@@ -542,7 +571,7 @@ __global__ void __launch_bounds__(256) drop_move_kernel(const Cache c, const uin
     T *base = (T *)(keys ? c.k : c.v) + (size_t)l * c.n_pages * c.n_kv * ((size_t)c.d << c.shift);
     const uint32_t *list = EVICT ? e.list + i * e.ld : nullptr;
     if (!keys || rot == 0) {
-        move_stream<T, kMoveVector, EVICT>(c, m, i, base, h, 0, true, cs, t0, slice, slices, list, turns);
+        move_stream<T, EVICT ? kMoveWhole : kMoveVector, EVICT>(c, m, i, base, h, 0, true, cs, t0, slice, slices, list, turns);
         return;
     }
     if constexpr (!EVICT) {
@@ -606,15 +635,20 @@ __device__ __forceinline__ uint32_t rank_of(float x)
 
 // Eviction, 1 of 4: which tokens of row rows[blockIdx.x] stay.  Of the tokens
 // between the first and the newest the k of greatest weight: the rank of the
-// k-th is found 8 bits at a time, by counting the weights that share the bits
+// k-th is found digit by digit, by counting the weights that share the bits
 // found so far; then one pass over the row writes the tokens above it, and the
-// lowest of those that have it, to the list.
+// lowest of those that have it, to the list.  The first digit has a sign, an
+// exponent and four bits more, so that weights of a few powers of two do not all
+// meet in the same counts, and kFar weights of a thread are under way at a time.
+// (us of 32768 tokens: four digits of 8 bits and one weight at a time 129, of
+// which most were atomics of a wave's lanes one after the other; like this 39.)
 __global__ void __launch_bounds__(kBook) evict_select_kernel(const Cache c, const uint32_t *rows, const uint32_t *budget,
                                                              uint32_t budget_all, uint32_t first, uint32_t recent, const Stays e)
 {
-    constexpr int kEach = 4;            // tokens of a thread in a step of the last pass
-    __shared__ uint32_t s_count[256], s_bin, s_above, s_from;
-    const uint32_t i = blockIdx.x, row = rows[i];
+    constexpr int kEach = 4, kFar = 8;  // tokens of a thread in a step of the last pass; reads of the passes before
+    constexpr int kBins = 1 << 13;
+    __shared__ uint32_t s_count[kBins], s_bin, s_above, s_from;
+    const uint32_t i = blockIdx.x, row = rows[i], lane = threadIdx.x & 63;
     bool again = row >= c.rows;         // (a row that an earlier i has counts there)
     for (uint32_t j = threadIdx.x; j < i; j += kBook) again |= rows[j] == row;
     again = __syncthreads_or(again);
@@ -637,55 +671,62 @@ __global__ void __launch_bounds__(kBook) evict_select_kernel(const Cache c, cons
     const uint32_t tail = m.len - min(recent, m.left), head = min(first, m.left - (m.len - tail));
     uint32_t want = m.left - head - (m.len - tail);     // of head .. tail - 1, which are more
     uint32_t rank = 0, known = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (threadIdx.x < 256) s_count[threadIdx.x] = 0;
+    auto digit = [&](auto at, auto bits) {
+        constexpr int kShift = decltype(at)::value, kAll = 1 << decltype(bits)::value, kMine = kAll / kBook;    // counts of a thread
+        for (uint32_t b = threadIdx.x; b < kAll; b += kBook) s_count[b] = 0;
         __syncthreads();
-        for (uint32_t t = head + threadIdx.x; t < tail; t += kBook) {
-            const uint32_t r = rank_of(mass[t]);
-            if ((r & known) == rank) atomicAdd(&s_count[r >> shift & 255], 1u);
-        }
-        __syncthreads();
-        if (threadIdx.x < 64) {         // four counts a lane, from the greatest down
-            uint32_t x[4], sum = 0;
+        for (uint32_t t = head + threadIdx.x; t < tail; t += kBook * kFar) {
+            float w[kFar];
 #pragma unroll
-            for (int k = 0; k < 4; k++) { x[k] = s_count[255 - (4 * threadIdx.x + k)]; sum += x[k]; }
-            uint32_t upto = sum;
+            for (int k = 0; k < kFar; k++) w[k] = mass[min(t + k * kBook, tail - 1)];
 #pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const uint32_t y = __shfl_up(upto, o);
-                if ((int)threadIdx.x >= o) upto += y;
-            }
-            uint32_t above = upto - sum;
-            // (want 0: the first bin, none of which is taken)
-            const bool mine = want == 0 ? threadIdx.x == 0 : above < want && want <= upto;
-            if (mine) {
-                int k = 0;
-                if (want)
-                    while (above + x[k & 3] < want && k < 3) above += x[k++ & 3];
-                s_bin = 255 - (4 * threadIdx.x + k);
-                s_above = above;
+            for (int k = 0; k < kFar; k++) {
+                const uint32_t r = rank_of(w[k]);
+                if (t + k * kBook < tail && (r & known) == rank) atomicAdd(&s_count[r >> kShift & (kAll - 1)], 1u);
             }
         }
         __syncthreads();
-        rank |= s_bin << shift;
-        known |= 255u << shift;
+        // from the greatest down, kMine counts a thread
+        uint32_t x[kMine], sum = 0, total;
+#pragma unroll
+        for (int k = 0; k < kMine; k++) { x[k] = s_count[kAll - 1 - (kMine * threadIdx.x + k)]; sum += x[k]; }
+        uint32_t above = scan(sum, total);
+        // (want 0: the greatest, none of which is taken)
+        if (want == 0 ? threadIdx.x == 0 : above < want && want <= above + sum) {
+            int bin = 0;
+#pragma unroll
+            for (int k = 0; k + 1 < kMine; k++)
+                if (bin == k && want && above + x[k] < want) { above += x[k]; bin++; }
+            s_bin = kAll - 1 - (kMine * threadIdx.x + bin);
+            s_above = above;
+        }
+        __syncthreads();
+        rank |= s_bin << kShift;
+        known |= (uint32_t)(kAll - 1) << kShift;
         want -= s_above;
+        __syncthreads();                // (s_bin and the counts are read)
+    };
+    if (head < tail) {
+        digit(std::integral_constant<int, 19>(), std::integral_constant<int, 13>());
+        digit(std::integral_constant<int, 9>(), std::integral_constant<int, 10>());
+        digit(std::integral_constant<int, 0>(), std::integral_constant<int, 10>());     // (a bit of the last digit again)
     }
     // those of rank `rank`: the lowest `want` stay
     if (threadIdx.x == 0) s_from = m.left;
     uint32_t sure = 0, even = 0;        // before this step's tokens: that stay, and that have that rank
+    uint32_t leaves = m.left;           // the first token of the thread's that does
     for (uint32_t t0 = 0; t0 < m.len; t0 += kBook * kEach) {
         uint32_t above = 0, same = 0;   // bits
+        float w[kEach];
+#pragma unroll
+        for (int k = 0; k < kEach; k++) w[k] = mass[min(t0 + threadIdx.x * kEach + k, m.len - 1)];
 #pragma unroll
         for (int k = 0; k < kEach; k++) {
-            const uint32_t t = t0 + threadIdx.x * kEach + k;
-            if (t >= m.len) break;
-            if (t < head || t >= tail) above |= 1u << k;
-            else {
-                const uint32_t r = rank_of(mass[t]);
-                above |= (uint32_t)(r > rank) << k;
-                same |= (uint32_t)(r == rank) << k;
-            }
+            const uint32_t t = t0 + threadIdx.x * kEach + k, r = rank_of(w[k]);
+            if (t >= m.len) continue;
+            const bool must = t < head || t >= tail;
+            above |= (uint32_t)(must || r > rank) << k;
+            same |= (uint32_t)(!must && r == rank) << k;
         }
         uint32_t total;
         const uint32_t before = scan(__popc(above) | __popc(same) << 16, total);
@@ -695,13 +736,16 @@ __global__ void __launch_bounds__(kBook) evict_select_kernel(const Cache c, cons
             const uint32_t t = t0 + threadIdx.x * kEach + k;
             const bool stays = above >> k & 1 || (same >> k & 1 && b < want);
             if (stays) list[a + min(b, want)] = t;
-            else if (t < m.len) atomicMin(&s_from, t);
+            else if (t < m.len) leaves = min(leaves, t);
             a += above >> k & 1;
             b += same >> k & 1;
         }
         sure += total & 0xffff;
         even += total >> 16;
     }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) leaves = min(leaves, (uint32_t)__shfl_xor(leaves, o));
+    if (lane == 0) atomicMin(&s_from, leaves);
     __syncthreads();
     m.from = s_from;
     if (threadIdx.x == 0) c.moves[i] = m;
@@ -760,7 +804,12 @@ void move_tokens(const gs_kv_cache *c, const gs::Cache &d, size_t n, const gs_ro
     // Several times as many workgroups as run at a time even out rows of unlike
     // lengths (16 rows of 2500 to 6000 tokens, us: 2048 workgroups 669, 4096
     // 611, 8192 586, 16384 567).
-    const dim3 grid((unsigned)streams, shares(n * streams, 16384, 64), (unsigned)n);
+    // An eviction's rows are known to hold no more than the list: each slice has two
+    // steps at least of 8192 / d tokens, since workgroups without any cost a launch
+    // too (one row of 8192 tokens to 2048, 28 layers of 4 heads: 103 us with 64
+    // slices, 90 with 16).
+    const size_t most = EVICT && e.ld * c->d / 16384 < 64 ? e.ld * c->d / 16384 + 1 : 64;
+    const dim3 grid((unsigned)streams, shares(n * streams, 16384, most), (unsigned)n);
     auto move = [&](auto t, auto mode) {
         hipLaunchKernelGGL((gs::drop_move_kernel<decltype(t), decltype(mode)::value, EVICT>), grid, dim3(256), 0, st, d, turns, rot, inter, e);
     };

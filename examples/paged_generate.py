@@ -9,9 +9,12 @@ different lengths go through in one call per layer, each conversation is forked
 into several answers that share the prompt's pages, the answers are generated
 token by token without a word to the host, and a conversation whose context is
 full loses its oldest tokens instead of running its prompt again
-(gguf-rs-cli's smart context, src/main.rs:205-256).
+(gguf-rs-cli's smart context, src/main.rs:205-256).  With --shared a prompt's
+pages are read once for all of its answers (KVCache.attend_shared); with
+--budget a full conversation is cut to that many tokens by the weight that they
+have had from the later ones (KVCache.weigh, evict).
 
-    python examples/paged_generate.py [--answers 4] [--new 48]
+    python examples/paged_generate.py [--answers 4] [--new 48] [--shared] [--budget 96]
 """
 import argparse
 import os
@@ -64,18 +67,26 @@ class PagedModel:
     def _norm(x):
         return x * torch.rsqrt(x.square().mean(-1, keepdim=True) + 1e-6)
 
-    def forward(self, tokens, rows, q_start=None, max_q=1):
+    def forward(self, tokens, rows, q_start=None, max_q=1, families=None, mass=None):
         """tokens [T] of `rows` (one each, or those from q_start[i] to
         q_start[i + 1]), for which extend() has made room; returns the hidden
-        states [T, hidden] before the output projection."""
+        states [T, hidden] before the output projection.  families: which of
+        the rows begin with the same pages; mass: gets the weights that the
+        rows' tokens have from these."""
         cfg, n = self.cfg, tokens.shape[0]
+        lse = None if mass is None else torch.empty((n, cfg["heads"]), device="cuda")
         x = self.embed[tokens.long()]
         for i, w in enumerate(self.w):
             heads = self._project(w["qkv"], self._norm(x)).view(n, -1, cfg["d"])
             q, k, v = heads.split([cfg["heads"], cfg["kv"], cfg["kv"]], 1)      # parts of one row: strides, no copies
             turned = torch.empty((n, cfg["heads"], cfg["d"]), device="cuda")
             self.cache.append(i, k, v, q=q, q_out=turned, rope=self.rope, rows=rows, q_start=q_start)
-            a = self.cache.attend(i, turned, rows=rows, q_start=q_start, max_q=max_q)
+            if families is None:
+                a = self.cache.attend(i, turned, rows=rows, q_start=q_start, max_q=max_q, lse=lse)
+            else:
+                a = self.cache.attend_shared(i, turned, families, rows=rows, q_start=q_start, max_q=max_q, lse=lse)
+            if mass is not None:
+                self.cache.weigh(i, turned, lse, mass, rows=rows, q_start=q_start, max_q=max_q)
             x = x + self._project(w["o"], a.view(n, -1))
             y = self._norm(x)
             y = torch.nn.functional.silu(self._project(w["gate"], y)) * self._project(w["up"], y)
@@ -87,9 +98,12 @@ def words(x):
     return torch.tensor(x, dtype=torch.int32, device="cuda")
 
 
-def generate(model, prompts, answers, new, seed=42, keep=8):
+def generate(model, prompts, answers, new, seed=42, keep=8, shared=False, budget=0):
     """`answers` continuations of each prompt, `new` tokens each; the oldest
-    half of what follows the first `keep` tokens leaves a row that is full.
+    half of what follows the first `keep` tokens leaves a row that is full, or
+    with a budget all but the first `keep`, the newest quarter of the budget and
+    those of greatest weight between.  shared: an answer's attention reads the
+    pages of its prompt together with the prompt's other answers.
     Returns the generated ids [prompts * answers][<= new]."""
     cfg, cache, n = model.cfg, model.cache, len(prompts)
     B = n * answers
@@ -99,11 +113,16 @@ def generate(model, prompts, answers, new, seed=42, keep=8):
     start = words(np.concatenate([[0], np.cumsum(lens)]).tolist())
     parents = words(list(range(n)))
     cache.extend(words(lens), rows=parents)
-    hidden = model.forward(words(np.concatenate(prompts).astype(np.int64).tolist()), parents, start, max(lens))
+    mass = cache.mass() if budget else None
+    families = words(list(range(0, B + 1, answers))) if shared else None
+    hidden = model.forward(words(np.concatenate(prompts).astype(np.int64).tolist()), parents, start, max(lens), mass=mass)
     # each answer is a row that shares its prompt's pages; the prompt's own row goes
     of = torch.arange(n, device="cuda", dtype=torch.int32).repeat_interleave(answers)
     cache.fork(of, kids)
     cache.free(parents)
+    if budget:
+        mass[kids.long()] = mass[of.long()]                     # the answers' tokens weigh what their prompts' do
+        mass[:n] = 0.0
     x = hidden[(start[1:] - 1).long()][of.long()].contiguous()
     sampler = gs.Sampler(0.8, 40, 0.95, 1.1, seed=seed)
     sampler.reserve(B, cfg["vocab"])
@@ -116,14 +135,18 @@ def generate(model, prompts, answers, new, seed=42, keep=8):
         if step + 1 == new:
             break
         full = [b for b in range(B) if held[b] == cfg["context"]]
-        if full:
+        if full and budget:
+            cache.evict(mass, budget, words([n + b for b in full]), first=keep, recent=budget // 4, rope=model.rope)
+            for b in full:
+                held[b] = budget
+        elif full:
             gone = (cfg["context"] - keep) // 2
             cache.drop(words([keep] * len(full)), words([keep + gone] * len(full)), words([n + b for b in full]), rope=model.rope)
             for b in full:
                 held[b] -= gone
         cache.extend(1, rows=kids)
         held = [x + 1 for x in held]
-        x = model.forward(dec.next, kids)
+        x = model.forward(dec.next, kids, families=families, mass=mass)
     return [g.tolist() for g in dec.generated_ids()]
 
 
@@ -131,13 +154,15 @@ def main():
     ap = argparse.ArgumentParser(description=__doc__.split("\n")[0])
     ap.add_argument("--answers", type=int, default=4)
     ap.add_argument("--new", type=int, default=48)
+    ap.add_argument("--shared", action="store_true")
+    ap.add_argument("--budget", type=int, default=0)
     a = ap.parse_args()
     rng = np.random.default_rng(1)
     prompts = [rng.integers(0, SMALL["vocab"], k) for k in (150, 37, 5)]
     rows = len(prompts) * (1 + a.answers)
     model = PagedModel(SMALL, rows, pages=rows * SMALL["context"] // SMALL["page"])
     t = time.perf_counter()
-    ids = generate(model, prompts, a.answers, a.new)
+    ids = generate(model, prompts, a.answers, a.new, shared=a.shared, budget=a.budget)
     t = time.perf_counter() - t
     for i, p in enumerate(prompts):
         print("prompt of %d tokens:" % len(p))

@@ -246,12 +246,15 @@ __global__ void __launch_bounds__(256) weigh_few_kernel(const WeighArgs a)
 
 // The shape of the kernel below for heads of D: four waves of kMine keys, tiles
 // of kRows query rows (in three parts twice as many would leave room for one
-// workgroup in a CU).
+// workgroup in a CU), and the workgroups that a CU takes.  (us with 64 keys of a
+// wave, two workgroups, and with 32, three: 4 x 2048 tokens over up to 8192, 350,
+// 363; 7 x 32 over up to 12000, 47, 45; one of 2000, 72, 62; 4 x 64 over up to
+// 12000, heads of 64, 32, 26.)
 template <int D, bool F32> struct Many {
-    static constexpr int kTiles = D == 256 ? 1 : 2, kMine = 32 * kTiles, kKeys = 4 * kMine, kRows = F32 ? 32 : 64;
+    static constexpr int kMine = 32, kKeys = 4 * kMine, kRows = F32 ? 32 : 64, kPerCU = F32 || D == 256 ? 2 : 3;
     static constexpr int kSetup = 1;                // the keys' way and the sums', dealt as tiles of rows
 };
-constexpr int kManyRuns = 512;                      // two workgroups per CU
+constexpr int kManyRuns = 3 * 256;                  // at most
 
 // A block of keys that a run begins and does not end.
 struct Left {
@@ -326,10 +329,10 @@ __device__ __forceinline__ void add_mass(const WeighArgs &a, uint32_t row, uint3
 // weights of query row lane & 31 for the keys that its results of S^T = K Q^T,
 // 32 x 32 x 16, are of.
 template <class T, int D, bool F32>
-__global__ void __launch_bounds__(256, F32 && D == 256 ? 1 : 2) weigh_many_kernel(const WeighArgs a)
+__global__ void __launch_bounds__(256, (F32 && D == 256 ? 1 : Many<D, F32>::kPerCU)) weigh_many_kernel(const WeighArgs a)
 {
     using M = Many<D, F32>;
-    constexpr int KT = M::kTiles, kMine = M::kMine, kKeys = M::kKeys, kSetup = M::kSetup, kRows = M::kRows, U = kRows / 32;
+    constexpr int kMine = M::kMine, kKeys = M::kKeys, kSetup = M::kSetup, kRows = M::kRows, U = kRows / 32;
     constexpr int KF = D / 16, NP = F32 ? 3 : 1, C = D / 8, kEach = C / 8;      // factors; parts; 16-byte pieces of a row, of a thread
     typedef typename Vec<T>::v8 v8;
     __shared__ __align__(16) T s_q[2][NP][kRows * D];
@@ -352,10 +355,10 @@ __global__ void __launch_bounds__(256, F32 && D == 256 ? 1 : 2) weigh_many_kerne
     uint64_t t = run.t0, skip = run.skip;
     uint32_t b = Dealt::find(a, s, skip);
     bool mine = is_first(a, si);
-    // Of two waves that want to issue the older one is taken: the first of a CU's
-    // two workgroups would be done long before the second.  The one that has
-    // more of its run before it goes first, by quarters.  (4 x 2048 tokens over
-    // up to 8192: 378 -> 348 us.)
+    // Of the waves that want to issue the oldest is taken: the first of a CU's
+    // workgroups would be done long before the others.  The one that has more of
+    // its run before it goes first, by quarters.  (4 x 2048 tokens over up to 8192:
+    // 378 -> 348 us, with two workgroups in a CU.)
     uint32_t done = 0, level = 3;
     const uint32_t quarter = (uint32_t)(run.t1 - run.t0) / 4;
     __builtin_amdgcn_s_setprio(3);
@@ -374,22 +377,18 @@ __global__ void __launch_bounds__(256, F32 && D == 256 ? 1 : 2) weigh_many_kerne
         const int base = (int)s.len - (int)s.nq;
         const uint32_t *table = a.table + (size_t)min(s.row, a.n_rows - 1) * a.ld_table;
 
-        float sum[KT][16];
+        float sum[16];
 #pragma unroll
-        for (int y = 0; y < KT; y++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) sum[y][i] = 0.0f;
+        for (int i = 0; i < 16; i++) sum[i] = 0.0f;
         // the last rows' exponents and factors, whose exponentials are still to come
-        float wait[KT][16], wait_by = 0.0f;
+        float wait[16], wait_by = 0.0f;
 #pragma unroll
-        for (int y = 0; y < KT; y++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) wait[y][i] = -INFINITY;
+        for (int i = 0; i < 16; i++) wait[i] = -INFINITY;
         auto weigh = [&](int i0, int i1) {
 #pragma unroll
-            for (int i = i0; i < i1 && i < 16 * KT; i++) {
-                sum[i >> 4][i & 15] = fmaf(__builtin_amdgcn_exp2f(wait[i >> 4][i & 15]), wait_by, sum[i >> 4][i & 15]);
-                asm volatile("" : "+v"(sum[i >> 4][i & 15]));       // (here: else it is put off past the branch that follows)
+            for (int i = i0; i < i1 && i < 16; i++) {
+                sum[i] = fmaf(__builtin_amdgcn_exp2f(wait[i]), wait_by, sum[i]);
+                asm volatile("" : "+v"(sum[i]));                    // (here: else it is put off past the branch that follows)
             }
         };
         const uint32_t kv0 = (uint32_t)quotient(skip, per), kv1 = (uint32_t)quotient(skip + part - 1, per);
@@ -403,18 +402,14 @@ __global__ void __launch_bounds__(256, F32 && D == 256 ? 1 : 2) weigh_many_kerne
             uint32_t x0, x1;
             tiles_of(kvh, x0, x1);
             if (x0 >= x1) continue;
-            v8 kf[KT][KF];
+            v8 kf[KF];
+            const uint32_t key = w0 + col, id = min(table[min(key, s.len - 1) >> a.shift], a.n_pages - 1);
+            const T *keys_at = (const T *)a.k + ((size_t)id * a.n_kv + kvh) * head + (size_t)(key & slot) * d;
 #pragma unroll
-            for (int y = 0; y < KT; y++) {
-                const uint32_t key = w0 + 32 * y + col;
-                const uint32_t id = min(table[min(key, s.len - 1) >> a.shift], a.n_pages - 1);
-                const T *p = (const T *)a.k + ((size_t)id * a.n_kv + kvh) * head + (size_t)(key & slot) * d;
-#pragma unroll
-                for (int c = 0; c < KF; c++) {
-                    v8 z = {};
-                    if (16 * c + 8 * hg < (int)d) z = *(const v8 *)(p + 16 * c + 8 * hg);
-                    kf[y][c] = z;
-                }
+            for (int c = 0; c < KF; c++) {
+                v8 z = {};
+                if (16 * c + 8 * hg < (int)d) z = *(const v8 *)(keys_at + 16 * c + 8 * hg);
+                kf[c] = z;
             }
             // A tile of queries through registers to LDS.  The bases of its rows are
             // a wave's, another one's for each tile.
@@ -533,43 +528,36 @@ __global__ void __launch_bounds__(256, F32 && D == 256 ? 1 : 2) weigh_many_kerne
                         const bool edge = (int)w0 + kMine > pa + 1 || (int64_t)w0 < (int64_t)pb + 1 - (int64_t)a.window;
                         // these scores while the last ones' exponentials run; the factors
                         // come from LDS kAhead products before theirs
-                        constexpr int kAll = NP * KF, kAhead = F32 ? 2 : 4, kFirst = 4 * KT, kTurn = (16 * KT - kFirst + kAll - 1) / kAll;
+                        constexpr int kAll = NP * KF, kAhead = 4, kFirst = 4, kTurn = (16 - kFirst + kAll - 1) / kAll;
                         v8 f[kAhead];
                         auto factor = [&](int p) {                          // (the small parts first)
                             f[p % kAhead] = *(const v8 *)&s_q[o][NP - 1 - p / KF][(32 * u + col) * D + 8 * place(col, 2 * (p % KF) + hg)];
                         };
-                        f16v z[KT];
+                        f16v z;
 #pragma unroll
-                        for (int y = 0; y < KT; y++)
-#pragma unroll
-                            for (int i = 0; i < 16; i++) z[y][i] = 0.0f;
+                        for (int i = 0; i < 16; i++) z[i] = 0.0f;
 #pragma unroll
                         for (int p = 0; p < kAhead; p++) factor(p);
                         weigh(0, kFirst);
                         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                         for (int p = 0; p < kAll; p++) {
-#pragma unroll
-                            for (int y = 0; y < KT; y++) z[y] = mfma(kf[y][p % KF], f[p % kAhead], z[y]);
+                            z = mfma(kf[p % KF], f[p % kAhead], z);
                             if (p + kAhead < kAll) factor(p + kAhead);
                             weigh(kFirst + kTurn * p, kFirst + kTurn * (p + 1));
                             __builtin_amdgcn_sched_barrier(0);
                         }
 #pragma unroll
-                        for (int y = 0; y < KT; y++)
-#pragma unroll
-                            for (int i = 0; i < 16; i++) wait[y][i] = fmaf(z[y][i], unscale, -n);
+                        for (int i = 0; i < 16; i++) wait[i] = fmaf(z[i], unscale, -n);
                         wait_by = by;
                         if (edge) {
                             const int pos = base + (int)(min(ra + col, rb) / a.group);
                             const int up = pos - (int)w0 - 4 * hg, down = (int)max((int64_t)-1, (int64_t)pos + 1 - (int64_t)a.window - w0) - 4 * hg;
 #pragma unroll
-                            for (int y = 0; y < KT; y++)
-#pragma unroll
-                                for (int i = 0; i < 16; i++) {
-                                    const int key = 32 * y + 8 * (i >> 2) + (i & 3);        // from the lane's first
-                                    if (key > up || key < down) wait[y][i] = -INFINITY;
-                                }
+                            for (int i = 0; i < 16; i++) {
+                                const int key = 8 * (i >> 2) + (i & 3);             // from the lane's first
+                                if (key > up || key < down) wait[i] = -INFINITY;
+                            }
                         }
                     }
                 }
@@ -578,17 +566,15 @@ __global__ void __launch_bounds__(256, F32 && D == 256 ? 1 : 2) weigh_many_kerne
             }
         }
 
-        weigh(0, 16 * KT);
+        weigh(0, 16);
 
         // ---- the block's sums, or this run's part of them
 #pragma unroll
-        for (int y = 0; y < KT; y++)
+        for (int i = 0; i < 16; i++) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) sum[y][i] += __shfl_xor(sum[y][i], o);
-                if (col == 0) s_sum[kMine * w + 32 * y + 8 * (i >> 2) + 4 * hg + (i & 3)] = sum[y][i];
-            }
+            for (int o = 1; o < 32; o <<= 1) sum[i] += __shfl_xor(sum[i], o);
+            if (col == 0) s_sum[kMine * w + 8 * (i >> 2) + 4 * hg + (i & 3)] = sum[i];
+        }
         if constexpr (F32) {                        // keys that met an infinity once more, by 64 lanes beside one another
             for (uint32_t k = 0; k < kMine; k++) {
                 const float old = s_sum[kMine * w + k];
@@ -661,7 +647,7 @@ template <class T, int D, bool F32> void by_rows(gs::WeighArgs a, uint64_t rows,
     if (few) return;
     a.min_rows = alike ? 0 : kFewRows + 1;
     a.max_rows = 0xffffffffu;
-    a.n_wg = gs::kManyRuns;
+    a.n_wg = 256 * gs::Many<D, F32>::kPerCU;
     hipLaunchKernelGGL((gs::weigh_many_kernel<T, D, F32>), dim3(a.n_wg), dim3(256), 0, st, a);
     hipLaunchKernelGGL(gs::weigh_join_kernel, dim3(a.n_wg), dim3(256), 0, st, a, gs::Many<D, F32>::kKeys);
 }

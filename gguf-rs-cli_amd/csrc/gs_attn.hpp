@@ -33,7 +33,6 @@ namespace gs {
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
-typedef float f2 __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ f4 mfma(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f4 mfma(b8 a, b8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -59,7 +58,7 @@ struct AttnArgs {
     const int32_t *pos;             // [n_tokens] positions
     uint32_t n_families;
     uint32_t *where;                // [2][n_tokens][heads] where the parts of a row's jobs are (common keys, its own)
-    float *whole;                   // [2][n_tokens][heads][D + 2] units that one run has whole
+    float *whole;                   // [2][n_tokens][heads][D + 4] units that one run has whole
     uint32_t second;                // 0 or kSecond: whose parts they are, of two kernels of a call
 };
 
@@ -800,7 +799,7 @@ __global__ void __launch_bounds__(256, rows_per_cu(D, NT)) attn_rows_kernel(cons
                     a.where[row] =
                         whole ? here ? kDone : common
                               : blockIdx.x | (run_with(run, end - 1) - blockIdx.x + 1) << 9 | (uint32_t)(16 * nt + rr) << 19 | a.second | common;
-                if (whole && !here) kept = a.whole + row * (D + 2);
+                if (whole && !here) kept = a.whole + row * (D + 4);
                 if (kept && c0 == 0) { kept[D] = lifted(a, top); kept[D + 1] = total; }
             }
             const size_t to = (size_t)(s.first + tok) * a.ld_out + (size_t)h * d;
@@ -811,7 +810,7 @@ __global__ void __launch_bounds__(256, rows_per_cu(D, NT)) attn_rows_kernel(cons
 #pragma unroll
                 for (int y = 0; y < 4; y++) x += *(const f4 *)&s_o[y][rr][dv] * by[y];
                 if (!whole) *(f4 *)(part + (size_t)(16 * nt + rr) * D + dv) = x;
-                else if (SHARED && kept) { *(f2 *)(kept + dv) = f2{x[0], x[1]}; *(f2 *)(kept + dv + 2) = f2{x[2], x[3]}; }
+                else if (SHARED && kept) *(f4 *)(kept + dv) = x;
                 else if (dv < (int)d) {
                     x *= inv;
                     if constexpr (F32) *(f4 *)((float *)a.out + to + dv) = x;
@@ -1285,13 +1284,14 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, 2) attn_chunk_kernel(const
                         }
                     }
             } else if (SHARED && whole) {
-                float *kept = a.whole + row * (D + 2);
+                float *kept = a.whole + row * (D + 4);
                 if (hg == 0) { kept[D] = lifted(a, mx); kept[D + 1] = sum; }
 #pragma unroll
                 for (int c = 0; c < DT; c++)
 #pragma unroll
-                    for (int i = 0; i < NA / 2; i++)
-                        *(f2 *)(kept + M * c + value_of(2 * i)) = f2{o[c][2 * i], o[c][2 * i + 1]};
+                    for (int i = 0; i < NA / 4; i++)
+                        *(f4 *)(kept + M * c + value_of(4 * i)) =
+                            f4{o[c][4 * i], o[c][4 * i + 1], o[c][4 * i + 2], o[c][4 * i + 3]};
             } else {
                 float *part = a.parts + (size_t)(2 * run_id + (first == 0)) * R * (D + 2);
                 const int rr = M * w + col;

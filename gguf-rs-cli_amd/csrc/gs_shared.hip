@@ -161,12 +161,12 @@ struct Parts {
 
 // A row of a token and head, by D / 4 threads: the parts of its two jobs.
 // The threads share out the parts' maximums and sums and then add the parts in
-// order, eight reads at a time.
+// order, kFar reads at a time.
 // R1, R2: rows of a unit of the call's two kernels.
 template <class TO, int D, int R1, int R2>
 __global__ void __launch_bounds__(256) shared_join_kernel(const AttnArgs a, const float *parts2, float lift2)
 {
-    constexpr int kCols = D / 4, kRows = 256 / kCols, kWide = kCols < 32 ? kCols : 32;
+    constexpr int kCols = D / 4, kRows = 256 / kCols, kWide = kCols < 32 ? kCols : 32, kFar = 8;
     const uint32_t heads = a.n_kv * a.group;
     const size_t rows = (size_t)a.n_tokens * heads, row = (size_t)blockIdx.x * kRows + threadIdx.x / kCols, here = min(row, rows - 1);
     const uint32_t dv = 4 * (threadIdx.x % kCols), j = threadIdx.x % kWide;
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(256) shared_join_kernel(const AttnArgs a, cons
         Parts &p = part[y];
         p.n = at >> 9 & 1023;
         if (p.n == 0) {
-            p.o = a.whole + ((y == 0 ? rows : 0) + here) * (D + 2);
+            p.o = a.whole + ((y == 0 ? rows : 0) + here) * (D + 4);
             p.m = p.o + D;
             p.sum = 1;
             p.lift = 0.0f;
@@ -222,19 +222,15 @@ __global__ void __launch_bounds__(256) shared_join_kernel(const AttnArgs a, cons
                 add = by * m[p.sum];
             }
             const uint32_t m = i0 < p.n ? min(p.n - i0, (uint32_t)kWide) : 0;
-            for (uint32_t i = 0; __any(i < m); i += 8) {
-                f4 v[8];
+            for (uint32_t i = 0; __any(i < m); i += kFar) {
+                f4 v[kFar];
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
+                for (int e = 0; e < kFar; e++) {
                     v[e] = f4{0, 0, 0, 0};
-                    if (i + e < m) {
-                        const float *o = p.o + at(p, i0 + i + e) + dv;
-                        const f2 lo = *(const f2 *)o, hi = *(const f2 *)(o + 2);
-                        v[e] = f4{lo[0], lo[1], hi[0], hi[1]};
-                    }
+                    if (i + e < m) v[e] = *(const f4 *)(p.o + at(p, i0 + i + e) + dv);
                 }
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
+                for (int e = 0; e < kFar; e++) {
                     const float b = __shfl(by, (int)((threadIdx.x & 63 & ~(kWide - 1)) + ((i + e) & (kWide - 1))));
                     if (i + e < m) x += v[e] * b;
                 }
@@ -279,7 +275,7 @@ Place place(const gs_kv_cache *c, uint32_t n_heads, size_t n, size_t n_families,
     p.pos = p.jobs + up16((n + n_families) * sizeof(gs::Job));
     p.where = p.pos + up16(n_tokens * 4);
     p.whole = p.where + up16(2 * rows * 4);
-    p.parts = p.whole + up16(2 * rows * (D + 2) * 4);
+    p.parts = p.whole + up16(2 * rows * (D + 4) * 4);
     p.parts2 = p.parts + up16(few_bytes(D));
     p.all = p.parts2 + parts_bytes(gs::kChunkRuns, D == 256 ? gs::Chunk<256>::kRows : gs::Chunk<128>::kRows, D);
     return p;

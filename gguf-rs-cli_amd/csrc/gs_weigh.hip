@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(256) weigh_few_kernel(const WeighArgs a)
                                 const bool sees = key <= pos && key > pos - (int64_t)a.window;
                                 float x = fmaf(z[y][e], unscale, -n);
                                 if constexpr (F32)
-                                    if (sees && x != x) {
+                                    if (sees && x != x && n == n) {
                                         const uint32_t p = min(table[(uint32_t)key >> a.shift], a.n_pages - 1);
                                         x = dot((const float *)a.q + at, (const T *)a.k + ((size_t)p * a.n_kv + kvh) * head + (size_t)((uint32_t)key & (page - 1)) * d, d) * a.scale - n;
                                     }
@@ -581,21 +581,25 @@ __global__ void __launch_bounds__(256, (F32 && D == 256 ? 1 : Many<D, F32>::kPer
                 if (__builtin_expect(old == old, 1)) continue;
                 const uint32_t key = w0 + k;
                 float add = 0.0f;
-                if (key < s.len)
-                    for (uint32_t kvh = kv0; kvh <= kv1; kvh++) {
-                        uint32_t x0, x1;
-                        tiles_of(kvh, x0, x1);
-                        const uint32_t id = min(table[key >> a.shift], a.n_pages - 1);
-                        const T *p = (const T *)a.k + ((size_t)id * a.n_kv + kvh) * head + (size_t)(key & slot) * d;
-                        for (uint32_t r = rows.r0 + kRows * x0 + lane; r < min(rows.r0 + kRows * x1, rows.r1); r += 64) {
-                            const uint32_t tok = r / a.group, h = kvh * a.group + (r - tok * a.group);
-                            const int pos = base + (int)tok;
-                            if ((int)key > pos || (int64_t)key <= (int64_t)pos - (int64_t)a.window) continue;
+                bool none = key >= s.len;           // (a NaN that is no infinity's ends it)
+                for (uint32_t kvh = kv0; kvh <= kv1 && !none; kvh++) {
+                    uint32_t x0, x1;
+                    tiles_of(kvh, x0, x1);
+                    const uint32_t id = min(table[key >> a.shift], a.n_pages - 1), end = min(rows.r0 + kRows * x1, rows.r1);
+                    const T *p = (const T *)a.k + ((size_t)id * a.n_kv + kvh) * head + (size_t)(key & slot) * d;
+                    for (uint32_t r0 = rows.r0 + kRows * x0; r0 < end && !none; r0 += 64) {
+                        const uint32_t r = min(r0 + lane, end - 1), tok = r / a.group, h = kvh * a.group + (r - tok * a.group);
+                        const int pos = base + (int)tok;
+                        if (r0 + lane < end && (int)key <= pos && (int64_t)key > (int64_t)pos - (int64_t)a.window) {
                             float n, c;
                             base_of(a, a.sums[(size_t)(s.first + tok) * a.n_kv * a.group + h], n, c);
-                            add += c * __builtin_amdgcn_exp2f(fmaf(dot((const float *)a.q + (size_t)(s.first + tok) * a.ld_q + (size_t)h * d, p, d), a.scale, -n));
+                            float x = n;
+                            if (n == n) x = fmaf(dot((const float *)a.q + (size_t)(s.first + tok) * a.ld_q + (size_t)h * d, p, d), a.scale, -n);
+                            add += c * __builtin_amdgcn_exp2f(x);
                         }
+                        none = __any(add != add);
                     }
+                }
 #pragma unroll
                 for (int o = 1; o < 64; o <<= 1) add += __shfl_xor(add, o);
                 if (lane == 0) s_sum[kMine * w + k] = add;

@@ -150,6 +150,22 @@ def test_rows_that_have_nothing_to_share(gpu, torch, dtype, cache):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,cache,each", [("float16", "float16", 3), ("bfloat16", "bfloat16", 30), ("float32", "float16", 9)])
+def test_scales(gpu, torch, dtype, cache, each):
+    """Scales given by the caller, also below 0, with scores far apart."""
+    c = family(gpu, torch, [300], [each], [1 + 3 * i for i in range(each)], 2, 64, 16, cache, seed=4)
+    rows = list(range(1, each + 1))
+    for t, f in ((3, 9.0), (120, 12.0)):
+        c.k[0, int(c.table[1, t // 16]), :, t % 16] *= f
+    q = torch.randn((each, 4, 64), generator=torch.Generator("cuda").manual_seed(8), device="cuda").to(getattr(torch, dtype))
+    for scale, window in ((0.3, 0), (-0.05, 0), (-0.2, 200)):
+        lse = torch.empty((each, 4), device="cuda")
+        out = c.attend_shared(0, q, words(torch, [0, each]), rows=words(torch, rows), scale=scale, window=window, lse=lse)
+        check(out, want(c, 0, q, rows, [1] * each, scale=float(np.float32(scale)), window=window))
+        check_lse(lse, want_lse(c, 0, q, rows, [1] * each, scale=float(np.float32(scale)), window=window))
+
+
+@pytest.mark.gpu
 def test_tokens_of_no_sequence_stay(gpu, torch):
     c = family(gpu, torch, [100], [2], [5, 9], 2, 64, 16, "float16")
     q = torch.randn((7, 4, 64), device="cuda").half()

@@ -141,6 +141,42 @@ def test_rows_twice_or_not_there(gpu, torch, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,cache", [("bfloat16", "bfloat16"), ("float32", "float16")])
+@pytest.mark.parametrize("news", [[1, 1, 1], [90, 33, 90]])
+def test_scales(gpu, torch, dtype, cache, news):
+    """Scales given by the caller, also below 0, with scores far apart; a chunk's row named twice."""
+    c = build(gpu, torch, [300, 170], 2, 64, 16, cache, seed=4)
+    for r, t, f in ((0, 3, 9.0), (0, 120, 12.0), (0, 299, 5.0), (1, 50, 10.0)):
+        c.k[0, int(c.table[r, t // 16]), :, t % 16] *= f
+    rows = [0, 1, 0]
+    q = torch.randn((sum(news), 4, 64), generator=torch.Generator("cuda").manual_seed(8), device="cuda").to(getattr(torch, dtype))
+    lse, start = torch.empty((sum(news), 4), device="cuda"), starts(torch, news)
+    for scale, window in ((0.3, 0), (-0.05, 0), (1e-6, 0), (-0.2, 40)):
+        c.attend(0, q, rows=words(torch, rows), q_start=start, scale=scale, window=window, lse=lse)
+        mass = fresh(torch, c)
+        ref = want(c, 0, q, lse, mass, rows, news, 1.0, scale=float(np.float32(scale)), window=window)
+        c.weigh(0, q, lse, mass, rows=words(torch, rows), q_start=start, scale=scale, window=window, max_q=max(news))
+        check(mass, ref)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float16", "float32"])
+@pytest.mark.parametrize("news", [3, 120])
+def test_queries_that_are_no_numbers(gpu, torch, dtype, news):
+    """A token whose query has a NaN makes the weights of what it sees none, and leaves the rest."""
+    c = build(gpu, torch, [260, 300], 2, 64, 16, "float16", seed=4)
+    q = torch.randn((2 * news, 4, 64), generator=torch.Generator("cuda").manual_seed(8), device="cuda").to(getattr(torch, dtype))
+    lse, start = torch.empty((2 * news, 4), device="cuda"), starts(torch, [news, news])
+    q[1, 2, 9] = math.nan
+    c.attend(0, q, q_start=start, lse=lse)
+    assert bool(lse[1, 2].isnan()) and int(lse.isnan().sum()) == 1
+    mass = c.mass()
+    c.weigh(0, q, lse, mass, q_start=start, max_q=news)
+    p = 260 - news + 1
+    assert bool(mass[0, :p + 1].isnan().all()) and bool(torch.isfinite(mass[0, p + 1:]).all()) and bool(torch.isfinite(mass[1]).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype,cache", [("float16", "float16"), ("float32", "float16"), ("float32", "bfloat16")])
 @pytest.mark.parametrize("news", [[1, 1], [3, 5], [70, 150]])
 def test_keys_that_are_no_numbers(gpu, torch, dtype, cache, news):

@@ -100,6 +100,13 @@ template <class T> __device__ __forceinline__ float dot(const float *q, const T 
     return z;
 }
 
+// A token's weight, with what it had before.
+__device__ __forceinline__ void add_mass(const WeighArgs &a, uint32_t row, uint32_t key, float sum)
+{
+    float *mass = a.mass + row * a.ld_mass + key;
+    *mass = a.keep == 0.0f ? sum : a.keep * *mass + sum;
+}
+
 // The few-rows kernel: kFewKeys keys of a wave, tiles dealt in equal runs.
 constexpr int kFewKeys = 32;
 struct FewDeal {
@@ -111,7 +118,10 @@ struct FewDeal {
 
 // For single tokens and few of them what bounds it is the read of the keys.  A
 // wave takes 32 keys and goes through the heads and the rows, 16 at a time; a
-// token's sum is made by one wave, in one order.
+// token's sum is made by one wave, in one order.  Runs of so few tiles that heads
+// of keys one after the other would take longer share out the heads instead, and
+// the waves' sums are added in order.  (us: one token over 4001, 28 / 4 heads, f32,
+// 10.7 and 9.4 so; 64 over 1000 to 32768, bf16, 112, which is 5.2 TB/s.)
 template <class T, int D, bool F32>
 __global__ void __launch_bounds__(256) weigh_few_kernel(const WeighArgs a)
 {
@@ -126,14 +136,17 @@ __global__ void __launch_bounds__(256) weigh_few_kernel(const WeighArgs a)
     uint32_t si = run.seq;
     WeighSeq s = run.s;
     uint64_t before = run.t0 - run.skip;            // tiles of the sequences before
-    for (uint64_t t = run.t0 + w;; si++, s = uniform(work_of<WeighSeq>(a, si))) {
+    __shared__ float s_part[4][kFewKeys];
+    const bool split = (run.t1 - run.t0) * ((a.n_kv + 3) / 4) < a.n_kv && run.t1 - run.t0 < 4;
+    const uint32_t kv0 = split ? w : 0, kv_step = split ? 4 : 1, t_step = split ? 1 : 4;
+    for (uint64_t t = run.t0 + (split ? 0 : w);; si++, s = uniform(work_of<WeighSeq>(a, si))) {
         const Keys<kFewKeys> keys(a, s);
         const uint64_t end = min(before + keys.tiles, run.t1);
         if (t < end) {
             const bool mine = is_first(a, si);
             const uint32_t *table = a.table + (size_t)min(s.row, a.n_rows - 1) * a.ld_table;
             const int64_t base = (int64_t)s.len - s.nq;
-            for (; t < end; t += 4) {
+            for (; t < end; t += t_step) {
                 if (!mine) continue;
                 const uint32_t key0 = (keys.tile0 + (uint32_t)(t - before)) * kFewKeys;
                 const Seers rows(a, s, key0, kFewKeys);
@@ -141,7 +154,7 @@ __global__ void __launch_bounds__(256) weigh_few_kernel(const WeighArgs a)
 #pragma unroll
                 for (int y = 0; y < 2; y++) id[y] = min(table[min(key0 + 16 * y + m, s.len - 1) >> a.shift], a.n_pages - 1);
                 float sum[2][4] = {};
-                for (uint32_t kvh = 0; kvh < a.n_kv && rows.r0 < rows.r1; kvh++) {
+                for (uint32_t kvh = kv0; kvh < a.n_kv && rows.r0 < rows.r1; kvh += kv_step) {
                     v8 kf[2][KS];
 #pragma unroll
                     for (int y = 0; y < 2; y++) {
@@ -227,15 +240,26 @@ __global__ void __launch_bounds__(256) weigh_few_kernel(const WeighArgs a)
                     for (int e = 0; e < 4; e++)
 #pragma unroll
                         for (int o = 1; o < 16; o <<= 1) sum[y][e] += __shfl_xor(sum[y][e], o);
+                if (split) {
+                    __syncthreads();                // (the last tile's sums are read)
+                    if (m == 0)
+#pragma unroll
+                        for (int y = 0; y < 2; y++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) s_part[w][16 * y + 4 * g + e] = sum[y][e];
+                    __syncthreads();
+                    const uint32_t key = key0 + lane;
+                    if (w == 0 && lane < kFewKeys && key >= keys.lo && key < keys.hi)
+                        add_mass(a, s.row, key, (s_part[0][lane] + s_part[1][lane]) + (s_part[2][lane] + s_part[3][lane]));
+                    continue;
+                }
                 if (m != 0) continue;
-                float *mass = a.mass + s.row * a.ld_mass;
 #pragma unroll
                 for (int y = 0; y < 2; y++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         const uint32_t key = key0 + 16 * y + 4 * g + e;
-                        if (key < keys.lo || key >= keys.hi) continue;
-                        mass[key] = a.keep == 0.0f ? sum[y][e] : a.keep * mass[key] + sum[y][e];
+                        if (key >= keys.lo && key < keys.hi) add_mass(a, s.row, key, sum[y][e]);
                     }
             }
         }
@@ -315,12 +339,6 @@ template <int D, bool F32> struct ManyDeal {
         }
     }
 };
-
-__device__ __forceinline__ void add_mass(const WeighArgs &a, uint32_t row, uint32_t key, float sum)
-{
-    float *mass = a.mass + row * a.ld_mass + key;
-    *mass = a.keep == 0.0f ? sum : a.keep * *mass + sum;
-}
 
 // For chunks of tokens what bounds it is the matrix cores and, beside them, the
 // exponentials.  A wave holds its keys of a head as factors, kRows rows of queries

@@ -353,7 +353,10 @@ __global__ void __launch_bounds__(256, (F32 && D == 256 ? 1 : Many<D, F32>::kPer
     constexpr int kMine = M::kMine, kKeys = M::kKeys, kSetup = M::kSetup, kRows = M::kRows, U = kRows / 32;
     constexpr int KF = D / 16, NP = F32 ? 3 : 1, C = D / 8, kEach = C / 8;      // factors; parts; 16-byte pieces of a row, of a thread
     typedef typename Vec<T>::v8 v8;
-    __shared__ __align__(16) T s_q[2][NP][kRows * D];
+    // (rows 16 bytes apart beyond their length: 16 of them meet no bank twice, and a
+    // lane's factors are at constant distances)
+    constexpr int kRow = D + 8;
+    __shared__ __align__(16) T s_q[2][NP][kRows * kRow];
     __shared__ float s_n[2][kRows], s_c[2][kRows], s_u[2][kRows];
     __shared__ float s_sum[kKeys];
     using Dealt = ManyDeal<D, F32>;
@@ -366,7 +369,6 @@ __global__ void __launch_bounds__(256, (F32 && D == 256 ? 1 : Many<D, F32>::kPer
     const int prow = threadIdx.x >> 3, pc = threadIdx.x & 7;        // this thread's first row of a tile of queries (the others 32 apart); its pieces pc + 8 i
     const uint32_t slot = (1u << a.shift) - 1, d = a.d;
     const size_t head = (size_t)d << a.shift;
-    auto place = [](int row, int c) { return c ^ (row & (C < 16 ? C - 1 : 15)); };
 
     uint32_t si = run.seq;
     WeighSeq s = run.s;
@@ -507,11 +509,11 @@ __global__ void __launch_bounds__(256, (F32 && D == 256 ? 1 : Many<D, F32>::kPer
                                 p[2][e] = (T)(y1 - (float)p[1][e]);
                             }
 #pragma unroll
-                            for (int q = 0; q < 3; q++) *(v8 *)&s_q[o][q % NP][row * D + 8 * place(row, pc + 8 * i)] = p[q];
+                            for (int q = 0; q < 3; q++) *(v8 *)&s_q[o][q % NP][row * kRow + 8 * (pc + 8 * i)] = p[q];
                         }
                     } else {
 #pragma unroll
-                        for (int i = 0; i < kEach; i++) *(v8 *)&s_q[o][0][row * D + 8 * place(row, pc + 8 * i)] = qr[u][i];
+                        for (int i = 0; i < kEach; i++) *(v8 *)&s_q[o][0][row * kRow + 8 * (pc + 8 * i)] = qr[u][i];
                     }
                 }
                 if (w == (x & 3) && lane < kRows) {
@@ -549,7 +551,7 @@ __global__ void __launch_bounds__(256, (F32 && D == 256 ? 1 : Many<D, F32>::kPer
                         constexpr int kAll = NP * KF, kAhead = 4, kFirst = 4, kTurn = (16 - kFirst + kAll - 1) / kAll;
                         v8 f[kAhead];
                         auto factor = [&](int p) {                          // (the small parts first)
-                            f[p % kAhead] = *(const v8 *)&s_q[o][NP - 1 - p / KF][(32 * u + col) * D + 8 * place(col, 2 * (p % KF) + hg)];
+                            f[p % kAhead] = *(const v8 *)&s_q[o][NP - 1 - p / KF][(32 * u + col) * kRow + 8 * (2 * (p % KF) + hg)];
                         };
                         f16v z;
 #pragma unroll

@@ -121,7 +121,7 @@ struct FewDeal {
 // token's sum is made by one wave, in one order.  Runs of so few tiles that heads
 // of keys one after the other would take longer share out the heads instead, and
 // the waves' sums are added in order.  (us: one token over 4001, 28 / 4 heads, f32,
-// 10.7 and 9.4 so; 64 over 1000 to 32768, bf16, 112, which is 5.2 TB/s.)
+// 10.7 and 8.2 so; 64 over 1000 to 32768, bf16, 112, which is 5.2 TB/s.)
 template <class T, int D, bool F32>
 __global__ void __launch_bounds__(256) weigh_few_kernel(const WeighArgs a)
 {

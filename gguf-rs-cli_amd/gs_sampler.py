@@ -1039,9 +1039,9 @@ class KVCache:
         families[j + 1] - 1 of the call, whose rows begin with the same pages,
         as fork() leaves them.  A family's common pages are read once, not once
         for each row; the result is attend()'s whatever the rows hold.
-        The cache keeps a workspace of 43 to 85 MB and 8 d + 44 bytes for each
-        token and head for each stream that attend_shared was called on, as
-        attend does."""
+        The cache keeps a workspace of 43 to 85 MB, and of 8 d + 44 bytes for each
+        token and head (d as 64, 128 or 256), for each stream that attend_shared
+        was called on, as attend does."""
         if not 0 <= window <= 0xFFFFFFFF:
             raise ValueError("window must be a number of positions")
         T, heads, _, ld_q = _heads(q, "q", self.dev, d=self.d)

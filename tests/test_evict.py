@@ -143,6 +143,10 @@ def test_evict(gpu, torch, shared, layout, rot, d, dtype):
         want, places = m.evict(rows, [9] * 3, 1, 3, turn)
         assert st == want
         m.check_all(c, mass, places, tol)
+        c.evict(mass, 0, words(torch, rows[:2]), first=2, recent=2)        # nothing is to stay
+        m.evict(rows[:2], [0, 0], 2, 2)
+        m.check_all(c, mass)
+        c.evict(mass, 0, words(torch, []))                            # no rows
 
 
 @pytest.mark.gpu

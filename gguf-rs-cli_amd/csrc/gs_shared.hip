@@ -24,7 +24,8 @@ constexpr int kPlan = 1024;
 // The common keys are whole pages that the tables of all rows with new tokens
 // have alike, and that all of the family's new tokens come after.  What bounds
 // it is its chain of reads (begins, rows, lengths, tables), so the tables are
-// compared kTables pieces of 64 pages at a time.
+// compared kTables pieces of 64 pages at a time.  Workgroups beyond the families
+// only mark rows.
 __global__ void __launch_bounds__(kPlan) shared_plan_kernel(const AttnArgs a, const uint32_t *families, uint32_t n, Job *jobs, int32_t *pos)
 {
     constexpr int kTables = 16;
@@ -34,6 +35,7 @@ __global__ void __launch_bounds__(kPlan) shared_plan_kernel(const AttnArgs a, co
     // (tokens of no sequence are left as they are)
     const size_t rows = (size_t)a.n_tokens * a.n_kv * a.group;
     for (size_t i = (size_t)j * kPlan + threadIdx.x; i < rows; i += (size_t)gridDim.x * kPlan) a.where[rows + i] = kDone;
+    if (j >= a.n_families) return;
     const uint32_t s0 = min(families[j], n), s1 = max(min(families[j + 1], n), s0);
     auto sequence = [&](uint32_t i) {
         Job x = {};
@@ -378,7 +380,9 @@ int gs_attn_shared(const gs_kv_cache *c, uint32_t layer, const gs_kv_batch *b, c
     a.whole = (float *)(ws + p.whole);
     a.parts = (float *)(ws + p.parts);
     hipStream_t st = (hipStream_t)stream;
-    hipLaunchKernelGGL(gs::shared_plan_kernel, dim3(n_families), dim3(gs::kPlan), 0, st, a, families, b->n, (gs::Job *)(ws + p.jobs), (int32_t *)(ws + p.pos));
+    // (16 rows of tokens and heads for each thread to mark)
+    const uint64_t marks = ((uint64_t)b->n_tokens * x->n_heads + 16 * gs::kPlan - 1) / (16 * gs::kPlan), most = marks < 256 ? marks : 256;
+    hipLaunchKernelGGL(gs::shared_plan_kernel, dim3(n_families > most ? n_families : (unsigned)most), dim3(gs::kPlan), 0, st, a, families, b->n, (gs::Job *)(ws + p.jobs), (int32_t *)(ws + p.pos));
     a.jobs = (const gs::Job *)(ws + p.jobs);
     a.pos = (const int32_t *)(ws + p.pos);
     a.n = b->n + n_families;

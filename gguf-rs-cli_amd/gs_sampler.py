@@ -1041,7 +1041,9 @@ class KVCache:
         for each row; the result is attend()'s whatever the rows hold.
         The cache keeps a workspace of 43 to 85 MB, and of 8 d + 44 bytes for each
         token and head (d as 64, 128 or 256), for each stream that attend_shared
-        was called on, as attend does."""
+        was called on, as attend does; a call of more tokens than those before
+        makes another, for twice as many at least, and the smaller one stays
+        with the cache for the graphs that use it."""
         if not 0 <= window <= 0xFFFFFFFF:
             raise ValueError("window must be a number of positions")
         T, heads, _, ld_q = _heads(q, "q", self.dev, d=self.d)

@@ -177,6 +177,21 @@ def test_tokens_of_no_sequence_stay(gpu, torch):
 
 
 @pytest.mark.gpu
+def test_more_rows_than_a_step(gpu, torch):
+    """Families of more rows than the plan's threads, and many of few."""
+    n = 1100
+    c = family(gpu, torch, [70], [n], [1 + i % 3 for i in range(n)], 1, 16, 16, "float16")
+    rows = list(range(1, n + 1))
+    q = torch.randn((n, 2, 16), generator=torch.Generator("cuda").manual_seed(1), device="cuda").half()
+    c.table[700, 2] = c.table[700, 0]                             # one row parts from the others at its third page
+    ref, ref_lse = want(c, 0, q, rows, [1] * n), want_lse(c, 0, q, rows, [1] * n)
+    for families in ([0, n], list(range(0, n + 1, 10)), [30, 1090]):
+        lse = torch.empty((n, 2), device="cuda")
+        check(c.attend_shared(0, q, words(torch, families), rows=words(torch, rows), lse=lse), ref)
+        check_lse(lse, ref_lse)
+
+
+@pytest.mark.gpu
 def test_the_table_says_what_is_common(gpu, torch):
     """Rows whose pages part in the middle, by an eviction of one of them: the
     pages behind are each row's own."""

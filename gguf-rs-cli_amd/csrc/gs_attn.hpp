@@ -346,6 +346,13 @@ template <class T> __device__ __forceinline__ bool not_finite(u4v x)
     return bad;
 }
 
+// Bits 15 and 31 say the same of the words x of two values each (a half's largest
+// exponent and one carry into its sign's place, no further).
+template <class T> __device__ __forceinline__ uint32_t exponents(uint32_t x)
+{
+    return (x & 0x7fff7fffu) + (__is_same(T, _Float16) ? 0x04000400u : 0x00800080u);
+}
+
 template <class T> struct Vec;
 template <> struct Vec<_Float16> { typedef h8 v8; };
 template <> struct Vec<__bf16> { typedef b8 v8; };
@@ -354,6 +361,14 @@ template <> struct Vec<__bf16> { typedef b8 v8; };
 // weights of 2^-15 of the largest would lose bits below 2^-14.
 template <class T> constexpr float kLift = __is_same(T, _Float16) ? 15.0f : 0.0f;
 template <class T> constexpr float kChunkLift = __is_same(T, _Float16) ? 7.0f : 0.0f;      // (the second kernel's, see there)
+// SHARED: the parts in which a weight reaches the values, of 16-bit queries: off
+// by 2^-22 (bf16: 2^-24) of it, so that a row's result is that of 32-bit weights,
+// rounded once, whichever of its keys are in common.  (us with one part and so: one
+// family of 64 rows over 16000, bf16, 63, 82 (two parts: 73); 16 of 16 over 700 to
+// 8192, f16, 187, 194; 32 rows of 8 tokens over 30001, heads of 256, bf16, 155, 198.
+// Results that are not the exact one's nearest, of these bf16, f16 and bf16:
+// 1e-4, 9e-4 and 1e-4 of all; of 32-bit torch operations 2e-4, 2e-3 and 5e-4.)
+template <class T> constexpr int kSharedParts = __is_same(T, _Float16) ? 2 : 3;
 
 constexpr int kRowTile = 128;           // keys of a tile: 32 for each wave
 
@@ -395,7 +410,7 @@ constexpr int rows_per_cu(int D, int NT) { return D == 64 || (D == 128 && NT == 
 template <class T, int D, int NT, bool F32, bool FULL, bool SHARED>
 __global__ void __launch_bounds__(256, rows_per_cu(D, NT)) attn_rows_kernel(const AttnArgs a)
 {
-    constexpr int R = 16 * NT, NP = F32 ? 3 : 1, NW = F32 ? 3 : __is_same(T, __bf16) && NT == 1 ? 2 : 1, KS = D / 32;
+    constexpr int R = 16 * NT, NP = F32 ? 3 : 1, NW = F32 ? 3 : SHARED ? kSharedParts<T> : __is_same(T, __bf16) && NT == 1 ? 2 : 1, KS = D / 32;
     constexpr int CW = D >= 128 ? 8 : D / 16, NC = D / (16 * CW);       // values of a lane's V chunk, chunks
     typedef typename Vec<T>::v8 v8;
     typedef T vw __attribute__((ext_vector_type(CW)));
@@ -651,7 +666,7 @@ __global__ void __launch_bounds__(256, rows_per_cu(D, NT)) attn_rows_kernel(cons
                     pf[nt][0][j] = (T)p[nt][j];
                     const float y = p[nt][j] - (float)pf[nt][0][j];
                     if constexpr (NW > 1) pf[nt][1][j] = (T)y;
-                    if constexpr (F32) pf[nt][2][j] = (T)(y - (float)pf[nt][1][j]);
+                    if constexpr (NW > 2) pf[nt][2][j] = (T)(y - (float)pf[nt][1][j]);
                 }
 #pragma unroll
             for (int c = 0; c < NC; c++)
@@ -855,9 +870,10 @@ template <int D> struct Chunk {
     static constexpr int kRows = 8 * kM, kThreads = 512;
     // What a tile costs beside its rows, in eighths of what 8 kM rows add, where
     // units of many and of few rows are dealt together.  (us of a tile of 64 keys
-    // of heads of 128, 8 waves with rows, 6 and 1: 2.4, 2.1, 1.5; of 32 keys of 256,
-    // 8 and 1: 1.7, 1.3.  One family of 64 rows over 16000 tokens, 28 / 4 heads:
-    // 63 us, with tiles dealt alike 70.)
+    // of heads of 128, all 256 workgroups at work, 8 waves with rows, 6 and 1: f16
+    // 4.3, 3.7, 1.9, bf16 4.9, 4.1, 2.2; of 32 keys of 256: 2.5, 2.2, 1.6 and 2.8,
+    // 2.4, 1.6.  One family of 64 rows over 16000 tokens, 28 / 4 heads, bf16: 84 us,
+    // with tiles dealt alike 95.)
     static constexpr int kBase = D == 256 ? 24 : 8;
     // (a run is at least as long as the heaviest tile, also where two share little more than twice that)
     static constexpr int kLeast = 3 * (kBase + 1) > 2 * (kBase + 8) ? 3 * (kBase + 1) : 2 * (kBase + 8);
@@ -878,8 +894,8 @@ constexpr int kChunkRuns = 256;         // one workgroup per CU
 // The running maximum is raised only when a score passes it by 2^8, so the
 // sums are seldom scaled: the weights then reach 2^8, which f32 sums and the
 // type's range (f16: 2^7 is the lift here) take without loss.  Each is rounded to
-// T once, off by 2^-11 of itself (bf16: 2^-8) at most and without a common
-// direction; the sum is of the unrounded ones.  A second part, as in the kernel
+// T once (SHARED: in kSharedParts), off by 2^-11 of itself (bf16: 2^-8) at most and
+// without a common direction; the sum is of the unrounded ones.  A second part, as in the kernel
 // above, would cost a quarter: 4 x 2048 over 8192, 32 / 8 heads of 128, f16, 1292
 // -> 1641 us; one chunk of 8192, bf16, 664 -> 827.  Without it the relative error
 // of the output, most of it the result's own rounding, is 2.16e-4 for 2.09e-4
@@ -1002,9 +1018,20 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, 2) attn_chunk_kernel(const
         };
         // Values of keys that no row of the unit sees are zeros, and so are
         // those of keys that some rows only see if an infinity or a NaN is
-        // among them; s_bad says which (bit: the key of the tile).
+        // among them; s_bad says which (bit: the key of the tile).  So are all
+        // such values where weights have parts (SHARED), of which some are 0 or
+        // below: an infinity would become a NaN.
         auto put = [&](uint32_t key0, int b, int bs) {
-            if ((int)key0 + kTile > unit_pos0 + 1 || (int)key0 < unit_lo1) {
+            bool look = (int)key0 + kTile > unit_pos0 + 1 || (int)key0 < unit_lo1;
+            if (SHARED && !look) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int i = 0; i < KP; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) top |= exponents<T>(vr[i][e]);
+                look = __any((top & 0x80008000u) != 0);
+            }
+            if (look) {
                 uint64_t bad = 0;
 #pragma unroll
                 for (int i = 0; i < KP; i++) {
@@ -1063,9 +1090,9 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, 2) attn_chunk_kernel(const
                 // the group before it run; the compiler would put every read
                 // right before its use.
                 constexpr int kGroups = KF / 4;         // of four factors
-                constexpr int NP = NZ / 8;
+                constexpr int NP = NZ / 8, NW = SHARED ? kSharedParts<T> : 1;
                 Acc z[KT][M == 32 ? 1 : 2];
-                v8 pf[KT][NP], kf[2][4], vf[2][4];
+                v8 pf[KT][NW][NP], kf[2][4], vf[2][4];
                 auto read_k = [&](int y, int gr) {      // of keys 32 y ..
 #pragma unroll
                     for (int c = 0; c < 4; c++) {
@@ -1098,10 +1125,12 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, 2) attn_chunk_kernel(const
                 };
                 auto add_v = [&](int y, int gr) {
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        const int f = 4 * gr + c;
-                        o[f % DT] = mfma(vf[(y * kGroups + gr) & 1][c], pf[y][f / DT], o[f % DT]);
-                    }
+                    for (int q = NW - 1; q >= 0; q--)   // (the small parts first)
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            const int f = 4 * gr + c;
+                            o[f % DT] = mfma(vf[(y * kGroups + gr) & 1][c], pf[y][q][f / DT], o[f % DT]);
+                        }
                 };
                 auto score_of = [&](int y, int i) -> float { return z[y][i / NA][i % NA]; };
                 float by = 1.0f;
@@ -1144,22 +1173,27 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, 2) attn_chunk_kernel(const
                 auto weigh = [&](int y, int i0, int n) {        // the weights of n scores, and their sum
 #pragma unroll
                     for (int i = i0; i < i0 + n; i++) {
-                        const float x = __builtin_amdgcn_exp2f(fmaf(score_of(y, i), scale, -ref));
+                        float x = __builtin_amdgcn_exp2f(fmaf(score_of(y, i), scale, -ref));
                         sum += x;
-                        pf[y][i >> 3][i & 7] = (T)x;
+#pragma unroll
+                        for (int q = 0; q < NW; q++) {
+                            pf[y][q][i >> 3][i & 7] = (T)x;
+                            if (q + 1 < NW) x -= (float)pf[y][q][i >> 3][i & 7];
+                        }
                     }
                 };
                 auto hold = [&](int y) {                // (computed here: else they are put off past the branch that follows)
 #pragma unroll
-                    for (int i = 0; i < NP; i++) asm volatile("" : "+v"(pf[y][i]));
+                    for (int i = 0; i < NW * NP; i++) asm volatile("" : "+v"(pf[y][i / NP][i % NP]));
                     asm volatile("" : "+v"(sum));
                 };
                 // one product and its share of the exponentials in turn
-                auto in_turn = [&] {
+                auto in_turn = [&](auto products) {
+                    constexpr int kAll = decltype(products)::value;
 #pragma unroll
-                    for (int i = 0; i < KF; i++) {
+                    for (int i = 0; i < kAll; i++) {
                         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                        __builtin_amdgcn_sched_group_barrier(0x002, NZ * 7 / 2 / KF, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x002, NZ * (2 + 5 * NW) / 2 / kAll, 0);
                     }
                 };
 #pragma unroll
@@ -1187,7 +1221,7 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, 2) attn_chunk_kernel(const
                         score(1, gr);
                         weigh(0, gr * NZ / kGroups, NZ / kGroups);
                     }
-                    in_turn();
+                    in_turn(std::integral_constant<int, KF>());
                     hold(0);
                     raise(1);
                     ref = mx == -INFINITY ? 0.0f : mx - kUp;
@@ -1199,7 +1233,7 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, 2) attn_chunk_kernel(const
                         add_v(0, gr);
                         weigh(1, gr * NZ / kGroups, NZ / kGroups);
                     }
-                    in_turn();
+                    in_turn(std::integral_constant<int, NW * KF>());
                     hold(1);
                     if (moved) scale_o();
                 } else weigh(0, 0, NZ);
@@ -1215,7 +1249,7 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, 2) attn_chunk_kernel(const
                 // (The first 32 keys' weights are those to the maximum before the
                 // second raise, which has scaled the sums since.)
                 const float since = KT > 1 && moved ? by : 1.0f;
-                if ((int)key0 + kTile > unit_pos0 + 1 || (int)key0 < unit_lo1)
+                if (SHARED || (int)key0 + kTile > unit_pos0 + 1 || (int)key0 < unit_lo1)
                     for (uint64_t bad = s_bad[bs]; bad; bad &= bad - 1) {
                         const int key = __ffsll((unsigned long long)bad) - 1, y = key & 31;
                         // the place and the lane of its weight
@@ -1225,7 +1259,11 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, 2) attn_chunk_kernel(const
                         float wt = 0.0f;
 #pragma unroll
                         for (int i = 0; i < NZ * KT; i++)
-                            if (i == at) wt = (float)pf[i / NZ][i % NZ >> 3][i & 7];
+                            if (i == at) {
+                                wt = (float)pf[i / NZ][NW - 1][i % NZ >> 3][i & 7];
+#pragma unroll
+                                for (int q = NW - 2; q >= 0; q--) wt += (float)pf[i / NZ][q][i % NZ >> 3][i & 7];
+                            }
                         wt = __shfl(wt, from);
                         if (key < 32) wt *= since;
                         if ((int)key0 + key > pos || (int)key0 + key < lo) continue;

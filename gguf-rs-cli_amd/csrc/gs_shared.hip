@@ -319,10 +319,10 @@ template <class T, int D, int NT, bool F32> void few_and_many(gs::AttnArgs &a, g
             b.second = gs::kSecond;
             // Few sequences' own keys do not fill a launch of their own.  (us with two
             // kernels and with the second alone, heads of 128: one family of 8 rows
-            // over 1000 tokens and up to 50 of their own, 8 heads of keys, 37.5, 26.9;
-            // 4 of 8 over 2000, 40.2, 33.7; one of 64 over 4000, 52.4, 54.4; 8 of 32 over
-            // 2000, 4 heads of keys, 77.9, 89.4.  Heads of 256, one of 16 over 8000, 57.9,
-            // 41.7; 16 of 16 over 2000 and up to 1000, 293, 306.)
+            // over 1000 tokens and up to 50 of their own, 8 heads of keys, 40.4, 29.5;
+            // 4 of 8 over 2000, 43.3, 38.2; one of 64 over 4000, 56.5, 54.8; 8 of 32 over
+            // 2000, 4 heads of keys, 86.6, 94.4.  Heads of 256, one of 16 over 8000, 62.4,
+            // 48.2; 16 of 16 over 2000 and up to 1000, 288, 319.)
             if ((uint64_t)(a.n - a.n_families) * a.n_kv > gs::kChunkRuns) {
                 a.max_rows = 16 * NT;
                 b.min_rows = 16 * NT + 1;

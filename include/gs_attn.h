@@ -66,7 +66,8 @@ int gs_attn_lse(const gs_kv_cache *c, uint32_t layer, const gs_kv_batch *b, cons
  * `families` [n_families + 1] is device memory, ascending; sequences before the
  * first or after the last family are by themselves.  The workspace is larger
  * and grows with the tokens: gs_attn_shared_workspace bytes.
- * 16-bit queries: weights are rounded to the cache's type once. */
+ * Weights reach the values in parts that hold 22 bits or more, of 16-bit queries
+ * too (gs_attn rounds theirs to the cache's type, but for few query rows). */
 int gs_attn_shared(const gs_kv_cache *c, uint32_t layer, const gs_kv_batch *b, const uint32_t *families, uint32_t n_families,
                    const gs_attn_args *a, float *lse, void *stream);
 

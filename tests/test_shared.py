@@ -125,6 +125,51 @@ def test_families(gpu, torch, prompts, each, adds, news, H, kv, d, page, dtype, 
     check_lse(lse, ref_lse)
 
 
+WEIGHTS = [  # prompts, rows of each, own tokens, new tokens, heads, kv, d, window: of the rows kernel alone, of the second alone, of both
+    ([300], [2], [5, 40], [1, 1], 8, 2, 128, 0),
+    ([300], [2], [5, 40], [2, 3], 8, 1, 64, 0),
+    ([300], [2], [5, 40], [1, 1], 8, 2, 256, 0),
+    ([600, 40], [9, 6], [1 + 3 * i for i in range(15)], [1] * 15, 16, 2, 128, 0),
+    ([600], [8], [1 + 3 * i for i in range(8)], [1, 1, 1, 2, 3, 4, 5, 6], 16, 2, 64, 200),
+    ([600], [8], [9 + 3 * i for i in range(8)], [1, 1, 1, 2, 3, 4, 5, 9], 12, 2, 256, 0),
+    ([300, 77], [20, 13], [1 + i % 9 for i in range(33)], [1] * 33, 16, 8, 128, 0),
+    ([300, 77], [20, 13], [1 + i % 9 for i in range(33)], [1] * 33, 16, 8, 256, 0),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("prompts,each,adds,news,H,kv,d,window", WEIGHTS)
+def test_weights_reach_the_values_in_parts(gpu, torch, dtype, prompts, each, adds, news, H, kv, d, window):
+    """16-bit queries and keys of small whole numbers, whose products have no
+    rounding.  With W the sum of the weights times the values' magnitudes, the
+    result is off by no more than
+      W 2^-22                         a weight's parts, two of f16, three of bf16,
+      W 2^-21 (1 + largest |score|)   the exponent, the reference it is taken
+                                      from and the exponential, of up to three
+                                      joined sums: four roundings of 2^-24 of
+                                      log2(e) |score| and two of 2^-23,
+      W (keys / 32 + 64) 2^-23        sums in 32 bits, as elsewhere,
+    and its own rounding.  A single rounding of a weight is up to 2^-11 (bf16:
+    2^-8) of it."""
+    c = family(gpu, torch, prompts, each, adds, kv, d, 16, dtype, seed=6)
+    g = torch.Generator("cuda").manual_seed(12)
+    t = getattr(torch, dtype)
+    c.k.copy_(torch.where(c.k.isnan(), c.k, torch.randint(-1, 2, c.k.shape, generator=g, device="cuda").to(t)))
+    c.v.copy_(torch.where(c.v.isnan(), c.v, torch.randn(c.v.shape, generator=g, device="cuda").to(t)))    # (sums near 0, which round little)
+    rows = list(range(len(prompts), len(prompts) + sum(each)))
+    q = torch.randint(-1, 2, (sum(news), H, d), generator=g, device="cuda").to(t)
+    families = words(torch, np.cumsum([0] + each))
+    scale = 1 / 16
+    got = c.attend_shared(0, q, families, rows=words(torch, rows), q_start=starts(torch, news), max_q=max(news), window=window, scale=scale)
+    out = want(c, 0, q.float(), rows, news, scale=scale, window=window)[0]
+    c.v.abs_()
+    W = want(c, 0, q.float(), rows, news, scale=scale, window=window)[0]
+    top, keys = scale * d, int(c.len.max())                       # (a score is d products of -1, 0 and 1)
+    tol = W * (2.0 ** -22 + 2.0 ** -21 * (1 + top) + (keys / 32 + 64) * 2.0 ** -23)
+    check(got, (out, tol + U[dtype] * (np.abs(out) + tol) + (2.0 ** -25 if dtype == "float16" else 0)))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,cache", [("float16", "float16"), ("float32", "bfloat16")])
 def test_rows_that_have_nothing_to_share(gpu, torch, dtype, cache):

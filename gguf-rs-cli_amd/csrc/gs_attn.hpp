@@ -62,6 +62,10 @@ struct AttnArgs {
     uint32_t second;                // 0 or kSecond: whose parts they are, of two kernels of a call
 };
 
+// What a call wants of the kernels below: gs_attn's result, the softmax's sums
+// too, or either for families.
+enum Kind { kPlain, kSums, kShared };
+
 // A row of `where`: the unit's first run (9 bits), its parts (10 bits; 0: in
 // `whole`), the row's place in the unit (8 bits), and these.
 constexpr uint32_t kSecond = 1u << 27;      // parts of the call's second kernel
@@ -179,6 +183,7 @@ template <int R_, int kTile_, int kSetup_, class S, int kBase = 0, int kM = 1> s
     // The first tile of a unit whose pieces begin at or after `piece` of its beginning.
     static __device__ __forceinline__ uint32_t tile_at(uint64_t piece, uint32_t weight)
     {
+        if constexpr (kBase == 0) return max((uint32_t)piece, (uint32_t)kSetup) - kSetup;
         return max((uint32_t)quotient(piece + weight - 1, weight), (uint32_t)kSetup) - kSetup;
     }
     static __device__ __forceinline__ uint32_t heads(const AttnArgs &a) { return a.n_kv; }
@@ -407,9 +412,10 @@ constexpr int rows_per_cu(int D, int NT) { return D == 64 || (D == 128 && NT == 
 // f16's range), and the weights too, so the products keep 24 bits.
 // FULL: heads of just D values (their strides are then constants, which takes
 // fewer registers and instructions).
-template <class T, int D, int NT, bool F32, bool FULL, bool SHARED>
+template <class T, int D, int NT, bool F32, bool FULL, Kind KIND>
 __global__ void __launch_bounds__(256, rows_per_cu(D, NT)) attn_rows_kernel(const AttnArgs a)
 {
+    constexpr bool SHARED = KIND == kShared;
     constexpr int R = 16 * NT, NP = F32 ? 3 : 1, NW = F32 ? 3 : SHARED ? kSharedParts<T> : __is_same(T, __bf16) && NT == 1 ? 2 : 1, KS = D / 32;
     constexpr int CW = D >= 128 ? 8 : D / 16, NC = D / (16 * CW);       // values of a lane's V chunk, chunks
     typedef typename Vec<T>::v8 v8;
@@ -806,7 +812,7 @@ __global__ void __launch_bounds__(256, rows_per_cu(D, NT)) attn_rows_kernel(cons
             const bool none = SHARED && s.family() ? false : (int64_t)s.len - s.nq + tok < 0;
             const float inv = none ? 0.0f : 1.0f / total;               // (no key: zeros)
             if (!whole && c0 == 0) { part[R * D + 16 * nt + rr] = top; part[R * D + R + 16 * nt + rr] = total; }
-            if (whole && here && c0 == 0 && a.lse) a.lse[(size_t)(s.first + tok) * heads + h] = log_sum(a, none, top, total);
+            if (KIND != kPlain && whole && here && c0 == 0 && a.lse) a.lse[(size_t)(s.first + tok) * heads + h] = log_sum(a, none, top, total);
             float *kept = nullptr;          // SHARED: a whole unit of a row that has another job
             if constexpr (SHARED) {
                 const size_t row = (s.family() ? 0 : (size_t)a.n_tokens * heads) + (size_t)(s.first + tok) * heads + h;
@@ -906,9 +912,10 @@ constexpr int kChunkRuns = 256;         // one workgroup per CU
 // vector issue is half of the clocks, the matrix cores two fifths.  Each pass of
 // keys and values through LDS serves 32 rows of a wave (64 do not fit its
 // registers).
-template <class T, int D, bool FULL, bool SHARED>
+template <class T, int D, bool FULL, Kind KIND>
 __global__ void __launch_bounds__(Chunk<D>::kThreads, 2) attn_chunk_kernel(const AttnArgs a)
 {
+    constexpr bool SHARED = KIND == kShared;
     constexpr int R = Chunk<D>::kRows, kTile = Chunk<D>::kTile, kThreads = Chunk<D>::kThreads;
     constexpr int C = D / 8, KP = kTile * C / kThreads;         // 16-byte pieces of a row; pieces of a thread
     constexpr int M = Chunk<D>::kM, KT = kTile / 32, DT = D / M;
@@ -965,7 +972,8 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, 2) attn_chunk_kernel(const
         const uint32_t weight = Dealt::weight(r0, r1);
         const uint32_t dealt = (span.tiles + Dealt::kSetup) * weight, part_of = (uint32_t)min((uint64_t)(dealt - skip), run.t1 - t);
         const uint32_t first = Dealt::tile_at(skip, weight), left = Dealt::tile_at((uint64_t)skip + part_of, weight) - first;
-        if (left == 0) {                                // (its setup only: the next run begins it; or a piece of its last tile)
+        if (!SHARED && left == 0) break;                // (its setup only: the next run begins it)
+        if (SHARED && left == 0) {                      // (or a piece of its last tile)
             t += part_of;
             skip = 0;
             r0 += R;
@@ -1307,7 +1315,7 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, 2) attn_chunk_kernel(const
                                      : run_id | (run_with(run, end - 1) - run_id + 1) << 9 | (uint32_t)(M * w + col) << 19 | a.second | common;
             if (whole && here) {
                 const float inv = pos < 0 ? 0.0f : 1.0f / sum;          // (no key: zeros)
-                if (hg == 0 && a.lse) a.lse[(size_t)(s.first + tok) * heads + hq] = log_sum(a, pos < 0, mx, sum);
+                if (KIND != kPlain && hg == 0 && a.lse) a.lse[(size_t)(s.first + tok) * heads + hq] = log_sum(a, pos < 0, mx, sum);
                 T *to = (T *)a.out + (size_t)(s.first + tok) * a.ld_out + (size_t)hq * d;
                 typedef T v4 __attribute__((ext_vector_type(4)));
 #pragma unroll
@@ -1364,7 +1372,7 @@ __global__ void __launch_bounds__(Chunk<D>::kThreads, 2) attn_chunk_kernel(const
 // 18 us.  Joining in the first kernel by the last run
 // to come needs a release to the other XCDs by each run: 64 single tokens 206
 // us like this, 368 so.)
-template <class TO, int D, int R> __device__ __forceinline__ void join_unit(const AttnArgs &a, uint32_t g)
+template <class TO, int D, int R, bool LSE> __device__ __forceinline__ void join_unit(const AttnArgs &a, uint32_t g)
 {
     const Cut c = a.cuts[g];
     if (c.last == 0) return;
@@ -1408,7 +1416,7 @@ template <class TO, int D, int R> __device__ __forceinline__ void join_unit(cons
     const uint32_t r = c.row0 + rr, tok = r / a.group;
     if (rr >= c.rows || dv >= a.d) return;
     x *= r < c.keyless ? 0.0f : 1.0f / total;
-    if (dv == 0 && a.lse) a.lse[(size_t)(c.first_token + tok) * a.n_kv * a.group + c.kvh * a.group + r - tok * a.group] = log_sum(a, r < c.keyless, top, total);
+    if (LSE && dv == 0 && a.lse) a.lse[(size_t)(c.first_token + tok) * a.n_kv * a.group + c.kvh * a.group + r - tok * a.group] = log_sum(a, r < c.keyless, top, total);
     const size_t to = (size_t)(c.first_token + tok) * a.ld_out + (size_t)(c.kvh * a.group + r - tok * a.group) * a.d + dv;
     if constexpr (sizeof(TO) == 4) *(f4 *)((float *)a.out + to) = x;
     else {
@@ -1417,17 +1425,17 @@ template <class TO, int D, int R> __device__ __forceinline__ void join_unit(cons
     }
 }
 
-template <class TO, int D, int R>
-__global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) { join_unit<TO, D, R>(a, blockIdx.x); }
+template <class TO, int D, int R, bool LSE>
+__global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) { join_unit<TO, D, R, LSE>(a, blockIdx.x); }
 
 // The parts of both kernels of a call that has sequences for each, in one
 // launch (a row of one token and one of 100, over up to 1000: 28.3 us with two,
 // 25.4; 24 rows over 700 to 8192, heads of 128: 220, 215).
-template <class TO, int D, int R, int R2>
+template <class TO, int D, int R, int R2, bool LSE>
 __global__ void __launch_bounds__(256) attn_join_both_kernel(const AttnArgs a, const AttnArgs b)
 {
-    if (blockIdx.x < a.n_wg) join_unit<TO, D, R>(a, blockIdx.x);
-    else join_unit<TO, D, R2>(b, blockIdx.x - a.n_wg);
+    if (blockIdx.x < a.n_wg) join_unit<TO, D, R, LSE>(a, blockIdx.x);
+    else join_unit<TO, D, R2, LSE>(b, blockIdx.x - a.n_wg);
 }
 
 } // namespace gs

@@ -290,8 +290,8 @@ template <class T, int D, int NT, bool F32> void rows_launch(gs::AttnArgs &a, hi
 {
     a.n_wg = kCUs * gs::rows_per_cu(D, NT);
     a.lift = gs::kLift<T>;
-    if (a.d == D) hipLaunchKernelGGL((gs::attn_rows_kernel<T, D, NT, F32, true, true>), dim3(a.n_wg), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((gs::attn_rows_kernel<T, D, NT, F32, false, true>), dim3(a.n_wg), dim3(256), 0, st, a);
+    if (a.d == D) hipLaunchKernelGGL((gs::attn_rows_kernel<T, D, NT, F32, true, gs::kShared>), dim3(a.n_wg), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((gs::attn_rows_kernel<T, D, NT, F32, false, gs::kShared>), dim3(a.n_wg), dim3(256), 0, st, a);
 }
 
 template <class T, int D> void chunk_launch(gs::AttnArgs &a, hipStream_t st)
@@ -299,8 +299,8 @@ template <class T, int D> void chunk_launch(gs::AttnArgs &a, hipStream_t st)
     a.n_wg = gs::kChunkRuns;
     a.lift = gs::kChunkLift<T>;
     const dim3 grid(a.n_wg), block(gs::Chunk<D>::kThreads);
-    if (a.d == D) hipLaunchKernelGGL((gs::attn_chunk_kernel<T, D, true, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((gs::attn_chunk_kernel<T, D, false, true>), grid, block, 0, st, a);
+    if (a.d == D) hipLaunchKernelGGL((gs::attn_chunk_kernel<T, D, true, gs::kShared>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((gs::attn_chunk_kernel<T, D, false, gs::kShared>), grid, block, 0, st, a);
 }
 
 template <class TO, int D, int R1, int R2> void join(const gs::AttnArgs &a, const gs::AttnArgs &b, hipStream_t st)

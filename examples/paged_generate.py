@@ -119,10 +119,9 @@ def generate(model, prompts, answers, new, seed=42, keep=8, shared=False, budget
     # each answer is a row that shares its prompt's pages; the prompt's own row goes
     of = torch.arange(n, device="cuda", dtype=torch.int32).repeat_interleave(answers)
     cache.fork(of, kids)
-    cache.free(parents)
     if budget:
         mass[kids.long()] = mass[of.long()]                     # the answers' tokens weigh what their prompts' do
-        mass[:n] = 0.0
+    cache.free(parents, mass=mass)
     x = hidden[(start[1:] - 1).long()][of.long()].contiguous()
     sampler = gs.Sampler(0.8, 40, 0.95, 1.1, seed=seed)
     sampler.reserve(B, cfg["vocab"])

@@ -36,7 +36,7 @@ struct Move {
 struct Stays {
     uint32_t *list;
     size_t ld;
-    float *mass;                // [rows][ld_mass]
+    float *mass;                // [rows][ld_mass] (of a drop: or null, and no list)
     size_t ld_mass;
 };
 
@@ -311,14 +311,16 @@ __global__ void __launch_bounds__(256) fork_write_kernel(const Cache c)
     if (threadIdx.x == 0) c.len[m.row] = m.len;
 }
 
-// Row rows[blockIdx.x] emptied.  Its length is taken by an exchange: a row
-// named twice is released once.  (Waits for three reads in a row: 3 to 5 us for
-// 8 to 256 rows.)
-__global__ void __launch_bounds__(256) free_kernel(const Cache c, const uint32_t *rows)
+// Row rows[blockIdx.x] emptied, with its weights (mass, or null).  Its length is
+// taken by an exchange: a row named twice is released once.  (Waits for three
+// reads in a row: 3 to 5 us for 8 to 256 rows.)
+__global__ void __launch_bounds__(256) free_kernel(const Cache c, const uint32_t *rows, float *mass, size_t ld_mass)
 {
     __shared__ uint32_t held;
     const uint32_t row = rows[blockIdx.x];
     if (row >= c.rows) return;
+    if (mass)
+        for (uint32_t x = threadIdx.x; x < c.ld << c.shift; x += 256) mass[row * ld_mass + x] = 0.0f;
     if (threadIdx.x == 0) held = min(atomicExch(&c.len[row], 0u), c.ld << c.shift);
     __syncthreads();
     uint32_t *table = c.table + (size_t)row * c.ld;
@@ -583,25 +585,26 @@ __global__ void __launch_bounds__(256) drop_move_kernel(const Cache c, const uin
     move_stream<T, MODE, EVICT>(c, m, i, base, h, rot, interleaved, cs, t0, slice, slices, list, turns);
 }
 
-// Drop, 3 of 3: row blockIdx.x's table, its released pages, its length.  (4.7
-// us: words only.)  EVICT: its weights too, kEach times 1024 at a time: they go
-// down in ascending order, and all of a step are read before one is written.
+// Drop, 3 of 3: row blockIdx.x's table, its released pages, its length, and its
+// weights where there are any, kEach times kThreads at a time: they go down in
+// ascending order, and all of a step are read before one is written.  (4.7 us:
+// words only.)
 template <bool EVICT> __global__ void __launch_bounds__(EVICT ? 1024 : 256) drop_write_kernel(const Cache c, const Stays e)
 {
     constexpr uint32_t kThreads = EVICT ? 1024 : 256;
     const uint32_t i = blockIdx.x;
     const Move m = c.moves[i];
     if (!m.ok) return;
-    if constexpr (EVICT) {
+    if (EVICT || e.mass) {
         constexpr int kEach = 8;
         float *mass = e.mass + m.row * e.ld_mass;
-        const uint32_t *list = e.list + i * e.ld;
+        const uint32_t *list = EVICT ? e.list + i * e.ld : nullptr, gone = m.len - m.left;
         for (uint32_t x0 = m.from; x0 < m.left; x0 += kEach * kThreads) {
             float w[kEach];
 #pragma unroll
             for (int k = 0; k < kEach; k++) {
                 const uint32_t x = x0 + k * kThreads + threadIdx.x;
-                w[k] = x < m.left ? mass[list[x]] : 0.0f;
+                w[k] = x < m.left ? mass[EVICT ? list[x] : x + gone] : 0.0f;
             }
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
@@ -781,6 +784,13 @@ int check_call(const gs_kv_cache *c, size_t n)
     return n <= c->rows && n <= 65535 ? GS_OK : GS_ERR_INVALID;     // (a grid's second and third sizes)
 }
 
+// Weights of the rows' tokens, [rows][ld_mass].
+int check_mass(const gs_kv_cache *c, const float *mass, size_t ld_mass)
+{
+    if (!mass || ((uintptr_t)mass & 3u) || ld_mass < (size_t)c->ld_table * c->page_size) return GS_ERR_INVALID;
+    return ld_mass > (size_t)1 << 40 ? GS_ERR_UNSUPPORTED : GS_OK;
+}
+
 int launched() { return hipGetLastError() == hipSuccess ? GS_OK : GS_ERR_HIP; }
 
 // Workgroups that share each of n pieces of data, up to `most`, so that there
@@ -871,26 +881,40 @@ int gs_kv_fork(const gs_kv_cache *c, const uint32_t *src, const uint32_t *dst, s
 
 int gs_kv_free(const gs_kv_cache *c, const uint32_t *rows, size_t n, void *stream)
 {
+    return gs_kv_free_mass(c, rows, n, nullptr, 0, stream);
+}
+
+int gs_kv_free_mass(const gs_kv_cache *c, const uint32_t *rows, size_t n, float *mass, size_t ld_mass, void *stream)
+{
     if (int rc = check_call(c, n)) return rc;
+    if (int rc = mass ? check_mass(c, mass, ld_mass) : GS_OK) return rc;
     if (n == 0) return GS_OK;
     if (!rows) return GS_ERR_INVALID;
-    hipLaunchKernelGGL(gs::free_kernel, dim3((unsigned)n), dim3(256), 0, (hipStream_t)stream, device_cache(c), rows);
+    hipLaunchKernelGGL(gs::free_kernel, dim3((unsigned)n), dim3(256), 0, (hipStream_t)stream, device_cache(c), rows, mass, ld_mass);
     return launched();
 }
 
 int gs_kv_drop(const gs_kv_cache *c, const uint32_t *rows, size_t n, const uint32_t *from, const uint32_t *to,
                const gs_rope *rope, int32_t *status, void *stream)
 {
+    return gs_kv_drop_mass(c, rows, n, from, to, rope, nullptr, 0, status, stream);
+}
+
+int gs_kv_drop_mass(const gs_kv_cache *c, const uint32_t *rows, size_t n, const uint32_t *from, const uint32_t *to,
+                    const gs_rope *rope, float *mass, size_t ld_mass, int32_t *status, void *stream)
+{
     if (int rc = check_call(c, n)) return rc;
     if (rope && (rope->d != c->d || !is_here(rope))) return GS_ERR_INVALID;
+    if (int rc = mass ? check_mass(c, mass, ld_mass) : GS_OK) return rc;
     if (n == 0) return GS_OK;
     if (!rows || !from || !to) return GS_ERR_INVALID;
     if (too_many_streams(c)) return GS_ERR_UNSUPPORTED;
     const gs::Cache d = device_cache(c);
     hipStream_t st = (hipStream_t)stream;
     hipLaunchKernelGGL(gs::drop_plan_kernel<false>, dim3(1), dim3(gs::kBook), 0, st, d, rows, (uint32_t)n, from, to, status);
-    move_tokens<false>(c, d, n, rope, gs::Stays(), st);
-    hipLaunchKernelGGL(gs::drop_write_kernel<false>, dim3((unsigned)n), dim3(256), 0, st, d, gs::Stays());
+    const gs::Stays e = {nullptr, 0, mass, ld_mass};
+    move_tokens<false>(c, d, n, rope, e, st);
+    hipLaunchKernelGGL(gs::drop_write_kernel<false>, dim3((unsigned)n), dim3(256), 0, st, d, e);
     return launched();
 }
 
@@ -908,8 +932,8 @@ int gs_kv_evict(const gs_kv_cache *c, const gs_kv_evict_args *x, void *stream)
     if (x->rope && (x->rope->d != c->d || !is_here(x->rope))) return GS_ERR_INVALID;
     if (x->n == 0) return GS_OK;
     const size_t most = (size_t)c->ld_table * c->page_size;
-    if (!x->rows || !x->mass || ((uintptr_t)x->mass & 3u) || x->ld_mass < most) return GS_ERR_INVALID;
-    if (x->ld_mass > (size_t)1 << 40) return GS_ERR_UNSUPPORTED;
+    if (!x->rows) return GS_ERR_INVALID;
+    if (int rc = check_mass(c, x->mass, x->ld_mass)) return rc;
     const uint32_t all = x->budget ? 0 : x->budget_all;
     if (!x->ws || ((uintptr_t)x->ws & 15u) || x->ws_bytes < gs_kv_evict_workspace(c, x->n, all)) return GS_ERR_INVALID;
     if (too_many_streams(c)) return GS_ERR_UNSUPPORTED;

@@ -54,7 +54,7 @@ EXPORTS = [
     "gs_rope_create", "gs_rope_destroy", "gs_rope_apply",
     # include/gs_cache.h
     "gs_kv_workspace", "gs_kv_reset", "gs_kv_extend", "gs_kv_fork", "gs_kv_free", "gs_kv_drop", "gs_kv_append",
-    "gs_kv_evict_workspace", "gs_kv_evict",
+    "gs_kv_evict_workspace", "gs_kv_evict", "gs_kv_free_mass", "gs_kv_drop_mass",
     # include/gs_attn.h
     "gs_attn_workspace", "gs_attn", "gs_attn_lse", "gs_attn_shared", "gs_attn_shared_workspace", "gs_attn_weigh",
     "gs_attn_weigh_workspace",
@@ -198,6 +198,8 @@ def load_library(path=LIB_PATH):
         "gs_kv_fork": ([ctypes.POINTER(GsKVCache), P, P, SZ, P, P], I),
         "gs_kv_free": ([ctypes.POINTER(GsKVCache), P, SZ, P], I),
         "gs_kv_drop": ([ctypes.POINTER(GsKVCache), P, SZ, P, P, P, P, P], I),
+        "gs_kv_free_mass": ([ctypes.POINTER(GsKVCache), P, SZ, P, SZ, P], I),
+        "gs_kv_drop_mass": ([ctypes.POINTER(GsKVCache), P, SZ, P, P, P, P, SZ, P, P], I),
         "gs_kv_evict_workspace": ([ctypes.POINTER(GsKVCache), SZ, ctypes.c_uint32], SZ),
         "gs_kv_evict": ([ctypes.POINTER(GsKVCache), ctypes.POINTER(GsKVEvictArgs), P], I),
         "gs_kv_append": ([ctypes.POINTER(GsKVCache), ctypes.c_uint32, ctypes.POINTER(GsKVBatch), P,
@@ -895,22 +897,28 @@ class KVCache:
         _call(dev, self._lib.gs_kv_fork, "gs_kv_fork", self._c, _words(src, "src", dev, n), _words(dst, "dst", dev), n,
               _words(status, "status", dev, n), _stream_of(self.dev, stream))
 
-    def free(self, rows, stream=None):
-        _call(self.dev, self._lib.gs_kv_free, "gs_kv_free", self._c, _words(rows, "rows", self.dev), rows.numel(),
+    def free(self, rows, stream=None, mass=None):
+        """`rows` become empty; their weights in `mass` (as mass() makes it) 0."""
+        at, ld = (None, 0) if mass is None else (mass.data_ptr(), self._mass(mass))
+        _call(self.dev, self._lib.gs_kv_free_mass, "gs_kv_free", self._c, _words(rows, "rows", self.dev), rows.numel(), at, ld,
               _stream_of(self.dev, stream))
 
-    def drop(self, start, end, rows, rope=None, status=None, stream=None):
+    def drop(self, start, end, rows, rope=None, status=None, stream=None, mass=None):
         """Tokens start .. end - 1 of each of `rows` leave it (gs_kv_drop); with
-        `rope` the keys after them are turned back to their new positions."""
+        `rope` the keys after them are turned back to their new positions, and
+        their weights in `mass` (as mass() makes it) move with them."""
         turn = _turn(rope)
         n, dev = rows.numel(), self.dev
-        _call(dev, self._lib.gs_kv_drop, "gs_kv_drop", self._c, _words(rows, "rows", dev), n, _words(start, "start", dev, n),
-              _words(end, "end", dev, n), turn, _words(status, "status", dev, n), _stream_of(self.dev, stream))
+        at, ld = (None, 0) if mass is None else (mass.data_ptr(), self._mass(mass))
+        _call(dev, self._lib.gs_kv_drop_mass, "gs_kv_drop", self._c, _words(rows, "rows", dev), n, _words(start, "start", dev, n),
+              _words(end, "end", dev, n), turn, at, ld, _words(status, "status", dev, n), _stream_of(self.dev, stream))
 
     def mass(self):
         """A new tensor for the weights that weigh() adds up and evict() goes by:
-        [rows, most tokens of a row] float32, zeros.  Its rows go with the
-        cache's: after fork, mass[dst] = mass[src] is the caller's to do."""
+        [rows, most tokens of a row] float32, zeros.  A weight belongs to a place
+        of a row, so give the tensor to free() and drop() too, or tokens have the
+        weights of those that were there before; after reset() the weights are
+        the caller's to clear, after fork(), mass[dst] = mass[src] to do."""
         import torch
         return torch.zeros((self.rows, self.table.shape[1] * self.page), device=self.k.device)
 

@@ -95,6 +95,17 @@ int gs_kv_fork(const gs_kv_cache *c, const uint32_t *src, const uint32_t *dst, s
  * out of range are skipped. */
 int gs_kv_free(const gs_kv_cache *c, const uint32_t *rows, size_t n, void *stream);
 
+/* Weights of cached tokens, mass[row * ld_mass + token] (gs_attn_weigh adds them
+ * up, gs_kv_evict goes by them), belong to places of rows, so they go with every
+ * call that moves or removes tokens: gs_kv_evict moves them, and these two do
+ * what gs_kv_free and gs_kv_drop do and clear a freed row's weights, or move
+ * those of a drop's tokens and clear the places behind.  ld_mass is at least
+ * ld_table * page_size; mass NULL: there are none.  After gs_kv_reset and
+ * gs_kv_fork the caller clears them, or copies row src[i]'s to row dst[i]. */
+int gs_kv_free_mass(const gs_kv_cache *c, const uint32_t *rows, size_t n, float *mass, size_t ld_mass, void *stream);
+int gs_kv_drop_mass(const gs_kv_cache *c, const uint32_t *rows, size_t n, const uint32_t *from, const uint32_t *to,
+                    const gs_rope *rope, float *mass, size_t ld_mass, int32_t *status, void *stream);
+
 /* Tokens from[i] .. to[i] - 1 (cut to the row's tokens) leave row rows[i], and
  * those after them move down to their place; with `rope` their keys are turned
  * by -(to - from) positions too, as if they had been written at their new

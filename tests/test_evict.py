@@ -245,6 +245,49 @@ def test_beside_other_calls(gpu, torch):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shared", [False, True])
+def test_weights_go_with_drops_and_frees(gpu, torch, shared):
+    """Rows that a drop has shortened, or that a free has emptied for others, are
+    cut by the weights that their tokens have."""
+    rows, lens = [4, 1, 6], [170, 33, 96]
+    c, mass, m = build(gpu, torch, lens, rows, shared, pages=90, max_len=176)
+    for start, end in (([20, 0, 96], [90, 33, 200]), ([3, 5, 10], [4, 5, 40]), ([0, 0, 65], [100, 0, 66])):
+        st = run(torch, c.drop, words(torch, start), words(torch, end), words(torch, rows), n=3, mass=mass)
+        for r, a, b in zip(rows, start, end):
+            n = m.len[r]
+            a, b = min(a, n), min(max(a, b), n)
+            m.mass[r, :n] = np.concatenate([m.mass[r, :a], m.mass[r, b:n], np.zeros(b - a, np.float32)])
+        assert st == m.drop(rows, start, end)[0]
+        m.check_all(c, mass)
+        c.extend(9)
+        m.extend(range(8), [9] * 8)
+    run(torch, c.evict, mass, 25, words(torch, rows), first=2, recent=5, n=3)
+    m.evict(rows, [25] * 3, 2, 5)
+    m.check_all(c, mass)
+    # one of a row twice, one that is not there, one that finds no page: weights are as before but for the first's
+    gone = words(torch, [4, 4, 9])
+    st = run(torch, c.drop, words(torch, [1, 2, 3]), words(torch, [9, 9, 9]), gone, n=3, mass=mass)
+    n = m.len[4]
+    m.mass[4, :n] = np.concatenate([m.mass[4, :1], m.mass[4, 9:n], np.zeros(8, np.float32)])
+    assert st == m.drop([4, 4, 9], [1, 2, 3], [9, 9, 9])[0] == [0, -1, -1]
+    m.check_all(c, mass)
+    c.free(words(torch, [6, 11, 4]), mass=mass)
+    m.fork([NONE] * 2, [6, 4])
+    m.mass[[6, 4]] = 0.0
+    m.check_all(c, mass)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,a,b", [(5000, 1, 2), (20011, 3, 7000), (8192, 0, 4096), (4100, 2049, 2050)])
+def test_weights_of_long_drops(gpu, torch, n, a, b):
+    c, mass, m = build(gpu, torch, [n], [1], False, layers=1, kv=1, d=8, pages=n // 16 + 9, max_len=n + 16)
+    c.drop(words(torch, [a]), words(torch, [b]), words(torch, [1]), mass=mass)
+    m.mass[1, :n] = np.concatenate([m.mass[1, :a], m.mass[1, b:n], np.zeros(b - a, np.float32)])
+    m.drop([1], [a], [b])
+    m.check_all(c, mass)
+
+
+@pytest.mark.gpu
 def test_graph_and_stream(gpu, torch):
     """extend and evict captured on a stream of their own, replayed with the
     program's own work between; a larger eager call after the capture, on the
@@ -303,6 +346,18 @@ def test_refusals_without_gpu():
     assert lib.gs_kv_evict_workspace(c, 5, 8) == 0
     # a budget given as a tensor may be anything
     assert call(c, budget=4096, ws_bytes=255) == gs.GS_ERR_INVALID
+
+
+def test_refusals_of_weights_without_gpu():
+    """Weights of a drop and a free: none, or room for each token."""
+    import gs_sampler as gs
+    lib, c = gs.load_library(), fake(gs)
+    for mass, ld, rc in ((None, 0, gs.GS_OK), (4096, 64, gs.GS_OK), (4098, 64, gs.GS_ERR_INVALID), (4096, 63, gs.GS_ERR_INVALID),
+                         (4096, (1 << 40) + 1, gs.GS_ERR_UNSUPPORTED)):
+        assert lib.gs_kv_free_mass(c, None, 0, mass, ld, None) == rc
+        assert lib.gs_kv_drop_mass(c, None, 0, None, None, None, mass, ld, None, None) == rc
+    assert lib.gs_kv_free_mass(c, None, 1, 4096, 64, None) == gs.GS_ERR_INVALID
+    assert lib.gs_kv_drop_mass(c, 4096, 1, 4096, None, None, 4096, 64, None, None) == gs.GS_ERR_INVALID
 
 
 @pytest.mark.gpu

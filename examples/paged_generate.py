@@ -106,6 +106,8 @@ def generate(model, prompts, answers, new, seed=42, keep=8, shared=False, budget
     pages of its prompt together with the prompt's other answers.
     Returns the generated ids [prompts * answers][<= new]."""
     cfg, cache, n = model.cfg, model.cache, len(prompts)
+    if not 0 <= budget < cfg["context"]:
+        raise ValueError("budget must be less than the context's %d tokens (0: none)" % cfg["context"])
     B = n * answers
     kids = words(list(range(n, n + B)))
     # the prompts, all at once
@@ -137,7 +139,7 @@ def generate(model, prompts, answers, new, seed=42, keep=8, shared=False, budget
         if full and budget:
             cache.evict(mass, budget, words([n + b for b in full]), first=keep, recent=budget // 4, rope=model.rope)
             for b in full:
-                held[b] = budget
+                held[b] = min(held[b], budget)
         elif full:
             gone = (cfg["context"] - keep) // 2
             cache.drop(words([keep] * len(full)), words([keep + gone] * len(full)), words([n + b for b in full]), rope=model.rope)

@@ -7,9 +7,14 @@ Weights: a score is off by about 2^-11 of scores of order 1, through the keys'
 rounding and through the queries', per layer: 8 x 2^-11 of their norm, as the
 logits.
 """
+import importlib.util
+import os
+import types
+
 import numpy as np
 import pytest
 
+from conftest import ROOT
 from test_paged_generate import Dense, example, logits_of  # noqa: F401  (a fixture)
 
 
@@ -129,3 +134,14 @@ def test_generate(example, torch):  # noqa: F811
         assert torch.equal(ref, m.cache.ref)
         assert m.cache.len.cpu().tolist()[:3] == [0, 0, 0] and int(m.cache.len.max()) <= 192
     assert runs[0] == runs[1] and all(len(r) == 120 for r in runs[0])
+
+
+@pytest.mark.parametrize("budget", [192, 193, 4096, -1])
+def test_budgets_that_cut_nothing(budget):
+    """A budget that a full row is within would leave it full: each later token
+    would be refused its place and written over the last one's."""
+    spec = importlib.util.spec_from_file_location("paged_generate", os.path.join(ROOT, "examples", "paged_generate.py"))
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    with pytest.raises(ValueError, match="budget"):
+        ex.generate(types.SimpleNamespace(cfg=ex.SMALL, cache=None), [np.arange(5)], 2, 8, budget=budget)

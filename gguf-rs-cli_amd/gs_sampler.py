@@ -758,6 +758,14 @@ def _stream_of(dev, stream):
     return _stream_handle(stream)
 
 
+def _may_capture(dev, st):
+    """Whether a call on the stream st of device dev may be recorded into a
+    graph now: it is unless st is torch's stream of the moment and records none."""
+    import torch
+    now = (_DT or _dtypes())[3]
+    return (now is not None and now() != dev) or st != _stream_of(dev, None) or torch.cuda.is_current_stream_capturing()
+
+
 def _empty_on(st, shape, dtype, like):
     """A new tensor on like's device for work on the HIP stream st.  Memory that
     torch's stream of the moment has freed may still be in use there: on
@@ -864,6 +872,7 @@ class KVCache:
         self.c.ws = self.ws.data_ptr()
         self._attn_ws = {}
         self._more_ws = {}
+        self._graph_ws = set()          # addresses of those that were given to a capture
 
     @classmethod
     def empty(cls, layers, pages, kv, d, rows, max_len, page=16, dtype=None, device="cuda"):
@@ -956,14 +965,23 @@ class KVCache:
 
     def _workspace(self, what, st, n, like):
         """A workspace of n bytes for the calls of one kind on the stream st,
-        where they do not overlap.  Larger ones come beside those that captured
-        graphs may hold, and are at least twice their size."""
+        where they do not overlap: up to an eighth more, so that calls of about
+        one size share it.  A larger one takes its place, unless a captured graph
+        may hold it: then it stays and the new one is at least twice its size."""
         import torch
         if not n:
             raise SamplerError(GS_ERR_INVALID, what)
         held = self._more_ws.setdefault((what, st), [])
         if not held or held[-1].numel() < n:
-            held.append(_empty_on(st, max(n, 2 * held[-1].numel() if held else 0), torch.uint8, like))
+            step = 1 << max(n.bit_length() - 4, 0)
+            size = -(-n // step) * step
+            if held and held[-1].data_ptr() in self._graph_ws:
+                size = max(size, 2 * held[-1].numel())
+            elif held:
+                held.pop()
+            held.append(_empty_on(st, size, torch.uint8, like))
+        if _may_capture(self.dev, st):
+            self._graph_ws.add(held[-1].data_ptr())
         return held[-1]
 
     def _batch(self, T, rows, q_start):
@@ -1051,8 +1069,9 @@ class KVCache:
         The cache keeps a workspace of 43 to 85 MB, and of 8 d + 44 bytes for each
         token and head (d as 64, 128 or 256), for each stream that attend_shared
         was called on, as attend does; a call of more tokens than those before
-        makes another, for twice as many at least, and the smaller one stays
-        with the cache for the graphs that use it."""
+        makes a larger one, and the smaller one stays only if a captured graph
+        may use it (it was given to a capture, or to a call on a stream that was
+        not torch's current one)."""
         if not 0 <= window <= 0xFFFFFFFF:
             raise ValueError("window must be a number of positions")
         T, heads, _, ld_q = _heads(q, "q", self.dev, d=self.d)

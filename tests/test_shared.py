@@ -316,6 +316,49 @@ def test_streams_and_graph(gpu, torch):
     assert len({w.data_ptr() for x in (a, b) for held in x._more_ws.values() for w in held}) >= 3
 
 
+@pytest.mark.gpu
+def test_workspaces_of_growing_calls(gpu, torch):
+    """A call that is a little larger than the last takes the same workspace or
+    one in its place; one that a capture has had stays."""
+    c = family(gpu, torch, [40], [2], [5, 9], 2, 64, 16, "float16")
+    rows, families = words(torch, [1, 2]), words(torch, [0, 2])
+
+    def need(n):
+        return c._lib.gs_attn_shared_workspace(c._c, 64, 2, 1, n)
+
+    def call(n):
+        q = torch.randn((n, 64, 64), device="cuda").half()
+        return c.attend_shared(0, q, families, rows=rows, q_start=words(torch, [0, 1, n]))
+
+    def held():
+        return [w.numel() for k, x in c._more_ws.items() if k[0] == "attend_shared" for w in x]
+
+    for n in (500, 501, 502, 4000, 4001):
+        call(n)
+        assert len(held()) == 1 and need(n) <= held()[0] <= need(n) * 9 // 8 + 1, n
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    q = torch.randn((600, 64, 64), device="cuda").half()
+    out, start = torch.empty_like(q), words(torch, [0, 1, 600])
+    c._more_ws.clear()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s):
+        with torch.cuda.graph(graph, stream=s):
+            c.attend_shared(0, q, families, out, rows=rows, q_start=start)
+        first = held()
+        for n in (2000, 4000, 8000):                              # (the ones between go, the graph's does not)
+            call(n)
+            assert held()[0] == first[0] and len(held()) == 2 and held()[1] >= max(need(n), 2 * first[0])
+    torch.cuda.synchronize()
+    want_out = c.attend_shared(0, q, families, rows=rows, q_start=start)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want_out)
+
+
 def test_refusals_without_gpu():
     import gs_sampler as gs
     lib = gs.load_library()

@@ -170,6 +170,57 @@ def test_weights_reach_the_values_in_parts(gpu, torch, dtype, prompts, each, add
     check(got, (out, tol + U[dtype] * (np.abs(out) + tol) + (2.0 ** -25 if dtype == "float16" else 0)))
 
 
+def many(n, each):
+    """n rows' own and new tokens, each as many new ones as `each` says in turn."""
+    news = [each[i % len(each)] for i in range(n)]
+    return [x + i % 21 for i, x in enumerate(news)], news
+
+
+BOTH = [  # prompts, rows of each, new tokens in turn, heads, kv, d, page, type, window: more heads of keys of sequences than the second kernel has runs
+    ([300, 77], [25, 11], [1], 16, 8, 128, 16, "float16", 0),
+    ([300, 77], [25, 11], [1], 16, 8, 128, 16, "bfloat16", 0),
+    ([300], [33], [1], 24, 8, 128, 32, "bfloat16", 150),           # windows that end inside the common pages,
+    ([300], [33], [1], 24, 8, 96, 16, "float16", 31),              # and past them for some rows
+    ([200], [34], [1], 8, 8, 192, 16, "bfloat16", 190),
+    ([200, 120], [20, 14], [1], 16, 8, 256, 16, "bfloat16", 0),
+    ([200, 120], [20, 14], [1], 16, 8, 256, 16, "float16", 180),
+    ([200], [36], [1], 40, 8, 80, 16, "float16", 0),
+    ([200], [34], [5], 32, 8, 128, 16, "bfloat16", 0),             # own rows of two tiles
+    ([200], [34], [5], 32, 8, 64, 16, "float16", 120),
+    ([200], [34], [7, 2, 0, 8], 32, 8, 128, 16, "float16", 0),
+    ([150], [34], [1, 1, 1, 40, 3], 16, 8, 128, 16, "bfloat16", 0),    # own keys of both kernels
+    ([150], [34], [1, 1, 1, 40, 3], 16, 8, 64, 16, "bfloat16", 100),
+    ([150], [34], [1, 20, 1, 9, 3], 16, 8, 256, 16, "float16", 0),
+    ([150], [34], [1, 20, 1, 17, 3], 16, 8, 192, 32, "bfloat16", 50),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("prompts,each,turn,H,kv,d,page,dtype,window", BOTH)
+def test_both_kernels(gpu, torch, prompts, each, turn, H, kv, d, page, dtype, window):
+    """Calls whose jobs of few rows go to one kernel and whose others go to a
+    second, of other parts, lifts and rows in a unit."""
+    n = sum(each)
+    assert n * kv > 256 and n * H // kv > 16
+    adds, news = many(n, turn)
+    c = family(gpu, torch, prompts, each, adds, kv, d, page, dtype, layers=2, seed=2)
+    rows = list(range(len(prompts), len(prompts) + n))
+    q = torch.randn((sum(news), H, d), generator=torch.Generator("cuda").manual_seed(3), device="cuda").to(getattr(torch, dtype)) * 2
+    start = None if set(news) == {1} else starts(torch, news)
+    ref, ref_lse = (f(c, 1, q, rows, news, window=window) for f in (want, want_lse))
+    ends = np.cumsum([0] + each).tolist()
+    outs = []
+    for families, most in ((ends, max(news)), (ends, 0), ([0, n], max(news)), ([3, n - 2], max(news)), (ends, 1)):   # (1: less than the most)
+        out = torch.full((sum(news), H, d), 99.0, dtype=q.dtype, device="cuda")
+        lse = torch.full((sum(news), H), 99.0, device="cuda")
+        c.attend_shared(1, q, words(torch, families), out, rows=words(torch, rows), q_start=start, window=window, max_q=most, lse=lse)
+        check(out, ref)
+        check_lse(lse, ref_lse)
+        outs.append(out)
+    again = c.attend_shared(1, q, words(torch, ends), rows=words(torch, rows), q_start=start, window=window, max_q=max(news))
+    assert torch.equal(outs[0], again)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,cache", [("float16", "float16"), ("float32", "bfloat16")])
 def test_rows_that_have_nothing_to_share(gpu, torch, dtype, cache):

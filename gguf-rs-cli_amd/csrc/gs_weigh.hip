@@ -273,9 +273,13 @@ __global__ void __launch_bounds__(256) weigh_few_kernel(const WeighArgs a)
 // workgroup in a CU), and the workgroups that a CU takes.  (us with 64 keys of a
 // wave, two workgroups, and with 32, three: 4 x 2048 tokens over up to 8192, 350,
 // 363; 7 x 32 over up to 12000, 47, 45; one of 2000, 72, 62; 4 x 64 over up to
-// 12000, heads of 64, 32, 26.)
+// 12000, heads of 64, 32, 26.)  With 32-bit queries LDS says how many: 29, 53 and
+// 101 KB of 160, of which three of 53 are not to be had.  (us with two for all heads,
+// and so: heads of 64, 4 x 1024 over 8192, 298, 236; 7 x 32 over up to 12000, 43, 38;
+// one of 2000, 56, 59; of 256, 4 x 256 over 8192, 291, 279; one of 2000, 125, 104.  Of
+// 128 with three: 4 x 512 over 8192, 318, 379.)
 template <int D, bool F32> struct Many {
-    static constexpr int kMine = 32, kKeys = 4 * kMine, kRows = F32 ? 32 : 64, kPerCU = F32 || D == 256 ? 2 : 3;
+    static constexpr int kMine = 32, kKeys = 4 * kMine, kRows = F32 ? 32 : 64, kPerCU = F32 ? D == 64 ? 3 : D == 128 ? 2 : 1 : D == 256 ? 2 : 3;
     static constexpr int kSetup = 1;                // the keys' way and the sums', dealt as tiles of rows
 };
 constexpr int kManyRuns = 3 * 256;                  // at most
@@ -351,7 +355,7 @@ template <int D, bool F32> struct ManyDeal {
 // twice.  7 x 32 over 3001 to 12000: 42 us, 2.2 TB/s: each head's keys are waited
 // for before 128 rows of queries.
 template <class T, int D, bool F32>
-__global__ void __launch_bounds__(256, (F32 && D == 256 ? 1 : Many<D, F32>::kPerCU)) weigh_many_kernel(const WeighArgs a)
+__global__ void __launch_bounds__(256, (Many<D, F32>::kPerCU)) weigh_many_kernel(const WeighArgs a)
 {
     using M = Many<D, F32>;
     constexpr int kMine = M::kMine, kKeys = M::kKeys, kSetup = M::kSetup, kRows = M::kRows, U = kRows / 32;
@@ -663,13 +667,22 @@ __global__ void __launch_bounds__(256) weigh_join_kernel(const WeighArgs a, int 
 namespace {
 
 constexpr size_t kLeftBytes = (gs::kManyRuns * sizeof(gs::Left) + 15) / 16 * 16;
-constexpr uint32_t kFewRows = 32;       // query rows per head of keys that the first kernel takes
+// Query rows per head of keys that the first kernel takes.  (us with 16, 32, 64; 16
+// sequences over up to 8000, 32 / 8 heads of 128, f16, 24 rows: 65, 56, 56; 32: 65, 59,
+// 59; 48: 66, 66, 67; 64: 67, 67, 77.  f32, 8 sequences, 24: 45, 51, 51; 48: 58, 58, 66;
+// 64: 58, 58, 78.  Four, heads of 64, 32: 16, 10, 10; heads of 256, eight, 24 to 64:
+// within 2 of one another.)
+constexpr uint32_t kFewRows = 32;
 
 template <class T, int D, bool F32> void by_rows(gs::WeighArgs a, uint64_t rows, hipStream_t st)
 {
     const bool few = rows <= kFewRows, alike = (uint64_t)a.n_tokens * a.group == rows * a.n;
     if (few || !alike) {
         a.max_rows = few ? 0xffffffffu : kFewRows;
+        // (us with 512, 1024, 2048 runs: 16 single tokens over up to 4000, 28 / 4 heads,
+        // bf16: 16.7, 14.9, 17.9; 64 over up to 32768: 115, 112, 108; 8 x 4 over up to
+        // 6000, 32 / 8, f16: 22.4, 20.4, 23.2; heads of 256, f32, 4 over up to 12000: 47,
+        // 53, 53)
         a.n_wg = 1024;
         hipLaunchKernelGGL((gs::weigh_few_kernel<T, D, F32>), dim3(a.n_wg), dim3(256), 0, st, a);
     }

@@ -687,14 +687,15 @@ _DT = None
 
 def _dtypes():
     """torch's value types and what they are here, its 4-byte integers, the
-    current stream's handle without an object on the way, and the current
-    device's number (None: there is one device)."""
+    current stream's handle without an object on the way, the current device's
+    number (None: there is one device), and whether its stream is captured."""
     global _DT
     if _DT is None:
         import torch
         _DT = ({torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}, (torch.int32, torch.uint32),
                getattr(torch._C, "_cuda_getCurrentRawStream", None),
-               torch.cuda.current_device if torch.cuda.device_count() > 1 else None)
+               torch.cuda.current_device if torch.cuda.device_count() > 1 else None,
+               getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing))
     return _DT
 
 
@@ -761,9 +762,8 @@ def _stream_of(dev, stream):
 def _may_capture(dev, st):
     """Whether a call on the stream st of device dev may be recorded into a
     graph now: it is unless st is torch's stream of the moment and records none."""
-    import torch
-    now = (_DT or _dtypes())[3]
-    return (now is not None and now() != dev) or st != _stream_of(dev, None) or torch.cuda.is_current_stream_capturing()
+    _, _, raw, now, capturing = _DT or _dtypes()
+    return (now is not None and now() != dev) or raw is None or st != raw(dev) or capturing()
 
 
 def _empty_on(st, shape, dtype, like):
@@ -872,7 +872,8 @@ class KVCache:
         self.c.ws = self.ws.data_ptr()
         self._attn_ws = {}
         self._more_ws = {}
-        self._graph_ws = set()          # addresses of those that were given to a capture
+        self._weigh_bytes = self._lib.gs_attn_weigh_workspace(self._c)
+        self._graph_ws = set()          # of these, whose last one a capture may have been given
 
     @classmethod
     def empty(cls, layers, pages, kv, d, rows, max_len, page=16, dtype=None, device="cuda"):
@@ -933,8 +934,7 @@ class KVCache:
 
     def _mass(self, mass):
         """Values from row to row of a tensor as mass() makes it."""
-        import torch
-        if mass.dtype != torch.float32 or mass.dim() != 2 or mass.get_device() != self.dev or mass.stride(1) != 1:
+        if (_DT or _dtypes())[0].get(mass.dtype) != TYPE_F32 or mass.dim() != 2 or mass.get_device() != self.dev or mass.stride(1) != 1:
             raise TypeError("mass must be a [rows, tokens] tensor of float32 on the cache's device")
         if mass.shape[0] != self.rows or mass.shape[1] < self.table.shape[1] * self.page:
             raise ValueError("mass must have the cache's rows and room for the most tokens of each")
@@ -968,20 +968,22 @@ class KVCache:
         where they do not overlap: up to an eighth more, so that calls of about
         one size share it.  A larger one takes its place, unless a captured graph
         may hold it: then it stays and the new one is at least twice its size."""
-        import torch
         if not n:
             raise SamplerError(GS_ERR_INVALID, what)
-        held = self._more_ws.setdefault((what, st), [])
+        key = (what, st)
+        held = self._more_ws.setdefault(key, [])
         if not held or held[-1].numel() < n:
+            import torch
             step = 1 << max(n.bit_length() - 4, 0)
             size = -(-n // step) * step
-            if held and held[-1].data_ptr() in self._graph_ws:
+            if key in self._graph_ws:
                 size = max(size, 2 * held[-1].numel())
+                self._graph_ws.remove(key)
             elif held:
                 held.pop()
             held.append(_empty_on(st, size, torch.uint8, like))
-        if _may_capture(self.dev, st):
-            self._graph_ws.add(held[-1].data_ptr())
+        if key not in self._graph_ws and _may_capture(self.dev, st):
+            self._graph_ws.add(key)
         return held[-1]
 
     def _batch(self, T, rows, q_start):
@@ -1017,10 +1019,9 @@ class KVCache:
 
     def _lse(self, lse, T, heads):
         """The address of a contiguous [T, heads] float32 tensor, or None."""
-        import torch
         if lse is None:
             return None
-        if lse.dtype != torch.float32 or lse.get_device() != self.dev or not lse.is_contiguous():
+        if (_DT or _dtypes())[0].get(lse.dtype) != TYPE_F32 or lse.get_device() != self.dev or not lse.is_contiguous():
             raise TypeError("lse must be a contiguous tensor of float32 on the cache's device")
         if lse.shape != (T, heads):
             raise ValueError("lse must be [tokens, heads]")
@@ -1107,7 +1108,7 @@ class KVCache:
         ld = self._mass(mass)
         b = self._batch(T, rows, q_start)
         st = _stream_of(self.dev, stream)
-        ws = self._workspace("weigh", st, self._lib.gs_attn_weigh_workspace(self._c), mass)
+        ws = self._workspace("weigh", st, self._weigh_bytes, mass)
         a = GsWeighArgs(_type(q, "q"), heads, q.data_ptr(), ld_q, self._lse(lse, T, heads), mass.data_ptr(), ld, keep, scale, window,
                         max_q, ws.data_ptr(), ws.numel())
         _call(self.dev, self._lib.gs_attn_weigh, "gs_attn_weigh", self._c, layer, ctypes.byref(b), ctypes.byref(a), st)

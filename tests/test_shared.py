@@ -393,6 +393,7 @@ def test_workspaces_of_growing_calls(gpu, torch):
     q = torch.randn((600, 64, 64), device="cuda").half()
     out, start = torch.empty_like(q), words(torch, [0, 1, 600])
     c._more_ws.clear()
+    c._graph_ws.clear()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.stream(s):
         with torch.cuda.graph(graph, stream=s):

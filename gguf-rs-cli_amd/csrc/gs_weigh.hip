@@ -350,9 +350,11 @@ template <int D, bool F32> struct ManyDeal {
 // next one's loads pass while this one is worked on), and a lane adds up the
 // weights of query row lane & 31 for the keys that its results of S^T = K Q^T,
 // 32 x 32 x 16, are of.  Measured: 4 x 2048 tokens over 2100 to 8192, 32 / 8 heads
-// of 128, bf16: 376 us, 650 TFLOP/s (a library product of 8192 x 8192 x 8192:
-// 1226); vector issue is 63 % of the clocks, the matrix cores 33 %, no bank is met
-// twice.  7 x 32 over 3001 to 12000: 42 us, 2.2 TB/s: each head's keys are waited
+// of 128, bf16: 372 us a call, of which weigh_join_kernel 5, 655 TFLOP/s (a library
+// product of 8192 x 8192 x 8192: 1226); by itself, under a profiler, whose load lowers
+// the clock, 381 to 437.  Vector issue is 63 % of the clocks, the matrix cores 33 %,
+// no bank is met twice.  7 x 32 over 3001 to 12000: 42 us, 2.3 TB/s: each head's keys
+// are waited
 // for before 128 rows of queries.
 template <class T, int D, bool F32>
 __global__ void __launch_bounds__(256, (Many<D, F32>::kPerCU)) weigh_many_kernel(const WeighArgs a)

@@ -1067,6 +1067,12 @@ class KVCache:
         as fork() leaves them.  A family's common pages are read once, not once
         for each row; the result is attend()'s formula's whatever the rows
         hold, and never less precise (gs_attn_shared).
+        It has three launches for attend()'s two, about 12 us more, so it pays
+        where attend() would read a family's common pages often: single tokens
+        of 16 bits from some 250 MB of keys and values a call on (rows x common
+        tokens x bytes; 16 rows over 4000, 8 heads of 128), with f32 queries from
+        2 GB on, in families of 16 rows or more.  For less, and for chunks of
+        hundreds of tokens, attend() is faster.
         The cache keeps a workspace of 43 to 85 MB, and of 8 d + 44 bytes for each
         token and head (d as 64, 128 or 256), for each stream that attend_shared
         was called on, as attend does; a call of more tokens than those before
